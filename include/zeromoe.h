@@ -39,6 +39,7 @@ typedef struct zm_tensor {
 /* ggml_type ids used on this path */
 enum {
   ZM_TYPE_F32 = 0,
+  ZM_TYPE_F16 = 1, /* F16, BF16: the dense operators below */
   ZM_TYPE_Q2_K = 10,
   ZM_TYPE_Q3_K = 11,
   ZM_TYPE_Q4_K = 12,
@@ -49,6 +50,7 @@ enum {
   ZM_TYPE_IQ3_XXS = 18,
   ZM_TYPE_IQ4_XS = 23,
   ZM_TYPE_I32 = 26,
+  ZM_TYPE_BF16 = 30,
 };
 
 /* ---------------------------------------------------------------- library */
@@ -319,6 +321,95 @@ int zm_expert_ffn_finish_stage1(zm_expert_scratch *s, const void *slab, size_t d
 int zm_expert_ffn_finish_stage2(zm_expert_scratch *s, float *host_out, int S, int D, void *stream);
 /* Read (and optionally reset) the NaN / Inf counters. */
 int zm_expert_bad_counts(zm_expert_scratch *s, int32_t counts[2], int reset);
+
+/* ---------------------------------------------------------------- dense operators around the layer
+ *
+ * What a block has next to its routed experts, with the gradients of a step
+ * that trains the router and the norm over frozen quantized experts: the
+ * unquantized matrix product (router, shared expert, attention output), the
+ * layer norm, the weighted sum of the experts' rows and the gradient of the
+ * routing.  No counterpart among the reference's kernels; the products of
+ * quantized weights are zm_f32_matmul and zm_mul_mat_id.
+ *
+ * Types are F32, F16 and BF16; all sums are f32 in a fixed order, so a call
+ * repeats its bits.  Rows have strides in elements (columns are contiguous);
+ * rows that are read may overlap, rows that are written may not.  Nothing is
+ * allocated and nothing synchronises: a call records into a HIP graph, given
+ * a workspace of its own for as long as the graph may run.  A workspace needs
+ * no clearing. */
+
+/* y[s] = act(x[s] . w^T + bias) + residual[s], x [S][I], w [O][I].
+ *   x F32 with w F32, F16 or BF16; x F16 with w F16; x BF16 with w BF16
+ *   y, residual and pre: F32 or x's type;  bias F32 [O]
+ * f32 operands keep their 24 bits (they enter as sums of bf16 terms); results
+ * are rounded once.  A row or column with an infinity or NaN gives non-finite
+ * results.  pre (optional) receives x . w^T + bias for the backward pass.
+ * residual (optional) may be y itself.  S may be 0. */
+enum {
+  ZM_ACT_NONE = 0,
+  ZM_ACT_RELU = 1,
+  ZM_ACT_GELU = 2,      /* z (1 + erf(z / sqrt 2)) / 2 */
+  ZM_ACT_GELU_TANH = 3, /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+  ZM_ACT_SILU = 4,
+  ZM_ACT_SIGMOID = 5,
+};
+typedef struct zm_linear_desc {
+  int32_t x_type, w_type, y_type; /* y_type: of y, residual, pre and dy */
+  int32_t act;
+  int64_t S, I, O;
+  int64_t x_stride, w_stride, y_stride, res_stride, pre_stride; /* y_stride: of y and dy */
+} zm_linear_desc;
+size_t zm_linear_workspace_size(const zm_linear_desc *desc);
+int zm_linear(const zm_linear_desc *desc, const void *x, const void *w, const float *bias, const void *residual, void *y,
+              void *pre, void *workspace, size_t workspace_size, void *stream);
+/* Gradients by dy [S][O]: dz = dy act'(pre), dx = dz w [S][I] of x's type,
+ * dw = dz^T x [O][I] f32, dbias = sum_s dz [O] f32; each is skipped when NULL,
+ * contiguous otherwise (the residual's gradient is dy).  pre is needed with an
+ * activation.  With S == 0 dw and dbias are zero.  x is read for dw alone, w
+ * for dx alone. */
+size_t zm_linear_backward_workspace_size(const zm_linear_desc *desc);
+int zm_linear_backward(const zm_linear_desc *desc, const void *dy, const void *x, const void *w, const void *pre,
+                       void *dx, float *dw, float *dbias, void *workspace, size_t workspace_size, void *stream);
+
+/* y[r] = (x[r] - mean_r) rstd_r weight + bias over rows of n values,
+ * rstd = 1 / sqrt(variance + eps); x and y of `type`, weight and bias F32 [n]
+ * (NULL: 1 and 0); mean and rstd F32 [rows] (optional) for the backward pass.
+ * y may be x. */
+int zm_layer_norm(int type, const void *x, int64_t x_stride, const float *weight, const float *bias, float eps,
+                  int64_t rows, int64_t n, void *y, int64_t y_stride, float *mean, float *rstd, void *stream);
+/* dx [rows][n] of `type`, dweight and dbias F32 [n], each skipped when NULL.
+ * The workspace is for dweight and dbias.  dx may be dy or x.  With rows == 0
+ * dweight and dbias are zero. */
+size_t zm_layer_norm_backward_workspace_size(int64_t rows, int64_t n);
+int zm_layer_norm_backward(int type, const void *dy, int64_t dy_stride, const void *x, int64_t x_stride,
+                           const float *weight, const float *mean, const float *rstd, int64_t rows, int64_t n, void *dx,
+                           int64_t dx_stride, float *dweight, float *dbias, void *workspace, size_t workspace_size,
+                           void *stream);
+
+/* out[s] = residual[s] + sum_k weights[s][k] y[s][k] over the experts' rows
+ * y [S][K][H] (strides in elements), as zm_mul_mat_id leaves them; all F32,
+ * weights and out contiguous, K <= 64.  A route with ids[s][k] < 0 (ids
+ * optional) takes no part and its row is not read.  residual (optional) may be
+ * out.  The sum inside zm_moe_forward, for callers that keep the rows. */
+int zm_combine(const float *y, int64_t y_tok, int64_t y_route, const float *weights, const int32_t *ids,
+               const float *residual, int64_t S, int K, int H, float *out, void *stream);
+/* dweights[s][k] = <dout[s], y[s][k]> and dy[s][k] = weights[s][k] dout[s]
+ * (contiguous), each skipped when NULL; zero for routes with a negative id.
+ * y is read for dweights alone, weights for dy alone. */
+int zm_combine_backward(const float *dout, const float *y, int64_t y_tok, int64_t y_route, const float *weights,
+                        const int32_t *ids, int64_t S, int K, int H, float *dweights, float *dy, void *stream);
+
+/* Gradient of zm_router's weights by its logits, the selection held fixed:
+ * dlogits [S][E] from dweights [S][K].  ids are expert ids, those zm_router
+ * gives without a slot table (an expert named twice counts twice); a negative
+ * one takes no part, a row of them alone (padding) has a zero gradient, and an
+ * id >= n_experts gives a NaN row.  dprobs [E] (optional) is added to the
+ * gradient of every token's gate probabilities (a balance loss on their mean;
+ * rows without a route excepted).  The gradient by logit_bias is the sum of
+ * dlogits over the tokens (zm_linear_backward's dbias).  spec as for
+ * zm_router; the groups do not matter here. */
+int zm_router_backward(const zm_router_spec *spec, const float *logits, const float *logit_bias, const int32_t *ids,
+                       const float *dweights, const float *dprobs, int S, float *dlogits, void *stream);
 
 /* ---------------------------------------------------------------- expert records
  *

@@ -21,11 +21,17 @@ libzeromoe_hip.so (include/zeromoe.h):
 * :func:`moe_unpack` -- expert-major [gate|up|down] transfer records to the
   planar expert tensors (launch_ggml_moe_unpack[_scatter],
   kernels/math/ggml_moe_pack.cu:127-179).
+* The dense operators around the layer, with their gradients: :func:`linear`
+  (unquantized matrix product with bias, activation and residual),
+  :func:`layer_norm`, :func:`combine` (weighted sum of the experts' rows) and
+  :func:`router_backward` (gradient of :func:`router`'s weights).
 
 Torch is used only for device memory and the current stream.
 """
 from __future__ import annotations
 
+from .dense import (combine, combine_backward, layer_norm, layer_norm_backward, linear, linear_backward,
+                    router_backward)
 from .ops import (GGML_TYPES, ColdLane, ExpertExecutor, MoELayer, block_dots, bucket, builtin_iq2xxs_grid, builtin_iq3xxs_grid,
                   builtin_iq4nl_table,                   f32_matmul,
                   glm5next_router_topk, init, moe_unpack, mul_mat_id, mul_mat_id_f32, quantize_q8_K, router, row_size,
@@ -34,4 +40,6 @@ from .ops import (GGML_TYPES, ColdLane, ExpertExecutor, MoELayer, block_dots, bu
 __all__ = ["GGML_TYPES", "ColdLane", "ExpertExecutor", "MoELayer", "block_dots", "bucket", "builtin_iq2xxs_grid", "builtin_iq3xxs_grid", "builtin_iq4nl_table",
            "f32_matmul",
            "glm5next_router_topk", "init", "moe_unpack", "mul_mat_id", "mul_mat_id_f32", "quantize_q8_K", "router", "row_size",
-           "scatter_accum", "set_iq2xxs_grid", "set_iq3xxs_grid", "set_iq4nl_table", "swiglu"]
+           "scatter_accum", "set_iq2xxs_grid", "set_iq3xxs_grid", "set_iq4nl_table", "swiglu",
+           "combine", "combine_backward", "layer_norm", "layer_norm_backward", "linear", "linear_backward",
+           "router_backward"]

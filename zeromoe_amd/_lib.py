@@ -49,6 +49,11 @@ class ZmColdLaneStats(C.Structure):
                 ("merge_ns", C.c_int64), ("vectorized", I32)]
 
 
+class ZmLinearDesc(C.Structure):
+    _fields_ = [("x_type", I32), ("w_type", I32), ("y_type", I32), ("act", I32), ("S", I64), ("I", I64), ("O", I64),
+                ("x_stride", I64), ("w_stride", I64), ("y_stride", I64), ("res_stride", I64), ("pre_stride", I64)]
+
+
 _MM = (None, [P, P, P, I, I, I])
 _MMS = (None, [P, P, P, I, I, I, P])
 _XS = C.POINTER(ZmExpertScratch)
@@ -106,6 +111,16 @@ SIGNATURES = {
     "zm_expert_ffn_finish_stage2": (I, [_XS, P, I, I, P]),
     "zm_expert_bad_counts": (I, [_XS, P, I]),
     "zm_moe_forward": (I, [C.POINTER(ZmMoeLayer), P, P, I, P, P, P, P, SZ, P]),
+    "zm_linear_workspace_size": (SZ, [C.POINTER(ZmLinearDesc)]),
+    "zm_linear": (I, [C.POINTER(ZmLinearDesc), P, P, P, P, P, P, P, SZ, P]),
+    "zm_linear_backward_workspace_size": (SZ, [C.POINTER(ZmLinearDesc)]),
+    "zm_linear_backward": (I, [C.POINTER(ZmLinearDesc), P, P, P, P, P, P, P, P, SZ, P]),
+    "zm_layer_norm": (I, [I, P, I64, P, P, F, I64, I64, P, I64, P, P, P]),
+    "zm_layer_norm_backward_workspace_size": (SZ, [I64, I64]),
+    "zm_layer_norm_backward": (I, [I, P, I64, P, I64, P, P, P, I64, I64, P, I64, P, P, P, SZ, P]),
+    "zm_combine": (I, [P, I64, I64, P, P, P, I64, I, I, P, P]),
+    "zm_combine_backward": (I, [P, P, I64, I64, P, P, I64, I, I, P, P, P]),
+    "zm_router_backward": (I, [C.POINTER(ZmRouterSpec), P, P, P, P, P, I, P, P]),
     "zm_cold_lane_create": (P, [C.POINTER(ZmColdLaneDesc)]),
     "zm_cold_lane_destroy": (None, [P]),
     "zm_cold_lane_fork": (I, [P, P, P, P, I, P]),

@@ -1,0 +1,281 @@
+// zm_linear.hip -- C ABI of the unquantized matrix product with bias, activation and residual, and of its gradients:
+// checks of the arguments, choice of tiles and k slices, workspace layout.  The kernels are in zm_linear.hpp; the
+// quantized counterpart is zm_f32_matmul.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/zeromoe.h"
+#include "zm_host.hpp"
+#include "zm_linear.hpp"
+
+using namespace zm;
+
+namespace {
+
+// ============================================================ dz and the bias gradient
+
+struct DzArgs {
+  const void *dy, *pre;  // [S][O] of `type`; pre null without an activation
+  int64_t ldy, ldp, S, O;
+  int type, act;
+  float *dz;         // [S][ldz] f32, or null (without an activation dy is dz)
+  int64_t ldz;
+  float *part;       // [gridDim.y][O] sums over this chunk of rows, or null
+  int64_t chunk;     // rows of a chunk
+};
+
+// One thread keeps one column of one chunk of rows: dz = dy * act'(pre), and the column's sum over the chunk in f32.
+__global__ __launch_bounds__(256) void k_linear_dz(DzArgs g) {
+  const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (o >= g.O) return;
+  const int64_t s0 = blockIdx.y * g.chunk, s1 = min(g.S, s0 + g.chunk);
+  float sum = 0.f;
+  for (int64_t s = s0; s < s1; ++s) {
+    float v = lin_load(g.dy, g.type, (size_t)(s * g.ldy + o));
+    if (g.act) v *= lin_act_slope(lin_load(g.pre, g.type, (size_t)(s * g.ldp + o)), g.act);
+    if (g.dz) g.dz[(size_t)(s * g.ldz + o)] = v;
+    sum += v;
+  }
+  if (g.part) g.part[(size_t)blockIdx.y * g.O + o] = sum;
+}
+
+// dst[i] = sum over z < n of part[z][i], z ascending
+__global__ __launch_bounds__(256) void k_linear_rows_sum(const float *__restrict__ part, int n, int64_t O,
+                                                         float *__restrict__ dst) {
+  const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (o >= O) return;
+  float v = 0.f;
+  for (int z = 0; z < n; ++z) v += part[(size_t)z * O + o];
+  dst[o] = v;
+}
+
+__global__ __launch_bounds__(256) void k_linear_zero(float *__restrict__ dst, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) dst[i] = 0.f;
+}
+
+// ============================================================ choices
+
+struct Plan {
+  int tile, tiles_m, tiles_n, slices;
+  int64_t kslice;
+  size_t part;  // bytes of the slices' partial results
+};
+
+// Tiles of 128 x 128, or 32 x 128 for up to 64 rows; k in as many slices as give about two workgroups per CU
+// (at least four tiles of k each), as long as the partial sums stay below 64 MB.
+Plan plan(int64_t M, int64_t N, int64_t K, bool vec) {
+  Plan p{};
+  p.tile = !vec || M <= 64;
+  const int bm = p.tile ? 32 : 128;
+  p.tiles_m = (int)((M + bm - 1) / bm);
+  p.tiles_n = (int)((N + 127) / 128);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  int64_t z = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), K / 256));
+  z = std::min(z, std::max<int64_t>(1, (int64_t)(64 << 20) / (M * N * 4)));
+  p.kslice = ((K + z - 1) / z + 63) / 64 * 64;
+  p.slices = (int)((K + p.kslice - 1) / p.kslice);
+  p.part = p.slices > 1 ? (size_t)p.slices * M * N * 4 : 0;
+  return p;
+}
+
+size_t size_of(int type) { return type == LIN_F32 ? 4 : 2; }
+bool lin_type(int t) { return t == LIN_F32 || t == LIN_F16 || t == LIN_BF16; }
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// whether an operand can be read 16 bytes at a time: `row` values contiguous in memory, taken 8 at a time where they
+// are k (kc), else in 16 bytes
+bool vec16(const void *p, int64_t ld, int64_t row, int type, bool kc) {
+  const size_t e = size_of(type);
+  return !((uintptr_t)p & 15) && !((size_t)ld * e & 15) && !(kc ? row & 7 : (int64_t)((size_t)row * e & 15));
+}
+
+int64_t dz_stride(int64_t O) { return (O + 3) / 4 * 4; }
+constexpr int DZ_CHUNK = 64;
+int64_t dz_chunks(int64_t S) { return std::min<int64_t>((S + DZ_CHUNK - 1) / DZ_CHUNK, 256); }
+
+// Workspace of the backward pass: dz in f32 (behind an activation) | bias partials | the larger product's partials.
+// It is sized for either choice of vector loads, so that it depends on the description alone.
+struct BackwardSpace {
+  size_t dz, bias, part, total;
+};
+BackwardSpace backward_space(const zm_linear_desc &d) {
+  BackwardSpace w{};
+  w.dz = d.act ? align256((size_t)d.S * dz_stride(d.O) * 4) : 0;
+  w.bias = align256((size_t)dz_chunks(d.S) * d.O * 4);
+  for (int vec = 0; vec < 2; ++vec) {
+    w.part = std::max(w.part, align256(plan(d.S, d.I, d.O, vec).part));
+    w.part = std::max(w.part, align256(plan(d.O, d.I, d.S, vec).part));
+  }
+  w.total = w.dz + w.bias + w.part;
+  return w;
+}
+
+int check_desc(const zm_linear_desc *d, const char *who) {
+  if (!d) return fail("%s: null description", who);
+  if (!lin_type(d->x_type) || !lin_type(d->w_type) || !lin_type(d->y_type))
+    return fail("%s: types are F32, F16 and BF16", who);
+  if (d->x_type != ZM_TYPE_F32 && d->w_type != d->x_type)
+    return fail("%s: 16-bit activations need weights of their own type", who);
+  if (d->y_type != ZM_TYPE_F32 && d->y_type != d->x_type)
+    return fail("%s: the result is F32 or of the activations' type", who);
+  if (d->act < 0 || d->act >= ACT_COUNT) return fail("%s: unknown activation %d", who, d->act);
+  if (d->S < 0 || d->I <= 0 || d->O <= 0) return fail("%s: S >= 0, I > 0 and O > 0 are needed", who);
+  const int64_t most = (int64_t)1 << 31;
+  if (d->S >= most || d->I >= most || d->O >= most) return fail("%s: S, I and O are below 2^31", who);
+  if (d->x_stride < 0 || d->w_stride < 0 || d->y_stride < 0 || d->res_stride < 0 || d->pre_stride < 0)
+    return fail("%s: negative stride", who);
+  if (((d->S + 31) / 32) * ((d->O + 127) / 128) > 0x3fffff || ((d->S + 31) / 32) * ((d->I + 127) / 128) > 0x3fffff ||
+      ((d->O + 31) / 32) * ((d->I + 127) / 128) > 0x3fffff)
+    return fail("%s: S x O, S x I or O x I too large for one launch", who);
+  return 0;
+}
+
+// the rows of a written matrix must not overlap
+int check_rows(int64_t rows, int64_t stride, int64_t width, const char *who, const char *what) {
+  if (rows > 1 && stride < width) return fail("%s: rows of %s overlap", who, what);
+  return 0;
+}
+
+int launched() {
+  HIP_OK(hipGetLastError());
+  return 0;
+}
+
+LinArgs product(const void *a, int64_t lda, const void *b, int64_t ldb, int64_t M, int64_t N, int64_t K, const Plan &p,
+                float *part) {
+  LinArgs g{};
+  g.a = a;
+  g.b = b;
+  g.lda = lda;
+  g.ldb = ldb;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.tiles_m = p.tiles_m;
+  g.tiles_n = p.tiles_n;
+  g.slices = p.slices;
+  g.kslice = p.kslice;
+  g.part = part;
+  return g;
+}
+
+int join(const LinArgs &g, hipStream_t st) {
+  if (g.slices > 1) {
+    const int64_t n = g.M * ((g.N + 3) / 4);
+    hipLaunchKernelGGL(k_linear_join, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g);
+  }
+  return launched();
+}
+
+bool vec4(const void *p, int64_t ld, int type) {
+  return !p || (!((uintptr_t)p & (4 * size_of(type) - 1)) && !(ld & 3));
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t zm_linear_workspace_size(const zm_linear_desc *d) {
+  if (check_desc(d, "zm_linear_workspace_size") || !d->S) return 0;
+  return std::max(align256(plan(d->S, d->O, d->I, false).part), align256(plan(d->S, d->O, d->I, true).part));
+}
+
+int zm_linear(const zm_linear_desc *d, const void *x, const void *w, const float *bias, const void *residual, void *y,
+              void *pre, void *workspace, size_t workspace_size, void *stream) {
+  if (check_desc(d, "zm_linear")) return -1;
+  if (check_rows(d->S, d->y_stride, d->O, "zm_linear", "y")) return -1;
+  if (pre && check_rows(d->S, d->pre_stride, d->O, "zm_linear", "pre")) return -1;
+  if (!d->S) return 0;
+  if (!x || !w || !y) return fail("zm_linear: null pointer");
+  const bool vec = vec16(x, d->x_stride, d->I, d->x_type, true) && vec16(w, d->w_stride, d->I, d->w_type, true);
+  const Plan p = plan(d->S, d->O, d->I, vec);
+  if (p.part && (!workspace || workspace_size < p.part || ((uintptr_t)workspace & 255)))
+    return fail("zm_linear: a 256-byte aligned workspace of zm_linear_workspace_size() bytes is needed");
+  LinArgs g = product(x, d->x_stride, w, d->w_stride, d->S, d->O, d->I, p, (float *)workspace);
+  g.e.y = y;
+  g.e.res = residual;
+  g.e.pre = pre;
+  g.e.bias = bias;
+  g.e.ldy = d->y_stride;
+  g.e.ldr = d->res_stride;
+  g.e.ldp = d->pre_stride;
+  g.e.type = d->y_type;
+  g.e.act = d->act;
+  g.e.vec = vec4(y, d->y_stride, d->y_type) && vec4(residual, d->res_stride, d->y_type) &&
+            vec4(pre, d->pre_stride, d->y_type) && vec4(bias, 0, LIN_F32);
+  lin_fwd(d->x_type, d->w_type, g, vec, p.tile, (hipStream_t)stream);
+  return join(g, (hipStream_t)stream);
+}
+
+size_t zm_linear_backward_workspace_size(const zm_linear_desc *d) {
+  if (check_desc(d, "zm_linear_backward_workspace_size") || !d->S) return 0;
+  return backward_space(*d).total;
+}
+
+int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, const void *w, const void *pre, void *dx,
+                       float *dw, float *dbias, void *workspace, size_t workspace_size, void *stream) {
+  if (check_desc(d, "zm_linear_backward")) return -1;
+  const hipStream_t st = (hipStream_t)stream;
+  if (!d->S) {  // no rows: the sums over them are zero
+    if (dw) hipLaunchKernelGGL(k_linear_zero, dim3(256), dim3(256), 0, st, dw, d->O * d->I);
+    if (dbias) hipLaunchKernelGGL(k_linear_zero, dim3(1), dim3(256), 0, st, dbias, d->O);
+    return launched();
+  }
+  if (!dy || (dw && !x) || (dx && !w)) return fail("zm_linear_backward: null pointer");
+  if (d->act && !pre) return fail("zm_linear_backward: an activation's gradient needs pre");
+  if (!dx && !dw && !dbias) return 0;
+  const BackwardSpace s = backward_space(*d);
+  if (s.total && (!workspace || workspace_size < s.total || ((uintptr_t)workspace & 255)))
+    return fail("zm_linear_backward: a 256-byte aligned workspace of zm_linear_backward_workspace_size() bytes is needed");
+  uint8_t *ws = (uint8_t *)workspace;
+  float *dz = (float *)ws, *bias_part = (float *)(ws + s.dz), *part = (float *)(ws + s.dz + s.bias);
+  if (d->act || dbias) {
+    DzArgs a{};
+    a.dy = dy;
+    a.pre = pre;
+    a.ldy = d->y_stride;
+    a.ldp = d->pre_stride;
+    a.S = d->S;
+    a.O = d->O;
+    a.type = d->y_type;
+    a.act = d->act;
+    a.dz = d->act ? dz : nullptr;
+    a.ldz = dz_stride(d->O);
+    a.part = dbias ? bias_part : nullptr;
+    const int64_t n = dz_chunks(d->S);
+    a.chunk = (d->S + n - 1) / n;
+    hipLaunchKernelGGL(k_linear_dz, dim3((unsigned)((d->O + 255) / 256), (unsigned)n), dim3(256), 0, st, a);
+    if (dbias)
+      hipLaunchKernelGGL(k_linear_rows_sum, dim3((unsigned)((d->O + 255) / 256)), dim3(256), 0, st, bias_part, (int)n,
+                         d->O, dbias);
+  }
+  const void *g_z = d->act ? (const void *)dz : dy;
+  const int64_t ldz = d->act ? dz_stride(d->O) : d->y_stride;
+  const int z_type = d->act ? (int)LIN_F32 : d->y_type;
+  if (dx) {  // M = S, N = I, K = O
+    const bool vec = vec16(g_z, ldz, d->O, z_type, true) && vec16(w, d->w_stride, d->I, d->w_type, false);
+    const Plan p = plan(d->S, d->I, d->O, vec);
+    LinArgs g = product(g_z, ldz, w, d->w_stride, d->S, d->I, d->O, p, part);
+    g.e.y = dx;
+    g.e.ldy = d->I;
+    g.e.type = d->x_type;
+    g.e.vec = vec4(dx, d->I, d->x_type);
+    lin_dx(d->x_type, d->w_type, z_type, g, vec, p.tile, st);
+    if (join(g, st)) return -1;
+  }
+  if (dw) {  // M = O, N = I, K = S
+    const bool vec = vec16(g_z, ldz, d->O, z_type, false) && vec16(x, d->x_stride, d->I, d->x_type, false);
+    const Plan p = plan(d->O, d->I, d->S, vec);
+    LinArgs g = product(g_z, ldz, x, d->x_stride, d->O, d->I, d->S, p, part);
+    g.e.y = dw;
+    g.e.ldy = d->I;
+    g.e.type = LIN_F32;
+    g.e.vec = vec4(dw, d->I, LIN_F32);
+    lin_dw(d->x_type, z_type, g, vec, p.tile, st);
+    if (join(g, st)) return -1;
+  }
+  return launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,518 @@
+// zm_linear.hpp -- matrix products of unquantized operands on the matrix cores:
+// C[m][n] = sum_k A(m, k) B(n, k) with an epilogue (bias, activation,
+// residual), and its gradients.
+//
+// f32 operands have no fast matrix instruction (the f32 forms run at 1/16 of the
+// bf16 rate), so an f32 value enters as a sum of bf16 terms
+//   v = t0 + t1 + t2,  t0 = bf16(v), t1 = bf16(v - t0), t2 = bf16(v - t0 - t1)
+// (3 x 8 significant bits cover the 24 of f32; the differences are exact), an f16
+// value as two (11 bits), a bf16 value as one.  A product of two sums keeps the
+// term pairs (i, j) with i + j <= 2 (each next pair is 2^-9 smaller with
+// round-to-nearest terms; what is left out is below 2^-26 of |a||b|): 6 bf16
+// products for f32 x f32, 5 for f32 x f16, 3 for f32 x bf16, accumulated in f32.
+// bf16 x bf16 and f16 x f16 are one product in their own type.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+namespace zm {
+
+struct bf16 {
+  uint16_t u;
+};
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+enum { LIN_F32 = 0, LIN_F16 = 1, LIN_BF16 = 30 };
+enum { ACT_NONE = 0, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU, ACT_SIGMOID, ACT_COUNT };
+
+template <class T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<_Float16>(_Float16 v) { return (float)v; }
+template <>
+__device__ __forceinline__ float to_f32<bf16>(bf16 v) { return __uint_as_float((uint32_t)v.u << 16); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ _Float16 from_f32<_Float16>(float v) { return (_Float16)v; }
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float v) { return bf16{__builtin_bit_cast(uint16_t, (__bf16)v)}; }
+
+__device__ __forceinline__ float lin_load(const void *p, int type, size_t i) {
+  if (type == LIN_F32) return ((const float *)p)[i];
+  if (type == LIN_F16) return (float)((const _Float16 *)p)[i];
+  return to_f32(((const bf16 *)p)[i]);
+}
+__device__ __forceinline__ void lin_store(void *p, int type, size_t i, float v) {
+  if (type == LIN_F32) ((float *)p)[i] = v;
+  else if (type == LIN_F16) ((_Float16 *)p)[i] = (_Float16)v;
+  else ((bf16 *)p)[i] = from_f32<bf16>(v);
+}
+// four values at an offset whose address is a multiple of 4 elements
+__device__ __forceinline__ v4f lin_load4(const void *p, int type, size_t i) {
+  if (type == LIN_F32) return *reinterpret_cast<const v4f *>((const float *)p + i);
+  const uint2 r = *reinterpret_cast<const uint2 *>((const uint16_t *)p + i);
+  if (type == LIN_F16) {
+    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+    const v4h h = __builtin_bit_cast(v4h, r);
+    return v4f{(float)h.x, (float)h.y, (float)h.z, (float)h.w};
+  }
+  return v4f{__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16),
+             __uint_as_float(r.y & 0xffff0000u)};
+}
+__device__ __forceinline__ void lin_store4(void *p, int type, size_t i, v4f v) {
+  if (type == LIN_F32) {
+    *reinterpret_cast<v4f *>((float *)p + i) = v;
+  } else if (type == LIN_F16) {
+    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<v4h *>((_Float16 *)p + i) =
+        v4h{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+  } else {
+    typedef __bf16 v4b __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<v4b *>((bf16 *)p + i) = v4b{(__bf16)v.x, (__bf16)v.y, (__bf16)v.z, (__bf16)v.w};
+  }
+}
+
+// act(z) and its slope; gelu by erf, gelu_tanh by its tanh form
+__device__ __forceinline__ float lin_act(float z, int act) {
+  switch (act) {
+  case ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
+  case ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  case ACT_GELU_TANH: return 0.5f * z * (1.0f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
+  case ACT_SILU: return z / (1.0f + expf(-z));
+  case ACT_SIGMOID: return 1.0f / (1.0f + expf(-z));
+  default: return z;
+  }
+}
+__device__ __forceinline__ float lin_act_slope(float z, int act) {
+  switch (act) {
+  case ACT_RELU: return z > 0.f ? 1.0f : 0.0f;
+  case ACT_GELU: {
+    const float zc = fminf(fmaxf(z, -20.f), 20.f);  // exp(-z^2/2) is 0 there; z * exp() has no inf * 0
+    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + zc * expf(-0.5f * zc * zc) * 0.39894228040143268f;
+  }
+  case ACT_GELU_TANH: {
+    const float zc = fminf(fmaxf(z, -20.f), 20.f);  // tanh is +-1 there: slope 0 or 1
+    const float t = tanhf(0.79788456080286536f * (zc + 0.044715f * zc * zc * zc));
+    return 0.5f * (1.0f + t) + 0.5f * zc * (1.0f - t * t) * 0.79788456080286536f * (1.0f + 0.134145f * zc * zc);
+  }
+  case ACT_SILU: {
+    const float zc = fminf(fmaxf(z, -120.f), 120.f);  // the sigmoid is 0 or 1 there
+    const float g = 1.0f / (1.0f + expf(-zc));
+    return g * (1.0f + zc * (1.0f - g));
+  }
+  case ACT_SIGMOID: {
+    const float g = 1.0f / (1.0f + expf(-z));
+    return g * (1.0f - g);
+  }
+  default: return 1.0f;
+  }
+}
+
+// ============================================================ terms
+
+constexpr float BF16_MOST = 3.38953139e38f;  // largest finite bf16
+
+// v[8] as NT bf16 terms.  Values past bf16's largest would round to infinity and
+// leave inf - inf behind: they are cut instead, and an infinity is one term.
+template <int NT>
+__device__ __forceinline__ void split_terms(const float (&v)[8], v8bf (&t)[NT]) {
+  if constexpr (NT == 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[0][i] = (__bf16)v[i];
+    return;
+  } else {
+    float r[8];
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      t[0][i] = (__bf16)v[i];
+      r[i] = v[i] - (float)t[0][i];
+      m = fmaxf(m, fabsf(v[i]));
+    }
+    if (m > BF16_MOST) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (fabsf(v[i]) > BF16_MOST) {
+          const float hi = __uint_as_float(__float_as_uint(v[i]) & 0xffff0000u);
+          t[0][i] = (__bf16)hi;
+          r[i] = fabsf(v[i]) == __builtin_inff() ? 0.f : v[i] - hi;
+        }
+    }
+#pragma unroll
+    for (int k = 1; k < NT; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        t[k][i] = (__bf16)r[i];
+        if (k + 1 < NT) r[i] -= (float)t[k][i];
+      }
+  }
+}
+
+template <class T>
+struct Is16 {
+  static constexpr bool value = sizeof(T) == 2;
+};
+
+// ============================================================ operands
+//
+// A tile of ROWS rows (m or n) x BK columns (k) goes from global memory through
+// registers into LDS, one plane per term: plane[row][BK] of 16-bit values, rows of
+// BK * 2 bytes whose 16-byte chunks are permuted by the row so that eight
+// neighbouring rows of one chunk lie in different banks (fragment reads), and
+// rows eight (16-bit) or four (f32) apart too (the writes of a row-contiguous
+// operand).
+//
+// A unit is one thread's part: 8 consecutive k of one row where k is contiguous
+// in memory (KC), else 16 bytes of rows for each of 8 consecutive k, transposed
+// in registers.
+template <int BK>
+__device__ __forceinline__ int chunk_at(int row, int c) {
+  if (BK == 64) return c ^ ((row ^ (row >> 3)) & 7);
+  const int v = row >> 1;
+  return c ^ ((v ^ (v >> 1)) & 3);
+}
+
+template <class T, int NT, bool KC, int ROWS, int BK, int NTHR, bool VEC>
+struct Operand {
+  static constexpr int R = KC ? 1 : 16 / (int)sizeof(T);  // rows of a unit
+  static constexpr int CH = BK / 8;
+  static constexpr int UNITS = ROWS / R * CH;
+  static constexpr int UPT = UNITS > NTHR ? UNITS / NTHR : 1;
+  static constexpr int NV = KC ? (int)sizeof(T) / 2 : 8;  // 16-byte registers of a unit
+  static constexpr int PLANE = ROWS * BK;                 // 16-bit values of a term plane
+  static_assert(UNITS % NTHR == 0 || UNITS < NTHR, "units split evenly over the threads");
+
+  const T *base;
+  int64_t ld;
+  int rows;   // of the matrix, from the tile's first row
+  int first;  // the thread's first unit
+  bool on;
+  v4u raw[UPT][NV];
+
+  // `row0`: the tile's first row; `total`: rows of the matrix
+  __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t total, int t) {
+    ld = ld_;
+    base = (const T *)p + (KC ? row0 * ld : row0);
+    rows = (int)(total - row0 < ROWS ? total - row0 : ROWS);
+    on = t >= 0 && t < UNITS;
+    first = t;
+  }
+  __device__ __forceinline__ static void place(int u, int &row, int &c) {
+    if (KC) {
+      row = u / CH;
+      c = u % CH;
+    } else {
+      row = u % (ROWS / R) * R;
+      c = u / (ROWS / R);
+    }
+  }
+  // columns [k, k + BK) of the tile, zeros from `kend` on; rows past the matrix
+  // repeat its last ones (their results are not stored)
+  __device__ __forceinline__ void load(int64_t k, int64_t kend) {
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      int row, c;
+      place(first + i * NTHR, row, c);
+      if (!on) continue;
+      const int64_t kc = k + 8 * c;
+      if constexpr (KC) {
+        const T *p = base + (int64_t)min(row, rows - 1) * ld + kc;
+        if constexpr (VEC) {
+#pragma unroll
+          for (int q = 0; q < NV; ++q)
+            raw[i][q] = kc < kend ? reinterpret_cast<const v4u *>(p)[q] : v4u{0, 0, 0, 0};
+        } else {
+          T e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = kc + j < kend ? p[j] : from_f32<T>(0.f);
+          __builtin_memcpy(raw[i], e, sizeof(e));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const T *p = base + (kc + j) * ld;
+          if constexpr (VEC) {
+            raw[i][j] = kc + j < kend ? *reinterpret_cast<const v4u *>(p + min(row, rows - R)) : v4u{0, 0, 0, 0};
+          } else {
+            T e[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) e[r] = kc + j < kend ? p[min(row + r, rows - 1)] : from_f32<T>(0.f);
+            __builtin_memcpy(&raw[i][j], e, sizeof(e));
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void put(uint16_t *lds, int row, int c, v8bf (&t)[NT]) const {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      *reinterpret_cast<v8bf *>(lds + n * PLANE + row * BK + chunk_at<BK>(row, c) * 8) = t[n];
+  }
+  __device__ __forceinline__ void store(uint16_t *lds) const {
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      int row, c;
+      place(first + i * NTHR, row, c);
+      if (!on) continue;
+      if constexpr (KC && sizeof(T) == 2) {
+        if constexpr (NT == 1) {
+          *reinterpret_cast<v4u *>(lds + row * BK + chunk_at<BK>(row, c) * 8) = raw[i][0];
+        } else {
+          T e[8];
+          float v[8];
+          __builtin_memcpy(e, raw[i], sizeof(e));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+          v8bf t[NT];
+          split_terms<NT>(v, t);
+          put(lds, row, c, t);
+        }
+      } else if constexpr (KC) {
+        float v[8];
+        __builtin_memcpy(v, raw[i], sizeof(v));
+        v8bf t[NT];
+        split_terms<NT>(v, t);
+        put(lds, row, c, t);
+      } else if constexpr (sizeof(T) == 2) {
+        // raw[j] holds rows (0,1)(2,3)(4,5)(6,7) at column j; row 2q + h: its halves of the eight columns
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            v4u o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              o[j] = __builtin_amdgcn_perm(raw[i][2 * j + 1][q], raw[i][2 * j][q], h ? 0x07060302u : 0x05040100u);
+            const int r = row + 2 * q + h;
+            if constexpr (NT == 1) {
+              *reinterpret_cast<v4u *>(lds + r * BK + chunk_at<BK>(r, c) * 8) = o;
+            } else {
+              T e[8];
+              float v[8];
+              __builtin_memcpy(e, &o, sizeof(e));
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+              v8bf t[NT];
+              split_terms<NT>(v, t);
+              put(lds, r, c, t);
+            }
+          }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw[i][j][r]);
+          v8bf t[NT];
+          split_terms<NT>(v, t);
+          put(lds, row + r, c, t);
+        }
+      }
+    }
+  }
+};
+
+// ============================================================ the product
+
+struct LinEpilogue {
+  void *y;             // [M][N], row stride ldy, of type `type`
+  const void *res;     // [M][N] of the same type, or null
+  void *pre;           // [M][N] of the same type: z = sum + bias before the activation, or null
+  const float *bias;   // [N] or null
+  int64_t ldy, ldr, ldp;
+  int type, act;
+  int vec;             // rows and bases of y, res, pre and bias allow 4 values at once
+};
+
+struct LinArgs {
+  const void *a, *b;
+  int64_t lda, ldb;
+  int64_t M, N, K;
+  int tiles_m, tiles_n;
+  int slices;      // of k
+  int64_t kslice;  // columns of a slice (a multiple of BK)
+  float *part;     // [slices][M][N] when slices > 1
+  LinEpilogue e;
+};
+
+__device__ __forceinline__ float lin_finish1(const LinEpilogue &e, int64_t m, int64_t n, float z) {
+  if (e.bias) z += e.bias[n];
+  if (e.pre) lin_store(e.pre, e.type, (size_t)(m * e.ldp + n), z);
+  float y = lin_act(z, e.act);
+  if (e.res) y += lin_load(e.res, e.type, (size_t)(m * e.ldr + n));
+  return y;
+}
+// four results of one row, columns n .. n + 3 of which those below N exist
+__device__ __forceinline__ void lin_finish4(const LinEpilogue &e, int64_t m, int64_t n, int64_t N, v4f z) {
+  if (e.vec && n + 4 <= N) {
+    if (e.bias) z += *reinterpret_cast<const v4f *>(e.bias + n);
+    if (e.pre) lin_store4(e.pre, e.type, (size_t)(m * e.ldp + n), z);
+    if (e.act) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[j] = lin_act(z[j], e.act);
+    }
+    if (e.res) z += lin_load4(e.res, e.type, (size_t)(m * e.ldr + n));
+    lin_store4(e.y, e.type, (size_t)(m * e.ldy + n), z);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (n + j < N) lin_store(e.y, e.type, (size_t)(m * e.ldy + n + j), lin_finish1(e, m, n + j, z[j]));
+}
+
+// Workgroup -> tile.  Workgroups go to the 8 XCDs in turn; each XCD takes a run
+// of neighbouring tiles instead, so that the operands they share meet in its L2.
+__device__ __forceinline__ int xcd_order(int b, int n) {
+  const int q = n / 8, r = n % 8, x = b % 8;
+  return x * q + min(x, r) + b / 8;
+}
+
+// The term pairs of a product: (0,0) first, then those 2^-9, 2^-18 smaller
+template <int NA, int NB>
+struct Pairs {
+  static constexpr int MOST = 2;  // i + j
+};
+
+// One workgroup: BM x BN results over one slice of k; WM x WN waves of 16 x 16
+// matrix instructions.  The next tile's global loads are in flight while the
+// current one is multiplied.  The instruction's rows are the results' columns n,
+// so that a lane ends with 4 neighbouring n of one row m.
+template <class TA, int NA, bool KCA, class TB, int NB, bool KCB, int BM, int BN, int WM, int WN, bool VEC>
+__global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
+  constexpr bool F16 = std::is_same<TA, _Float16>::value && std::is_same<TB, _Float16>::value && NA == 1 && NB == 1;
+  constexpr int BK = NA * NB == 1 ? 64 : 32;
+  constexpr int NTHR = 64 * WM * WN;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  typedef Operand<TA, NA, KCA, BM, BK, NTHR, VEC> OA;
+  typedef Operand<TB, NB, KCB, BN, BK, NTHR, VEC> OB;
+  __shared__ __attribute__((aligned(16))) uint16_t lds_a[NA * BM * BK];
+  __shared__ __attribute__((aligned(16))) uint16_t lds_b[NB * BN * BK];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tile = xcd_order(blockIdx.x, gridDim.x);
+  const int per = g.tiles_m * g.tiles_n;
+  const int z = tile / per, tt = tile - z * per;
+  const int64_t m0 = (int64_t)(tt / g.tiles_n) * BM, n0 = (int64_t)(tt % g.tiles_n) * BN;
+  const int64_t kb = z * g.kslice, ke = min(g.K, kb + g.kslice);
+  OA a;
+  OB b;
+  a.init(g.a, g.lda, m0, g.M, tid);
+  // an operand with fewer units than threads is loaded by the last threads: the other one's units are with the first
+  b.init(g.b, g.ldb, n0, g.N, OB::UNITS < NTHR ? tid - (NTHR - OB::UNITS) : tid);
+  v4f acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const int fr = lane & 15, fc = lane >> 4;
+  a.load(kb, ke);
+  b.load(kb, ke);
+  for (int64_t k = kb; k < ke; k += BK) {
+    a.store(lds_a);
+    b.store(lds_b);
+    __syncthreads();
+    if (k + BK < ke) {
+      a.load(k + BK, ke);
+      b.load(k + BK, ke);
+    }
+#pragma unroll
+    for (int s = 0; s < BK / 32; ++s) {
+      v8bf fa[FM][NA], fb[FN][NB];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int r = wm + 16 * i + fr;
+#pragma unroll
+        for (int t = 0; t < NA; ++t)
+          fa[i][t] = *reinterpret_cast<const v8bf *>(lds_a + t * BM * BK + r * BK + chunk_at<BK>(r, 4 * s + fc) * 8);
+      }
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int r = wn + 16 * j + fr;
+#pragma unroll
+        for (int t = 0; t < NB; ++t)
+          fb[j][t] = *reinterpret_cast<const v8bf *>(lds_b + t * BN * BK + r * BK + chunk_at<BK>(r, 4 * s + fc) * 8);
+      }
+#pragma unroll
+      for (int ta = 0; ta < NA; ++ta)
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb) {
+          if (ta + tb > Pairs<NA, NB>::MOST) continue;
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+              if constexpr (F16)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, fb[j][tb]),
+                                                                  __builtin_bit_cast(v8h, fa[i][ta]), acc[i][j], 0, 0, 0);
+              else
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j][tb], fa[i][ta], acc[i][j], 0, 0, 0);
+            }
+        }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int64_t m = m0 + wm + 16 * i + fr, n = n0 + wn + 16 * j + 4 * fc;
+      if (m >= g.M || n >= g.N) continue;
+      if (g.slices > 1) {
+        float *p = g.part + ((size_t)z * g.M + m) * g.N + n;
+        if (!(g.N & 3)) *reinterpret_cast<v4f *>(p) = acc[i][j];
+        else
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (n + q < g.N) p[q] = acc[i][j][q];
+      } else {
+        lin_finish4(g.e, m, n, g.N, acc[i][j]);
+      }
+    }
+}
+
+// Results of the k slices added in order (the same bits on every call), then the epilogue.
+static __global__ __launch_bounds__(256) void k_linear_join(LinArgs g) {
+  const int64_t nq = (g.N + 3) / 4, q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (q >= g.M * nq) return;
+  const int64_t m = q / nq, n = (q - m * nq) * 4;
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+  const size_t plane = (size_t)g.M * g.N;
+  const float *p = g.part + (size_t)m * g.N + n;
+  if (!(g.N & 3)) {
+    for (int z = 0; z < g.slices; ++z) v += *reinterpret_cast<const v4f *>(p + z * plane);
+  } else {
+    for (int z = 0; z < g.slices; ++z)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < g.N) v[j] += p[z * plane + j];
+  }
+  lin_finish4(g.e, m, n, g.N, v);
+}
+
+// The launch of one kernel instance.  `tile` 0 = 128 x 128, 1 = 32 x 128; operands without 16-byte loads (`vec`
+// false) take 32 x 128.
+template <class TA, int NA, bool KCA, class TB, int NB, bool KCB>
+void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices));
+  if (!vec) hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 4, false>), grid, dim3(256), 0, st, g);
+  else if (tile) hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 4, true>), grid, dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 2, true>), grid, dim3(256), 0, st, g);
+}
+
+// the products by what their operands are: forward (x, w), dx (dz, w), dw (dz, x)
+void lin_fwd(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
+void lin_dx(int x_type, int w_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
+void lin_dw(int x_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
+
+}  // namespace zm
