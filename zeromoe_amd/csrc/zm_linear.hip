@@ -23,31 +23,61 @@ struct DzArgs {
   int64_t ldz;
   float *part;       // [gridDim.y][O] sums over this chunk of rows, or null
   int64_t chunk;     // rows of a chunk
+  int packs, side;   // packs of V columns that a workgroup takes, and rows that it takes at once
 };
 
-// One thread keeps one column of one chunk of rows: dz = dy * act'(pre), and the column's sum over the chunk in f32.
+// dz = dy * act'(pre), and its sums over a chunk of rows in f32.  A thread keeps V columns and takes every side-th row
+// of the chunk, four at a time; the rows' sums meet in LDS in order.
+template <int V>
 __global__ __launch_bounds__(256) void k_linear_dz(DzArgs g) {
-  const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (o >= g.O) return;
+  __shared__ float red[256 * V];
+  const int c = threadIdx.x % g.packs, r = threadIdx.x / g.packs;
+  const int64_t o = ((int64_t)blockIdx.x * g.packs + c) * V;
   const int64_t s0 = blockIdx.y * g.chunk, s1 = min(g.S, s0 + g.chunk);
-  float sum = 0.f;
-  for (int64_t s = s0; s < s1; ++s) {
-    float v = lin_load(g.dy, g.type, (size_t)(s * g.ldy + o));
-    if (g.act) v *= lin_act_slope(lin_load(g.pre, g.type, (size_t)(s * g.ldp + o)), g.act);
-    if (g.dz) g.dz[(size_t)(s * g.ldz + o)] = v;
-    sum += v;
+  v4f sum = {0.f, 0.f, 0.f, 0.f};
+  if (o < g.O && r < g.side) {
+    for (int64_t s = s0 + r; s < s1; s += 4 * g.side) {
+      v4f v[4], p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t su = s + u * g.side;
+        const bool in = su < s1;
+        if constexpr (V == 4) {
+          v[u] = in ? lin_load4(g.dy, g.type, (size_t)(su * g.ldy + o)) : v4f{0.f, 0.f, 0.f, 0.f};
+          if (g.act) p[u] = in ? lin_load4(g.pre, g.type, (size_t)(su * g.ldp + o)) : v4f{0.f, 0.f, 0.f, 0.f};
+        } else {
+          v[u].x = in ? lin_load(g.dy, g.type, (size_t)(su * g.ldy + o)) : 0.f;
+          if (g.act) p[u].x = in ? lin_load(g.pre, g.type, (size_t)(su * g.ldp + o)) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t su = s + u * g.side;
+        if (su >= s1) break;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (g.act) v[u][j] *= lin_act_slope(p[u][j], g.act);
+          sum[j] += v[u][j];
+        }
+        if (g.dz) {
+          float *d = g.dz + su * g.ldz + o;
+          if constexpr (V == 4) *reinterpret_cast<v4f *>(d) = v[u];
+          else *d = v[u].x;
+        }
+      }
+    }
   }
-  if (g.part) g.part[(size_t)blockIdx.y * g.O + o] = sum;
-}
-
-// dst[i] = sum over z < n of part[z][i], z ascending
-__global__ __launch_bounds__(256) void k_linear_rows_sum(const float *__restrict__ part, int n, int64_t O,
-                                                         float *__restrict__ dst) {
-  const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (o >= O) return;
-  float v = 0.f;
-  for (int z = 0; z < n; ++z) v += part[(size_t)z * O + o];
-  dst[o] = v;
+  if (!g.part) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) red[(r * g.packs + c) * V + j] = sum[j];  // (threads past side * packs have sums of zero)
+  __syncthreads();
+  for (int j = threadIdx.x; j < g.packs * V; j += 256) {
+    const int64_t k = (int64_t)blockIdx.x * g.packs * V + j;
+    if (k >= g.O) break;
+    float a = 0.f;
+    for (int q = 0; q < g.side; ++q) a += red[q * g.packs * V + j];
+    g.part[(size_t)blockIdx.y * g.O + k] = a;
+  }
 }
 
 __global__ __launch_bounds__(256) void k_linear_zero(float *__restrict__ dst, int64_t n) {
@@ -91,8 +121,8 @@ bool vec16(const void *p, int64_t ld, int64_t row, int type, bool kc) {
 }
 
 int64_t dz_stride(int64_t O) { return (O + 3) / 4 * 4; }
-constexpr int DZ_CHUNK = 64;
-int64_t dz_chunks(int64_t S) { return std::min<int64_t>((S + DZ_CHUNK - 1) / DZ_CHUNK, 256); }
+// chunks of rows of the bias gradient: 32 rows each, at most 256
+int64_t dz_chunks(int64_t S) { return std::min<int64_t>((S + 31) / 32, 256); }
 
 // Workspace of the backward pass: dz in f32 (behind an activation) | bias partials | the larger product's partials.
 // It is sized for either choice of vector loads, so that it depends on the description alone.
@@ -245,10 +275,14 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
     a.part = dbias ? bias_part : nullptr;
     const int64_t n = dz_chunks(d->S);
     a.chunk = (d->S + n - 1) / n;
-    hipLaunchKernelGGL(k_linear_dz, dim3((unsigned)((d->O + 255) / 256), (unsigned)n), dim3(256), 0, st, a);
-    if (dbias)
-      hipLaunchKernelGGL(k_linear_rows_sum, dim3((unsigned)((d->O + 255) / 256)), dim3(256), 0, st, bias_part, (int)n,
-                         d->O, dbias);
+    const bool v = !(d->O & 3) && vec4(dy, d->y_stride, d->y_type) && (!d->act || vec4(pre, d->pre_stride, d->y_type));
+    const int64_t packs = v ? d->O / 4 : d->O;
+    a.packs = (int)std::min<int64_t>(packs, 64);
+    a.side = 256 / a.packs;
+    const dim3 grid((unsigned)((packs + a.packs - 1) / a.packs), (unsigned)n);
+    if (v) hipLaunchKernelGGL((k_linear_dz<4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_linear_dz<1>), grid, dim3(256), 0, st, a);
+    if (dbias) parts_sum(bias_part, (int)n, d->O, d->O, dbias, nullptr, st);
   }
   const void *g_z = d->act ? (const void *)dz : dy;
   const int64_t ldz = d->act ? dz_stride(d->O) : d->y_stride;

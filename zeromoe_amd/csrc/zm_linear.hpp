@@ -164,6 +164,58 @@ struct Is16 {
   static constexpr bool value = sizeof(T) == 2;
 };
 
+// ============================================================ sums over partial rows
+
+// dst0[i] (i < n0) and dst1[i - n0] (n0 <= i < n) = sum over p < parts of part[p][i], either null: not wanted.  A
+// workgroup takes 16 packs of V columns; its 16 groups of 16 threads take every 16th part, eight loads in flight, and
+// their sums meet in LDS, all in a fixed order.  512 parts of 14336 columns (29 MB): 9 us, against 123 us with a
+// thread per column going through all parts.
+template <int V>
+static __global__ __launch_bounds__(256) void k_parts_sum(const float *__restrict__ part, int parts, int64_t n, int64_t n0,
+                                                          float *__restrict__ dst0, float *__restrict__ dst1) {
+  __shared__ float red[16][16 * V];
+  const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int64_t i = ((int64_t)blockIdx.x * 16 + c) * V;
+  float v[V] = {};
+  if (i < n) {
+    for (int p0 = g; p0 < parts; p0 += 128) {
+      float t[8][V];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int p = p0 + 16 * u;
+        if constexpr (V == 4) {
+          const v4f r = p < parts ? *reinterpret_cast<const v4f *>(part + (size_t)p * n + i) : v4f{0.f, 0.f, 0.f, 0.f};
+          t[u][0] = r.x, t[u][1] = r.y, t[u][2] = r.z, t[u][3] = r.w;
+        } else {
+          t[u][0] = p < parts ? part[(size_t)p * n + i] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += t[u][j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) red[g][c * V + j] = v[j];
+  __syncthreads();
+  for (int j = threadIdx.x; j < 16 * V; j += 256) {
+    const int64_t k = (int64_t)blockIdx.x * 16 * V + j;
+    if (k >= n) break;
+    float a = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) a += red[q][j];
+    float *dst = k < n0 ? dst0 : dst1;
+    if (dst) dst[k < n0 ? k : k - n0] = a;
+  }
+}
+static inline void parts_sum(const float *part, int parts, int64_t n, int64_t n0, float *dst0, float *dst1, hipStream_t st) {
+  if (!(n & 3) && !((uintptr_t)part & 15))
+    hipLaunchKernelGGL((k_parts_sum<4>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, part, parts, n, n0, dst0, dst1);
+  else
+    hipLaunchKernelGGL((k_parts_sum<1>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, part, parts, n, n0, dst0, dst1);
+}
+
 // ============================================================ operands
 //
 // A tile of ROWS rows (m or n) x BK columns (k) goes from global memory through

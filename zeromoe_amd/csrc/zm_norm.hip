@@ -32,19 +32,33 @@ struct NormArgs {
   float eps;
 };
 
-// sum over the TPR threads of a row (64 or 256); every one of them gets it
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float *red) {
+// sums over the TPR threads of a row (64 and more); every one of them gets them.  `red`: one entry for each wave of
+// the workgroup, not in use by another sum; all threads of the workgroup call together where TPR > 64.
+template <int TPR, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[N]) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  for (int o = 32; o; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], o);
   if (TPR > 64) {
-    const int wave = threadIdx.x >> 6;
-    __syncthreads();  // the last sum has been read
-    if (!(threadIdx.x & 63)) red[wave] = v;
+    const int wave = threadIdx.x >> 6, first = wave / (TPR / 64) * (TPR / 64);
+    if (!(threadIdx.x & 63))
+#pragma unroll
+      for (int k = 0; k < N; ++k) red[wave][k] = v[k];
     __syncthreads();
-    v = (red[0] + red[1]) + (red[2] + red[3]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      v[k] = red[first][k];
+#pragma unroll
+      for (int w = 1; w < TPR / 64; ++w) v[k] += red[first + w][k];
+    }
   }
-  return v;
+}
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float (*red)[1]) {
+  float a[1] = {v};
+  row_sums<TPR, 1>(a, red);
+  return a[0];
 }
 
 // 16 bytes of T as floats
@@ -75,71 +89,88 @@ __device__ __forceinline__ void load_vec(const float *p, int i, bool on, int V, 
   }
 }
 
-// TPR threads keep one row in C packs of 16 bytes each; 256 / TPR rows per workgroup.
-template <class T, int TPR, int C>
-__global__ __launch_bounds__(256) void k_norm(NormArgs g) {
-  constexpr int V = Pack<T>::V;
-  __shared__ float red[4];
+// Workgroups of NT threads go over the rows; TPR = 64 or NT threads keep one row in C packs of 16 bytes each.  Weight
+// and bias stay in registers (from L2 they are 8 bytes a value next to 4 of a 16-bit row), and the next row's loads are
+// in flight while this one's sums are taken.  Buffers of the sums alternate, so that one barrier a sum is enough.
+template <class T, int NT, int TPR, int C>
+__global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
+  constexpr int V = Pack<T>::V, RPB = NT / TPR;
+  __shared__ float red[2][2][NT / 64][1];
   const int t = threadIdx.x & (TPR - 1);
-  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  if (TPR == 64 && row >= g.rows) return;
-  const T *x = (const T *)g.x + row * g.ldx;
-  float v[C][V];
-  float sum = 0.f;
+  float w[C][V], b[C][V];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = (t + TPR * c) * V;
-    unpack<T>(i < g.n ? *reinterpret_cast<const v4u *>(x + i) : v4u{0, 0, 0, 0}, v[c]);
+    load_vec(g.weight, i, i < g.n, V, 1.0f, w[c]);
+    load_vec(g.bias, i, i < g.n, V, 0.0f, b[c]);
   }
+  const float n = (float)g.n;
+  v4u next[C];
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  auto fetch = [&](int64_t r) {
+    const T *x = (const T *)g.x + r * g.ldx;
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int j = 0; j < V; ++j) sum += v[c][j];
-  const float mean = row_sum<TPR>(sum, red) / (float)g.n;
-  float sq = 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const bool in = (t + TPR * c) * V < g.n;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      v[c][j] = in ? v[c][j] - mean : 0.f;
-      sq += v[c][j] * v[c][j];
+    for (int c = 0; c < C; ++c) {
+      const int i = (t + TPR * c) * V;
+      next[c] = r < g.rows && i < g.n ? *reinterpret_cast<const v4u *>(x + i) : v4u{0, 0, 0, 0};
     }
-  }
-  const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, red) / (float)g.n + g.eps);
-  T *y = (T *)g.y + row * g.ldy;
+  };
+  fetch(row);
+  // (with one row per workgroup all threads leave the loop together)
+  for (int par = 0; row < g.rows; row += step, par ^= 1) {
+    float v[C][V];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int i = (t + TPR * c) * V;
-    if (i >= g.n) continue;
-    float w[V], b[V];
-    load_vec(g.weight, i, true, V, 1.0f, w);
-    load_vec(g.bias, i, true, V, 0.0f, b);
+    for (int c = 0; c < C; ++c) unpack<T>(next[c], v[c]);
+    fetch(row + step);
+    float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[c][j] = v[c][j] * rstd * w[j] + b[j];
-    *reinterpret_cast<v4u *>(y + i) = pack<T>(v[c]);
-  }
-  if (!t) {
-    if (g.mean) g.mean[row] = mean;
-    if (g.rstd) g.rstd[row] = rstd;
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum += v[c][j];
+    const float mean = row_sum<TPR>(sum, red[par][0]) / n;
+    float sq = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const bool in = (t + TPR * c) * V < g.n;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[c][j] = in ? v[c][j] - mean : 0.f;
+        sq = __builtin_fmaf(v[c][j], v[c][j], sq);
+      }
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, red[par][1]) / n + g.eps);
+    T *y = (T *)g.y + row * g.ldy;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int i = (t + TPR * c) * V;
+      if (i >= g.n) continue;
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[c][j] = __builtin_fmaf(v[c][j] * rstd, w[c][j], b[c][j]);
+      __builtin_nontemporal_store(pack<T>(v[c]), reinterpret_cast<v4u *>(y + i));
+    }
+    if (!t) {
+      if (g.mean) g.mean[row] = mean;
+      if (g.rstd) g.rstd[row] = rstd;
+    }
   }
 }
 
 // Any width and alignment: a row is read three times (the later ones from L2).
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_any(NormArgs g) {
-  __shared__ float red[4];
+  __shared__ float red[2][4][1];
   const int64_t row = blockIdx.x;
   const T *x = (const T *)g.x + row * g.ldx;
   float sum = 0.f;
   for (int i = threadIdx.x; i < g.n; i += 256) sum += to_f32(x[i]);
-  const float mean = row_sum<256>(sum, red) / (float)g.n;
+  const float mean = row_sum<256>(sum, red[0]) / (float)g.n;
   float sq = 0.f;
   for (int i = threadIdx.x; i < g.n; i += 256) {
     const float d = to_f32(x[i]) - mean;
     sq += d * d;
   }
-  const float rstd = 1.0f / sqrtf(row_sum<256>(sq, red) / (float)g.n + g.eps);
+  const float rstd = 1.0f / sqrtf(row_sum<256>(sq, red[1]) / (float)g.n + g.eps);
   T *y = (T *)g.y + row * g.ldy;
   for (int i = threadIdx.x; i < g.n; i += 256) {
     const float h = (to_f32(x[i]) - mean) * rstd;
@@ -151,73 +182,113 @@ __global__ __launch_bounds__(256) void k_norm_any(NormArgs g) {
   }
 }
 
-// Workgroup b takes rows b, b + gridDim.x, ...: each thread keeps the same columns throughout, so the sums over the
-// rows stay in its registers until the end.
-template <class T, int C>
-__global__ __launch_bounds__(256) void k_norm_backward(NormArgs g) {
-  constexpr int V = Pack<T>::V;
-  __shared__ float red[4];
-  const int t = threadIdx.x;
-  float dw[C][V], db[C][V];
+// NT threads, TPR of them for a row: a workgroup goes over rows b * NT / TPR + ..., and each thread keeps the same
+// columns throughout, so the sums over the rows stay in its registers until the end, and the weight too.  The next
+// rows' loads are in flight while this one's sums are taken.
+template <class T, int NT, int TPR, int C>
+__global__ __launch_bounds__(NT) void k_norm_backward(NormArgs g) {
+  constexpr int V = Pack<T>::V, RPB = NT / TPR;
+  __shared__ float red[2][NT / 64][2];
+  __shared__ __attribute__((aligned(16))) float meet[RPB > 1 ? 2 * TPR * C * V : 4];
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  float dw[C][V], db[C][V], w[C][V];
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+  for (int c = 0; c < C; ++c) {
+    const int i = (t + TPR * c) * V;
+    load_vec(g.weight, i, i < g.n, V, 1.0f, w[c]);
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[c][j] = db[c][j] = 0.f;
-  for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
-    const T *x = (const T *)g.x + row * g.ldx, *dy = (const T *)g.dy + row * g.ldg;
-    const float mean = g.mean[row], rstd = g.rstd[row];
+  }
+  v4u nx[C], ng[C];
+  float nm, nr;
+  auto fetch = [&](int64_t r) {
+    const T *x = (const T *)g.x + r * g.ldx, *dy = (const T *)g.dy + r * g.ldg;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int i = (t + TPR * c) * V;
+      const bool in = r < g.rows && i < g.n;
+      nx[c] = in ? *reinterpret_cast<const v4u *>(x + i) : v4u{0, 0, 0, 0};
+      ng[c] = in ? *reinterpret_cast<const v4u *>(dy + i) : v4u{0, 0, 0, 0};
+    }
+    nm = r < g.rows ? g.mean[r] : 0.f;
+    nr = r < g.rows ? g.rstd[r] : 0.f;
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t first = (int64_t)blockIdx.x * RPB;
+  fetch(first + group);
+  int par = 0;
+  for (; first < g.rows; first += step, par ^= 1) {  // the same for the whole workgroup: a row past the end adds zeros
+    const int64_t row = first + group;
+    const float mean = nm, rstd = nr;
     v4u rx[C], rg[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int i = (t + 256 * c) * V;
-      rx[c] = i < g.n ? *reinterpret_cast<const v4u *>(x + i) : v4u{0, 0, 0, 0};
-      rg[c] = i < g.n ? *reinterpret_cast<const v4u *>(dy + i) : v4u{0, 0, 0, 0};
-    }
-    float s1 = 0.f, s2 = 0.f;
+    for (int c = 0; c < C; ++c) rx[c] = nx[c], rg[c] = ng[c];
+    fetch(row + step);
+    float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int i = (t + 256 * c) * V;
-      float xv[V], gv[V], w[V];
+      float xv[V], gv[V];
       unpack<T>(rx[c], xv);
       unpack<T>(rg[c], gv);
-      load_vec(g.weight, i, i < g.n, V, 1.0f, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float h = (xv[j] - mean) * rstd;  // past n: dy is 0, so nothing is added
-        dw[c][j] += gv[j] * h;
+        const float gw = gv[j] * w[c][j];
+        dw[c][j] = __builtin_fmaf(gv[j], h, dw[c][j]);
         db[c][j] += gv[j];
-        s1 += gv[j] * w[j];
-        s2 += gv[j] * w[j] * h;
+        s[0] += gw;
+        s[1] = __builtin_fmaf(gw, h, s[1]);
       }
     }
-    s1 = row_sum<256>(s1, red) / (float)g.n;
-    s2 = row_sum<256>(s2, red) / (float)g.n;
-    if (g.y) {
-      T *dx = (T *)g.y + row * g.ldy;
+    row_sums<TPR, 2>(s, red[par]);
+    if (!g.y || row >= g.rows) continue;
+    const float s1 = s[0] / (float)g.n, rs2 = s[1] / (float)g.n * rstd;
+    T *dx = (T *)g.y + row * g.ldy;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int i = (t + 256 * c) * V;
-        if (i >= g.n) continue;
-        float xv[V], gv[V], w[V];
-        unpack<T>(rx[c], xv);
-        unpack<T>(rg[c], gv);
-        load_vec(g.weight, i, true, V, 1.0f, w);
+    for (int c = 0; c < C; ++c) {
+      const int i = (t + TPR * c) * V;
+      if (i >= g.n) continue;
+      float xv[V], gv[V];
+      unpack<T>(rx[c], xv);
+      unpack<T>(rg[c], gv);
 #pragma unroll
-        for (int j = 0; j < V; ++j) xv[j] = rstd * (gv[j] * w[j] - s1 - (xv[j] - mean) * rstd * s2);
-        *reinterpret_cast<v4u *>(dx + i) = pack<T>(xv);
-      }
+      for (int j = 0; j < V; ++j) xv[j] = rstd * __builtin_fmaf(mean - xv[j], rs2, __builtin_fmaf(gv[j], w[c][j], -s1));
+      __builtin_nontemporal_store(pack<T>(xv), reinterpret_cast<v4u *>(dx + i));
     }
   }
   if (!g.part) return;
+  if (RPB > 1) {  // the groups' sums, one group after the other
+    for (int q = 0; q < RPB; ++q) {
+      if (group == q) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            float *m = meet + (c * V + j) * TPR + t;
+            m[0] = q ? m[0] + dw[c][j] : dw[c][j];
+            m[TPR * C * V] = q ? m[TPR * C * V] + db[c][j] : db[c][j];
+          }
+      }
+      __syncthreads();
+    }
+    if (group) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        dw[c][j] = meet[(c * V + j) * TPR + t];
+        db[c][j] = meet[(C * V + c * V + j) * TPR + t];
+      }
+  }
   float *pw = g.part + (size_t)blockIdx.x * 2 * g.n, *pb = pw + g.n;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int i = (t + 256 * c) * V;
+    const int i = (t + TPR * c) * V;
     if (i >= g.n) continue;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      pw[i + j] = dw[c][j];
-      pb[i + j] = db[c][j];
+    for (int j = 0; j < V; j += 4) {
+      *reinterpret_cast<v4f *>(pw + i + j) = v4f{dw[c][j], dw[c][j + 1], dw[c][j + 2], dw[c][j + 3]};
+      *reinterpret_cast<v4f *>(pb + i + j) = v4f{db[c][j], db[c][j + 1], db[c][j + 2], db[c][j + 3]};
     }
   }
 }
@@ -226,25 +297,26 @@ __global__ __launch_bounds__(256) void k_norm_backward(NormArgs g) {
 // alone touches at columns t, t + 256, ...
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_backward_any(NormArgs g) {
-  __shared__ float red[4];
+  __shared__ float red[2][4][2];
+  int par = 0;
   float *pw = g.part ? g.part + (size_t)blockIdx.x * 2 * g.n : nullptr, *pb = pw + g.n;
   if (pw)
     for (int i = threadIdx.x; i < g.n; i += 256) pw[i] = pb[i] = 0.f;
-  for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
+  for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x, par ^= 1) {
     const T *x = (const T *)g.x + row * g.ldx, *dy = (const T *)g.dy + row * g.ldg;
     const float mean = g.mean[row], rstd = g.rstd[row];
-    float s1 = 0.f, s2 = 0.f;
+    float s[2] = {0.f, 0.f};
     for (int i = threadIdx.x; i < g.n; i += 256) {
       const float h = (to_f32(x[i]) - mean) * rstd, d = to_f32(dy[i]), w = d * (g.weight ? g.weight[i] : 1.0f);
       if (pw) {
         pw[i] += d * h;
         pb[i] += d;
       }
-      s1 += w;
-      s2 += w * h;
+      s[0] += w;
+      s[1] += w * h;
     }
-    s1 = row_sum<256>(s1, red) / (float)g.n;
-    s2 = row_sum<256>(s2, red) / (float)g.n;
+    row_sums<256, 2>(s, red[par]);
+    const float s1 = s[0] / (float)g.n, s2 = s[1] / (float)g.n;
     if (g.y) {
       T *dx = (T *)g.y + row * g.ldy;
       for (int i = threadIdx.x; i < g.n; i += 256) {
@@ -255,19 +327,13 @@ __global__ __launch_bounds__(256) void k_norm_backward_any(NormArgs g) {
   }
 }
 
-// dweight and dbias: the workgroups' sums added in order
-__global__ __launch_bounds__(256) void k_norm_sum(const float *__restrict__ part, int parts, int n,
-                                                  float *__restrict__ dweight, float *__restrict__ dbias) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= 2 * n) return;
-  float v = 0.f;
-  for (int p = 0; p < parts; ++p) v += part[(size_t)p * 2 * n + i];
-  float *dst = i < n ? dweight : dbias;
-  if (dst) dst[i < n ? i : i - n] = v;
+// Workgroups of the backward pass: every one leaves a row of sums behind (8 n bytes written and read again), so not
+// more than two a CU, and as few as go over the rows in as many rounds.
+constexpr int NORM_PARTS = 512;
+int norm_parts(int64_t rows) {
+  const int64_t rounds = (rows + NORM_PARTS - 1) / NORM_PARTS;
+  return (int)((rows + rounds - 1) / rounds);
 }
-
-// rows' worth of workgroups of the backward pass: two per CU
-int norm_parts(int64_t rows) { return (int)std::min<int64_t>(rows, 512); }
 
 bool aligned(const void *p, int64_t ld, size_t e) { return !p || (!((uintptr_t)p & 15) && !((size_t)ld * e & 15)); }
 
@@ -281,27 +347,33 @@ int check(const char *who, int type, int64_t rows, int64_t n) {
 template <class T>
 void norm(const NormArgs &g, bool vec, hipStream_t st) {
   constexpr int V = Pack<T>::V;
-  const unsigned rows = (unsigned)g.rows, quads = (unsigned)((g.rows + 3) / 4);
+  const int64_t quads = (g.rows + 3) / 4;
   const int packs = (g.n + V - 1) / V;
-  const dim3 b(256);
-  if (!vec || packs > 8 * 256) hipLaunchKernelGGL((k_norm_any<T>), dim3(rows), b, 0, st, g);
-  else if (packs <= 64) hipLaunchKernelGGL((k_norm<T, 64, 1>), dim3(quads), b, 0, st, g);
-  else if (packs <= 128) hipLaunchKernelGGL((k_norm<T, 64, 2>), dim3(quads), b, 0, st, g);
-  else if (packs <= 256) hipLaunchKernelGGL((k_norm<T, 256, 1>), dim3(rows), b, 0, st, g);
-  else if (packs <= 512) hipLaunchKernelGGL((k_norm<T, 256, 2>), dim3(rows), b, 0, st, g);
-  else if (packs <= 1024) hipLaunchKernelGGL((k_norm<T, 256, 4>), dim3(rows), b, 0, st, g);
-  else hipLaunchKernelGGL((k_norm<T, 256, 8>), dim3(rows), b, 0, st, g);
+  // as many workgroups as fit the chip at once (`most`), or as few as take as many rounds
+  auto grid = [](int64_t n, int64_t most) {
+    const int64_t rounds = (n + most - 1) / most;
+    return dim3((unsigned)((n + rounds - 1) / rounds));
+  };
+  if (!vec || packs > 4 * 512) hipLaunchKernelGGL((k_norm_any<T>), dim3((unsigned)g.rows), dim3(256), 0, st, g);
+  else if (packs <= 64) hipLaunchKernelGGL((k_norm<T, 256, 64, 1>), grid(quads, 2048), dim3(256), 0, st, g);
+  else if (packs <= 128) hipLaunchKernelGGL((k_norm<T, 256, 64, 2>), grid(quads, 1536), dim3(256), 0, st, g);
+  else if (packs <= 256) hipLaunchKernelGGL((k_norm<T, 256, 256, 1>), grid(g.rows, 2048), dim3(256), 0, st, g);
+  else if (packs <= 512) hipLaunchKernelGGL((k_norm<T, 512, 512, 1>), grid(g.rows, 1024), dim3(512), 0, st, g);
+  else if (packs <= 1024) hipLaunchKernelGGL((k_norm<T, 512, 512, 2>), grid(g.rows, 1024), dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((k_norm<T, 512, 512, 4>), grid(g.rows, 512), dim3(512), 0, st, g);
 }
 
 template <class T>
 void norm_backward(const NormArgs &g, bool vec, unsigned parts, hipStream_t st) {
   constexpr int V = Pack<T>::V;
   const int packs = (g.n + V - 1) / V;
-  const dim3 b(256);
-  if (!vec || packs > 4 * 256) hipLaunchKernelGGL((k_norm_backward_any<T>), dim3(parts), b, 0, st, g);
-  else if (packs <= 256) hipLaunchKernelGGL((k_norm_backward<T, 1>), dim3(parts), b, 0, st, g);
-  else if (packs <= 512) hipLaunchKernelGGL((k_norm_backward<T, 2>), dim3(parts), b, 0, st, g);
-  else hipLaunchKernelGGL((k_norm_backward<T, 4>), dim3(parts), b, 0, st, g);
+  if (!vec || packs > 4 * 512) hipLaunchKernelGGL((k_norm_backward_any<T>), dim3(parts), dim3(256), 0, st, g);
+  else if (packs <= 64) hipLaunchKernelGGL((k_norm_backward<T, 512, 64, 1>), dim3(parts), dim3(512), 0, st, g);
+  else if (packs <= 128) hipLaunchKernelGGL((k_norm_backward<T, 512, 128, 1>), dim3(parts), dim3(512), 0, st, g);
+  else if (packs <= 256) hipLaunchKernelGGL((k_norm_backward<T, 512, 256, 1>), dim3(parts), dim3(512), 0, st, g);
+  else if (packs <= 512) hipLaunchKernelGGL((k_norm_backward<T, 512, 512, 1>), dim3(parts), dim3(512), 0, st, g);
+  else if (packs <= 1024) hipLaunchKernelGGL((k_norm_backward<T, 512, 512, 2>), dim3(parts), dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((k_norm_backward<T, 512, 512, 4>), dim3(parts), dim3(512), 0, st, g);
 }
 
 __global__ __launch_bounds__(256) void k_norm_zero(float *dweight, float *dbias, int n) {
@@ -386,9 +458,7 @@ int zm_layer_norm_backward(int type, const void *dy, int64_t dy_stride, const vo
   if (type == LIN_F32) norm_backward<float>(g, vec, parts, st);
   else if (type == LIN_F16) norm_backward<_Float16>(g, vec, parts, st);
   else norm_backward<bf16>(g, vec, parts, st);
-  if (sums)
-    hipLaunchKernelGGL(k_norm_sum, dim3((unsigned)((2 * n + 255) / 256)), dim3(256), 0, st, (const float *)workspace,
-                       (int)parts, (int)n, dweight, dbias);
+  if (sums) parts_sum((const float *)workspace, (int)parts, 2 * n, n, dweight, dbias, st);
   HIP_OK(hipGetLastError());
   return 0;
 }

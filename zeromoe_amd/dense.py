@@ -6,7 +6,6 @@ allocator for that stream, so a call may be captured into a graph.  Gradients ar
 recorded by autograd."""
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional
 
 import torch
@@ -17,36 +16,43 @@ from .ops import _spec
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _F32, _I32 = torch.float32, torch.int32
+_F32S, _I32S = (_F32,), (_I32,)
+
+
+# the current stream's handle without a Stream object around it: 0.1 us of a call's 7, against 1.1
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
 
 
 def _on(fn):
     """Runs the call where its first tensor lies and on `stream`, whose allocations are then that stream's."""
+    name = fn.__code__.co_varnames[2]
+
     def call(*args, stream=None, **kw):
-        t = args[0]
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        first = args[0] if args else kw.get(name)
+        if not isinstance(first, torch.Tensor) or not first.is_cuda:
             raise ValueError(f"{fn.__name__}: device tensors are needed")
-        d = t.get_device()
-        if stream is not None:
-            if stream.device.index != d:
-                raise ValueError(f"{fn.__name__}: the stream belongs to another device than the tensors")
-            with torch.cuda.stream(stream):
-                return fn(stream.cuda_stream, *args, **kw)
-        if d != torch.cuda.current_device():
+        d = first.get_device()
+        if stream is None:
+            if d == torch.cuda.current_device():
+                return fn(_raw_stream(d), d, *args, **kw)
             with torch.cuda.device(d):
-                return fn(torch.cuda.current_stream(d).cuda_stream, *args, **kw)
-        return fn(torch.cuda.current_stream(d).cuda_stream, *args, **kw)
+                return fn(_raw_stream(d), d, *args, **kw)
+        if stream.device.index != d:
+            raise ValueError(f"{fn.__name__}: the stream belongs to another device than the tensors")
+        with torch.cuda.stream(stream):
+            return fn(stream.cuda_stream, d, *args, **kw)
 
     call.__name__, call.__qualname__, call.__doc__, call.__wrapped__ = fn.__name__, fn.__qualname__, fn.__doc__, fn
     return call
 
 
-def _need(t: torch.Tensor, what: str, like: torch.Tensor, dtypes, shape) -> torch.Tensor:
+def _need(t: torch.Tensor, what: str, d: int, dtypes, shape) -> torch.Tensor:
     """`t` with the device, type and shape that the call needs."""
-    if t.device != like.device:
+    if t.get_device() != d:
         raise ValueError(f"{what} is on another device")
     if t.dtype not in dtypes:
-        raise ValueError(f"{what} is {t.dtype}: {', '.join(str(d) for d in dtypes)} needed")
-    if tuple(t.shape) != shape:
+        raise ValueError(f"{what} is {t.dtype}: {', '.join(str(x) for x in dtypes)} needed")
+    if t.shape != shape:
         raise ValueError(f"{what} has shape {tuple(t.shape)}: {shape} needed")
     return t
 
@@ -56,15 +62,19 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _out(t: torch.Tensor, what: str, like: torch.Tensor, dtype, shape) -> torch.Tensor:
-    _need(t, what, like, (dtype,), shape)
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _out(t: torch.Tensor, what: str, d: int, dtype, shape) -> torch.Tensor:
+    _need(t, what, d, (dtype,), shape)
     if t.stride(-1) != 1 and shape[-1] != 1:
         raise ValueError(f"{what} needs contiguous columns")
     return t
 
 
-def _vector(t: Optional[torch.Tensor], what: str, like: torch.Tensor, n: int):
-    return None if t is None else _need(t, what, like, (_F32,), (n,)).contiguous()
+def _vector(t: Optional[torch.Tensor], what: str, d: int, n: int):
+    return None if t is None else _flat(_need(t, what, d, _F32S, (n,)))
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -72,7 +82,7 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _space(n: int, like: torch.Tensor):
-    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
+    return like.new_empty(n, dtype=torch.uint8) if n else None
 
 
 def _act(act) -> int:
@@ -81,11 +91,11 @@ def _act(act) -> int:
     return ACTIVATIONS[act]
 
 
-def _linear_types(x, w):
+def _linear_types(d, x, w):
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"x (S, I) and w (O, I) are needed, not {tuple(x.shape)} and {tuple(w.shape)}")
-    if w.device != x.device:
-        raise ValueError("w is on another device")
+    if x.get_device() != d or w.get_device() != d:
+        raise ValueError("x or w is on another device")
     if x.dtype not in _TYPES or w.dtype not in _TYPES or (x.dtype != _F32 and w.dtype != x.dtype):
         raise ValueError(f"x {x.dtype} with w {w.dtype}: float32 activations with float32, float16 or bfloat16 weights, "
                          "or both of one 16-bit type")
@@ -94,104 +104,105 @@ def _linear_types(x, w):
 
 
 @_on
-def linear(st, x: torch.Tensor, w: torch.Tensor, bias=None, act: str = "none", residual=None, out=None, out_dtype=None,
+def linear(st, d, x: torch.Tensor, w: torch.Tensor, bias=None, act: str = "none", residual=None, out=None, out_dtype=None,
            save_pre: bool = False):
     """act(x w^T + bias) + residual: x (S, I), w (O, I), bias (O) float32, residual (S, O) of the result's type.
 
     x float32 with w float32, float16 or bfloat16, or both float16 or both bfloat16; the result is of x's type or
     float32 (`out_dtype`, or `out`'s type).  act: none, relu, gelu, gelu_tanh, silu, sigmoid.  `out` may be `residual`
-    itself.  save_pre: also returns x w^T + bias, in the result's type, for linear_backward.  (zm_linear)"""
-    _linear_types(x, w)
+    itself, and overlaps no other operand.  save_pre: also returns x w^T + bias, in the result's type, for linear_backward.  (zm_linear)"""
+    _linear_types(d, x, w)
     S, I = x.shape
     O = w.shape[0]
     x = _rows(x)
     dtype = out_dtype or (out.dtype if out is not None else x.dtype)
     if dtype != _F32 and dtype != x.dtype:
         raise ValueError(f"the result is float32 or {x.dtype}, not {dtype}")
-    y = torch.empty((S, O), dtype=dtype, device=x.device) if out is None else _out(out, "out", x, dtype, (S, O))
+    y = x.new_empty((S, O), dtype=dtype) if out is None else _out(out, "out", d, dtype, (S, O))
     if residual is not None:
-        residual = _rows(_need(residual, "residual", x, (dtype,), (S, O)))
-    bias = _vector(bias, "bias", x, O)
-    pre = torch.empty((S, O), dtype=dtype, device=x.device) if save_pre else None
-    d = ZmLinearDesc(_TYPES[x.dtype], _TYPES[w.dtype], _TYPES[dtype], _act(act), S, I, O, x.stride(0), w.stride(0),
-                     y.stride(0), residual.stride(0) if residual is not None else 0, O)
+        residual = _rows(_need(residual, "residual", d, (dtype,), (S, O)))
+    bias = _vector(bias, "bias", d, O)
+    pre = x.new_empty((S, O), dtype=dtype) if save_pre else None
+    desc = ZmLinearDesc(_TYPES[x.dtype], _TYPES[w.dtype], _TYPES[dtype], _act(act), S, I, O, x.stride(0), w.stride(0),
+                        y.stride(0), residual.stride(0) if residual is not None else 0, O)
     L = lib()
-    ws = _space(L.zm_linear_workspace_size(d), x)
-    check(L.zm_linear(d, x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(pre), _ptr(ws),
+    ws = _space(L.zm_linear_workspace_size(desc), x)
+    check(L.zm_linear(desc, x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(pre), _ptr(ws),
                       0 if ws is None else ws.numel(), st), "zm_linear")
     return (y, pre) if save_pre else y
 
 
 @_on
-def linear_backward(st, dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str = "none", pre=None,
+def linear_backward(st, d, dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str = "none", pre=None,
                     need_dx: bool = True, need_dw: bool = True, need_dbias: bool = True):
     """(dx, dw, dbias) of linear() for dy (S, O), its gradient by the result: dx (S, I) of x's type, dw (O, I) and
     dbias (O) float32; None in the place of one that is not needed.  The residual's gradient is dy itself.  pre: what
     linear(save_pre=True) returned, needed with an activation.  (zm_linear_backward)"""
-    _linear_types(x, w)
+    _linear_types(d, x, w)
     S, I = x.shape
     O = w.shape[0]
     x = _rows(x)
-    dy = _rows(_need(dy, "dy", x, (_F32, x.dtype), (S, O)))
+    dy = _rows(_need(dy, "dy", d, (_F32, x.dtype), (S, O)))
     a = _act(act)
     if a:
         if pre is None:
             raise ValueError("an activation's gradient needs pre")
-        pre = _rows(_need(pre, "pre", x, (dy.dtype,), (S, O)))
+        pre = _rows(_need(pre, "pre", d, (dy.dtype,), (S, O)))
     else:
         pre = None
-    dev = x.device
-    dx = torch.empty((S, I), dtype=x.dtype, device=dev) if need_dx else None
-    dw = torch.empty((O, I), dtype=_F32, device=dev) if need_dw else None
-    db = torch.empty(O, dtype=_F32, device=dev) if need_dbias else None
-    d = ZmLinearDesc(_TYPES[x.dtype], _TYPES[w.dtype], _TYPES[dy.dtype], a, S, I, O, x.stride(0), w.stride(0),
-                     dy.stride(0), 0, pre.stride(0) if pre is not None else 0)
+    dx = x.new_empty((S, I)) if need_dx else None
+    dw = x.new_empty((O, I), dtype=_F32) if need_dw else None
+    db = x.new_empty(O, dtype=_F32) if need_dbias else None
+    desc = ZmLinearDesc(_TYPES[x.dtype], _TYPES[w.dtype], _TYPES[dy.dtype], a, S, I, O, x.stride(0), w.stride(0),
+                        dy.stride(0), 0, pre.stride(0) if pre is not None else 0)
     L = lib()
-    ws = _space(L.zm_linear_backward_workspace_size(d), x)
-    check(L.zm_linear_backward(d, dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db),
+    ws = _space(L.zm_linear_backward_workspace_size(desc), x)
+    check(L.zm_linear_backward(desc, dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db),
                                _ptr(ws), 0 if ws is None else ws.numel(), st), "zm_linear_backward")
     return dx, dw, db
 
 
-def _norm_rows(x, what="x"):
+def _norm_rows(d, x):
+    if x.get_device() != d:
+        raise ValueError("x is on another device")
     if x.dim() != 2 or x.shape[1] == 0:
-        raise ValueError(f"{what} (rows, n) is needed, not {tuple(x.shape)}")
+        raise ValueError(f"x (rows, n) is needed, not {tuple(x.shape)}")
     if x.dtype not in _TYPES:
-        raise ValueError(f"{what} is {x.dtype}: float32, float16 or bfloat16 needed")
+        raise ValueError(f"x is {x.dtype}: float32, float16 or bfloat16 needed")
 
 
 @_on
-def layer_norm(st, x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=None, stats: bool = False):
+def layer_norm(st, d, x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=None, stats: bool = False):
     """(x - mean) / sqrt(variance + eps) * weight + bias over the rows of x (rows, n), in x's type; weight and bias (n)
     float32.  `out` may be x itself.  stats: also returns each row's mean and 1 / sqrt(variance + eps), for
     layer_norm_backward.  (zm_layer_norm)"""
-    _norm_rows(x)
+    _norm_rows(d, x)
     rows, n = x.shape
     x = _rows(x)
-    y = torch.empty((rows, n), dtype=x.dtype, device=x.device) if out is None else _out(out, "out", x, x.dtype, (rows, n))
-    weight, bias = _vector(weight, "weight", x, n), _vector(bias, "bias", x, n)
+    y = x.new_empty((rows, n)) if out is None else _out(out, "out", d, x.dtype, (rows, n))
+    weight, bias = _vector(weight, "weight", d, n), _vector(bias, "bias", d, n)
     mean = rstd = None
     if stats:
-        mean, rstd = torch.empty((2, rows), dtype=_F32, device=x.device).unbind(0)
+        mean, rstd = x.new_empty((2, rows), dtype=_F32).unbind(0)
     check(lib().zm_layer_norm(_TYPES[x.dtype], x.data_ptr(), x.stride(0), _ptr(weight), _ptr(bias), eps, rows, n,
                               y.data_ptr(), y.stride(0), _ptr(mean), _ptr(rstd), st), "zm_layer_norm")
     return (y, mean, rstd) if stats else y
 
 
 @_on
-def layer_norm_backward(st, dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight=None,
+def layer_norm_backward(st, d, dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight=None,
                         need_dx: bool = True, need_dweight: bool = True, need_dbias: bool = True):
     """(dx, dweight, dbias) of layer_norm() for dy (rows, n) of x's type, with the statistics that it returned: dx of
     x's type, dweight and dbias (n) float32; None in the place of one that is not needed.  (zm_layer_norm_backward)"""
-    _norm_rows(x)
+    _norm_rows(d, x)
     rows, n = x.shape
     x = _rows(x)
-    dy = _rows(_need(dy, "dy", x, (x.dtype,), (rows, n)))
-    mean, rstd = _vector(mean, "mean", x, rows), _vector(rstd, "rstd", x, rows)
-    weight = _vector(weight, "weight", x, n)
-    dx = torch.empty((rows, n), dtype=x.dtype, device=x.device) if need_dx else None
-    dw = torch.empty(n, dtype=_F32, device=x.device) if need_dweight else None
-    db = torch.empty(n, dtype=_F32, device=x.device) if need_dbias else None
+    dy = _rows(_need(dy, "dy", d, (x.dtype,), (rows, n)))
+    mean, rstd = _vector(mean, "mean", d, rows), _vector(rstd, "rstd", d, rows)
+    weight = _vector(weight, "weight", d, n)
+    dx = x.new_empty((rows, n)) if need_dx else None
+    dw = x.new_empty(n, dtype=_F32) if need_dweight else None
+    db = x.new_empty(n, dtype=_F32) if need_dbias else None
     L = lib()
     ws = _space(L.zm_layer_norm_backward_workspace_size(rows, n) if need_dweight or need_dbias else 0, x)
     check(L.zm_layer_norm_backward(_TYPES[x.dtype], dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), _ptr(weight),
@@ -200,27 +211,27 @@ def layer_norm_backward(st, dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
     return dx, dw, db
 
 
-def _routes(y, what="y"):
+def _routes(y):
     if y.dim() != 3 or y.dtype != _F32:
-        raise ValueError(f"{what} (S, K, H) float32 is needed, not {tuple(y.shape)} {y.dtype}")
+        raise ValueError(f"y (S, K, H) float32 is needed, not {tuple(y.shape)} {y.dtype}")
     return _rows(y)
 
 
 @_on
-def combine(st, y: torch.Tensor, weights: torch.Tensor, ids=None, residual=None, out=None):
+def combine(st, d, y: torch.Tensor, weights: torch.Tensor, ids=None, residual=None, out=None):
     """residual + sum over k of weights[:, k] * y[:, k]: the experts' rows y (S, K, H) as mul_mat_id returns them,
     weights (S, K), residual (S, H) and the result, all float32.  A route with a negative id in ids (S, K) int32 takes
     no part.  `out` may be `residual` itself.  (zm_combine)"""
     y = _routes(y)
     S, K, H = y.shape
-    weights = _need(weights, "weights", y, (_F32,), (S, K)).contiguous()
+    weights = _flat(_need(weights, "weights", d, _F32S, (S, K)))
     if ids is not None:
-        ids = _need(ids, "ids", y, (_I32,), (S, K)).contiguous()
+        ids = _flat(_need(ids, "ids", d, _I32S, (S, K)))
     if residual is not None:
-        residual = _need(residual, "residual", y, (_F32,), (S, H)).contiguous()
+        residual = _flat(_need(residual, "residual", d, _F32S, (S, H)))
     if out is None:
-        out = torch.empty((S, H), dtype=_F32, device=y.device)
-    elif not _out(out, "out", y, _F32, (S, H)).is_contiguous():
+        out = y.new_empty((S, H))
+    elif not _out(out, "out", d, _F32, (S, H)).is_contiguous():
         raise ValueError("out needs to be contiguous")
     check(lib().zm_combine(y.data_ptr(), y.stride(0), y.stride(1), weights.data_ptr(), _ptr(ids), _ptr(residual), S, K, H,
                            out.data_ptr(), st), "zm_combine")
@@ -228,28 +239,30 @@ def combine(st, y: torch.Tensor, weights: torch.Tensor, ids=None, residual=None,
 
 
 @_on
-def combine_backward(st, dout: torch.Tensor, y: torch.Tensor, weights=None, ids=None, need_dy: bool = False):
+def combine_backward(st, d, dout: torch.Tensor, y: torch.Tensor, weights=None, ids=None, need_dy: bool = False):
     """dweights (S, K) of combine() for dout (S, H): the dot products of dout with the experts' rows, 0 for a route with
     a negative id.  need_dy: (dweights, dy), dy (S, K, H) = weights * dout, which needs weights.  The residual's
     gradient is dout itself.  (zm_combine_backward)"""
     y = _routes(y)
     S, K, H = y.shape
-    dout = _need(dout, "dout", y, (_F32,), (S, H)).contiguous()
+    if y.get_device() != d:
+        raise ValueError("y is on another device")
+    dout = _flat(_need(dout, "dout", d, _F32S, (S, H)))
     if ids is not None:
-        ids = _need(ids, "ids", y, (_I32,), (S, K)).contiguous()
+        ids = _flat(_need(ids, "ids", d, _I32S, (S, K)))
     if need_dy and weights is None:
         raise ValueError("dy needs weights")
     if weights is not None:
-        weights = _need(weights, "weights", y, (_F32,), (S, K)).contiguous()
-    dweights = torch.empty((S, K), dtype=_F32, device=y.device)
-    dy = torch.empty((S, K, H), dtype=_F32, device=y.device) if need_dy else None
+        weights = _flat(_need(weights, "weights", d, _F32S, (S, K)))
+    dweights = y.new_empty((S, K))
+    dy = y.new_empty((S, K, H)) if need_dy else None
     check(lib().zm_combine_backward(dout.data_ptr(), y.data_ptr(), y.stride(0), y.stride(1), _ptr(weights), _ptr(ids), S,
                                     K, H, dweights.data_ptr(), _ptr(dy), st), "zm_combine_backward")
     return (dweights, dy) if need_dy else dweights
 
 
 @_on
-def router_backward(st, logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Tensor, gating="softmax",
+def router_backward(st, d, logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Tensor, gating="softmax",
                     logit_bias=None, weights_norm: bool = False, weights_scale: float = 0.0, dprobs=None):
     """The gradient of router()'s weights by its logits (S, E) float32, the selection held fixed: ids (S, K) int32 are
     expert ids (router() without a slot table), dweights (S, K).  A negative id takes no part; a row of them alone has
@@ -257,13 +270,13 @@ def router_backward(st, logits: torch.Tensor, ids: torch.Tensor, dweights: torch
     on their mean has it.  The gradient by logit_bias is the result's sum over the tokens.  (zm_router_backward)"""
     if logits.dim() != 2 or logits.dtype != _F32 or ids.dim() != 2:
         raise ValueError("logits (S, E) float32 and ids (S, K) are needed")
-    logits = logits.contiguous()
+    logits = _flat(logits)
     S, E = logits.shape
     K = ids.shape[1]
-    ids = _need(ids, "ids", logits, (_I32,), (S, K)).contiguous()
-    dweights = _need(dweights, "dweights", logits, (_F32,), (S, K)).contiguous()
-    logit_bias, dprobs = _vector(logit_bias, "logit_bias", logits, E), _vector(dprobs, "dprobs", logits, E)
-    out = torch.empty((S, E), dtype=_F32, device=logits.device)
+    ids = _flat(_need(ids, "ids", d, _I32S, (S, K)))
+    dweights = _flat(_need(dweights, "dweights", d, _F32S, (S, K)))
+    logit_bias, dprobs = _vector(logit_bias, "logit_bias", d, E), _vector(dprobs, "dprobs", d, E)
+    out = logits.new_empty((S, E))
     spec = _spec(E, K, gating, 0, 0, weights_norm, weights_scale)
     check(lib().zm_router_backward(spec, logits.data_ptr(), _ptr(logit_bias), ids.data_ptr(), dweights.data_ptr(),
                                    _ptr(dprobs), S, out.data_ptr(), st), "zm_router_backward")
