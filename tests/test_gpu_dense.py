@@ -122,6 +122,19 @@ def test_linear_strides_and_alignment(xt, wt, S):
         Z.linear(x, rand(I, O, seed=7, dtype=TYPES[wt]).t())
 
 
+@pytest.mark.parametrize("xt,wt", PAIRS)
+@pytest.mark.parametrize("S", [1, 4, 5, 40, 150])
+def test_linear_on_odd_addresses(S, xt, wt):
+    """Shapes that allow 16-byte loads on addresses that do not: of x, of w, of the result alone; long rows too."""
+    for I, O in ((264, 72), (4104, 40)):
+        xb, wb = rand(S * (I + 8) + 16, seed=3, dtype=TYPES[xt]), rand(O * (I + 8) + 16, seed=4, scale=0.06, dtype=TYPES[wt])
+        for ox, ow, oy in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (8, 8, 8)):
+            x, w = (b[off:off + n * (I + 8)].view(n, I + 8)[:, :I] for b, off, n in ((xb, ox, S), (wb, ow, O)))
+            yb = torch.full((S, O + 8), 7.0, device="cuda", dtype=TYPES[xt])
+            check_linear(S, I, O, xt, wt, x=x, w=w, out=yb[:, oy:oy + O])
+            assert (yb[:, :oy] == 7.0).all() and (yb[:, oy + O:] == 7.0).all()
+
+
 def test_linear_no_rows_pre_and_in_place():
     import zeromoe_amd as Z
 

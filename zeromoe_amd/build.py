@@ -14,7 +14,7 @@ SRC = os.path.join(PKG_DIR, "csrc")
 OUT = os.path.join(PKG_DIR, "lib", "libzeromoe_hip.so")
 SOURCES = ("zm_api.hip", "zm_dec_a.hip", "zm_dec_b.hip", "zm_mmq_a.hip", "zm_mmq_b.hip", "zm_mmq_c.hip",
            "zm_mmq_d.hip", "zm_exec.hip", "zm_pack.hip", "zm_lane.hip", "zm_linear.hip", "zm_linear_a.hip", "zm_linear_b.hip",
-           "zm_linear_c.hip", "zm_norm.hip", "zm_combine.hip")
+           "zm_linear_c.hip", "zm_linear_d.hip", "zm_norm.hip", "zm_combine.hip")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 # -ffp-contract=off: the quantizer, router and SwiGLU are bit-reproducible

@@ -93,8 +93,8 @@ struct Plan {
 };
 
 // Tiles of 128 x 128, or 32 x 128 for up to 64 rows; k in as many slices as give about two workgroups per CU
-// (at least four tiles of k each), as long as the partial sums stay below 64 MB.
-Plan plan(int64_t M, int64_t N, int64_t K, bool vec) {
+// (at least four tiles of k each), as long as the partial sums stay below `most` bytes.
+Plan plan(int64_t M, int64_t N, int64_t K, bool vec, size_t most = 64 << 20) {
   Plan p{};
   p.tile = !vec || M <= 64;
   const int bm = p.tile ? 32 : 128;
@@ -102,7 +102,7 @@ Plan plan(int64_t M, int64_t N, int64_t K, bool vec) {
   p.tiles_n = (int)((N + 127) / 128);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   int64_t z = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), K / 256));
-  z = std::min(z, std::max<int64_t>(1, (int64_t)(64 << 20) / (M * N * 4)));
+  z = std::min(z, std::max<int64_t>(1, (int64_t)(most / ((size_t)M * N * 4))));
   p.kslice = ((K + z - 1) / z + 63) / 64 * 64;
   p.slices = (int)((K + p.kslice - 1) / p.kslice);
   p.part = p.slices > 1 ? (size_t)p.slices * M * N * 4 : 0;
@@ -113,11 +113,35 @@ size_t size_of(int type) { return type == LIN_F32 ? 4 : 2; }
 bool lin_type(int t) { return t == LIN_F32 || t == LIN_F16 || t == LIN_BF16; }
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// whether an operand can be read 16 bytes at a time: `row` values contiguous in memory, taken 8 at a time where they
-// are k (kc), else in 16 bytes
-bool vec16(const void *p, int64_t ld, int64_t row, int type, bool kc) {
+// Whether an operand can be read 16 bytes at a time: `row` values contiguous in memory, taken 8 at a time where they
+// are k (kc), else in 16 bytes.  By its shape, and by where it lies.
+bool vec_shape(int64_t ld, int64_t row, int type, bool kc) {
   const size_t e = size_of(type);
-  return !((uintptr_t)p & 15) && !((size_t)ld * e & 15) && !(kc ? row & 7 : (int64_t)((size_t)row * e & 15));
+  return !((size_t)ld * e & 15) && !(kc ? row & 7 : (int64_t)((size_t)row * e & 15));
+}
+bool vec_at(const void *p) { return !((uintptr_t)p & 15); }
+
+// One of a call's products: its shape decides the workspace; where the pointers then forbid 16-byte loads the plan has
+// to do with that.
+struct Product {
+  int64_t M, N, K;
+  bool shaped;
+  size_t space() const { return rows() ? 0 : plan(M, N, K, shaped).part; }
+  bool rows() const { return shaped && few && M <= LIN_ROWS && N < (1 << 26) && K < (1 << 30); }  // 32-bit columns, 2^32 threads
+  bool few;  // the product has the kernel for few rows
+};
+Product forward(const zm_linear_desc &d) {
+  return {d.S, d.O, d.I, vec_shape(d.x_stride, d.I, d.x_type, true) && vec_shape(d.w_stride, d.I, d.w_type, true), true};
+}
+int64_t dz_stride(int64_t O);
+// what dz is: dy itself, or f32 of the workspace behind an activation
+int dz_type(const zm_linear_desc &d) { return d.act ? (int)LIN_F32 : d.y_type; }
+int64_t dz_ld(const zm_linear_desc &d) { return d.act ? dz_stride(d.O) : d.y_stride; }
+Product by_x(const zm_linear_desc &d) {
+  return {d.S, d.I, d.O, vec_shape(dz_ld(d), d.O, dz_type(d), true) && vec_shape(d.w_stride, d.I, d.w_type, false), false};
+}
+Product by_w(const zm_linear_desc &d) {
+  return {d.O, d.I, d.S, vec_shape(dz_ld(d), d.O, dz_type(d), false) && vec_shape(d.x_stride, d.I, d.x_type, false), false};
 }
 
 int64_t dz_stride(int64_t O) { return (O + 3) / 4 * 4; }
@@ -125,7 +149,6 @@ int64_t dz_stride(int64_t O) { return (O + 3) / 4 * 4; }
 int64_t dz_chunks(int64_t S) { return std::min<int64_t>((S + 31) / 32, 256); }
 
 // Workspace of the backward pass: dz in f32 (behind an activation) | bias partials | the larger product's partials.
-// It is sized for either choice of vector loads, so that it depends on the description alone.
 struct BackwardSpace {
   size_t dz, bias, part, total;
 };
@@ -133,10 +156,7 @@ BackwardSpace backward_space(const zm_linear_desc &d) {
   BackwardSpace w{};
   w.dz = d.act ? align256((size_t)d.S * dz_stride(d.O) * 4) : 0;
   w.bias = align256((size_t)dz_chunks(d.S) * d.O * 4);
-  for (int vec = 0; vec < 2; ++vec) {
-    w.part = std::max(w.part, align256(plan(d.S, d.I, d.O, vec).part));
-    w.part = std::max(w.part, align256(plan(d.O, d.I, d.S, vec).part));
-  }
+  w.part = align256(std::max(by_x(d).space(), by_w(d).space()));
   w.total = w.dz + w.bias + w.part;
   return w;
 }
@@ -172,16 +192,17 @@ int launched() {
   return 0;
 }
 
-LinArgs product(const void *a, int64_t lda, const void *b, int64_t ldb, int64_t M, int64_t N, int64_t K, const Plan &p,
-                float *part) {
+Plan plan_of(const Product &q, bool vec) { return plan(q.M, q.N, q.K, vec, vec == q.shaped ? 64 << 20 : q.space()); }
+
+LinArgs product(const Product &q, const void *a, int64_t lda, const void *b, int64_t ldb, const Plan &p, float *part) {
   LinArgs g{};
   g.a = a;
   g.b = b;
   g.lda = lda;
   g.ldb = ldb;
-  g.M = M;
-  g.N = N;
-  g.K = K;
+  g.M = q.M;
+  g.N = q.N;
+  g.K = q.K;
   g.tiles_m = p.tiles_m;
   g.tiles_n = p.tiles_n;
   g.slices = p.slices;
@@ -208,7 +229,7 @@ extern "C" {
 
 size_t zm_linear_workspace_size(const zm_linear_desc *d) {
   if (check_desc(d, "zm_linear_workspace_size") || !d->S) return 0;
-  return std::max(align256(plan(d->S, d->O, d->I, false).part), align256(plan(d->S, d->O, d->I, true).part));
+  return align256(forward(*d).space());
 }
 
 int zm_linear(const zm_linear_desc *d, const void *x, const void *w, const float *bias, const void *residual, void *y,
@@ -218,11 +239,13 @@ int zm_linear(const zm_linear_desc *d, const void *x, const void *w, const float
   if (pre && check_rows(d->S, d->pre_stride, d->O, "zm_linear", "pre")) return -1;
   if (!d->S) return 0;
   if (!x || !w || !y) return fail("zm_linear: null pointer");
-  const bool vec = vec16(x, d->x_stride, d->I, d->x_type, true) && vec16(w, d->w_stride, d->I, d->w_type, true);
-  const Plan p = plan(d->S, d->O, d->I, vec);
-  if (p.part && (!workspace || workspace_size < p.part || ((uintptr_t)workspace & 255)))
+  const Product q = forward(*d);
+  const bool vec = q.shaped && vec_at(x) && vec_at(w);
+  const Plan p = plan_of(q, vec);
+  const bool rows = vec && q.rows();
+  if (!rows && p.part && (!workspace || workspace_size < p.part || ((uintptr_t)workspace & 255)))
     return fail("zm_linear: a 256-byte aligned workspace of zm_linear_workspace_size() bytes is needed");
-  LinArgs g = product(x, d->x_stride, w, d->w_stride, d->S, d->O, d->I, p, (float *)workspace);
+  LinArgs g = product(q, x, d->x_stride, w, d->w_stride, p, (float *)workspace);
   g.e.y = y;
   g.e.res = residual;
   g.e.pre = pre;
@@ -234,6 +257,10 @@ int zm_linear(const zm_linear_desc *d, const void *x, const void *w, const float
   g.e.act = d->act;
   g.e.vec = vec4(y, d->y_stride, d->y_type) && vec4(residual, d->res_stride, d->y_type) &&
             vec4(pre, d->pre_stride, d->y_type) && vec4(bias, 0, LIN_F32);
+  if (rows) {
+    lin_rows(d->x_type, d->w_type, g, (hipStream_t)stream);
+    return launched();
+  }
   lin_fwd(d->x_type, d->w_type, g, vec, p.tile, (hipStream_t)stream);
   return join(g, (hipStream_t)stream);
 }
@@ -284,13 +311,13 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
     else hipLaunchKernelGGL((k_linear_dz<1>), grid, dim3(256), 0, st, a);
     if (dbias) parts_sum(bias_part, (int)n, d->O, d->O, dbias, nullptr, st);
   }
-  const void *g_z = d->act ? (const void *)dz : dy;
-  const int64_t ldz = d->act ? dz_stride(d->O) : d->y_stride;
-  const int z_type = d->act ? (int)LIN_F32 : d->y_type;
-  if (dx) {  // M = S, N = I, K = O
-    const bool vec = vec16(g_z, ldz, d->O, z_type, true) && vec16(w, d->w_stride, d->I, d->w_type, false);
-    const Plan p = plan(d->S, d->I, d->O, vec);
-    LinArgs g = product(g_z, ldz, w, d->w_stride, d->S, d->I, d->O, p, part);
+  const void *z = d->act ? (const void *)dz : dy;
+  const int z_type = dz_type(*d);
+  if (dx) {
+    const Product q = by_x(*d);
+    const bool vec = q.shaped && vec_at(z) && vec_at(w);
+    const Plan p = plan_of(q, vec);
+    LinArgs g = product(q, z, dz_ld(*d), w, d->w_stride, p, part);
     g.e.y = dx;
     g.e.ldy = d->I;
     g.e.type = d->x_type;
@@ -298,10 +325,11 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
     lin_dx(d->x_type, d->w_type, z_type, g, vec, p.tile, st);
     if (join(g, st)) return -1;
   }
-  if (dw) {  // M = O, N = I, K = S
-    const bool vec = vec16(g_z, ldz, d->O, z_type, false) && vec16(x, d->x_stride, d->I, d->x_type, false);
-    const Plan p = plan(d->O, d->I, d->S, vec);
-    LinArgs g = product(g_z, ldz, x, d->x_stride, d->O, d->I, d->S, p, part);
+  if (dw) {
+    const Product q = by_w(*d);
+    const bool vec = q.shaped && vec_at(z) && vec_at(x);
+    const Plan p = plan_of(q, vec);
+    LinArgs g = product(q, z, dz_ld(*d), x, d->x_stride, p, part);
     g.e.y = dw;
     g.e.ldy = d->I;
     g.e.type = LIN_F32;

@@ -552,6 +552,80 @@ static __global__ __launch_bounds__(256) void k_linear_join(LinArgs g) {
   lin_finish4(g.e, m, n, g.N, v);
 }
 
+// ============================================================ few rows
+//
+// Up to four rows of x: bound by reading w once.  WPR waves share a row of w (one wave a row, or four where there are
+// few rows); a lane multiplies 16 bytes of it at a time by the same columns of each row of x, in f32, eight such loads
+// in flight before the first product.  x comes from L2 (it is short).
+constexpr int LIN_ROWS = 4;
+template <class TX, class TW, int S, int WPR>
+__global__ __launch_bounds__(256) void k_linear_rows(LinArgs g) {
+  constexpr int V = 16 / (int)sizeof(TW), U = 8;
+  __shared__ float red[4][S];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t o = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  if (WPR == 1 && o >= g.N) return;
+  const TW *w = (const TW *)g.b + o * g.ldb;
+  const TX *x = (const TX *)g.a;
+  float acc[S] = {};
+  const int K = (int)g.K, first = ((WPR == 1 ? 0 : wave * 64) + lane) * V, step = 64 * WPR * V;
+  for (int k0 = first; k0 < K; k0 += U * step) {
+    v4u rw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * step;
+      rw[u] = k < K ? __builtin_nontemporal_load(reinterpret_cast<const v4u *>(w + k)) : v4u{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * step;
+      if (k >= K) break;
+      TW e[V];
+      __builtin_memcpy(e, &rw[u], 16);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        TX f[V];
+        __builtin_memcpy(f, x + s * g.lda + k, sizeof(f));
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[s] = __builtin_fmaf(to_f32(e[j]), to_f32(f[j]), acc[s]);
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int q = 32; q; q >>= 1) acc[s] += __shfl_xor(acc[s], q);
+  if (WPR > 1) {
+    if (!lane)
+#pragma unroll
+      for (int s = 0; s < S; ++s) red[wave][s] = acc[s];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int s = 0; s < S; ++s) acc[s] = (red[0][s] + red[1][s]) + (red[2][s] + red[3][s]);
+  }
+  float z = acc[0];
+#pragma unroll
+  for (int s = 1; s < S; ++s) z = lane == s ? acc[s] : z;
+  if (lane < S) lin_store(g.e.y, g.e.type, (size_t)(lane * g.e.ldy + o), lin_finish1(g.e, lane, o, z));
+}
+
+template <class TX, class TW, int S>
+void lin_rows_launch(const LinArgs &g, hipStream_t st) {
+  // one wave a row from 2048 rows on, else four
+  if (g.N >= 2048) hipLaunchKernelGGL((k_linear_rows<TX, TW, S, 1>), dim3((unsigned)((g.N + 3) / 4)), dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((k_linear_rows<TX, TW, S, 4>), dim3((unsigned)g.N), dim3(256), 0, st, g);
+}
+template <class TX, class TW>
+void lin_rows_of(const LinArgs &g, hipStream_t st) {
+  switch (g.M) {
+  case 1: lin_rows_launch<TX, TW, 1>(g, st); break;
+  case 2: lin_rows_launch<TX, TW, 2>(g, st); break;
+  case 3: lin_rows_launch<TX, TW, 3>(g, st); break;
+  default: lin_rows_launch<TX, TW, 4>(g, st); break;
+  }
+}
+
 // The launch of one kernel instance.  `tile` 0 = 128 x 128, 1 = 32 x 128; operands without 16-byte loads (`vec`
 // false) take 32 x 128.
 template <class TA, int NA, bool KCA, class TB, int NB, bool KCB>
@@ -563,6 +637,7 @@ void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
 }
 
 // the products by what their operands are: forward (x, w), dx (dz, w), dw (dz, x)
+void lin_rows(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // M <= LIN_ROWS, operands with 16-byte loads
 void lin_fwd(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dx(int x_type, int w_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dw(int x_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
