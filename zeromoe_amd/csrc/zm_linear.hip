@@ -87,23 +87,37 @@ __global__ __launch_bounds__(256) void k_linear_zero(float *__restrict__ dst, in
 // ============================================================ choices
 
 struct Plan {
-  int tile, tiles_m, tiles_n, slices;
+  int kind, tile, tiles_m, tiles_n, slices;
   int64_t kslice;
   size_t part;  // bytes of the slices' partial results
 };
 
-// Tiles of 128 x 128, or 32 x 128 for up to 64 rows; k in as many slices as give about two workgroups per CU
-// (at least four tiles of k each), as long as the partial sums stay below `most` bytes.
-Plan plan(int64_t M, int64_t N, int64_t K, bool vec, size_t most = 64 << 20) {
+// the kernels of a product, by its rows and by whether its operands can be read 16 bytes at a time
+enum Kind { ROWS, FEW, TILES };
+
+Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, bool vec, size_t most) {
   Plan p{};
-  p.tile = !vec || M <= 64;
-  const int bm = p.tile ? 32 : 128;
-  p.tiles_m = (int)((M + bm - 1) / bm);
-  p.tiles_n = (int)((N + 127) / 128);
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  int64_t z = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), K / 256));
-  z = std::min(z, std::max<int64_t>(1, (int64_t)(most / ((size_t)M * N * 4))));
-  p.kslice = ((K + z - 1) / z + 63) / 64 * 64;
+  p.kind = kind;
+  int64_t z = 1, bk = 64;
+  if (kind == FEW) {
+    // 256 columns a workgroup where w is wide, else 128; slices of k until there are two workgroups per CU, at least
+    // one unit (256 of k) each
+    p.tile = N >= 4096;
+    p.tiles_m = (int)((M + FEW_ROWS - 1) / FEW_ROWS);
+    p.tiles_n = (int)(p.tile ? (N + 255) / 256 : (N + 127) / 128);
+    bk = 256;
+    z = std::min<int64_t>(512 / ((int64_t)p.tiles_m * p.tiles_n), (K + 255) / 256);
+  } else if (kind == TILES) {
+    // 128 x 128, or 32 x 128 for up to 64 rows; k in as many slices as give about two workgroups per CU (at least four
+    // tiles of k each)
+    p.tile = !vec || M <= 64;
+    const int bm = p.tile ? 32 : 128;
+    p.tiles_m = (int)((M + bm - 1) / bm);
+    p.tiles_n = (int)((N + 127) / 128);
+    z = std::min<int64_t>(512 / std::max<int64_t>((int64_t)p.tiles_m * p.tiles_n, 1), K / 256);
+  }
+  z = std::max<int64_t>(1, std::min<int64_t>(z, (int64_t)(most / ((size_t)M * N * 4))));
+  p.kslice = ((K + z - 1) / z + bk - 1) / bk * bk;
   p.slices = (int)((K + p.kslice - 1) / p.kslice);
   p.part = p.slices > 1 ? (size_t)p.slices * M * N * 4 : 0;
   return p;
@@ -125,10 +139,15 @@ bool vec_at(const void *p) { return !((uintptr_t)p & 15); }
 // to do with that.
 struct Product {
   int64_t M, N, K;
-  bool shaped;
-  size_t space() const { return rows() ? 0 : plan(M, N, K, shaped).part; }
-  bool rows() const { return shaped && few && M <= LIN_ROWS && N < (1 << 26) && K < (1 << 30); }  // 32-bit columns, 2^32 threads
-  bool few;  // the product has the kernel for few rows
+  bool shaped;   // strides and widths allow 16-byte loads
+  bool forward;  // the product has kernels for few rows
+  Kind kind(bool vec) const {
+    if (!vec || !forward || N >= (1 << 26) || K >= (1 << 30)) return TILES;
+    return M <= LIN_ROWS ? ROWS : M <= LIN_FEW ? FEW : TILES;
+  }
+  // partial sums of at most 64 MB
+  size_t space() const { return plan(kind(shaped), M, N, K, shaped, 64 << 20).part; }
+  Plan planned(bool vec) const { return plan(kind(vec), M, N, K, vec, vec == shaped ? 64 << 20 : space()); }
 };
 Product forward(const zm_linear_desc &d) {
   return {d.S, d.O, d.I, vec_shape(d.x_stride, d.I, d.x_type, true) && vec_shape(d.w_stride, d.I, d.w_type, true), true};
@@ -192,8 +211,6 @@ int launched() {
   return 0;
 }
 
-Plan plan_of(const Product &q, bool vec) { return plan(q.M, q.N, q.K, vec, vec == q.shaped ? 64 << 20 : q.space()); }
-
 LinArgs product(const Product &q, const void *a, int64_t lda, const void *b, int64_t ldb, const Plan &p, float *part) {
   LinArgs g{};
   g.a = a;
@@ -212,10 +229,7 @@ LinArgs product(const Product &q, const void *a, int64_t lda, const void *b, int
 }
 
 int join(const LinArgs &g, hipStream_t st) {
-  if (g.slices > 1) {
-    const int64_t n = g.M * ((g.N + 3) / 4);
-    hipLaunchKernelGGL(k_linear_join, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g);
-  }
+  if (g.slices > 1) lin_join(g, st);
   return launched();
 }
 
@@ -241,9 +255,8 @@ int zm_linear(const zm_linear_desc *d, const void *x, const void *w, const float
   if (!x || !w || !y) return fail("zm_linear: null pointer");
   const Product q = forward(*d);
   const bool vec = q.shaped && vec_at(x) && vec_at(w);
-  const Plan p = plan_of(q, vec);
-  const bool rows = vec && q.rows();
-  if (!rows && p.part && (!workspace || workspace_size < p.part || ((uintptr_t)workspace & 255)))
+  const Plan p = q.planned(vec);
+  if (p.part && (!workspace || workspace_size < p.part || ((uintptr_t)workspace & 255)))
     return fail("zm_linear: a 256-byte aligned workspace of zm_linear_workspace_size() bytes is needed");
   LinArgs g = product(q, x, d->x_stride, w, d->w_stride, p, (float *)workspace);
   g.e.y = y;
@@ -257,11 +270,9 @@ int zm_linear(const zm_linear_desc *d, const void *x, const void *w, const float
   g.e.act = d->act;
   g.e.vec = vec4(y, d->y_stride, d->y_type) && vec4(residual, d->res_stride, d->y_type) &&
             vec4(pre, d->pre_stride, d->y_type) && vec4(bias, 0, LIN_F32);
-  if (rows) {
-    lin_rows(d->x_type, d->w_type, g, (hipStream_t)stream);
-    return launched();
-  }
-  lin_fwd(d->x_type, d->w_type, g, vec, p.tile, (hipStream_t)stream);
+  if (p.kind == ROWS) lin_rows(d->x_type, d->w_type, g, (hipStream_t)stream);
+  else if (p.kind == FEW) lin_few(d->x_type, d->w_type, g, p.tile, (hipStream_t)stream);
+  else lin_fwd(d->x_type, d->w_type, g, vec, p.tile, (hipStream_t)stream);
   return join(g, (hipStream_t)stream);
 }
 
@@ -316,7 +327,7 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
   if (dx) {
     const Product q = by_x(*d);
     const bool vec = q.shaped && vec_at(z) && vec_at(w);
-    const Plan p = plan_of(q, vec);
+    const Plan p = q.planned(vec);
     LinArgs g = product(q, z, dz_ld(*d), w, d->w_stride, p, part);
     g.e.y = dx;
     g.e.ldy = d->I;
@@ -328,7 +339,7 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
   if (dw) {
     const Product q = by_w(*d);
     const bool vec = q.shaped && vec_at(z) && vec_at(x);
-    const Plan p = plan_of(q, vec);
+    const Plan p = q.planned(vec);
     LinArgs g = product(q, z, dz_ld(*d), x, d->x_stride, p, part);
     g.e.y = dw;
     g.e.ldy = d->I;

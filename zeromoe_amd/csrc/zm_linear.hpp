@@ -423,6 +423,20 @@ __device__ __forceinline__ void lin_finish4(const LinEpilogue &e, int64_t m, int
     if (n + j < N) lin_store(e.y, e.type, (size_t)(m * e.ldy + n + j), lin_finish1(e, m, n + j, z[j]));
 }
 
+// four sums of slice z: into its plane, or finished where there is one slice
+__device__ __forceinline__ void lin_result(const LinArgs &g, int z, int64_t m, int64_t n, v4f v) {
+  if (m >= g.M || n >= g.N) return;
+  if (g.slices == 1) return lin_finish4(g.e, m, n, g.N, v);
+  float *p = g.part + ((size_t)z * g.M + m) * g.N + n;
+  if (!(g.N & 3)) {
+    *reinterpret_cast<v4f *>(p) = v;
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (n + q < g.N) p[q] = v[q];
+  }
+}
+
 // Workgroup -> tile.  Workgroups go to the 8 XCDs in turn; each XCD takes a run
 // of neighbouring tiles instead, so that the operands they share meet in its L2.
 __device__ __forceinline__ int xcd_order(int b, int n) {
@@ -517,39 +531,57 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int64_t m = m0 + wm + 16 * i + fr, n = n0 + wn + 16 * j + 4 * fc;
-      if (m >= g.M || n >= g.N) continue;
-      if (g.slices > 1) {
-        float *p = g.part + ((size_t)z * g.M + m) * g.N + n;
-        if (!(g.N & 3)) *reinterpret_cast<v4f *>(p) = acc[i][j];
-        else
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (n + q < g.N) p[q] = acc[i][j][q];
-      } else {
-        lin_finish4(g.e, m, n, g.N, acc[i][j]);
-      }
-    }
+    for (int j = 0; j < FN; ++j) lin_result(g, z, m0 + wm + 16 * i + fr, n0 + wn + 16 * j + 4 * fc, acc[i][j]);
 }
 
-// Results of the k slices added in order (the same bits on every call), then the epilogue.
+// Results of the k slices added in order (the same bits on every call), then the epilogue.  G threads share four
+// results where there are many slices: each adds every G-th, four loads in flight, and their sums meet in LDS.
+template <int G>
 static __global__ __launch_bounds__(256) void k_linear_join(LinArgs g) {
-  const int64_t nq = (g.N + 3) / 4, q = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (q >= g.M * nq) return;
+  constexpr int Q = 256 / G;  // quads of results of a workgroup
+  __shared__ v4f red[G][Q];
+  const int64_t nq = (g.N + 3) / 4, q = (int64_t)blockIdx.x * Q + threadIdx.x % Q;
+  const int first = threadIdx.x / Q;
+  const bool in = q < g.M * nq;
   const int64_t m = q / nq, n = (q - m * nq) * 4;
   v4f v = {0.f, 0.f, 0.f, 0.f};
   const size_t plane = (size_t)g.M * g.N;
   const float *p = g.part + (size_t)m * g.N + n;
-  if (!(g.N & 3)) {
-    for (int z = 0; z < g.slices; ++z) v += *reinterpret_cast<const v4f *>(p + z * plane);
-  } else {
-    for (int z = 0; z < g.slices; ++z)
+  if (in) {
+    for (int z0 = first; z0 < g.slices; z0 += 4 * G) {
+      v4f t[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < g.N) v[j] += p[z * plane + j];
+      for (int u = 0; u < 4; ++u) {
+        const int z = z0 + u * G;
+        t[u] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (z < g.slices) {
+          if (!(g.N & 3)) {
+            t[u] = *reinterpret_cast<const v4f *>(p + z * plane);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (n + j < g.N) t[u][j] = p[z * plane + j];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v += t[u];
+    }
   }
-  lin_finish4(g.e, m, n, g.N, v);
+  if (G > 1) {
+    red[first][threadIdx.x % Q] = v;
+    __syncthreads();
+    if (first) return;
+#pragma unroll
+    for (int k = 1; k < G; ++k) v += red[k][threadIdx.x];
+  }
+  if (in) lin_finish4(g.e, m, n, g.N, v);
+}
+static inline void lin_join(const LinArgs &g, hipStream_t st) {
+  const int64_t quads = g.M * ((g.N + 3) / 4);
+  if (g.slices > 8 && quads < (1 << 26))
+    hipLaunchKernelGGL((k_linear_join<16>), dim3((unsigned)((quads + 15) / 16)), dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((k_linear_join<1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, g);
 }
 
 // ============================================================ few rows
@@ -626,6 +658,118 @@ void lin_rows_of(const LinArgs &g, hipStream_t st) {
   }
 }
 
+// A few dozen rows of x: bound by reading w once, multiplied on the matrix cores.  A workgroup takes 128 NF columns of
+// the result, 16 MT rows and a slice of k in units of KS: each of its 8 waves asks for all of a unit's w at once,
+// straight from global memory into the instruction's operands (a lane's 16 or 32 bytes of its row of w: no other wave
+// needs them); while those are on their way x's part goes into LDS as terms, once for all waves.  So a unit costs one
+// trip to memory.
+template <class T>
+struct Eight {  // 8 consecutive values as they lie in memory
+  v4u r[sizeof(T) / 2];
+};
+template <class T>
+__device__ __forceinline__ Eight<T> load8(const T *p, bool in) {
+  Eight<T> e;
+#pragma unroll
+  for (int q = 0; q < (int)sizeof(T) / 2; ++q) e.r[q] = in ? reinterpret_cast<const v4u *>(p)[q] : v4u{0, 0, 0, 0};
+  return e;
+}
+template <class T, int NT>
+__device__ __forceinline__ void terms_of(const Eight<T> &e, v8bf (&t)[NT]) {
+  if constexpr (sizeof(T) == 2 && NT == 1) {
+    t[0] = __builtin_bit_cast(v8bf, e.r[0]);
+  } else {
+    T f[8];
+    float v[8];
+    __builtin_memcpy(f, &e, sizeof(f));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f32(f[j]);
+    split_terms<NT>(v, t);
+  }
+}
+
+constexpr int LIN_FEW = 128, FEW_ROWS = 64;
+template <class TX, int NX, class TW, int NW, int MT, int NF>
+__global__ __launch_bounds__(512) void k_linear_few(LinArgs g) {
+  constexpr bool F16 = std::is_same<TX, _Float16>::value && NX == 1;
+  constexpr int KS = sizeof(TW) == 2 ? 256 : 128, CH = KS / 8, ROWS = 16 * MT;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[NX * ROWS * KS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int fr = lane & 15, fc = lane >> 4;
+  const int per = g.tiles_m * g.tiles_n;
+  const int z = blockIdx.x / per, tile = blockIdx.x - z * per;
+  const int64_t m0 = (int64_t)(tile % g.tiles_m) * ROWS, n0 = (int64_t)(tile / g.tiles_m) * 128 * NF + wave * 16 * NF;
+  const int64_t kb = z * g.kslice, ke = min(g.K, kb + g.kslice);
+  const int rows = (int)min(g.M - m0, (int64_t)ROWS);
+  const TW *w[NF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) w[j] = (const TW *)g.b + min(n0 + 16 * j + fr, g.N - 1) * g.ldb + 8 * fc;
+  const TX *x = (const TX *)g.a + m0 * g.lda;
+  v4f acc[MT][NF];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int64_t k = kb; k < ke; k += KS) {
+    Eight<TW> rw[KS / 32][NF];
+#pragma unroll
+    for (int h = 0; h < KS / 32; ++h)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) rw[h][j] = load8(w[j] + k + 32 * h, k + 32 * h + 8 * fc < ke);
+    if (k > kb) __syncthreads();  // x's last part has been used
+    for (int u = threadIdx.x; u < rows * CH; u += 512) {
+      const int r = u / CH, c = u % CH;
+      v8bf t[NX];
+      terms_of<TX, NX>(load8(x + r * g.lda + k + 8 * c, k + 8 * c < ke), t);
+#pragma unroll
+      for (int a = 0; a < NX; ++a) *reinterpret_cast<v8bf *>(lds + (a * ROWS + r) * KS + (c ^ (r & 7)) * 8) = t[a];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < KS / 32; ++h) {
+      v8bf tw[NF][NW];
+#pragma unroll
+      for (int j = 0; j < NF; ++j) terms_of<TW, NW>(rw[h][j], tw[j]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int a = 0; a < NX; ++a) {
+          const int r = 16 * i + fr;
+          const v8bf tx = *reinterpret_cast<const v8bf *>(lds + (a * ROWS + r) * KS + ((4 * h + fc) ^ (r & 7)) * 8);
+#pragma unroll
+          for (int b = 0; b < NW; ++b) {
+            if (a + b > Pairs<NX, NW>::MOST) continue;
+#pragma unroll
+            for (int j = 0; j < NF; ++j) {
+              if constexpr (F16)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, tw[j][b]),
+                                                                  __builtin_bit_cast(v8h, tx), acc[i][j], 0, 0, 0);
+              else
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(tw[j][b], tx, acc[i][j], 0, 0, 0);
+            }
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) lin_result(g, z, m0 + 16 * i + fr, n0 + 16 * j + 4 * fc, acc[i][j]);
+}
+
+template <class TX, int NX, class TW, int NW, int NF>
+void lin_few_launch(const LinArgs &g, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices)), b(512);
+  if (g.M <= 16) hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, 1, NF>), grid, b, 0, st, g);
+  else if (g.M <= 32) hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, 2, NF>), grid, b, 0, st, g);
+  else hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, 4, NF>), grid, b, 0, st, g);
+}
+template <class TX, int NX, class TW, int NW>
+void lin_few_of(const LinArgs &g, int wide, hipStream_t st) {
+  if (wide) lin_few_launch<TX, NX, TW, NW, 2>(g, st);
+  else lin_few_launch<TX, NX, TW, NW, 1>(g, st);
+}
+
 // The launch of one kernel instance.  `tile` 0 = 128 x 128, 1 = 32 x 128; operands without 16-byte loads (`vec`
 // false) take 32 x 128.
 template <class TA, int NA, bool KCA, class TB, int NB, bool KCB>
@@ -638,6 +782,7 @@ void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
 
 // the products by what their operands are: forward (x, w), dx (dz, w), dw (dz, x)
 void lin_rows(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // M <= LIN_ROWS, operands with 16-byte loads
+void lin_few(int x_type, int w_type, const LinArgs &g, int wide, hipStream_t st);  // likewise; 128 or 256 (wide) columns
 void lin_fwd(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dx(int x_type, int w_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dw(int x_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
