@@ -100,13 +100,13 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, bool vec, size_t most) {
   p.kind = kind;
   int64_t z = 1, bk = 64;
   if (kind == FEW) {
-    // 256 columns a workgroup where w is wide, else 128; slices of k until there are two workgroups per CU, at least
-    // one unit (256 of k) each
-    p.tile = N >= 4096;
+    // slices of k until there is a workgroup of 8 waves, or two of 4, per CU
+    const int cols = few_columns(M, N);
     p.tiles_m = (int)((M + FEW_ROWS - 1) / FEW_ROWS);
-    p.tiles_n = (int)(p.tile ? (N + 255) / 256 : (N + 127) / 128);
-    bk = 256;
-    z = std::min<int64_t>(512 / ((int64_t)p.tiles_m * p.tiles_n), (K + 255) / 256);
+    p.tiles_n = (int)((N + cols - 1) / cols);
+    bk = FEW_UNIT;
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, want = cols == 64 ? 512 : 256;
+    z = std::min<int64_t>((want - 1 + tiles) / tiles, (K + bk - 1) / bk);
   } else if (kind == TILES) {
     // 128 x 128, or 32 x 128 for up to 64 rows; k in as many slices as give about two workgroups per CU (at least four
     // tiles of k each)
@@ -131,7 +131,7 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // are k (kc), else in 16 bytes.  By its shape, and by where it lies.
 bool vec_shape(int64_t ld, int64_t row, int type, bool kc) {
   const size_t e = size_of(type);
-  return !((size_t)ld * e & 15) && !(kc ? row & 7 : (int64_t)((size_t)row * e & 15));
+  return !((size_t)ld * e & 15) && ld < BUF_ROW / (int64_t)e && !(kc ? row & 7 : (int64_t)((size_t)row * e & 15));
 }
 bool vec_at(const void *p) { return !((uintptr_t)p & 15); }
 
@@ -271,7 +271,7 @@ int zm_linear(const zm_linear_desc *d, const void *x, const void *w, const float
   g.e.vec = vec4(y, d->y_stride, d->y_type) && vec4(residual, d->res_stride, d->y_type) &&
             vec4(pre, d->pre_stride, d->y_type) && vec4(bias, 0, LIN_F32);
   if (p.kind == ROWS) lin_rows(d->x_type, d->w_type, g, (hipStream_t)stream);
-  else if (p.kind == FEW) lin_few(d->x_type, d->w_type, g, p.tile, (hipStream_t)stream);
+  else if (p.kind == FEW) lin_few(d->x_type, d->w_type, g, (hipStream_t)stream);
   else lin_fwd(d->x_type, d->w_type, g, vec, p.tile, (hipStream_t)stream);
   return join(g, (hipStream_t)stream);
 }

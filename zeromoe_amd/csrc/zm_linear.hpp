@@ -18,6 +18,8 @@
 
 #include <type_traits>
 
+#include "zm_device.hpp"
+
 namespace zm {
 
 struct bf16 {
@@ -123,46 +125,30 @@ __device__ __forceinline__ float lin_act_slope(float z, int act) {
 
 constexpr float BF16_MOST = 3.38953139e38f;  // largest finite bf16
 
-// v[8] as NT bf16 terms.  Values past bf16's largest would round to infinity and
-// leave inf - inf behind: they are cut instead, and an infinity is one term.
-template <int NT>
+// v[8] as NT bf16 terms, without a branch.  T is what the values came from: an f32 past bf16's largest is cut to that
+// for its first term (it would round to infinity and leave inf - inf behind); an infinity ends as a NaN term.
+template <class T, int NT>
 __device__ __forceinline__ void split_terms(const float (&v)[8], v8bf (&t)[NT]) {
-  if constexpr (NT == 1) {
+  float r[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[0][i] = (__bf16)v[i];
-    return;
-  } else {
-    float r[8];
-    float m = 0.f;
+  for (int i = 0; i < 8; ++i) {
+    t[0][i] = (__bf16)(NT > 1 && sizeof(T) == 4 ? __builtin_amdgcn_fmed3f(v[i], -BF16_MOST, BF16_MOST) : v[i]);
+    if (NT > 1) r[i] = v[i] - (float)t[0][i];
+  }
+#pragma unroll
+  for (int k = 1; k < NT; ++k)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      t[0][i] = (__bf16)v[i];
-      r[i] = v[i] - (float)t[0][i];
-      m = fmaxf(m, fabsf(v[i]));
+      t[k][i] = (__bf16)r[i];
+      if (k + 1 < NT) r[i] -= (float)t[k][i];
     }
-    if (m > BF16_MOST) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (fabsf(v[i]) > BF16_MOST) {
-          const float hi = __uint_as_float(__float_as_uint(v[i]) & 0xffff0000u);
-          t[0][i] = (__bf16)hi;
-          r[i] = fabsf(v[i]) == __builtin_inff() ? 0.f : v[i] - hi;
-        }
-    }
-#pragma unroll
-    for (int k = 1; k < NT; ++k)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        t[k][i] = (__bf16)r[i];
-        if (k + 1 < NT) r[i] -= (float)t[k][i];
-      }
-  }
 }
 
-template <class T>
-struct Is16 {
-  static constexpr bool value = sizeof(T) == 2;
-};
+// 16 bytes from a buffer resource; an offset of OOR reads as zeros and touches no memory.  Bases move along k with the
+// loop, so offsets stay within the tile: rows shorter than 8 MB.
+__device__ __forceinline__ v4u buf16(rsrc_t r, int vo, int so) { return __builtin_bit_cast(v4u, bld16(r, vo, so)); }
+__device__ __forceinline__ rsrc_t buf_at(const void *p) { return make_rsrc(p, 0x7ffffff0u); }
+constexpr int64_t BUF_ROW = 1 << 23;  // bytes of a row, less than: 256 rows of a tile stay below 2^31
 
 // ============================================================ sums over partial rows
 
@@ -218,21 +204,19 @@ static inline void parts_sum(const float *part, int parts, int64_t n, int64_t n0
 
 // ============================================================ operands
 //
-// A tile of ROWS rows (m or n) x BK columns (k) goes from global memory through
-// registers into LDS, one plane per term: plane[row][BK] of 16-bit values, rows of
-// BK * 2 bytes whose 16-byte chunks are permuted by the row so that eight
-// neighbouring rows of one chunk lie in different banks (fragment reads), and
-// rows eight (16-bit) or four (f32) apart too (the writes of a row-contiguous
-// operand).
+// A tile of ROWS rows (m or n) x BK columns (k) goes from global memory through registers into LDS, one plane per term:
+// plane[row][BK] of 16-bit values.  LDS has 64 banks of 4 bytes, and 16 lanes read 16 bytes each at once: the 16-byte
+// chunks of a row are permuted by the row so that one chunk of 16 neighbouring rows (a fragment) covers all banks; rows
+// eight apart, which a row-contiguous operand writes together, fall apart too.
 //
 // A unit is one thread's part: 8 consecutive k of one row where k is contiguous
 // in memory (KC), else 16 bytes of rows for each of 8 consecutive k, transposed
 // in registers.
 template <int BK>
 __device__ __forceinline__ int chunk_at(int row, int c) {
-  if (BK == 64) return c ^ ((row ^ (row >> 3)) & 7);
-  const int v = row >> 1;
-  return c ^ ((v ^ (v >> 1)) & 3);
+  if (BK == 128) return c ^ (row & 15);
+  if (BK == 64) return c ^ (((row >> 1) ^ (row >> 4)) & 7);
+  return c ^ (((row >> 2) ^ (row >> 4)) & 3);
 }
 
 template <class T, int NT, bool KC, int ROWS, int BK, int NTHR, bool VEC>
@@ -245,11 +229,12 @@ struct Operand {
   static constexpr int PLANE = ROWS * BK;                 // 16-bit values of a term plane
   static_assert(UNITS % NTHR == 0 || UNITS < NTHR, "units split evenly over the threads");
 
-  const T *base;
+  const T *base;  // the tile's first row
   int64_t ld;
-  int rows;   // of the matrix, from the tile's first row
-  int first;  // the thread's first unit
+  int rows;       // of the matrix, from the tile's first row
+  int first;      // the thread's first unit
   bool on;
+  int off[UPT];   // bytes from the tile's first row and column (16-byte loads)
   v4u raw[UPT][NV];
 
   // `row0`: the tile's first row; `total`: rows of the matrix
@@ -259,6 +244,13 @@ struct Operand {
     rows = (int)(total - row0 < ROWS ? total - row0 : ROWS);
     on = t >= 0 && t < UNITS;
     first = t;
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      int row, c;
+      place(first + i * NTHR, row, c);
+      if (KC) off[i] = (min(row, rows - 1) * (int)ld + 8 * c) * (int)sizeof(T);
+      else off[i] = (8 * c * (int)ld + min(row, rows - R)) * (int)sizeof(T);
+    }
   }
   __device__ __forceinline__ static void place(int u, int &row, int &c) {
     if (KC) {
@@ -272,34 +264,34 @@ struct Operand {
   // columns [k, k + BK) of the tile, zeros from `kend` on; rows past the matrix
   // repeat its last ones (their results are not stored)
   __device__ __forceinline__ void load(int64_t k, int64_t kend) {
+    const int left = (int)min(kend - k, (int64_t)BK);
+    const rsrc_t r = buf_at(base + (KC ? k : k * ld));
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       int row, c;
       place(first + i * NTHR, row, c);
-      if (!on) continue;
-      const int64_t kc = k + 8 * c;
-      if constexpr (KC) {
-        const T *p = base + (int64_t)min(row, rows - 1) * ld + kc;
-        if constexpr (VEC) {
+      if constexpr (VEC && KC) {
+        const int vo = on && 8 * c < left ? off[i] : OOR;
 #pragma unroll
-          for (int q = 0; q < NV; ++q)
-            raw[i][q] = kc < kend ? reinterpret_cast<const v4u *>(p)[q] : v4u{0, 0, 0, 0};
-        } else {
+        for (int q = 0; q < NV; ++q) raw[i][q] = buf16(r, vo, 16 * q);
+      } else if constexpr (VEC) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          raw[i][j] = buf16(r, on && 8 * c + j < left ? off[i] : OOR, j * (int)ld * (int)sizeof(T));
+      } else if (on) {
+        if constexpr (KC) {
+          const T *p = base + (int64_t)min(row, rows - 1) * ld + k + 8 * c;
           T e[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) e[j] = kc + j < kend ? p[j] : from_f32<T>(0.f);
+          for (int j = 0; j < 8; ++j) e[j] = 8 * c + j < left ? p[j] : from_f32<T>(0.f);
           __builtin_memcpy(raw[i], e, sizeof(e));
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const T *p = base + (kc + j) * ld;
-          if constexpr (VEC) {
-            raw[i][j] = kc + j < kend ? *reinterpret_cast<const v4u *>(p + min(row, rows - R)) : v4u{0, 0, 0, 0};
-          } else {
+          for (int j = 0; j < 8; ++j) {
+            const T *p = base + (k + 8 * c + j) * ld;
             T e[R];
 #pragma unroll
-            for (int r = 0; r < R; ++r) e[r] = kc + j < kend ? p[min(row + r, rows - 1)] : from_f32<T>(0.f);
+            for (int q = 0; q < R; ++q) e[q] = 8 * c + j < left ? p[min(row + q, rows - 1)] : from_f32<T>(0.f);
             __builtin_memcpy(&raw[i][j], e, sizeof(e));
           }
         }
@@ -327,14 +319,14 @@ struct Operand {
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
           v8bf t[NT];
-          split_terms<NT>(v, t);
+          split_terms<T, NT>(v, t);
           put(lds, row, c, t);
         }
       } else if constexpr (KC) {
         float v[8];
         __builtin_memcpy(v, raw[i], sizeof(v));
         v8bf t[NT];
-        split_terms<NT>(v, t);
+        split_terms<T, NT>(v, t);
         put(lds, row, c, t);
       } else if constexpr (sizeof(T) == 2) {
         // raw[j] holds rows (0,1)(2,3)(4,5)(6,7) at column j; row 2q + h: its halves of the eight columns
@@ -356,7 +348,7 @@ struct Operand {
 #pragma unroll
               for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
               v8bf t[NT];
-              split_terms<NT>(v, t);
+              split_terms<T, NT>(v, t);
               put(lds, r, c, t);
             }
           }
@@ -367,7 +359,7 @@ struct Operand {
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw[i][j][r]);
           v8bf t[NT];
-          split_terms<NT>(v, t);
+          split_terms<T, NT>(v, t);
           put(lds, row + r, c, t);
         }
       }
@@ -659,19 +651,19 @@ void lin_rows_of(const LinArgs &g, hipStream_t st) {
 }
 
 // A few dozen rows of x: bound by reading w once, multiplied on the matrix cores.  A workgroup takes 128 NF columns of
-// the result, 16 MT rows and a slice of k in units of KS: each of its 8 waves asks for all of a unit's w at once,
-// straight from global memory into the instruction's operands (a lane's 16 or 32 bytes of its row of w: no other wave
-// needs them); while those are on their way x's part goes into LDS as terms, once for all waves.  So a unit costs one
-// trip to memory.
+// the result, 16 MT rows and a slice of k in units of KS.  Each of its 8 waves reads its rows of w straight from global
+// memory into the instruction's operands (a lane's 16 or 32 bytes: no other wave needs them); x's part of a unit goes
+// into LDS as terms, once for all waves.  The next unit's loads are in flight while one is multiplied; x's are asked
+// for before w's, since loads are waited for in order.
 template <class T>
 struct Eight {  // 8 consecutive values as they lie in memory
   v4u r[sizeof(T) / 2];
 };
 template <class T>
-__device__ __forceinline__ Eight<T> load8(const T *p, bool in) {
+__device__ __forceinline__ Eight<T> load8(rsrc_t r, int vo) {
   Eight<T> e;
 #pragma unroll
-  for (int q = 0; q < (int)sizeof(T) / 2; ++q) e.r[q] = in ? reinterpret_cast<const v4u *>(p)[q] : v4u{0, 0, 0, 0};
+  for (int q = 0; q < (int)sizeof(T) / 2; ++q) e.r[q] = buf16(r, vo, 16 * q);
   return e;
 }
 template <class T, int NT>
@@ -684,58 +676,80 @@ __device__ __forceinline__ void terms_of(const Eight<T> &e, v8bf (&t)[NT]) {
     __builtin_memcpy(f, &e, sizeof(f));
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = to_f32(f[j]);
-    split_terms<NT>(v, t);
+    split_terms<T, NT>(v, t);
   }
 }
 
 constexpr int LIN_FEW = 128, FEW_ROWS = 64;
-template <class TX, int NX, class TW, int NW, int MT, int NF>
-__global__ __launch_bounds__(512) void k_linear_few(LinArgs g) {
+constexpr int FEW_UNIT = 128;  // a slice is a multiple of it: one unit of a 16-bit w, two of an f32 one
+template <class TX, int NX, class TW, int NW, int MT, int NF, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
   constexpr bool F16 = std::is_same<TX, _Float16>::value && NX == 1;
-  constexpr int KS = sizeof(TW) == 2 ? 256 : 128, CH = KS / 8, ROWS = 16 * MT;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[NX * ROWS * KS];
+  constexpr int KS = sizeof(TW) == 2 ? FEW_UNIT : FEW_UNIT / 2, CH = KS / 8, ROWS = 16 * MT;
+  constexpr int THREADS = 64 * WAVES, UX = (ROWS * CH + THREADS - 1) / THREADS, PLANE = ROWS * KS;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][NX * PLANE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int fr = lane & 15, fc = lane >> 4;
   const int per = g.tiles_m * g.tiles_n;
   const int z = blockIdx.x / per, tile = blockIdx.x - z * per;
-  const int64_t m0 = (int64_t)(tile % g.tiles_m) * ROWS, n0 = (int64_t)(tile / g.tiles_m) * 128 * NF + wave * 16 * NF;
+  const int64_t m0 = (int64_t)(tile % g.tiles_m) * ROWS, n0 = (int64_t)(tile / g.tiles_m) * (16 * NF * WAVES);
+  const int64_t n1 = n0 + wave * 16 * NF;
   const int64_t kb = z * g.kslice, ke = min(g.K, kb + g.kslice);
   const int rows = (int)min(g.M - m0, (int64_t)ROWS);
-  const TW *w[NF];
-#pragma unroll
-  for (int j = 0; j < NF; ++j) w[j] = (const TW *)g.b + min(n0 + 16 * j + fr, g.N - 1) * g.ldb + 8 * fc;
+  // bytes from the workgroup's first column, and from its first row of x
+  const TW *w = (const TW *)g.b + n0 * g.ldb;
   const TX *x = (const TX *)g.a + m0 * g.lda;
+  int wo[NF], xo[UX];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) wo[j] = (int)((min(n1 + 16 * j + fr, g.N - 1) - n0) * g.ldb + 8 * fc) * (int)sizeof(TW);
+#pragma unroll
+  for (int u = 0; u < UX; ++u) {
+    const int q = threadIdx.x + THREADS * u, r = q / CH, c = q % CH;
+    xo[u] = r < rows ? (r * (int)g.lda + 8 * c) * (int)sizeof(TX) : OOR;
+  }
   v4f acc[MT][NF];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int64_t k = kb; k < ke; k += KS) {
-    Eight<TW> rw[KS / 32][NF];
+  struct Unit {
+    Eight<TX> x[UX];
+    Eight<TW> w[KS / 32][NF];
+  };
+  auto load = [&](Unit &t, int64_t k) {
+    const int left = (int)min(ke - k, (int64_t)KS);
+    const rsrc_t rx = buf_at(x + k), rw = buf_at(w + k);
+#pragma unroll
+    for (int u = 0; u < UX; ++u) t.x[u] = load8<TX>(rx, 8 * ((threadIdx.x + THREADS * u) % CH) < left ? xo[u] : OOR);
 #pragma unroll
     for (int h = 0; h < KS / 32; ++h)
 #pragma unroll
-      for (int j = 0; j < NF; ++j) rw[h][j] = load8(w[j] + k + 32 * h, k + 32 * h + 8 * fc < ke);
-    if (k > kb) __syncthreads();  // x's last part has been used
-    for (int u = threadIdx.x; u < rows * CH; u += 512) {
-      const int r = u / CH, c = u % CH;
-      v8bf t[NX];
-      terms_of<TX, NX>(load8(x + r * g.lda + k + 8 * c, k + 8 * c < ke), t);
+      for (int j = 0; j < NF; ++j)
+        t.w[h][j] = load8<TW>(rw, 32 * h + 8 * fc < left ? wo[j] + 32 * h * (int)sizeof(TW) : OOR);
+  };
+  // x's terms into `to` (which the waves have left behind a barrier ago), then the unit's products
+  auto step = [&](Unit &t, uint16_t *to) {
 #pragma unroll
-      for (int a = 0; a < NX; ++a) *reinterpret_cast<v8bf *>(lds + (a * ROWS + r) * KS + (c ^ (r & 7)) * 8) = t[a];
+    for (int u = 0; u < UX; ++u) {
+      const int q = threadIdx.x + THREADS * u, r = q / CH, c = q % CH;
+      if (r >= ROWS) break;
+      v8bf e[NX];
+      terms_of<TX, NX>(t.x[u], e);
+#pragma unroll
+      for (int a = 0; a < NX; ++a) *reinterpret_cast<v8bf *>(to + a * PLANE + r * KS + chunk_at<KS>(r, c) * 8) = e[a];
     }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < KS / 32; ++h) {
       v8bf tw[NF][NW];
 #pragma unroll
-      for (int j = 0; j < NF; ++j) terms_of<TW, NW>(rw[h][j], tw[j]);
+      for (int j = 0; j < NF; ++j) terms_of<TW, NW>(t.w[h][j], tw[j]);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int a = 0; a < NX; ++a) {
           const int r = 16 * i + fr;
-          const v8bf tx = *reinterpret_cast<const v8bf *>(lds + (a * ROWS + r) * KS + ((4 * h + fc) ^ (r & 7)) * 8);
+          const v8bf tx = *reinterpret_cast<const v8bf *>(to + a * PLANE + r * KS + chunk_at<KS>(r, 4 * h + fc) * 8);
 #pragma unroll
           for (int b = 0; b < NW; ++b) {
             if (a + b > Pairs<NX, NW>::MOST) continue;
@@ -750,24 +764,39 @@ __global__ __launch_bounds__(512) void k_linear_few(LinArgs g) {
           }
         }
     }
+  };
+  Unit p, q;
+  load(p, kb);
+  for (int64_t k = kb; k < ke; k += 2 * KS) {
+    if (k + KS < ke) load(q, k + KS);
+    step(p, lds[0]);
+    if (k + KS >= ke) break;
+    if (k + 2 * KS < ke) load(p, k + 2 * KS);
+    step(q, lds[1]);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NF; ++j) lin_result(g, z, m0 + 16 * i + fr, n0 + 16 * j + 4 * fc, acc[i][j]);
+    for (int j = 0; j < NF; ++j) lin_result(g, z, m0 + 16 * i + fr, n1 + 16 * j + 4 * fc, acc[i][j]);
 }
 
-template <class TX, int NX, class TW, int NW, int NF>
-void lin_few_launch(const LinArgs &g, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices)), b(512);
-  if (g.M <= 16) hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, 1, NF>), grid, b, 0, st, g);
-  else if (g.M <= 32) hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, 2, NF>), grid, b, 0, st, g);
-  else hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, 4, NF>), grid, b, 0, st, g);
+// columns of a workgroup (one wave each 16 of them): 64 where w is narrow, so that more of them share its reading, else
+// 128; 32 for each wave where the rows are many too
+inline int few_columns(int64_t M, int64_t N) { return M <= 32 ? (N < 2048 ? 64 : 128) : (N < 4096 ? 128 : 256); }
+template <class TX, int NX, class TW, int NW, int MT>
+void lin_few_rows(const LinArgs &g, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices));
+  switch (few_columns(g.M, g.N)) {
+  case 64: hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, MT, 1, 4>), grid, dim3(256), 0, st, g); break;
+  case 128: hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, MT, 1, 8>), grid, dim3(512), 0, st, g); break;
+  default: hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, MT, 2, 8>), grid, dim3(512), 0, st, g);
+  }
 }
 template <class TX, int NX, class TW, int NW>
-void lin_few_of(const LinArgs &g, int wide, hipStream_t st) {
-  if (wide) lin_few_launch<TX, NX, TW, NW, 2>(g, st);
-  else lin_few_launch<TX, NX, TW, NW, 1>(g, st);
+void lin_few_of(const LinArgs &g, hipStream_t st) {
+  if (g.M <= 16) lin_few_rows<TX, NX, TW, NW, 1>(g, st);
+  else if (g.M <= 32) lin_few_rows<TX, NX, TW, NW, 2>(g, st);
+  else lin_few_rows<TX, NX, TW, NW, 4>(g, st);
 }
 
 // The launch of one kernel instance.  `tile` 0 = 128 x 128, 1 = 32 x 128; operands without 16-byte loads (`vec`
@@ -782,7 +811,7 @@ void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
 
 // the products by what their operands are: forward (x, w), dx (dz, w), dw (dz, x)
 void lin_rows(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // M <= LIN_ROWS, operands with 16-byte loads
-void lin_few(int x_type, int w_type, const LinArgs &g, int wide, hipStream_t st);  // likewise; 128 or 256 (wide) columns
+void lin_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // likewise
 void lin_fwd(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dx(int x_type, int w_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dw(int x_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
