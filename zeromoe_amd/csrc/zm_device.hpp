@@ -696,4 +696,39 @@ __device__ __forceinline__ float quarter_dot(const WSlice &w, int q, const Q8Sli
   }
 }
 
+typedef unsigned v4u_t __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------- buffer-to-LDS loads
+//
+// Lane L's 16 bytes land at lds + 16 * L (inactive lanes write nothing,
+// out-of-range dwords write zeros).  Inline asm: the compiler's wait insertion
+// does not track them, so the caller counts them and waits itself.
+__device__ __forceinline__ v4u_t dma_rsrc(const void *p, uint32_t bytes) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  return v4u_t{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, bytes, 0x00020000u};
+}
+__device__ __forceinline__ uint32_t lds_addr(const void *p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
+}
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is written by the asm and by nothing else here
+__device__ __forceinline__ void dma_lds16(v4u_t rs, uint32_t lds, int vo, int so) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(vo), "s"(rs), "s"(so)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// at most N vector memory operations of this wave outstanding
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// the same, then the workgroup barrier (this wave's LDS reads are complete)
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
 }  // namespace zm

@@ -19,7 +19,8 @@ struct DzArgs {
   const void *dy, *pre;  // [S][O] of `type`; pre null without an activation
   int64_t ldy, ldp, S, O;
   int type, act;
-  float *dz;         // [S][ldz] f32, or null (without an activation dy is dz)
+  float *dz;         // [S][ldz] f32, or
+  bf16 *terms;       // [3][S][ldz], its bf16 terms, or neither (dy is dz)
   int64_t ldz;
   float *part;       // [gridDim.y][O] sums over this chunk of rows, or null
   int64_t chunk;     // rows of a chunk
@@ -64,6 +65,21 @@ __global__ __launch_bounds__(256) void k_linear_dz(DzArgs g) {
           if constexpr (V == 4) *reinterpret_cast<v4f *>(d) = v[u];
           else *d = v[u].x;
         }
+        if (g.terms) {
+          v4f r = v[u];
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            bf16 *d = g.terms + (k * g.S + su) * g.ldz + o;
+            bf16 e[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              e[j] = from_f32<bf16>(k ? r[j] : __builtin_amdgcn_fmed3f(r[j], -BF16_MOST, BF16_MOST));
+              r[j] -= to_f32(e[j]);
+            }
+            if constexpr (V == 4) __builtin_memcpy(__builtin_assume_aligned(d, 8), e, 8);
+            else *d = e[0];
+          }
+        }
       }
     }
   }
@@ -95,7 +111,8 @@ struct Plan {
 // the kernels of a product, by its rows and by whether its operands can be read 16 bytes at a time
 enum Kind { ROWS, FEW, TILES };
 
-Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, bool vec, size_t most) {
+// `step`: k of a step of the tiles; `dma`: 16-bit operands of one type
+Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int step, bool dma, bool vec, size_t most) {
   Plan p{};
   p.kind = kind;
   int64_t z = 1, bk = 64;
@@ -108,13 +125,24 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, bool vec, size_t most) {
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, want = cols == 64 ? 512 : 256;
     z = std::min<int64_t>((want - 1 + tiles) / tiles, (K + bk - 1) / bk);
   } else if (kind == TILES) {
-    // 128 x 128, or 32 x 128 for up to 64 rows; k in as many slices as give about two workgroups per CU (at least four
-    // tiles of k each)
+    // 128 x 128, or 32 x 128 for up to 64 rows; 256 x 256 for 16-bit operands where that leaves no CU idle in most of
+    // its rounds; k in as many slices as give about two workgroups per CU (at least four steps each)
     p.tile = !vec || M <= 64;
-    const int bm = p.tile ? 32 : 128;
+    int bm = p.tile ? 32 : 128, bn = 128;
+    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
+    if (dma && !p.tile && big >= 224 && big * 100 >= (big + 255) / 256 * 256 * 85) {
+      p.tile = 2;
+      bm = bn = 256;
+    }
     p.tiles_m = (int)((M + bm - 1) / bm);
-    p.tiles_n = (int)((N + 127) / 128);
-    z = std::min<int64_t>(512 / std::max<int64_t>((int64_t)p.tiles_m * p.tiles_n, 1), K / 256);
+    p.tiles_n = (int)((N + bn - 1) / bn);
+    if (p.tile != 2) z = std::min<int64_t>(512 / std::max<int64_t>((int64_t)p.tiles_m * p.tiles_n, 1), planes * K / 256);
+    z = std::max<int64_t>(1, std::min<int64_t>(z, (int64_t)(most / ((size_t)M * N * 4))));
+    const int64_t steps = planes * ((K + step - 1) / step);
+    p.kslice = (steps + z - 1) / z;
+    p.slices = (int)((steps + p.kslice - 1) / p.kslice);
+    p.part = p.slices > 1 ? (size_t)p.slices * M * N * 4 : 0;
+    return p;
   }
   z = std::max<int64_t>(1, std::min<int64_t>(z, (int64_t)(most / ((size_t)M * N * 4))));
   p.kslice = ((K + z - 1) / z + bk - 1) / bk * bk;
@@ -139,41 +167,57 @@ bool vec_at(const void *p) { return !((uintptr_t)p & 15); }
 // to do with that.
 struct Product {
   int64_t M, N, K;
+  int a_type, b_type, planes;
   bool shaped;   // strides and widths allow 16-byte loads
   bool forward;  // the product has kernels for few rows
   Kind kind(bool vec) const {
     if (!vec || !forward || N >= (1 << 26) || K >= (1 << 30)) return TILES;
     return M <= LIN_ROWS ? ROWS : M <= LIN_FEW ? FEW : TILES;
   }
+  Plan plan_for(bool vec, size_t most) const {
+    const bool dma = a_type == b_type && a_type != LIN_F32;
+    return plan(kind(vec), M, N, K, planes, dma ? 64 : 32, dma, vec, most);
+  }
   // partial sums of at most 64 MB
-  size_t space() const { return plan(kind(shaped), M, N, K, shaped, 64 << 20).part; }
-  Plan planned(bool vec) const { return plan(kind(vec), M, N, K, vec, vec == shaped ? 64 << 20 : space()); }
+  size_t space() const { return plan_for(shaped, 64 << 20).part; }
+  Plan planned(bool vec) const { return plan_for(vec, vec == shaped ? 64 << 20 : space()); }
 };
 Product forward(const zm_linear_desc &d) {
-  return {d.S, d.O, d.I, vec_shape(d.x_stride, d.I, d.x_type, true) && vec_shape(d.w_stride, d.I, d.w_type, true), true};
+  return {d.S, d.O, d.I, d.x_type, d.w_type, 1,
+          vec_shape(d.x_stride, d.I, d.x_type, true) && vec_shape(d.w_stride, d.I, d.w_type, true), true};
 }
-int64_t dz_stride(int64_t O);
-// what dz is: dy itself, or f32 of the workspace behind an activation
-int dz_type(const zm_linear_desc &d) { return d.act ? (int)LIN_F32 : d.y_type; }
-int64_t dz_ld(const zm_linear_desc &d) { return d.act ? dz_stride(d.O) : d.y_stride; }
+// What the products of the backward pass take for dz: dy itself; behind an activation f32 in the workspace; next to
+// bf16, where it is not bf16 itself, three planes of bf16 terms there.
+enum DzForm { DZ_DY, DZ_F32, DZ_TERMS };
+DzForm dz_form(const zm_linear_desc &d) {
+  if (d.x_type == LIN_BF16 && (d.act || d.y_type == LIN_F32)) return DZ_TERMS;
+  return d.act ? DZ_F32 : DZ_DY;
+}
+int dz_type(const zm_linear_desc &d) {
+  const DzForm f = dz_form(d);
+  return f == DZ_TERMS ? (int)LIN_BF16 : f == DZ_F32 ? (int)LIN_F32 : d.y_type;
+}
+int64_t dz_ld(const zm_linear_desc &d) { return dz_form(d) == DZ_DY ? d.y_stride : (d.O + 7) / 8 * 8; }
 Product by_x(const zm_linear_desc &d) {
-  return {d.S, d.I, d.O, vec_shape(dz_ld(d), d.O, dz_type(d), true) && vec_shape(d.w_stride, d.I, d.w_type, false), false};
+  return {d.S, d.I, d.O, dz_type(d), d.w_type, 1,
+          vec_shape(dz_ld(d), d.O, dz_type(d), true) && vec_shape(d.w_stride, d.I, d.w_type, false), false};
 }
 Product by_w(const zm_linear_desc &d) {
-  return {d.O, d.I, d.S, vec_shape(dz_ld(d), d.O, dz_type(d), false) && vec_shape(d.x_stride, d.I, d.x_type, false), false};
+  return {d.O, d.I, d.S, dz_type(d), d.x_type, dz_form(d) == DZ_TERMS ? 3 : 1,
+          vec_shape(dz_ld(d), d.O, dz_type(d), false) && vec_shape(d.x_stride, d.I, d.x_type, false), false};
 }
 
-int64_t dz_stride(int64_t O) { return (O + 3) / 4 * 4; }
 // chunks of rows of the bias gradient: 32 rows each, at most 256
 int64_t dz_chunks(int64_t S) { return std::min<int64_t>((S + 31) / 32, 256); }
 
-// Workspace of the backward pass: dz in f32 (behind an activation) | bias partials | the larger product's partials.
+// Workspace of the backward pass: dz (unless it is dy) | bias partials | the larger product's partials.
 struct BackwardSpace {
   size_t dz, bias, part, total;
 };
 BackwardSpace backward_space(const zm_linear_desc &d) {
   BackwardSpace w{};
-  w.dz = d.act ? align256((size_t)d.S * dz_stride(d.O) * 4) : 0;
+  const size_t n = (size_t)d.S * dz_ld(d);
+  w.dz = dz_form(d) == DZ_DY ? 0 : align256(dz_form(d) == DZ_F32 ? n * 4 : n * 6);
   w.bias = align256((size_t)dz_chunks(d.S) * d.O * 4);
   w.part = align256(std::max(by_x(d).space(), by_w(d).space()));
   w.total = w.dz + w.bias + w.part;
@@ -220,6 +264,8 @@ LinArgs product(const Product &q, const void *a, int64_t lda, const void *b, int
   g.M = q.M;
   g.N = q.N;
   g.K = q.K;
+  g.planes = q.planes;
+  g.plane = q.planes > 1 ? q.K * lda : 0;
   g.tiles_m = p.tiles_m;
   g.tiles_n = p.tiles_n;
   g.slices = p.slices;
@@ -298,7 +344,8 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
     return fail("zm_linear_backward: a 256-byte aligned workspace of zm_linear_backward_workspace_size() bytes is needed");
   uint8_t *ws = (uint8_t *)workspace;
   float *dz = (float *)ws, *bias_part = (float *)(ws + s.dz), *part = (float *)(ws + s.dz + s.bias);
-  if (d->act || dbias) {
+  const DzForm form = dz_form(*d);
+  if (form != DZ_DY || dbias) {
     DzArgs a{};
     a.dy = dy;
     a.pre = pre;
@@ -308,8 +355,9 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
     a.O = d->O;
     a.type = d->y_type;
     a.act = d->act;
-    a.dz = d->act ? dz : nullptr;
-    a.ldz = dz_stride(d->O);
+    a.dz = form == DZ_F32 ? dz : nullptr;
+    a.terms = form == DZ_TERMS ? (bf16 *)dz : nullptr;
+    a.ldz = dz_ld(*d);
     a.part = dbias ? bias_part : nullptr;
     const int64_t n = dz_chunks(d->S);
     a.chunk = (d->S + n - 1) / n;
@@ -322,7 +370,7 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
     else hipLaunchKernelGGL((k_linear_dz<1>), grid, dim3(256), 0, st, a);
     if (dbias) parts_sum(bias_part, (int)n, d->O, d->O, dbias, nullptr, st);
   }
-  const void *z = d->act ? (const void *)dz : dy;
+  const void *z = form == DZ_DY ? dy : (const void *)dz;
   const int z_type = dz_type(*d);
   if (dx) {
     const Product q = by_x(*d);

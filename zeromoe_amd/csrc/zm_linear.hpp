@@ -261,11 +261,12 @@ struct Operand {
       c = u / (ROWS / R);
     }
   }
-  // columns [k, k + BK) of the tile, zeros from `kend` on; rows past the matrix
+  // columns [k, k + BK) of the tile, `skip` values on, zeros from `kend` on; rows past the matrix
   // repeat its last ones (their results are not stored)
-  __device__ __forceinline__ void load(int64_t k, int64_t kend) {
+  __device__ __forceinline__ void load(int64_t k, int64_t kend, int64_t skip) {
     const int left = (int)min(kend - k, (int64_t)BK);
-    const rsrc_t r = buf_at(base + (KC ? k : k * ld));
+    const T *at = base + skip + (KC ? k : k * ld);
+    const rsrc_t r = buf_at(at);
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       int row, c;
@@ -280,7 +281,7 @@ struct Operand {
           raw[i][j] = buf16(r, on && 8 * c + j < left ? off[i] : OOR, j * (int)ld * (int)sizeof(T));
       } else if (on) {
         if constexpr (KC) {
-          const T *p = base + (int64_t)min(row, rows - 1) * ld + k + 8 * c;
+          const T *p = at + (int64_t)min(row, rows - 1) * ld + 8 * c;
           T e[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) e[j] = 8 * c + j < left ? p[j] : from_f32<T>(0.f);
@@ -288,7 +289,7 @@ struct Operand {
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const T *p = base + (k + 8 * c + j) * ld;
+            const T *p = at + (int64_t)(8 * c + j) * ld;
             T e[R];
 #pragma unroll
             for (int q = 0; q < R; ++q) e[q] = 8 * c + j < left ? p[min(row + q, rows - 1)] : from_f32<T>(0.f);
@@ -384,8 +385,10 @@ struct LinArgs {
   int64_t lda, ldb;
   int64_t M, N, K;
   int tiles_m, tiles_n;
+  int planes;      // of a, to be added: each `plane` values after the last, all times the same b
+  int64_t plane;
   int slices;      // of k
-  int64_t kslice;  // columns of a slice (a multiple of BK)
+  int64_t kslice;  // k of a slice; k_linear, k_linear_dma: steps of a slice
   float *part;     // [slices][M][N] when slices > 1
   LinEpilogue e;
 };
@@ -436,6 +439,24 @@ __device__ __forceinline__ int xcd_order(int b, int n) {
   return x * q + min(x, r) + b / 8;
 }
 
+// The steps of one slice: BK of k each, through the planes of `a` one after the other.
+struct LinSteps {
+  int64_t k, left, per;  // where the step is; steps left; steps of a plane
+  int p;
+  __device__ __forceinline__ LinSteps(const LinArgs &g, int z, int bk) {
+    per = (g.K + bk - 1) / bk;
+    const int64_t first = z * g.kslice;
+    left = min(g.planes * per - first, g.kslice);
+    p = g.planes > 1 ? (int)(first / per) : 0;
+    k = (first - p * per) * bk;
+  }
+  __device__ __forceinline__ bool next(int bk) {
+    k += bk;
+    if (k >= per * bk) k = 0, ++p;
+    return --left > 0;
+  }
+};
+
 // The term pairs of a product: (0,0) first, then those 2^-9, 2^-18 smaller
 template <int NA, int NB>
 struct Pairs {
@@ -461,7 +482,6 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
   const int per = g.tiles_m * g.tiles_n;
   const int z = tile / per, tt = tile - z * per;
   const int64_t m0 = (int64_t)(tt / g.tiles_n) * BM, n0 = (int64_t)(tt % g.tiles_n) * BN;
-  const int64_t kb = z * g.kslice, ke = min(g.K, kb + g.kslice);
   OA a;
   OB b;
   a.init(g.a, g.lda, m0, g.M, tid);
@@ -474,16 +494,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
     for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const int fr = lane & 15, fc = lane >> 4;
-  a.load(kb, ke);
-  b.load(kb, ke);
-  for (int64_t k = kb; k < ke; k += BK) {
+  LinSteps at(g, z, BK);
+  auto load = [&] {
+    a.load(at.k, g.K, at.p * g.plane);
+    b.load(at.k, g.K, 0);
+  };
+  load();
+  for (;;) {
     a.store(lds_a);
     b.store(lds_b);
     __syncthreads();
-    if (k + BK < ke) {
-      a.load(k + BK, ke);
-      b.load(k + BK, ke);
-    }
+    const bool more = at.next(BK);
+    if (more) load();
 #pragma unroll
     for (int s = 0; s < BK / 32; ++s) {
       v8bf fa[FM][NA], fb[FN][NB];
@@ -518,8 +540,138 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
             }
         }
     }
+    if (!more) break;
     __syncthreads();
   }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) lin_result(g, z, m0 + wm + 16 * i + fr, n0 + wn + 16 * j + 4 * fc, acc[i][j]);
+}
+
+// ============================================================ 16-bit operands, large
+//
+// The same product for 16-bit operands of one type, bound by the matrix cores: tiles go from global memory straight
+// into LDS (16 bytes a lane), the next step's while this one's are multiplied; a barrier a step of 64.  An operand
+// whose k is contiguous lies in LDS as above; a row-contiguous one as it is in memory, a row of LDS for each k, and is
+// turned by the transposing reads (16 lanes read 4 k of 16 rows and get 4 k of one row each).  Its 32-byte pieces are
+// permuted by k so that the 8 k that 32 lanes read fall into different banks.  LDS is written in the lanes' order, so
+// the permutation is in what each lane asks for.
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+template <bool KC, int ROWS, int NTHR>
+struct DmaOperand {
+  static constexpr int BK = 64, PER = ROWS * BK / 8 / NTHR, WIDE = ROWS / 8;  // 16-byte chunks of a thread; of a row of k
+  static constexpr int BYTES = ROWS * BK * 2;
+  const uint16_t *base;
+  int64_t ld;
+  int off[PER];
+  __device__ __forceinline__ static int turn(int k) { return (k & 3) | ((k >> 3) & 1) << 2; }
+  __device__ __forceinline__ static void place(int i, int &r, int &c) {  // KC: row, chunk; else k, first row
+    const int s = i * NTHR + (int)threadIdx.x;
+    if (KC) {
+      r = s / 8;
+      c = chunk_at<64>(r, s % 8);
+    } else {
+      r = s / WIDE;
+      const int q = s % WIDE;
+      c = 8 * ((((q >> 1) ^ turn(r)) << 1) | (q & 1));
+    }
+  }
+  __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t total) {
+    ld = ld_;
+    base = (const uint16_t *)p + (KC ? row0 * ld : row0);
+    const int rows = (int)(total - row0 < ROWS ? total - row0 : ROWS);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int r, c;
+      place(i, r, c);
+      off[i] = 2 * (KC ? min(r, rows - 1) * (int)ld + 8 * c : r * (int)ld + min(c, rows - 8));
+    }
+  }
+  // the step at k into `lds`: zeros from `kend` on
+  __device__ __forceinline__ void load(uint32_t lds, int64_t k, int64_t kend, int64_t skip) const {
+    const int left = (int)min(kend - k, (int64_t)BK);
+    const v4u_t rs = dma_rsrc(base + skip + (KC ? k : k * ld), 0x7ffffff0u);
+    const uint32_t to = lds + (threadIdx.x >> 6) * 1024u;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int r, c;
+      place(i, r, c);
+      dma_lds16(rs, to + i * NTHR * 16u, (KC ? 8 * c : r) < left ? off[i] : OOR, 0);
+    }
+  }
+  // the fragment of 16 rows from `row` on, 32 k from 32 * s on
+  __device__ __forceinline__ static v8bf frag(const uint16_t *lds, int row, int s) {
+    const int lane = threadIdx.x & 63, fr = lane & 15, fc = lane >> 4;
+    if constexpr (KC) {
+      const int r = row + fr;
+      return *reinterpret_cast<const v8bf *>(lds + r * BK + chunk_at<64>(r, 4 * s + fc) * 8);
+    } else {
+      const int k = 32 * s + 8 * fc + (fr >> 2);
+      const uint16_t *q = lds + k * ROWS + (((row >> 4) ^ turn(k)) << 4) + 4 * (fr & 3);
+      typedef __attribute__((address_space(3))) v4s *lp;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 4 * ROWS));
+      return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+template <bool F16, bool KCA, bool KCB, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
+  constexpr int NTHR = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, BK = 64;
+  typedef DmaOperand<KCA, BM, NTHR> OA;
+  typedef DmaOperand<KCB, BN, NTHR> OB;
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[2][(OA::BYTES + OB::BYTES) / 2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tile = xcd_order(blockIdx.x, gridDim.x);
+  const int per = g.tiles_m * g.tiles_n;
+  const int z = tile / per, tt = tile - z * per;
+  const int64_t m0 = (int64_t)(tt / g.tiles_n) * BM, n0 = (int64_t)(tt % g.tiles_n) * BN;
+  OA a;
+  OB b;
+  a.init(g.a, g.lda, m0, g.M);
+  b.init(g.b, g.ldb, n0, g.N);
+  v4f acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  LinSteps at(g, z, BK);
+  const uint32_t l0 = lds_addr(lds[0]), l1 = lds_addr(lds[1]);
+  auto load = [&](int buf) {
+    const uint32_t to = buf ? l1 : l0;
+    a.load(to, at.k, g.K, at.p * g.plane);
+    b.load(to + OA::BYTES, at.k, g.K, 0);
+  };
+  load(0);
+  for (int buf = 0;; buf ^= 1) {
+    const bool more = at.next(BK);
+    wait_barrier<0>();  // this step's tiles have landed for all waves, and all have read the other buffer's
+    if (more) load(buf ^ 1);
+    const uint16_t *la = lds[buf], *lb = la + OA::BYTES / 2;
+#pragma unroll
+    for (int s = 0; s < BK / 32; ++s) {
+      v8bf fa[FM], fb[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[i] = OA::frag(la, wm + 16 * i, s);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = OB::frag(lb, wn + 16 * j, s);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          if constexpr (F16)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, fb[j]), __builtin_bit_cast(v8h, fa[i]),
+                                                              acc[i][j], 0, 0, 0);
+          else
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+        }
+    }
+    if (!more) break;
+  }
+  const int fr = lane & 15, fc = lane >> 4;
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -799,19 +951,27 @@ void lin_few_of(const LinArgs &g, hipStream_t st) {
   else lin_few_rows<TX, NX, TW, NW, 4>(g, st);
 }
 
-// The launch of one kernel instance.  `tile` 0 = 128 x 128, 1 = 32 x 128; operands without 16-byte loads (`vec`
-// false) take 32 x 128.
+// The launch of one kernel instance.  `tile`: 0 = 128 x 128, 1 = 32 x 128, 2 = 256 x 256 (16-bit operands); operands
+// without 16-byte loads (`vec` false) take 32 x 128.
 template <class TA, int NA, bool KCA, class TB, int NB, bool KCB>
 void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices));
-  if (!vec) hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 4, false>), grid, dim3(256), 0, st, g);
-  else if (tile) hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 4, true>), grid, dim3(256), 0, st, g);
-  else hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 2, true>), grid, dim3(256), 0, st, g);
+  if (!vec) {
+    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 4, false>), grid, dim3(256), 0, st, g);
+  } else if (tile == 1) {
+    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 4, true>), grid, dim3(256), 0, st, g);
+  } else if constexpr (std::is_same<TA, TB>::value && sizeof(TA) == 2) {
+    constexpr bool F16 = std::is_same<TA, _Float16>::value;
+    if (tile == 2) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 256, 2, 4>), grid, dim3(512), 0, st, g);
+    else hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
+  } else {
+    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 2, true>), grid, dim3(256), 0, st, g);
+  }
 }
 
 // the products by what their operands are: forward (x, w), dx (dz, w), dw (dz, x)
 void lin_rows(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // M <= LIN_ROWS, operands with 16-byte loads
-void lin_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // likewise
+void lin_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);   // M <= LIN_FEW, likewise
 void lin_fwd(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dx(int x_type, int w_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dw(int x_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);

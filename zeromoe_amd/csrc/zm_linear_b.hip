@@ -1,8 +1,8 @@
 // zm_linear_b.hip -- products of the gradient by x: dz [S][O] by w [O][I], k = O contiguous in dz, rows in w.
 //
-// The result has x's type.  Where that is 16 bits and dz is held in f32 (behind an activation, or from an f32
-// result), dz enters with fewer terms: one bf16 term for bf16 (its rounding, 2^-9, is the result's own), two for
-// f16 (2^-17 against the result's 2^-12; one f16 term could overflow or lose small gradients).
+// The result has x's type.  Where that is 16 bits and dz is not (behind an activation, or from an f32 result), dz enters
+// with fewer terms: for bf16 its first bf16 term alone (its rounding, 2^-9, is the result's own), for f16 two of them
+// (2^-17 against the result's 2^-12; one f16 term could overflow or lose small gradients).
 #include <hip/hip_runtime.h>
 
 #include "zm_linear.hpp"
@@ -11,8 +11,7 @@ namespace zm {
 
 void lin_dx(int x_type, int w_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st) {
   if (x_type == LIN_BF16) {
-    if (dz_type == LIN_F32) lin_launch<float, 1, true, bf16, 1, false>(g, vec, tile, st);
-    else lin_launch<bf16, 1, true, bf16, 1, false>(g, vec, tile, st);
+    lin_launch<bf16, 1, true, bf16, 1, false>(g, vec, tile, st);
   } else if (x_type == LIN_F16) {
     if (dz_type == LIN_F32) lin_launch<float, 2, true, _Float16, 2, false>(g, vec, tile, st);
     else lin_launch<_Float16, 1, true, _Float16, 1, false>(g, vec, tile, st);
