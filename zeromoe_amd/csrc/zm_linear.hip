@@ -125,23 +125,45 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int step, bool
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, want = cols == 64 ? 512 : 256;
     z = std::min<int64_t>((want - 1 + tiles) / tiles, (K + bk - 1) / bk);
   } else if (kind == TILES) {
-    // 128 x 128, or 32 x 128 for up to 64 rows; 256 x 256 for 16-bit operands where that leaves no CU idle in most of
-    // its rounds; k in as many slices as give about two workgroups per CU (at least four steps each)
+    const int64_t steps = planes * ((K + step - 1) / step);
+    const size_t plane = (size_t)M * N * 4;
     p.tile = !vec || M <= 64;
     int bm = p.tile ? 32 : 128, bn = 128;
-    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    if (dma && !p.tile && big >= 224 && big * 100 >= (big + 255) / 256 * 256 * 85) {
-      p.tile = 2;
-      bm = bn = 256;
+    if (dma && !p.tile) {
+      // The cheapest of three tiles and some numbers of slices, by what they measured: us of a step in which every CU
+      // has one tile of 256 x 256, one of 256 x 128, one of 128 x 128 and two of 128 x 128; and a join of the slices
+      // at 5 TB/s with 4 us to start.
+      double best = 1e30;
+      for (int tile : {2, 3, 0}) {
+        const int64_t h = tile ? 256 : 128, w = tile == 2 ? 256 : 128;
+        const int64_t tiles = ((M + h - 1) / h) * ((N + w - 1) / w);
+        for (int64_t s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+          if (s > 1 && (s * plane > most || steps < 4 * s || tiles * s > 1024)) break;
+          const int64_t n = tiles * s;
+          const double rounds = tile ? (double)((n + 255) / 256) * (tile == 2 ? 1.9 : 1.04)
+                                     : n / 512 * 1.09 + (n % 512 > 256 ? 1.09 : n % 512 ? 0.75 : 0.0);
+          const double us = rounds * (double)((steps + s - 1) / s) + (s > 1 ? 4.0 + s * plane * 2 / 5e6 : 0.0);
+          if (us < best) {
+            best = us;
+            z = s;
+            p.tile = tile;
+            bm = (int)h;
+            bn = (int)w;
+          }
+        }
+      }
     }
     p.tiles_m = (int)((M + bm - 1) / bm);
     p.tiles_n = (int)((N + bn - 1) / bn);
-    if (p.tile != 2) z = std::min<int64_t>(512 / std::max<int64_t>((int64_t)p.tiles_m * p.tiles_n, 1), planes * K / 256);
-    z = std::max<int64_t>(1, std::min<int64_t>(z, (int64_t)(most / ((size_t)M * N * 4))));
-    const int64_t steps = planes * ((K + step - 1) / step);
+    if (!dma || p.tile == 1) {
+      // 128 x 128, or 32 x 128 for up to 64 rows; k in as many slices as give about two workgroups per CU (at least
+      // 256 of k each)
+      z = std::min<int64_t>(512 / std::max<int64_t>((int64_t)p.tiles_m * p.tiles_n, 1), planes * K / 256);
+      z = std::max<int64_t>(1, std::min<int64_t>(z, (int64_t)(most / plane)));
+    }
     p.kslice = (steps + z - 1) / z;
     p.slices = (int)((steps + p.kslice - 1) / p.kslice);
-    p.part = p.slices > 1 ? (size_t)p.slices * M * N * 4 : 0;
+    p.part = p.slices > 1 ? (size_t)p.slices * plane : 0;
     return p;
   }
   z = std::max<int64_t>(1, std::min<int64_t>(z, (int64_t)(most / ((size_t)M * N * 4))));
@@ -176,7 +198,7 @@ struct Product {
   }
   Plan plan_for(bool vec, size_t most) const {
     const bool dma = a_type == b_type && a_type != LIN_F32;
-    return plan(kind(vec), M, N, K, planes, dma ? 64 : 32, dma, vec, most);
+    return plan(kind(vec), M, N, K, planes, dma ? DMA_BK : 32, dma, vec, most);
   }
   // partial sums of at most 64 MB
   size_t space() const { return plan_for(shaped, 64 << 20).part; }

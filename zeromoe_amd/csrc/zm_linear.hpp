@@ -551,34 +551,42 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
 
 // ============================================================ 16-bit operands, large
 //
-// The same product for 16-bit operands of one type, bound by the matrix cores: tiles go from global memory straight
-// into LDS (16 bytes a lane), the next step's while this one's are multiplied; a barrier a step of 64.  An operand
-// whose k is contiguous lies in LDS as above; a row-contiguous one as it is in memory, a row of LDS for each k, and is
-// turned by the transposing reads (16 lanes read 4 k of 16 rows and get 4 k of one row each).  Its 32-byte pieces are
-// permuted by k so that the 8 k that 32 lanes read fall into different banks.  LDS is written in the lanes' order, so
-// the permutation is in what each lane asks for.
+// The same product for 16-bit operands of one type, bound by the matrix cores.  Tiles go from global memory straight
+// into LDS (16 bytes a lane, whole cache lines of 64 k), two steps deep; fragments are read into registers half a step
+// ahead; one barrier a step.  8192^3 in bf16: 945 us, 1160 TFLOP/s (without its loads the loop does 1460; with them
+// answered by L2 alone 1290; reading them where a step of 32 k is four deep, in half lines, 780).
+//
+// An operand whose k is contiguous lies in LDS in rows of 64 k, its 16-byte chunks permuted by the row so that 16 rows
+// of a fragment cover all banks.  A row-contiguous one lies as it is in memory, a row of LDS for each k, and is turned
+// by the transposing reads (16 lanes read 4 k of 16 rows and get 4 k of one row each); its 32-byte pieces are permuted
+// by k so that the 8 k that 32 lanes read fall into different banks.  LDS is written in the lanes' order, so the
+// permutation is in what each lane asks for.
 typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+constexpr int DMA_BK = 64;
 
-template <bool KC, int ROWS, int NTHR>
+template <bool KC, int ROWS, int NTHR, int FR>
 struct DmaOperand {
-  static constexpr int BK = 64, PER = ROWS * BK / 8 / NTHR, WIDE = ROWS / 8;  // 16-byte chunks of a thread; of a row of k
+  static constexpr int BK = DMA_BK, PER = ROWS * BK / 8 / NTHR, WIDE = ROWS / 8;  // 16-byte chunks of a thread; of a row of k
   static constexpr int BYTES = ROWS * BK * 2;
   const uint16_t *base;
   int64_t ld;
   int off[PER];
+  uint32_t at[KC ? 2 : FR];  // where the lane's part of each fragment is (KC: of each half of the step)
   __device__ __forceinline__ static int turn(int k) { return (k & 3) | ((k >> 3) & 1) << 2; }
   __device__ __forceinline__ static void place(int i, int &r, int &c) {  // KC: row, chunk; else k, first row
     const int s = i * NTHR + (int)threadIdx.x;
     if (KC) {
       r = s / 8;
-      c = chunk_at<64>(r, s % 8);
+      c = s % 8 ^ (r >> 1 & 7);
     } else {
       r = s / WIDE;
       const int q = s % WIDE;
       c = 8 * ((((q >> 1) ^ turn(r)) << 1) | (q & 1));
     }
   }
-  __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t total) {
+  // `w0`: the wave's first row of the tile
+  __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t total, int w0) {
     ld = ld_;
     base = (const uint16_t *)p + (KC ? row0 * ld : row0);
     const int rows = (int)(total - row0 < ROWS ? total - row0 : ROWS);
@@ -588,30 +596,34 @@ struct DmaOperand {
       place(i, r, c);
       off[i] = 2 * (KC ? min(r, rows - 1) * (int)ld + 8 * c : r * (int)ld + min(c, rows - 8));
     }
-  }
-  // the step at k into `lds`: zeros from `kend` on
-  __device__ __forceinline__ void load(uint32_t lds, int64_t k, int64_t kend, int64_t skip) const {
-    const int left = (int)min(kend - k, (int64_t)BK);
-    const v4u_t rs = dma_rsrc(base + skip + (KC ? k : k * ld), 0x7ffffff0u);
-    const uint32_t to = lds + (threadIdx.x >> 6) * 1024u;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      int r, c;
-      place(i, r, c);
-      dma_lds16(rs, to + i * NTHR * 16u, (KC ? 8 * c : r) < left ? off[i] : OOR, 0);
-    }
-  }
-  // the fragment of 16 rows from `row` on, 32 k from 32 * s on
-  __device__ __forceinline__ static v8bf frag(const uint16_t *lds, int row, int s) {
     const int lane = threadIdx.x & 63, fr = lane & 15, fc = lane >> 4;
     if constexpr (KC) {
-      const int r = row + fr;
-      return *reinterpret_cast<const v8bf *>(lds + r * BK + chunk_at<64>(r, 4 * s + fc) * 8);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) at[s] = 2 * ((w0 + fr) * BK + ((4 * s + fc) ^ (fr >> 1)) * 8);  // (w0 is a multiple of 16)
     } else {
-      const int k = 32 * s + 8 * fc + (fr >> 2);
-      const uint16_t *q = lds + k * ROWS + (((row >> 4) ^ turn(k)) << 4) + 4 * (fr & 3);
+      const int k = 8 * fc + (fr >> 2);
+#pragma unroll
+      for (int i = 0; i < FR; ++i) at[i] = 2 * (k * ROWS + (((w0 >> 4) + i ^ turn(k)) << 4) + 4 * (fr & 3));
+    }
+  }
+  __device__ __forceinline__ v4u_t source(int64_t k, int64_t skip) const {
+    return dma_rsrc(base + skip + (KC ? k : k * ld), 0x7ffffff0u);
+  }
+  // the i-th request of a step into the buffer at `lds`; `left`: k of the step that exist (zeros past them)
+  __device__ __forceinline__ void ask(v4u_t rs, uint32_t lds, int i, int left) const {
+    int r, c;
+    place(i, r, c);
+    dma_lds16(rs, lds + (threadIdx.x >> 6) * 1024u + i * NTHR * 16u, (KC ? 8 * c : r) < left ? off[i] : OOR, 0);
+  }
+  // fragment i of the wave, half s of the step, from the buffer at `lds`
+  __device__ __forceinline__ v8bf frag(uint32_t lds, int i, int s) const {
+    if constexpr (KC) {
+      typedef __attribute__((address_space(3))) v8s *lp;
+      return __builtin_bit_cast(v8bf, *(lp)(lds + at[s] + 2 * 16 * BK * i));
+    } else {
       typedef __attribute__((address_space(3))) v4s *lp;
-      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 4 * ROWS));
+      const uint32_t q = lds + at[i] + 64 * ROWS * s;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 8 * ROWS));
       return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
@@ -619,58 +631,102 @@ struct DmaOperand {
 
 template <bool F16, bool KCA, bool KCB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
-  constexpr int NTHR = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, BK = 64;
-  typedef DmaOperand<KCA, BM, NTHR> OA;
-  typedef DmaOperand<KCB, BN, NTHR> OB;
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[2][(OA::BYTES + OB::BYTES) / 2];
+  constexpr int NTHR = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+  typedef DmaOperand<KCA, BM, NTHR, FM> OA;
+  typedef DmaOperand<KCB, BN, NTHR, FN> OB;
+  constexpr int BYTES = OA::BYTES + OB::BYTES;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BYTES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int tile = xcd_order(blockIdx.x, gridDim.x);
   const int per = g.tiles_m * g.tiles_n;
   const int z = tile / per, tt = tile - z * per;
-  const int64_t m0 = (int64_t)(tt / g.tiles_n) * BM, n0 = (int64_t)(tt % g.tiles_n) * BN;
+  // four rows of tiles at a time, so that the 32 tiles of an XCD read about 4 x 8 tiles' operands
+  const int band = tt / (4 * g.tiles_n), in = tt - band * 4 * g.tiles_n, hi = min(4, g.tiles_m - 4 * band);
+  const int64_t m0 = (int64_t)(4 * band + in % hi) * BM, n0 = (int64_t)(in / hi) * BN;
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   OA a;
   OB b;
-  a.init(g.a, g.lda, m0, g.M);
-  b.init(g.b, g.ldb, n0, g.N);
+  a.init(g.a, g.lda, m0, g.M, wm);
+  b.init(g.b, g.ldb, n0, g.N, wn);
   v4f acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-  LinSteps at(g, z, BK);
-  const uint32_t l0 = lds_addr(lds[0]), l1 = lds_addr(lds[1]);
-  auto load = [&](int buf) {
-    const uint32_t to = buf ? l1 : l0;
-    a.load(to, at.k, g.K, at.p * g.plane);
-    b.load(to + OA::BYTES, at.k, g.K, 0);
+  LinSteps at(g, z, DMA_BK);  // the step to be asked for
+  const uint32_t l0 = lds_addr(lds);
+  const int64_t steps = at.left;
+  int left = (int)min(g.K - at.k, (int64_t)DMA_BK);
+  auto next = [&] {
+    at.next(DMA_BK);
+    left = at.left > 0 ? (int)min(g.K - at.k, (int64_t)DMA_BK) : 0;
   };
-  load(0);
-  for (int buf = 0;; buf ^= 1) {
-    const bool more = at.next(BK);
-    wait_barrier<0>();  // this step's tiles have landed for all waves, and all have read the other buffer's
-    if (more) load(buf ^ 1);
-    const uint16_t *la = lds[buf], *lb = la + OA::BYTES / 2;
+  auto load = [&](uint32_t to) {
+    const v4u_t ra = a.source(at.k, at.p * g.plane), rb = b.source(at.k, 0);
 #pragma unroll
-    for (int s = 0; s < BK / 32; ++s) {
-      v8bf fa[FM], fb[FN];
+    for (int i = 0; i < OA::PER; ++i) a.ask(ra, to, i, left);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = OA::frag(la, wm + 16 * i, s);
+    for (int i = 0; i < OB::PER; ++i) b.ask(rb, to + OA::BYTES, i, left);
+    next();
+  };
+  auto row = [&](int i, const v8bf &fa, const v8bf (&fb)[FN]) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = OB::frag(lb, wn + 16 * j, s);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          if constexpr (F16)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, fb[j]), __builtin_bit_cast(v8h, fa[i]),
-                                                              acc[i][j], 0, 0, 0);
-          else
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
-        }
+    for (int j = 0; j < FN; ++j) {
+      if constexpr (F16)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, fb[j]), __builtin_bit_cast(v8h, fa),
+                                                          acc[i][j], 0, 0, 0);
+      else
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa, acc[i][j], 0, 0, 0);
     }
-    if (!more) break;
+  };
+  // Step t lies in one buffer, step t + 1 lands in the other.  While the step's first half is multiplied its second
+  // half is read; then all waves have read the buffer and step t + 1 has landed, and while the second half is multiplied
+  // the first half of step t + 1 is read and step t + 2 asked for, into the buffer that is free.
+  load(l0);
+  wait_barrier<0>();
+  load(l0 + BYTES);
+  v8bf a0[FM], b0[FN], a1[FM], b1[FN];
+#pragma unroll
+  for (int j = 0; j < FN; ++j) b0[j] = b.frag(l0 + OA::BYTES, j, 0);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) a0[i] = a.frag(l0, i, 0);
+  uint32_t cur = l0, other = l0 + BYTES;
+  // the fragments of half s in the buffer at `from`, a few behind each row of products, the first ones needed first
+  auto read = [&](int i, v8bf (&fa)[FM], v8bf (&fb)[FN], uint32_t from, int s) {
+    constexpr int EACH = (FM + FN + FM / 2 - 1) / (FM / 2);
+#pragma unroll
+    for (int q = i * EACH; q < (i + 1) * EACH && q < FM + FN; ++q) {
+      if (q < FN) fb[q] = b.frag(from + OA::BYTES, q, s);
+      else fa[q - FN] = a.frag(from, q - FN, s);
+    }
+  };
+  for (int64_t t = 0; t < steps; ++t) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      row(i, a0[i], b0);
+      __builtin_amdgcn_sched_barrier(0);
+      read(i, a1, b1, cur, 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_barrier<0>();
+    const v4u_t ra = a.source(at.k, at.p * g.plane), rb = b.source(at.k, 0);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      row(i, a1[i], b1);
+      __builtin_amdgcn_sched_barrier(0);
+      read(i, a0, b0, other, 0);
+#pragma unroll
+      for (int q = i * OA::PER / FM; q < (i + 1) * OA::PER / FM; ++q) a.ask(ra, cur, q, left);
+#pragma unroll
+      for (int q = i * OB::PER / FM; q < (i + 1) * OB::PER / FM; ++q) b.ask(rb, cur + OA::BYTES, q, left);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    next();
+    const uint32_t swap = cur;
+    cur = other;
+    other = swap;
   }
+  wait_vm<0>();  // (what was asked for past the end writes zeros: not into another workgroup's LDS)
   const int fr = lane & 15, fc = lane >> 4;
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -951,8 +1007,8 @@ void lin_few_of(const LinArgs &g, hipStream_t st) {
   else lin_few_rows<TX, NX, TW, NW, 4>(g, st);
 }
 
-// The launch of one kernel instance.  `tile`: 0 = 128 x 128, 1 = 32 x 128, 2 = 256 x 256 (16-bit operands); operands
-// without 16-byte loads (`vec` false) take 32 x 128.
+// The launch of one kernel instance.  `tile`: 0 = 128 x 128, 1 = 32 x 128, for 16-bit operands 2 = 256 x 256 and
+// 3 = 256 x 128; operands without 16-byte loads (`vec` false) take 32 x 128.
 template <class TA, int NA, bool KCA, class TB, int NB, bool KCB>
 void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices));
@@ -963,7 +1019,8 @@ void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
   } else if constexpr (std::is_same<TA, TB>::value && sizeof(TA) == 2) {
     constexpr bool F16 = std::is_same<TA, _Float16>::value;
     if (tile == 2) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 256, 2, 4>), grid, dim3(512), 0, st, g);
-    else hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
+    else if (tile == 3) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 128, 4, 2>), grid, dim3(512), 0, st, g);
+    else hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 128, 128, 2, 4>), grid, dim3(512), 0, st, g);
   } else {
     hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 2, true>), grid, dim3(256), 0, st, g);
   }
