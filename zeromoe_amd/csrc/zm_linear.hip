@@ -111,8 +111,10 @@ struct Plan {
 // the kernels of a product, by its rows and by whether its operands can be read 16 bytes at a time
 enum Kind { ROWS, FEW, TILES };
 
-// `step`: k of a step of the tiles; `dma`: 16-bit operands of one type
-Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int step, bool dma, bool vec, size_t most) {
+// `products`: of terms, for each product of values; 1: 16-bit operands of one type, which go straight into LDS
+Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, bool vec, size_t most) {
+  const bool dma = products == 1;
+  const int step = dma ? DMA_BK : 32;
   Plan p{};
   p.kind = kind;
   int64_t z = 1, bk = 64;
@@ -129,38 +131,42 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int step, bool
     const size_t plane = (size_t)M * N * 4;
     p.tile = !vec || M <= 64;
     int bm = p.tile ? 32 : 128, bn = 128;
-    if (dma && !p.tile) {
-      // The cheapest of three tiles and some numbers of slices, by what they measured: us of a step in which every CU
-      // has one tile of 256 x 256, one of 256 x 128, one of 128 x 128 and two of 128 x 128; and a join of the slices
-      // at 5 TB/s with 4 us to start.
+    if (p.tile) {
+      // 32 x 128 for up to 64 rows; k in as many slices as give two workgroups per CU, at least 256 of it each
+      const int64_t tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+      z = std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), planes * K / 256);
+      z = std::max<int64_t>(1, std::min<int64_t>(z, (int64_t)(most / plane)));
+    } else {
+      // The cheapest tile and number of slices by what they measured: us of a step with one tile a CU and, where two
+      // fit, with two; and a join of the slices at 5 TB/s with 4 us to start.
+      struct Tile {
+        int kind, bm, bn;
+        double one, two;
+      };
+      static const Tile dma_tiles[] = {{2, 256, 256, 1.9, 0}, {3, 256, 128, 1.04, 0}, {0, 128, 128, 0.75, 1.09}};
+      static const Tile term_tiles[] = {{0, 128, 128, 1.0, 1.5}, {0, 128, 128, 1.2, 2.1}, {0, 128, 128, 1.3, 0}};
+      const Tile *first = dma ? dma_tiles : term_tiles + (products <= 3 ? 0 : products <= 5 ? 1 : 2);
       double best = 1e30;
-      for (int tile : {2, 3, 0}) {
-        const int64_t h = tile ? 256 : 128, w = tile == 2 ? 256 : 128;
-        const int64_t tiles = ((M + h - 1) / h) * ((N + w - 1) / w);
-        for (int64_t s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      for (const Tile *t = first; t < first + (dma ? 3 : 1); ++t) {
+        const int64_t tiles = ((M + t->bm - 1) / t->bm) * ((N + t->bn - 1) / t->bn);
+        for (int64_t s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
           if (s > 1 && (s * plane > most || steps < 4 * s || tiles * s > 1024)) break;
           const int64_t n = tiles * s;
-          const double rounds = tile ? (double)((n + 255) / 256) * (tile == 2 ? 1.9 : 1.04)
-                                     : n / 512 * 1.09 + (n % 512 > 256 ? 1.09 : n % 512 ? 0.75 : 0.0);
+          const double rounds = t->two ? n / 512 * t->two + (n % 512 > 256 ? t->two : n % 512 ? t->one : 0.0)
+                                       : (double)((n + 255) / 256) * t->one;
           const double us = rounds * (double)((steps + s - 1) / s) + (s > 1 ? 4.0 + s * plane * 2 / 5e6 : 0.0);
           if (us < best) {
             best = us;
             z = s;
-            p.tile = tile;
-            bm = (int)h;
-            bn = (int)w;
+            p.tile = t->kind;
+            bm = t->bm;
+            bn = t->bn;
           }
         }
       }
     }
     p.tiles_m = (int)((M + bm - 1) / bm);
     p.tiles_n = (int)((N + bn - 1) / bn);
-    if (!dma || p.tile == 1) {
-      // 128 x 128, or 32 x 128 for up to 64 rows; k in as many slices as give about two workgroups per CU (at least
-      // 256 of k each)
-      z = std::min<int64_t>(512 / std::max<int64_t>((int64_t)p.tiles_m * p.tiles_n, 1), planes * K / 256);
-      z = std::max<int64_t>(1, std::min<int64_t>(z, (int64_t)(most / plane)));
-    }
     p.kslice = (steps + z - 1) / z;
     p.slices = (int)((steps + p.kslice - 1) / p.kslice);
     p.part = p.slices > 1 ? (size_t)p.slices * plane : 0;
@@ -194,11 +200,11 @@ struct Product {
   bool forward;  // the product has kernels for few rows
   Kind kind(bool vec) const {
     if (!vec || !forward || N >= (1 << 26) || K >= (1 << 30)) return TILES;
-    return M <= LIN_ROWS ? ROWS : M <= LIN_FEW ? FEW : TILES;
+    return M <= LIN_ROWS ? ROWS : lin_few_rows(M, N) ? FEW : TILES;
   }
   Plan plan_for(bool vec, size_t most) const {
-    const bool dma = a_type == b_type && a_type != LIN_F32;
-    return plan(kind(vec), M, N, K, planes, dma ? DMA_BK : 32, dma, vec, most);
+    const int f32_by = b_type == LIN_BF16 ? 3 : b_type == LIN_F16 ? 5 : 6;
+    return plan(kind(vec), M, N, K, planes, a_type == LIN_F32 ? f32_by : 1, vec, most);
   }
   // partial sums of at most 64 MB
   size_t space() const { return plan_for(shaped, 64 << 20).part; }

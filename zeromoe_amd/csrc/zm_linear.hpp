@@ -210,8 +210,8 @@ static inline void parts_sum(const float *part, int parts, int64_t n, int64_t n0
 // eight apart, which a row-contiguous operand writes together, fall apart too.
 //
 // A unit is one thread's part: 8 consecutive k of one row where k is contiguous
-// in memory (KC), else 16 bytes of rows for each of 8 consecutive k, transposed
-// in registers.
+// in memory (KC), else 4 bytes of rows (one f32, two 16-bit) for each of 8 consecutive k, transposed in registers:
+// small enough for every thread to have its share of the splitting into terms.
 template <int BK>
 __device__ __forceinline__ int chunk_at(int row, int c) {
   if (BK == 128) return c ^ (row & 15);
@@ -221,29 +221,29 @@ __device__ __forceinline__ int chunk_at(int row, int c) {
 
 template <class T, int NT, bool KC, int ROWS, int BK, int NTHR, bool VEC>
 struct Operand {
-  static constexpr int R = KC ? 1 : 16 / (int)sizeof(T);  // rows of a unit
+  static constexpr int R = KC ? 1 : 4 / (int)sizeof(T);  // rows of a unit
   static constexpr int CH = BK / 8;
   static constexpr int UNITS = ROWS / R * CH;
   static constexpr int UPT = UNITS > NTHR ? UNITS / NTHR : 1;
-  static constexpr int NV = KC ? (int)sizeof(T) / 2 : 8;  // 16-byte registers of a unit
+  static constexpr int NW = KC ? 2 * (int)sizeof(T) : 8;  // words of a unit
   static constexpr int PLANE = ROWS * BK;                 // 16-bit values of a term plane
   static_assert(UNITS % NTHR == 0 || UNITS < NTHR, "units split evenly over the threads");
 
   const T *base;  // the tile's first row
   int64_t ld;
   int rows;       // of the matrix, from the tile's first row
-  int first;      // the thread's first unit
-  bool on;
+  int first;      // the thread's first unit (where there are fewer units than threads some are loaded and stored twice)
   int off[UPT];   // bytes from the tile's first row and column (16-byte loads)
-  v4u raw[UPT][NV];
+  struct Raw {    // a step of the tile as it came from memory: the thread's units
+    uint32_t r[UPT][NW];
+  };
 
   // `row0`: the tile's first row; `total`: rows of the matrix
   __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t total, int t) {
     ld = ld_;
     base = (const T *)p + (KC ? row0 * ld : row0);
     rows = (int)(total - row0 < ROWS ? total - row0 : ROWS);
-    on = t >= 0 && t < UNITS;
-    first = t;
+    first = t % UNITS;
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       int row, c;
@@ -261,10 +261,9 @@ struct Operand {
       c = u / (ROWS / R);
     }
   }
-  // columns [k, k + BK) of the tile, `skip` values on, zeros from `kend` on; rows past the matrix
+  // columns [k, k + left) of the tile, `skip` values on, and zeros; rows past the matrix
   // repeat its last ones (their results are not stored)
-  __device__ __forceinline__ void load(int64_t k, int64_t kend, int64_t skip) {
-    const int left = (int)min(kend - k, (int64_t)BK);
+  __device__ __forceinline__ void load(Raw &to, int64_t k, int left, int64_t skip) const {
     const T *at = base + skip + (KC ? k : k * ld);
     const rsrc_t r = buf_at(at);
 #pragma unroll
@@ -272,20 +271,24 @@ struct Operand {
       int row, c;
       place(first + i * NTHR, row, c);
       if constexpr (VEC && KC) {
-        const int vo = on && 8 * c < left ? off[i] : OOR;
+        const int vo = 8 * c < left ? off[i] : OOR;
 #pragma unroll
-        for (int q = 0; q < NV; ++q) raw[i][q] = buf16(r, vo, 16 * q);
+        for (int q = 0; q < NW / 4; ++q) {
+          const v4u v = buf16(r, vo, 16 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to.r[i][4 * q + j] = v[j];
+        }
       } else if constexpr (VEC) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          raw[i][j] = buf16(r, on && 8 * c + j < left ? off[i] : OOR, j * (int)ld * (int)sizeof(T));
-      } else if (on) {
+          to.r[i][j] = bld4(r, 8 * c + j < left ? off[i] : OOR, j * (int)ld * (int)sizeof(T));
+      } else {
         if constexpr (KC) {
           const T *p = at + (int64_t)min(row, rows - 1) * ld + 8 * c;
           T e[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) e[j] = 8 * c + j < left ? p[j] : from_f32<T>(0.f);
-          __builtin_memcpy(raw[i], e, sizeof(e));
+          __builtin_memcpy(to.r[i], e, sizeof(e));
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -293,77 +296,49 @@ struct Operand {
             T e[R];
 #pragma unroll
             for (int q = 0; q < R; ++q) e[q] = 8 * c + j < left ? p[min(row + q, rows - 1)] : from_f32<T>(0.f);
-            __builtin_memcpy(&raw[i][j], e, sizeof(e));
+            __builtin_memcpy(&to.r[i][j], e, 4);
           }
         }
       }
     }
   }
-  __device__ __forceinline__ void put(uint16_t *lds, int row, int c, v8bf (&t)[NT]) const {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      *reinterpret_cast<v8bf *>(lds + n * PLANE + row * BK + chunk_at<BK>(row, c) * 8) = t[n];
-  }
-  __device__ __forceinline__ void store(uint16_t *lds) const {
+  __device__ __forceinline__ void store(uint16_t *lds, const Raw &from) const {
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       int row, c;
       place(first + i * NTHR, row, c);
-      if (!on) continue;
-      if constexpr (KC && sizeof(T) == 2) {
-        if constexpr (NT == 1) {
-          *reinterpret_cast<v4u *>(lds + row * BK + chunk_at<BK>(row, c) * 8) = raw[i][0];
-        } else {
-          T e[8];
-          float v[8];
-          __builtin_memcpy(e, raw[i], sizeof(e));
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
-          v8bf t[NT];
-          split_terms<T, NT>(v, t);
-          put(lds, row, c, t);
-        }
-      } else if constexpr (KC) {
-        float v[8];
-        __builtin_memcpy(v, raw[i], sizeof(v));
-        v8bf t[NT];
-        split_terms<T, NT>(v, t);
-        put(lds, row, c, t);
-      } else if constexpr (sizeof(T) == 2) {
-        // raw[j] holds rows (0,1)(2,3)(4,5)(6,7) at column j; row 2q + h: its halves of the eight columns
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            v4u o;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              o[j] = __builtin_amdgcn_perm(raw[i][2 * j + 1][q], raw[i][2 * j][q], h ? 0x07060302u : 0x05040100u);
-            const int r = row + 2 * q + h;
-            if constexpr (NT == 1) {
-              *reinterpret_cast<v4u *>(lds + r * BK + chunk_at<BK>(r, c) * 8) = o;
-            } else {
-              T e[8];
-              float v[8];
-              __builtin_memcpy(e, &o, sizeof(e));
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
-              v8bf t[NT];
-              split_terms<T, NT>(v, t);
-              put(lds, r, c, t);
-            }
-          }
+      if constexpr (KC) {
+        put8(lds, row, c, from.r[i]);
+      } else if constexpr (sizeof(T) == 4) {
+        put8(lds, row, c, from.r[i]);
       } else {
+        // word j holds rows 0 and 1 at column j
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float v[8];
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[4];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw[i][j][r]);
-          v8bf t[NT];
-          split_terms<T, NT>(v, t);
-          put(lds, row + r, c, t);
+          for (int j = 0; j < 4; ++j)
+            o[j] = __builtin_amdgcn_perm(from.r[i][2 * j + 1], from.r[i][2 * j], h ? 0x07060302u : 0x05040100u);
+          put8(lds, row + h, c, o);
         }
       }
+    }
+  }
+  // 8 values of one row, as they came, into the planes
+  __device__ __forceinline__ void put8(uint16_t *lds, int row, int c, const uint32_t *w) const {
+    uint16_t *at = lds + row * BK + chunk_at<BK>(row, c) * 8;
+    if constexpr (NT == 1 && sizeof(T) == 2) {
+      *reinterpret_cast<v4u *>(at) = v4u{w[0], w[1], w[2], w[3]};
+    } else {
+      T e[8];
+      float v[8];
+      __builtin_memcpy(e, w, sizeof(e));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+      v8bf t[NT];
+      split_terms<T, NT>(v, t);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) *reinterpret_cast<v8bf *>(at + n * PLANE) = t[n];
     }
   }
 };
@@ -463,10 +438,11 @@ struct Pairs {
   static constexpr int MOST = 2;  // i + j
 };
 
-// One workgroup: BM x BN results over one slice of k; WM x WN waves of 16 x 16
-// matrix instructions.  The next tile's global loads are in flight while the
-// current one is multiplied.  The instruction's rows are the results' columns n,
-// so that a lane ends with 4 neighbouring n of one row m.
+// One workgroup: BM x BN results over one slice of k; WM x WN waves of 16 x 16 matrix instructions.  Two steps of BK
+// deep in LDS: while one is multiplied, the next one, in registers, is split into terms and stored, and the one after
+// that is on its way from memory; one barrier a step.  The instruction's rows are the results' columns n, so that a
+// lane ends with 4 neighbouring n of one row m.  f32 by f32, 2048^3: 95 us, 181 TFLOP/s of f32 products (1085 of bf16
+// ones), against 103 us with one buffer, the splitting in front of the products and two workgroups a CU.
 template <class TA, int NA, bool KCA, class TB, int NB, bool KCB, int BM, int BN, int WM, int WN, bool VEC>
 __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
   constexpr bool F16 = std::is_same<TA, _Float16>::value && std::is_same<TB, _Float16>::value && NA == 1 && NB == 1;
@@ -475,8 +451,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   typedef Operand<TA, NA, KCA, BM, BK, NTHR, VEC> OA;
   typedef Operand<TB, NB, KCB, BN, BK, NTHR, VEC> OB;
-  __shared__ __attribute__((aligned(16))) uint16_t lds_a[NA * BM * BK];
-  __shared__ __attribute__((aligned(16))) uint16_t lds_b[NB * BN * BK];
+  constexpr int LA = NA * BM * BK, LDS = LA + NB * BN * BK;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tile = xcd_order(blockIdx.x, gridDim.x);
   const int per = g.tiles_m * g.tiles_n;
@@ -485,8 +461,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
   OA a;
   OB b;
   a.init(g.a, g.lda, m0, g.M, tid);
-  // an operand with fewer units than threads is loaded by the last threads: the other one's units are with the first
-  b.init(g.b, g.ldb, n0, g.N, OB::UNITS < NTHR ? tid - (NTHR - OB::UNITS) : tid);
+  b.init(g.b, g.ldb, n0, g.N, tid);
   v4f acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -494,18 +469,20 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
     for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const int fr = lane & 15, fc = lane >> 4;
-  LinSteps at(g, z, BK);
-  auto load = [&] {
-    a.load(at.k, g.K, at.p * g.plane);
-    b.load(at.k, g.K, 0);
+  LinSteps at(g, z, BK);  // the step to be asked for
+  const int64_t steps = at.left;
+  struct Raw {
+    typename OA::Raw a;
+    typename OB::Raw b;
   };
-  load();
-  for (;;) {
-    a.store(lds_a);
-    b.store(lds_b);
-    __syncthreads();
-    const bool more = at.next(BK);
-    if (more) load();
+  auto load = [&](Raw &to) {  // zeros behind the last step
+    const int left = at.left > 0 ? (int)min(g.K - at.k, (int64_t)BK) : 0;
+    a.load(to.a, at.k, left, at.p * g.plane);
+    b.load(to.b, at.k, left, 0);
+    at.next(BK);
+  };
+  auto step = [&](const uint16_t *from, uint16_t *to, const Raw &next, Raw &after) {
+    load(after);
 #pragma unroll
     for (int s = 0; s < BK / 32; ++s) {
       v8bf fa[FM][NA], fb[FN][NB];
@@ -514,14 +491,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
         const int r = wm + 16 * i + fr;
 #pragma unroll
         for (int t = 0; t < NA; ++t)
-          fa[i][t] = *reinterpret_cast<const v8bf *>(lds_a + t * BM * BK + r * BK + chunk_at<BK>(r, 4 * s + fc) * 8);
+          fa[i][t] = *reinterpret_cast<const v8bf *>(from + t * BM * BK + r * BK + chunk_at<BK>(r, 4 * s + fc) * 8);
       }
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         const int r = wn + 16 * j + fr;
 #pragma unroll
         for (int t = 0; t < NB; ++t)
-          fb[j][t] = *reinterpret_cast<const v8bf *>(lds_b + t * BN * BK + r * BK + chunk_at<BK>(r, 4 * s + fc) * 8);
+          fb[j][t] = *reinterpret_cast<const v8bf *>(from + LA + t * BN * BK + r * BK + chunk_at<BK>(r, 4 * s + fc) * 8);
+      }
+      if (s == BK / 32 - 1) {
+        a.store(to, next.a);
+        b.store(to + LA, next.b);
       }
 #pragma unroll
       for (int ta = 0; ta < NA; ++ta)
@@ -540,8 +521,27 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
             }
         }
     }
-    if (!more) break;
+
+    if (NA * NB > 1) {
+      // the splitting into terms goes between the products, which leave the vector units three of four issues
+#pragma unroll
+      for (int i = 0; i < FM * FN * NA * NB; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
+      }
+    }
     __syncthreads();
+  };
+  Raw p, q;
+  load(p);
+  load(q);
+  a.store(lds[0], p.a);
+  b.store(lds[0] + LA, p.b);
+  __syncthreads();
+  for (int64_t t = 0; t < steps; t += 2) {
+    step(lds[0], lds[1], q, p);
+    if (t + 1 >= steps) break;
+    step(lds[1], lds[0], p, q);
   }
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -888,7 +888,11 @@ __device__ __forceinline__ void terms_of(const Eight<T> &e, v8bf (&t)[NT]) {
   }
 }
 
-constexpr int LIN_FEW = 128, FEW_ROWS = 64;
+constexpr int FEW_ROWS = 64;
+// where it is the faster one (us, tiles -> this): w of 256 x 7168 f32, 192 rows 25.1 -> 16.6, 384 rows 28.7 -> 22.3,
+// 1024 rows 35.5 -> 36.9; w of 4096 x 4096 bf16, 128 rows 23.4 -> 25.3, 192 rows 26.7 -> 37.7; w of 1536 x 4096 bf16
+// under f32 rows, 128 rows 27.1 -> 24.5, 256 rows 31.8 -> 31.1
+inline bool lin_few_rows(int64_t M, int64_t N) { return M <= 128 || (M <= 384 && N <= 512); }
 constexpr int FEW_UNIT = 128;  // a slice is a multiple of it: one unit of a 16-bit w, two of an f32 one
 template <class TX, int NX, class TW, int NW, int MT, int NF, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
@@ -992,7 +996,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
 // 128; 32 for each wave where the rows are many too
 inline int few_columns(int64_t M, int64_t N) { return M <= 32 ? (N < 2048 ? 64 : 128) : (N < 4096 ? 128 : 256); }
 template <class TX, int NX, class TW, int NW, int MT>
-void lin_few_rows(const LinArgs &g, hipStream_t st) {
+void lin_few_launch(const LinArgs &g, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices));
   switch (few_columns(g.M, g.N)) {
   case 64: hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, MT, 1, 4>), grid, dim3(256), 0, st, g); break;
@@ -1002,9 +1006,9 @@ void lin_few_rows(const LinArgs &g, hipStream_t st) {
 }
 template <class TX, int NX, class TW, int NW>
 void lin_few_of(const LinArgs &g, hipStream_t st) {
-  if (g.M <= 16) lin_few_rows<TX, NX, TW, NW, 1>(g, st);
-  else if (g.M <= 32) lin_few_rows<TX, NX, TW, NW, 2>(g, st);
-  else lin_few_rows<TX, NX, TW, NW, 4>(g, st);
+  if (g.M <= 16) lin_few_launch<TX, NX, TW, NW, 1>(g, st);
+  else if (g.M <= 32) lin_few_launch<TX, NX, TW, NW, 2>(g, st);
+  else lin_few_launch<TX, NX, TW, NW, 4>(g, st);
 }
 
 // The launch of one kernel instance.  `tile`: 0 = 128 x 128, 1 = 32 x 128, for 16-bit operands 2 = 256 x 256 and
@@ -1015,20 +1019,20 @@ void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
   if (!vec) {
     hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 4, false>), grid, dim3(256), 0, st, g);
   } else if (tile == 1) {
-    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 4, true>), grid, dim3(256), 0, st, g);
+    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 8, true>), grid, dim3(512), 0, st, g);
   } else if constexpr (std::is_same<TA, TB>::value && sizeof(TA) == 2) {
     constexpr bool F16 = std::is_same<TA, _Float16>::value;
     if (tile == 2) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 256, 2, 4>), grid, dim3(512), 0, st, g);
     else if (tile == 3) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 128, 4, 2>), grid, dim3(512), 0, st, g);
     else hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 128, 128, 2, 4>), grid, dim3(512), 0, st, g);
   } else {
-    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 2, true>), grid, dim3(256), 0, st, g);
+    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 4, true>), grid, dim3(512), 0, st, g);
   }
 }
 
 // the products by what their operands are: forward (x, w), dx (dz, w), dw (dz, x)
 void lin_rows(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // M <= LIN_ROWS, operands with 16-byte loads
-void lin_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);   // M <= LIN_FEW, likewise
+void lin_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);   // where lin_few_rows(), likewise
 void lin_fwd(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dx(int x_type, int w_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dw(int x_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
