@@ -17,33 +17,30 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigm
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _F32, _I32 = torch.float32, torch.int32
 _F32S, _I32S = (_F32,), (_I32,)
+_ROWS = torch.contiguous_format
 
 
-# the current stream's handle without a Stream object around it: 0.1 us of a call's 7, against 1.1
+# the current stream's handle without a Stream object around it, and the current device: 0.1 us each of a call's 7,
+# against 1.1 and 0.3
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _on(fn):
-    """Runs the call where its first tensor lies and on `stream`, whose allocations are then that stream's."""
-    name = fn.__code__.co_varnames[2]
+def _index(t: torch.Tensor, who: str) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{who}: device tensors are needed")
+    return t.get_device()
 
-    def call(*args, stream=None, **kw):
-        first = args[0] if args else kw.get(name)
-        if not isinstance(first, torch.Tensor) or not first.is_cuda:
-            raise ValueError(f"{fn.__name__}: device tensors are needed")
-        d = first.get_device()
-        if stream is None:
-            if d == torch.cuda.current_device():
-                return fn(_raw_stream(d), d, *args, **kw)
-            with torch.cuda.device(d):
-                return fn(_raw_stream(d), d, *args, **kw)
-        if stream.device.index != d:
-            raise ValueError(f"{fn.__name__}: the stream belongs to another device than the tensors")
-        with torch.cuda.stream(stream):
-            return fn(stream.cuda_stream, d, *args, **kw)
 
-    call.__name__, call.__qualname__, call.__doc__, call.__wrapped__ = fn.__name__, fn.__qualname__, fn.__doc__, fn
-    return call
+def _there(fn, d: int, stream, *args):
+    """The call on the device of its tensors and on `stream`, whose allocations are then that stream's."""
+    if stream is None:
+        with torch.cuda.device(d):
+            return fn(*args)
+    if stream.device.index != d:
+        raise ValueError(f"{fn.__name__}: the stream belongs to another device than the tensors")
+    with torch.cuda.stream(stream):
+        return fn(*args)
 
 
 def _need(t: torch.Tensor, what: str, d: int, dtypes, shape) -> torch.Tensor:
@@ -103,14 +100,18 @@ def _linear_types(d, x, w):
         raise ValueError("w needs contiguous columns")
 
 
-@_on
-def linear(st, d, x: torch.Tensor, w: torch.Tensor, bias=None, act: str = "none", residual=None, out=None, out_dtype=None,
-           save_pre: bool = False):
+def linear(x: torch.Tensor, w: torch.Tensor, bias=None, act: str = "none", residual=None, out=None, out_dtype=None,
+           save_pre: bool = False, stream=None):
     """act(x w^T + bias) + residual: x (S, I), w (O, I), bias (O) float32, residual (S, O) of the result's type.
 
     x float32 with w float32, float16 or bfloat16, or both float16 or both bfloat16; the result is of x's type or
     float32 (`out_dtype`, or `out`'s type).  act: none, relu, gelu, gelu_tanh, silu, sigmoid.  `out` may be `residual`
-    itself, and overlaps no other operand.  save_pre: also returns x w^T + bias, in the result's type, for linear_backward.  (zm_linear)"""
+    itself, and overlaps no other operand.  save_pre: also returns x w^T + bias, in the result's type, for
+    linear_backward.  (zm_linear)"""
+    d = _index(x, "linear")
+    if stream is not None or d != _device():
+        return _there(linear, d, stream, x, w, bias, act, residual, out, out_dtype, save_pre)
+    st = _raw_stream(d)
     _linear_types(d, x, w)
     S, I = x.shape
     O = w.shape[0]
@@ -132,12 +133,15 @@ def linear(st, d, x: torch.Tensor, w: torch.Tensor, bias=None, act: str = "none"
     return (y, pre) if save_pre else y
 
 
-@_on
-def linear_backward(st, d, dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str = "none", pre=None,
-                    need_dx: bool = True, need_dw: bool = True, need_dbias: bool = True):
+def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str = "none", pre=None,
+                    need_dx: bool = True, need_dw: bool = True, need_dbias: bool = True, stream=None):
     """(dx, dw, dbias) of linear() for dy (S, O), its gradient by the result: dx (S, I) of x's type, dw (O, I) and
     dbias (O) float32; None in the place of one that is not needed.  The residual's gradient is dy itself.  pre: what
     linear(save_pre=True) returned, needed with an activation.  (zm_linear_backward)"""
+    d = _index(dy, "linear_backward")
+    if stream is not None or d != _device():
+        return _there(linear_backward, d, stream, dy, x, w, act, pre, need_dx, need_dw, need_dbias)
+    st = _raw_stream(d)
     _linear_types(d, x, w)
     S, I = x.shape
     O = w.shape[0]
@@ -171,15 +175,18 @@ def _norm_rows(d, x):
         raise ValueError(f"x is {x.dtype}: float32, float16 or bfloat16 needed")
 
 
-@_on
-def layer_norm(st, d, x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=None, stats: bool = False):
+def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=None, stats: bool = False, stream=None):
     """(x - mean) / sqrt(variance + eps) * weight + bias over the rows of x (rows, n), in x's type; weight and bias (n)
     float32.  `out` may be x itself.  stats: also returns each row's mean and 1 / sqrt(variance + eps), for
     layer_norm_backward.  (zm_layer_norm)"""
+    d = _index(x, "layer_norm")
+    if stream is not None or d != _device():
+        return _there(layer_norm, d, stream, x, weight, bias, eps, out, stats)
+    st = _raw_stream(d)
     _norm_rows(d, x)
     rows, n = x.shape
     x = _rows(x)
-    y = x.new_empty((rows, n)) if out is None else _out(out, "out", d, x.dtype, (rows, n))
+    y = torch.empty_like(x, memory_format=_ROWS) if out is None else _out(out, "out", d, x.dtype, (rows, n))
     weight, bias = _vector(weight, "weight", d, n), _vector(bias, "bias", d, n)
     mean = rstd = None
     if stats:
@@ -189,18 +196,21 @@ def layer_norm(st, d, x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5
     return (y, mean, rstd) if stats else y
 
 
-@_on
-def layer_norm_backward(st, d, dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight=None,
-                        need_dx: bool = True, need_dweight: bool = True, need_dbias: bool = True):
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight=None,
+                        need_dx: bool = True, need_dweight: bool = True, need_dbias: bool = True, stream=None):
     """(dx, dweight, dbias) of layer_norm() for dy (rows, n) of x's type, with the statistics that it returned: dx of
     x's type, dweight and dbias (n) float32; None in the place of one that is not needed.  (zm_layer_norm_backward)"""
+    d = _index(dy, "layer_norm_backward")
+    if stream is not None or d != _device():
+        return _there(layer_norm_backward, d, stream, dy, x, mean, rstd, weight, need_dx, need_dweight, need_dbias)
+    st = _raw_stream(d)
     _norm_rows(d, x)
     rows, n = x.shape
     x = _rows(x)
     dy = _rows(_need(dy, "dy", d, (x.dtype,), (rows, n)))
     mean, rstd = _vector(mean, "mean", d, rows), _vector(rstd, "rstd", d, rows)
     weight = _vector(weight, "weight", d, n)
-    dx = x.new_empty((rows, n)) if need_dx else None
+    dx = torch.empty_like(x, memory_format=_ROWS) if need_dx else None
     dw = x.new_empty(n, dtype=_F32) if need_dweight else None
     db = x.new_empty(n, dtype=_F32) if need_dbias else None
     L = lib()
@@ -217,11 +227,14 @@ def _routes(y):
     return _rows(y)
 
 
-@_on
-def combine(st, d, y: torch.Tensor, weights: torch.Tensor, ids=None, residual=None, out=None):
+def combine(y: torch.Tensor, weights: torch.Tensor, ids=None, residual=None, out=None, stream=None):
     """residual + sum over k of weights[:, k] * y[:, k]: the experts' rows y (S, K, H) as mul_mat_id returns them,
     weights (S, K), residual (S, H) and the result, all float32.  A route with a negative id in ids (S, K) int32 takes
     no part.  `out` may be `residual` itself.  (zm_combine)"""
+    d = _index(y, "combine")
+    if stream is not None or d != _device():
+        return _there(combine, d, stream, y, weights, ids, residual, out)
+    st = _raw_stream(d)
     y = _routes(y)
     S, K, H = y.shape
     weights = _flat(_need(weights, "weights", d, _F32S, (S, K)))
@@ -238,11 +251,14 @@ def combine(st, d, y: torch.Tensor, weights: torch.Tensor, ids=None, residual=No
     return out
 
 
-@_on
-def combine_backward(st, d, dout: torch.Tensor, y: torch.Tensor, weights=None, ids=None, need_dy: bool = False):
+def combine_backward(dout: torch.Tensor, y: torch.Tensor, weights=None, ids=None, need_dy: bool = False, stream=None):
     """dweights (S, K) of combine() for dout (S, H): the dot products of dout with the experts' rows, 0 for a route with
     a negative id.  need_dy: (dweights, dy), dy (S, K, H) = weights * dout, which needs weights.  The residual's
     gradient is dout itself.  (zm_combine_backward)"""
+    d = _index(dout, "combine_backward")
+    if stream is not None or d != _device():
+        return _there(combine_backward, d, stream, dout, y, weights, ids, need_dy)
+    st = _raw_stream(d)
     y = _routes(y)
     S, K, H = y.shape
     if y.get_device() != d:
@@ -261,13 +277,17 @@ def combine_backward(st, d, dout: torch.Tensor, y: torch.Tensor, weights=None, i
     return (dweights, dy) if need_dy else dweights
 
 
-@_on
-def router_backward(st, d, logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Tensor, gating="softmax",
-                    logit_bias=None, weights_norm: bool = False, weights_scale: float = 0.0, dprobs=None):
+def router_backward(logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Tensor, gating="softmax",
+                    logit_bias=None, weights_norm: bool = False, weights_scale: float = 0.0, dprobs=None, stream=None):
     """The gradient of router()'s weights by its logits (S, E) float32, the selection held fixed: ids (S, K) int32 are
     expert ids (router() without a slot table), dweights (S, K).  A negative id takes no part; a row of them alone has
     a zero gradient.  dprobs (E): added to the gradient of every routed token's gate probabilities, as a balance loss
     on their mean has it.  The gradient by logit_bias is the result's sum over the tokens.  (zm_router_backward)"""
+    d = _index(logits, "router_backward")
+    if stream is not None or d != _device():
+        return _there(router_backward, d, stream, logits, ids, dweights, gating, logit_bias, weights_norm, weights_scale,
+                      dprobs)
+    st = _raw_stream(d)
     if logits.dim() != 2 or logits.dtype != _F32 or ids.dim() != 2:
         raise ValueError("logits (S, E) float32 and ids (S, K) are needed")
     logits = _flat(logits)
@@ -276,7 +296,7 @@ def router_backward(st, d, logits: torch.Tensor, ids: torch.Tensor, dweights: to
     ids = _flat(_need(ids, "ids", d, _I32S, (S, K)))
     dweights = _flat(_need(dweights, "dweights", d, _F32S, (S, K)))
     logit_bias, dprobs = _vector(logit_bias, "logit_bias", d, E), _vector(dprobs, "dprobs", d, E)
-    out = logits.new_empty((S, E))
+    out = torch.empty_like(logits)
     spec = _spec(E, K, gating, 0, 0, weights_norm, weights_scale)
     check(lib().zm_router_backward(spec, logits.data_ptr(), _ptr(logit_bias), ids.data_ptr(), dweights.data_ptr(),
                                    _ptr(dprobs), S, out.data_ptr(), st), "zm_router_backward")
