@@ -129,7 +129,7 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, 
   } else if (kind == TILES) {
     const int64_t steps = planes * ((K + step - 1) / step);
     const size_t plane = (size_t)M * N * 4;
-    p.tile = !vec || M <= 64;
+    p.tile = M <= 64;
     int bm = p.tile ? 32 : 128, bn = 128;
     if (p.tile) {
       // 32 x 128 for up to 64 rows; k in as many slices as give two workgroups per CU, at least 256 of it each
@@ -145,9 +145,10 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, 
       };
       static const Tile dma_tiles[] = {{2, 256, 256, 1.9, 0}, {3, 256, 128, 1.04, 0}, {0, 128, 128, 0.75, 1.09}};
       static const Tile term_tiles[] = {{0, 128, 128, 1.0, 1.5}, {0, 128, 128, 1.2, 2.1}, {0, 128, 128, 1.3, 0}};
-      const Tile *first = dma ? dma_tiles : term_tiles + (products <= 3 ? 0 : products <= 5 ? 1 : 2);
+      const bool lds = dma && vec;  // (without 16-byte loads 16-bit operands go through registers too)
+      const Tile *first = lds ? dma_tiles : term_tiles + (products <= 3 ? 0 : products <= 5 ? 1 : 2);
       double best = 1e30;
-      for (const Tile *t = first; t < first + (dma ? 3 : 1); ++t) {
+      for (const Tile *t = first; t < first + (lds ? 3 : 1); ++t) {
         const int64_t tiles = ((M + t->bm - 1) / t->bm) * ((N + t->bn - 1) / t->bn);
         for (int64_t s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
           if (s > 1 && (s * plane > most || steps < 4 * s || tiles * s > 1024)) break;

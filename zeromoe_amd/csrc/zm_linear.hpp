@@ -282,22 +282,32 @@ struct Operand {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           to.r[i][j] = bld4(r, 8 * c + j < left ? off[i] : OOR, j * (int)ld * (int)sizeof(T));
-      } else {
+      } else if (left == BK && (KC || rows >= R)) {
+        // any alignment: memory takes it, the whole step exists
         if constexpr (KC) {
-          const T *p = at + (int64_t)min(row, rows - 1) * ld + 8 * c;
-          T e[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) e[j] = 8 * c + j < left ? p[j] : from_f32<T>(0.f);
-          __builtin_memcpy(to.r[i], e, sizeof(e));
+          __builtin_memcpy(to.r[i], at + (int64_t)min(row, rows - 1) * ld + 8 * c, sizeof(to.r[i]));
         } else {
+          const T *p = at + (int64_t)8 * c * ld + min(row, rows - R);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const T *p = at + (int64_t)(8 * c + j) * ld;
-            T e[R];
-#pragma unroll
-            for (int q = 0; q < R; ++q) e[q] = 8 * c + j < left ? p[min(row + q, rows - 1)] : from_f32<T>(0.f);
-            __builtin_memcpy(&to.r[i][j], e, 4);
+            __builtin_memcpy(&to.r[i][j], p + j * ld, 4);
+            if (R == 2 && row > rows - R) to.r[i][j] >>= 16;  // the last row of an odd number of them
           }
+        }
+      } else if constexpr (KC) {
+        const T *p = at + (int64_t)min(row, rows - 1) * ld + 8 * c;
+        T e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = 8 * c + j < left ? p[j] : from_f32<T>(0.f);
+        __builtin_memcpy(to.r[i], e, sizeof(e));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const T *p = at + (int64_t)(8 * c + j) * ld;
+          T e[R];
+#pragma unroll
+          for (int q = 0; q < R; ++q) e[q] = 8 * c + j < left ? p[min(row + q, rows - 1)] : from_f32<T>(0.f);
+          __builtin_memcpy(&to.r[i][j], e, 4);
         }
       }
     }
@@ -1011,22 +1021,23 @@ void lin_few_of(const LinArgs &g, hipStream_t st) {
   else lin_few_launch<TX, NX, TW, NW, 4>(g, st);
 }
 
-// The launch of one kernel instance.  `tile`: 0 = 128 x 128, 1 = 32 x 128, for 16-bit operands 2 = 256 x 256 and
-// 3 = 256 x 128; operands without 16-byte loads (`vec` false) take 32 x 128.
+// The launch of one kernel instance.  `tile`: 0 = 128 x 128, 1 = 32 x 128, for 16-bit operands with 16-byte loads
+// (`vec`) 2 = 256 x 256 and 3 = 256 x 128.
 template <class TA, int NA, bool KCA, class TB, int NB, bool KCB>
 void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices));
-  if (!vec) {
-    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 4, false>), grid, dim3(256), 0, st, g);
-  } else if (tile == 1) {
-    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 8, true>), grid, dim3(512), 0, st, g);
+  const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices)), b(512);
+  if (tile == 1) {
+    if (vec) hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 8, true>), grid, b, 0, st, g);
+    else hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 32, 128, 1, 8, false>), grid, b, 0, st, g);
+  } else if (!vec) {
+    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 4, false>), grid, b, 0, st, g);
   } else if constexpr (std::is_same<TA, TB>::value && sizeof(TA) == 2) {
     constexpr bool F16 = std::is_same<TA, _Float16>::value;
-    if (tile == 2) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 256, 2, 4>), grid, dim3(512), 0, st, g);
-    else if (tile == 3) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 128, 4, 2>), grid, dim3(512), 0, st, g);
-    else hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 128, 128, 2, 4>), grid, dim3(512), 0, st, g);
+    if (tile == 2) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 256, 2, 4>), grid, b, 0, st, g);
+    else if (tile == 3) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 128, 4, 2>), grid, b, 0, st, g);
+    else hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 128, 128, 2, 4>), grid, b, 0, st, g);
   } else {
-    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 4, true>), grid, dim3(512), 0, st, g);
+    hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 4, true>), grid, b, 0, st, g);
   }
 }
 

@@ -82,17 +82,56 @@ __device__ __forceinline__ v4u pack(const float (&v)[Pack<T>::V]) {
   __builtin_memcpy(&r, e, 16);
   return r;
 }
-__device__ __forceinline__ void load_vec(const float *p, int i, bool on, int V, float other, float *v) {
+// V values from i on of a row of n (zeros past it); ALIGNED: n and the addresses allow whole packs, else memory takes
+// whole packs where they lie and the last one goes value by value
+template <class T, bool ALIGNED>
+__device__ __forceinline__ v4u load_pack(const T *p, int i, int n) {
+  constexpr int V = Pack<T>::V;
+  if (ALIGNED) return i < n ? *reinterpret_cast<const v4u *>(p + i) : v4u{0, 0, 0, 0};
+  v4u r = {0, 0, 0, 0};
+  if (i + V <= n) {
+    __builtin_memcpy(&r, p + i, 16);
+  } else if (i < n) {
+    T e[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) e[j] = i + j < n ? p[i + j] : from_f32<T>(0.f);
+    __builtin_memcpy(&r, e, 16);
+  }
+  return r;
+}
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void store_pack(T *p, int i, int n, const float (&v)[Pack<T>::V]) {
+  constexpr int V = Pack<T>::V;
+  const v4u r = pack<T>(v);
+  if (ALIGNED) {
+    if (i < n) __builtin_nontemporal_store(r, reinterpret_cast<v4u *>(p + i));
+  } else if (i + V <= n) {
+    __builtin_memcpy(p + i, &r, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (i + j < n) p[i + j] = from_f32<T>(v[j]);
+  }
+}
+// V floats of a vector of n, `other` where it is null or past its end
+template <int V, bool ALIGNED>
+__device__ __forceinline__ void load_vec(const float *p, int i, int n, float other, float (&v)[V]) {
+#pragma unroll
   for (int j = 0; j < V; j += 4) {
-    const v4f f = p && on ? *reinterpret_cast<const v4f *>(p + i + j) : v4f{other, other, other, other};
-    v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
+    if (ALIGNED) {
+      const v4f f = p && i < n ? *reinterpret_cast<const v4f *>(p + i + j) : v4f{other, other, other, other};
+      v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
+    } else {
+#pragma unroll
+      for (int q = j; q < j + 4; ++q) v[q] = p && i + q < n ? p[i + q] : other;
+    }
   }
 }
 
 // Workgroups of NT threads go over the rows; TPR = 64 or NT threads keep one row in C packs of 16 bytes each.  Weight
 // and bias stay in registers (from L2 they are 8 bytes a value next to 4 of a 16-bit row), and the next row's loads are
 // in flight while this one's sums are taken.  Buffers of the sums alternate, so that one barrier a sum is enough.
-template <class T, int NT, int TPR, int C>
+template <class T, int NT, int TPR, int C, bool ALIGNED>
 __global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
   constexpr int V = Pack<T>::V, RPB = NT / TPR;
   __shared__ float red[2][2][NT / 64][1];
@@ -101,8 +140,8 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = (t + TPR * c) * V;
-    load_vec(g.weight, i, i < g.n, V, 1.0f, w[c]);
-    load_vec(g.bias, i, i < g.n, V, 0.0f, b[c]);
+    load_vec<V, ALIGNED>(g.weight, i, g.n, 1.0f, w[c]);
+    load_vec<V, ALIGNED>(g.bias, i, g.n, 0.0f, b[c]);
   }
   const float n = (float)g.n;
   v4u next[C];
@@ -113,7 +152,7 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int i = (t + TPR * c) * V;
-      next[c] = r < g.rows && i < g.n ? *reinterpret_cast<const v4u *>(x + i) : v4u{0, 0, 0, 0};
+      next[c] = r < g.rows ? load_pack<T, ALIGNED>(x, i, g.n) : v4u{0, 0, 0, 0};
     }
   };
   fetch(row);
@@ -132,10 +171,10 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
     float sq = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const bool in = (t + TPR * c) * V < g.n;
+      const int i = (t + TPR * c) * V;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[c][j] = in ? v[c][j] - mean : 0.f;
+        v[c][j] = (ALIGNED ? i : i + j) < g.n ? v[c][j] - mean : 0.f;
         sq = __builtin_fmaf(v[c][j], v[c][j], sq);
       }
     }
@@ -144,10 +183,9 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int i = (t + TPR * c) * V;
-      if (i >= g.n) continue;
 #pragma unroll
       for (int j = 0; j < V; ++j) v[c][j] = __builtin_fmaf(v[c][j] * rstd, w[c][j], b[c][j]);
-      __builtin_nontemporal_store(pack<T>(v[c]), reinterpret_cast<v4u *>(y + i));
+      store_pack<T, ALIGNED>(y, i, g.n, v[c]);
     }
     if (!t) {
       if (g.mean) g.mean[row] = mean;
@@ -156,7 +194,7 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
   }
 }
 
-// Any width and alignment: a row is read three times (the later ones from L2).
+// Rows too long for registers: read three times (the later ones from L2).
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_any(NormArgs g) {
   __shared__ float red[2][4][1];
@@ -185,7 +223,7 @@ __global__ __launch_bounds__(256) void k_norm_any(NormArgs g) {
 // NT threads, TPR of them for a row: a workgroup goes over rows b * NT / TPR + ..., and each thread keeps the same
 // columns throughout, so the sums over the rows stay in its registers until the end, and the weight too.  The next
 // rows' loads are in flight while this one's sums are taken.
-template <class T, int NT, int TPR, int C>
+template <class T, int NT, int TPR, int C, bool ALIGNED>
 __global__ __launch_bounds__(NT) void k_norm_backward(NormArgs g) {
   constexpr int V = Pack<T>::V, RPB = NT / TPR;
   __shared__ float red[2][NT / 64][2];
@@ -195,7 +233,7 @@ __global__ __launch_bounds__(NT) void k_norm_backward(NormArgs g) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = (t + TPR * c) * V;
-    load_vec(g.weight, i, i < g.n, V, 1.0f, w[c]);
+    load_vec<V, ALIGNED>(g.weight, i, g.n, 1.0f, w[c]);
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[c][j] = db[c][j] = 0.f;
   }
@@ -206,9 +244,8 @@ __global__ __launch_bounds__(NT) void k_norm_backward(NormArgs g) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int i = (t + TPR * c) * V;
-      const bool in = r < g.rows && i < g.n;
-      nx[c] = in ? *reinterpret_cast<const v4u *>(x + i) : v4u{0, 0, 0, 0};
-      ng[c] = in ? *reinterpret_cast<const v4u *>(dy + i) : v4u{0, 0, 0, 0};
+      nx[c] = r < g.rows ? load_pack<T, ALIGNED>(x, i, g.n) : v4u{0, 0, 0, 0};
+      ng[c] = r < g.rows ? load_pack<T, ALIGNED>(dy, i, g.n) : v4u{0, 0, 0, 0};
     }
     nm = r < g.rows ? g.mean[r] : 0.f;
     nr = r < g.rows ? g.rstd[r] : 0.f;
@@ -247,13 +284,12 @@ __global__ __launch_bounds__(NT) void k_norm_backward(NormArgs g) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int i = (t + TPR * c) * V;
-      if (i >= g.n) continue;
       float xv[V], gv[V];
       unpack<T>(rx[c], xv);
       unpack<T>(rg[c], gv);
 #pragma unroll
       for (int j = 0; j < V; ++j) xv[j] = rstd * __builtin_fmaf(mean - xv[j], rs2, __builtin_fmaf(gv[j], w[c][j], -s1));
-      __builtin_nontemporal_store(pack<T>(xv), reinterpret_cast<v4u *>(dx + i));
+      store_pack<T, ALIGNED>(dx, i, g.n, xv);
     }
   }
   if (!g.part) return;
@@ -285,15 +321,24 @@ __global__ __launch_bounds__(NT) void k_norm_backward(NormArgs g) {
   for (int c = 0; c < C; ++c) {
     const int i = (t + TPR * c) * V;
     if (i >= g.n) continue;
+    if (ALIGNED) {
 #pragma unroll
-    for (int j = 0; j < V; j += 4) {
-      *reinterpret_cast<v4f *>(pw + i + j) = v4f{dw[c][j], dw[c][j + 1], dw[c][j + 2], dw[c][j + 3]};
-      *reinterpret_cast<v4f *>(pb + i + j) = v4f{db[c][j], db[c][j + 1], db[c][j + 2], db[c][j + 3]};
+      for (int j = 0; j < V; j += 4) {
+        *reinterpret_cast<v4f *>(pw + i + j) = v4f{dw[c][j], dw[c][j + 1], dw[c][j + 2], dw[c][j + 3]};
+        *reinterpret_cast<v4f *>(pb + i + j) = v4f{db[c][j], db[c][j + 1], db[c][j + 2], db[c][j + 3]};
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (i + j < g.n) {
+          pw[i + j] = dw[c][j];
+          pb[i + j] = db[c][j];
+        }
     }
   }
 }
 
-// Any width and alignment; the sums over the rows are kept in the workgroup's part of the workspace, which thread t
+// Rows too long for registers; the sums over the rows are kept in the workgroup's part of the workspace, which thread t
 // alone touches at columns t, t + 256, ...
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_backward_any(NormArgs g) {
@@ -344,36 +389,45 @@ int check(const char *who, int type, int64_t rows, int64_t n) {
   return 0;
 }
 
-template <class T>
-void norm(const NormArgs &g, bool vec, hipStream_t st) {
-  constexpr int V = Pack<T>::V;
+template <class T, bool ALIGNED>
+void norm_rows(const NormArgs &g, int packs, hipStream_t st) {
   const int64_t quads = (g.rows + 3) / 4;
-  const int packs = (g.n + V - 1) / V;
   // as many workgroups as fit the chip at once (`most`), or as few as take as many rounds
   auto grid = [](int64_t n, int64_t most) {
     const int64_t rounds = (n + most - 1) / most;
     return dim3((unsigned)((n + rounds - 1) / rounds));
   };
-  if (!vec || packs > 4 * 512) hipLaunchKernelGGL((k_norm_any<T>), dim3((unsigned)g.rows), dim3(256), 0, st, g);
-  else if (packs <= 64) hipLaunchKernelGGL((k_norm<T, 256, 64, 1>), grid(quads, 2048), dim3(256), 0, st, g);
-  else if (packs <= 128) hipLaunchKernelGGL((k_norm<T, 256, 64, 2>), grid(quads, 1536), dim3(256), 0, st, g);
-  else if (packs <= 256) hipLaunchKernelGGL((k_norm<T, 256, 256, 1>), grid(g.rows, 2048), dim3(256), 0, st, g);
-  else if (packs <= 512) hipLaunchKernelGGL((k_norm<T, 512, 512, 1>), grid(g.rows, 1024), dim3(512), 0, st, g);
-  else if (packs <= 1024) hipLaunchKernelGGL((k_norm<T, 512, 512, 2>), grid(g.rows, 1024), dim3(512), 0, st, g);
-  else hipLaunchKernelGGL((k_norm<T, 512, 512, 4>), grid(g.rows, 512), dim3(512), 0, st, g);
+  if (packs <= 64) hipLaunchKernelGGL((k_norm<T, 256, 64, 1, ALIGNED>), grid(quads, 2048), dim3(256), 0, st, g);
+  else if (packs <= 128) hipLaunchKernelGGL((k_norm<T, 256, 64, 2, ALIGNED>), grid(quads, 1536), dim3(256), 0, st, g);
+  else if (packs <= 256) hipLaunchKernelGGL((k_norm<T, 256, 256, 1, ALIGNED>), grid(g.rows, 2048), dim3(256), 0, st, g);
+  else if (packs <= 512) hipLaunchKernelGGL((k_norm<T, 512, 512, 1, ALIGNED>), grid(g.rows, 1024), dim3(512), 0, st, g);
+  else if (packs <= 1024) hipLaunchKernelGGL((k_norm<T, 512, 512, 2, ALIGNED>), grid(g.rows, 1024), dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((k_norm<T, 512, 512, 4, ALIGNED>), grid(g.rows, 512), dim3(512), 0, st, g);
+}
+template <class T>
+void norm(const NormArgs &g, bool vec, hipStream_t st) {
+  const int packs = (g.n + Pack<T>::V - 1) / Pack<T>::V;
+  if (packs > 4 * 512) hipLaunchKernelGGL((k_norm_any<T>), dim3((unsigned)g.rows), dim3(256), 0, st, g);
+  else if (vec) norm_rows<T, true>(g, packs, st);
+  else norm_rows<T, false>(g, packs, st);
 }
 
+template <class T, bool ALIGNED>
+void norm_backward_rows(const NormArgs &g, int packs, unsigned parts, hipStream_t st) {
+  const dim3 grid(parts), b(512);
+  if (packs <= 64) hipLaunchKernelGGL((k_norm_backward<T, 512, 64, 1, ALIGNED>), grid, b, 0, st, g);
+  else if (packs <= 128) hipLaunchKernelGGL((k_norm_backward<T, 512, 128, 1, ALIGNED>), grid, b, 0, st, g);
+  else if (packs <= 256) hipLaunchKernelGGL((k_norm_backward<T, 512, 256, 1, ALIGNED>), grid, b, 0, st, g);
+  else if (packs <= 512) hipLaunchKernelGGL((k_norm_backward<T, 512, 512, 1, ALIGNED>), grid, b, 0, st, g);
+  else if (packs <= 1024) hipLaunchKernelGGL((k_norm_backward<T, 512, 512, 2, ALIGNED>), grid, b, 0, st, g);
+  else hipLaunchKernelGGL((k_norm_backward<T, 512, 512, 4, ALIGNED>), grid, b, 0, st, g);
+}
 template <class T>
 void norm_backward(const NormArgs &g, bool vec, unsigned parts, hipStream_t st) {
-  constexpr int V = Pack<T>::V;
-  const int packs = (g.n + V - 1) / V;
-  if (!vec || packs > 4 * 512) hipLaunchKernelGGL((k_norm_backward_any<T>), dim3(parts), dim3(256), 0, st, g);
-  else if (packs <= 64) hipLaunchKernelGGL((k_norm_backward<T, 512, 64, 1>), dim3(parts), dim3(512), 0, st, g);
-  else if (packs <= 128) hipLaunchKernelGGL((k_norm_backward<T, 512, 128, 1>), dim3(parts), dim3(512), 0, st, g);
-  else if (packs <= 256) hipLaunchKernelGGL((k_norm_backward<T, 512, 256, 1>), dim3(parts), dim3(512), 0, st, g);
-  else if (packs <= 512) hipLaunchKernelGGL((k_norm_backward<T, 512, 512, 1>), dim3(parts), dim3(512), 0, st, g);
-  else if (packs <= 1024) hipLaunchKernelGGL((k_norm_backward<T, 512, 512, 2>), dim3(parts), dim3(512), 0, st, g);
-  else hipLaunchKernelGGL((k_norm_backward<T, 512, 512, 4>), dim3(parts), dim3(512), 0, st, g);
+  const int packs = (g.n + Pack<T>::V - 1) / Pack<T>::V;
+  if (packs > 4 * 512) hipLaunchKernelGGL((k_norm_backward_any<T>), dim3(parts), dim3(256), 0, st, g);
+  else if (vec) norm_backward_rows<T, true>(g, packs, parts, st);
+  else norm_backward_rows<T, false>(g, packs, parts, st);
 }
 
 __global__ __launch_bounds__(256) void k_norm_zero(float *dweight, float *dbias, int n) {
