@@ -200,8 +200,8 @@ struct Product {
   bool shaped;   // strides and widths allow 16-byte loads
   bool forward;  // the product has kernels for few rows
   Kind kind(bool vec) const {
-    if (!vec || !forward || N >= (1 << 26) || K >= (1 << 30)) return TILES;
-    return M <= LIN_ROWS ? ROWS : lin_few_rows(M, N) ? FEW : TILES;
+    if (!forward || N >= (1 << 26) || K >= (1 << 30)) return TILES;
+    return M <= LIN_ROWS ? ROWS : vec && lin_few_rows(M, N) ? FEW : TILES;
   }
   Plan plan_for(bool vec, size_t most) const {
     const int f32_by = b_type == LIN_BF16 ? 3 : b_type == LIN_F16 ? 5 : 6;
@@ -308,10 +308,6 @@ int join(const LinArgs &g, hipStream_t st) {
   return launched();
 }
 
-bool vec4(const void *p, int64_t ld, int type) {
-  return !p || (!((uintptr_t)p & (4 * size_of(type) - 1)) && !(ld & 3));
-}
-
 }  // namespace
 
 extern "C" {
@@ -343,8 +339,6 @@ int zm_linear(const zm_linear_desc *d, const void *x, const void *w, const float
   g.e.ldp = d->pre_stride;
   g.e.type = d->y_type;
   g.e.act = d->act;
-  g.e.vec = vec4(y, d->y_stride, d->y_type) && vec4(residual, d->res_stride, d->y_type) &&
-            vec4(pre, d->pre_stride, d->y_type) && vec4(bias, 0, LIN_F32);
   if (p.kind == ROWS) lin_rows(d->x_type, d->w_type, g, (hipStream_t)stream);
   else if (p.kind == FEW) lin_few(d->x_type, d->w_type, g, (hipStream_t)stream);
   else lin_fwd(d->x_type, d->w_type, g, vec, p.tile, (hipStream_t)stream);
@@ -390,7 +384,7 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
     a.part = dbias ? bias_part : nullptr;
     const int64_t n = dz_chunks(d->S);
     a.chunk = (d->S + n - 1) / n;
-    const bool v = !(d->O & 3) && vec4(dy, d->y_stride, d->y_type) && (!d->act || vec4(pre, d->pre_stride, d->y_type));
+    const bool v = !(d->O & 3);
     const int64_t packs = v ? d->O / 4 : d->O;
     a.packs = (int)std::min<int64_t>(packs, 64);
     a.side = 256 / a.packs;
@@ -409,7 +403,6 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
     g.e.y = dx;
     g.e.ldy = d->I;
     g.e.type = d->x_type;
-    g.e.vec = vec4(dx, d->I, d->x_type);
     lin_dx(d->x_type, d->w_type, z_type, g, vec, p.tile, st);
     if (join(g, st)) return -1;
   }
@@ -421,7 +414,6 @@ int zm_linear_backward(const zm_linear_desc *d, const void *dy, const void *x, c
     g.e.y = dw;
     g.e.ldy = d->I;
     g.e.type = LIN_F32;
-    g.e.vec = vec4(dw, d->I, LIN_F32);
     lin_dw(d->x_type, z_type, g, vec, p.tile, st);
     if (join(g, st)) return -1;
   }

@@ -60,10 +60,12 @@ __device__ __forceinline__ void lin_store(void *p, int type, size_t i, float v) 
   else if (type == LIN_F16) ((_Float16 *)p)[i] = (_Float16)v;
   else ((bf16 *)p)[i] = from_f32<bf16>(v);
 }
-// four values at an offset whose address is a multiple of 4 elements
+// four neighbouring values, at any address that their type allows (memory takes whole accesses at any alignment)
+typedef v4f v4fu __attribute__((aligned(4)));
 __device__ __forceinline__ v4f lin_load4(const void *p, int type, size_t i) {
-  if (type == LIN_F32) return *reinterpret_cast<const v4f *>((const float *)p + i);
-  const uint2 r = *reinterpret_cast<const uint2 *>((const uint16_t *)p + i);
+  if (type == LIN_F32) return *reinterpret_cast<const v4fu *>((const float *)p + i);
+  uint2 r;
+  __builtin_memcpy(&r, (const uint16_t *)p + i, 8);
   if (type == LIN_F16) {
     typedef _Float16 v4h __attribute__((ext_vector_type(4)));
     const v4h h = __builtin_bit_cast(v4h, r);
@@ -74,14 +76,15 @@ __device__ __forceinline__ v4f lin_load4(const void *p, int type, size_t i) {
 }
 __device__ __forceinline__ void lin_store4(void *p, int type, size_t i, v4f v) {
   if (type == LIN_F32) {
-    *reinterpret_cast<v4f *>((float *)p + i) = v;
+    *reinterpret_cast<v4fu *>((float *)p + i) = v;
   } else if (type == LIN_F16) {
     typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<v4h *>((_Float16 *)p + i) =
-        v4h{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+    const v4h h = {(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+    __builtin_memcpy((_Float16 *)p + i, &h, 8);
   } else {
     typedef __bf16 v4b __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<v4b *>((bf16 *)p + i) = v4b{(__bf16)v.x, (__bf16)v.y, (__bf16)v.z, (__bf16)v.w};
+    const v4b h = {(__bf16)v.x, (__bf16)v.y, (__bf16)v.z, (__bf16)v.w};
+    __builtin_memcpy((bf16 *)p + i, &h, 8);
   }
 }
 
@@ -362,7 +365,6 @@ struct LinEpilogue {
   const float *bias;   // [N] or null
   int64_t ldy, ldr, ldp;
   int type, act;
-  int vec;             // rows and bases of y, res, pre and bias allow 4 values at once
 };
 
 struct LinArgs {
@@ -387,8 +389,8 @@ __device__ __forceinline__ float lin_finish1(const LinEpilogue &e, int64_t m, in
 }
 // four results of one row, columns n .. n + 3 of which those below N exist
 __device__ __forceinline__ void lin_finish4(const LinEpilogue &e, int64_t m, int64_t n, int64_t N, v4f z) {
-  if (e.vec && n + 4 <= N) {
-    if (e.bias) z += *reinterpret_cast<const v4f *>(e.bias + n);
+  if (n + 4 <= N) {
+    if (e.bias) z += *reinterpret_cast<const v4fu *>(e.bias + n);
     if (e.pre) lin_store4(e.pre, e.type, (size_t)(m * e.ldp + n), z);
     if (e.act) {
 #pragma unroll
@@ -408,8 +410,8 @@ __device__ __forceinline__ void lin_result(const LinArgs &g, int z, int64_t m, i
   if (m >= g.M || n >= g.N) return;
   if (g.slices == 1) return lin_finish4(g.e, m, n, g.N, v);
   float *p = g.part + ((size_t)z * g.M + m) * g.N + n;
-  if (!(g.N & 3)) {
-    *reinterpret_cast<v4f *>(p) = v;
+  if (n + 4 <= g.N) {
+    *reinterpret_cast<v4fu *>(p) = v;
   } else {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -765,8 +767,8 @@ static __global__ __launch_bounds__(256) void k_linear_join(LinArgs g) {
         const int z = z0 + u * G;
         t[u] = v4f{0.f, 0.f, 0.f, 0.f};
         if (z < g.slices) {
-          if (!(g.N & 3)) {
-            t[u] = *reinterpret_cast<const v4f *>(p + z * plane);
+          if (n + 4 <= g.N) {
+            t[u] = *reinterpret_cast<const v4fu *>(p + z * plane);
           } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -811,17 +813,18 @@ __global__ __launch_bounds__(256) void k_linear_rows(LinArgs g) {
   const TX *x = (const TX *)g.a;
   float acc[S] = {};
   const int K = (int)g.K, first = ((WPR == 1 ? 0 : wave * 64) + lane) * V, step = 64 * WPR * V;
-  for (int k0 = first; k0 < K; k0 += U * step) {
+  typedef v4u v4uu __attribute__((aligned(2)));
+  for (int k0 = first; k0 + V <= K; k0 += U * step) {
     v4u rw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = k0 + u * step;
-      rw[u] = k < K ? __builtin_nontemporal_load(reinterpret_cast<const v4u *>(w + k)) : v4u{0, 0, 0, 0};
+      rw[u] = k + V <= K ? __builtin_nontemporal_load(reinterpret_cast<const v4uu *>(w + k)) : v4u{0, 0, 0, 0};
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = k0 + u * step;
-      if (k >= K) break;
+      if (k + V > K) break;
       TW e[V];
       __builtin_memcpy(e, &rw[u], 16);
 #pragma unroll
@@ -833,6 +836,11 @@ __global__ __launch_bounds__(256) void k_linear_rows(LinArgs g) {
       }
     }
   }
+  // the last, partial pack: a value a lane
+  const int last = K / V * V + lane;
+  if (last < K && (WPR == 1 || wave == 0))
+#pragma unroll
+    for (int s = 0; s < S; ++s) acc[s] = __builtin_fmaf(to_f32(w[last]), to_f32(x[s * g.lda + last]), acc[s]);
 #pragma unroll
   for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -1042,8 +1050,8 @@ void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
 }
 
 // the products by what their operands are: forward (x, w), dx (dz, w), dw (dz, x)
-void lin_rows(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // M <= LIN_ROWS, operands with 16-byte loads
-void lin_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);   // where lin_few_rows(), likewise
+void lin_rows(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // M <= LIN_ROWS, any alignment
+void lin_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);   // where lin_few_rows(), operands with 16-byte loads
 void lin_fwd(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dx(int x_type, int w_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dw(int x_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
