@@ -179,6 +179,73 @@ def test_linear_f32_keeps_its_digits():
         assert not y[:2].isfinite().any() and y[2:].isfinite().all()
 
 
+@pytest.mark.parametrize("S", [2, 40, 200])
+def test_linear_smallest_values(S):
+    """Subnormal f16 and bf16 values, and f32 values whose last bf16 term is one (steps of 2^-133)."""
+    import zeromoe_amd as Z
+
+    for dtype, e in ((torch.float16, -20.0), (torch.bfloat16, -128.0)):
+        x = torch.ldexp(rand(S, 128, seed=1), torch.tensor(e, device="cuda")).to(dtype)
+        w = (rand(64, 128, seed=2) * (64.0 if dtype == torch.float16 else 2.0 ** 60)).to(dtype)
+        y = Z.linear(x, w, out_dtype=torch.float32)
+        # (what an instruction adds in one go may be rounded at its largest product's place: up to 32 products)
+        close(y, x.double() @ w.double().t(), 8 * sum_tol(128, x.double().abs() @ w.double().abs().t()))
+    for e in (-100.0, -115.0, -126.0):
+        x, w = torch.ldexp(rand(S, 128, seed=3), torch.tensor(e, device="cuda")), rand(64, 128, seed=4) * 2.0 ** 60
+        a = x.double().abs() @ w.double().abs().t()
+        lost = 2.0 ** -133 * w.double().abs().sum(1)[None]
+        close(Z.linear(x, w), x.double() @ w.double().t(), sum_tol(128, a) + lost)
+
+
+def test_offsets_past_32_bits():
+    """Operands and results of more than 2^31 values: the last rows against the same rows by themselves."""
+    import zeromoe_amd as Z
+
+    S, I, O = (1 << 20) + 7, 2056, 40
+    x, w = torch.empty(S, I, device="cuda", dtype=torch.bfloat16), rand(O, I, seed=1, scale=0.02, dtype=torch.bfloat16)
+    x.copy_(rand(1, I, seed=2).to(torch.bfloat16).expand(S, I))
+    x[-300:] = rand(300, I, seed=3, dtype=torch.bfloat16)
+    y = Z.linear(x, w, out_dtype=torch.float32)
+    z = x[-300:].double() @ w.double().t()
+    close(y[-300:], z, sum_tol(I, x[-300:].double().abs() @ w.double().abs().t()))
+    h, mean, rstd = Z.layer_norm(x, stats=True)
+    assert torch.equal(h[-300:], Z.layer_norm(x[-300:]))
+    dy = torch.zeros_like(x)
+    dy[-300:] = rand(300, I, seed=4, dtype=torch.bfloat16)
+    dx, dw, db = Z.layer_norm_backward(dy, x, mean, rstd)
+    ex, ew, eb = Z.layer_norm_backward(dy[-300:], x[-300:], mean[-300:], rstd[-300:])
+    assert torch.equal(dx[-300:], ex) and (dx[:-300] == 0).all()
+    assert (dw - ew).abs().max() <= 1e-5 * ew.abs().max() and (db - eb).abs().max() <= 1e-5 * eb.abs().max()  # 300 f32 additions
+    del h, dy, dx
+    dx = Z.linear_backward(y, x, w, need_dw=False, need_dbias=False)[0]
+    assert torch.equal(dx[-128:], Z.linear_backward(y[-128 * 3:], x[-128 * 3:], w, need_dw=False, need_dbias=False)[0][-128:])
+    del x, y, dx
+    S, K, H = 70000, 8, 4100
+    r, wt, d = torch.zeros(S, K, H, device="cuda"), rand(S, K, seed=5), rand(S, H, seed=6)
+    r[-50:] = rand(50, K, H, seed=7)
+    assert torch.equal(Z.combine(r, wt, residual=d)[-50:], Z.combine(r[-50:], wt[-50:], residual=d[-50:]))
+    dw, dy = Z.combine_backward(d, r, weights=wt, need_dy=True)
+    assert torch.equal(dw[-50:], Z.combine_backward(d[-50:], r[-50:])) and torch.equal(dy[-1, -1], wt[-1, -1] * d[-1])
+
+
+@pytest.mark.parametrize("S", [3, 40, 200])
+def test_linear_rows_far_apart(S):
+    """Rows up to 8 MB apart, where 32-bit offsets of a tile end, and further."""
+    import zeromoe_amd as Z
+
+    w = rand(24, 72, seed=1)
+    for ld in ((1 << 21) - 4, 1 << 21, (1 << 21) + 4):
+        x = torch.empty((S - 1) * ld + 72, device="cuda").as_strided((S, 72), (ld, 1))
+        x.copy_(rand(S, 72, seed=2))
+        assert torch.equal(Z.linear(x[:3], w), Z.linear(x[:3].contiguous(), w))
+        close(Z.linear(x, w), x.double() @ w.double().t(), sum_tol(72, x.double().abs() @ w.double().abs().t()))
+        dy = rand(S, 24, seed=3)
+        dw = Z.linear_backward(dy, x, w, need_dx=False)[1]
+        close(dw, dy.double().t() @ x.double(), sum_tol(S, dy.double().abs().t() @ x.double().abs()) + U)
+        h = Z.layer_norm(x)
+        assert torch.equal(h, Z.layer_norm(x.contiguous()))
+
+
 def check_linear_backward(S, I, O, xt, wt, act="none", ydt=None, seed=1, need=(True, True, True)):
     import zeromoe_amd as Z
 
@@ -496,6 +563,23 @@ def test_router_backward_masked_logits_and_odd_ids(gating):
     ids[0, 0], ids[1, 2] = E, 2 ** 31 - 1
     got = Z.router_backward(logits, ids, dw, gating=gating)
     assert got[:2].isnan().all() and got[2:].isfinite().all()
+
+
+@pytest.mark.parametrize("gating", ["sigmoid", "sqrt_softplus"])
+def test_router_backward_small_sums(gating):
+    """Weights whose sum is below the least that they are divided by: the divisor is a constant there."""
+    import zeromoe_amd as Z
+
+    logits = rand(6, 40, seed=1) - (13.0 if gating == "sigmoid" else 25.0)
+    ids = torch.topk(logits, 4)[1].int()
+    dw = rand(6, 4, seed=2)
+    got = Z.router_backward(logits, ids, dw, gating=gating, weights_norm=True, weights_scale=2.0)
+    want = route_grad64(logits, ids, dw, gating, None, True, 2.0, None)
+    p = gate64(logits.double(), gating)
+    total = p.gather(1, ids.long()).sum(-1, keepdim=True)
+    assert (total < 2.0 ** -14).any()
+    # exp's argument is up to 28 (its rounding is 28 of the result's), then a few roundings of d and sum d p / N
+    close(got, want, 60 * U * p * 4 * dw.abs().double().sum(-1, keepdim=True) / total.clamp(min=2.0 ** -14) + 1e-37)
 
 
 def test_router_backward_by_differences():
