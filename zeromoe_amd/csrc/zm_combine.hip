@@ -95,8 +95,7 @@ __global__ __launch_bounds__(256) void k_combine_backward(CombineArgs g) {
     float sum;
     if constexpr (V == 4) sum = (acc.x + acc.y) + (acc.z + acc.w);
     else sum = acc;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    sum = group_sum<64>(sum);
     if (!lane) g.dweights[r] = sum;
   }
   if (g.dy) {
@@ -120,22 +119,27 @@ struct RouteGradArgs {
   float scale;
 };
 
-__device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
 // One wave per token; expert e = lane + 64 i is register i of its lane (E <= 64 P), route k is lane k (K <= 64).
+constexpr int ROUTE_WAVES = 4;
 template <int P>
-__global__ __launch_bounds__(256) void k_router_backward(RouteGradArgs g) {
-  __shared__ float prob[4][64 * P];
+__global__ __launch_bounds__(64 * ROUTE_WAVES) void k_router_backward(RouteGradArgs g) {
+  __shared__ float prob[ROUTE_WAVES][64 * P];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t s = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t s = (int64_t)blockIdx.x * ROUTE_WAVES + wave;
   if (s >= g.S) return;
   const float INF = __builtin_inff();
+  // everything the token needs is asked for at once: a memory latency is most of this kernel's time
+  float z[P], p[P], u[P], gr[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int e = lane + 64 * i;
+    z[i] = e < g.E ? g.logits[s * g.E + e] : -INF;
+    p[i] = g.logit_bias && e < g.E ? g.logit_bias[e] : 0.f;
+    gr[i] = g.dprobs && e < g.E ? g.dprobs[e] : 0.f;
+  }
   const int id = lane < g.K ? g.ids[s * g.K + lane] : -1;
-  float d = lane < g.K && id >= 0 ? g.dweights[s * g.K + lane] : 0.f;
+  float d = lane < g.K ? g.dweights[s * g.K + lane] : 0.f;
+  d = id >= 0 ? d : 0.f;
   float *out = g.dlogits + s * g.E;
   const bool any = __ballot(id >= 0) != 0, bad = __ballot(id >= g.E) != 0;
   if (!any || bad) {  // a skipped row has no gradient; an id that does not exist has none that could be told
@@ -144,24 +148,21 @@ __global__ __launch_bounds__(256) void k_router_backward(RouteGradArgs g) {
       if (lane + 64 * i < g.E) out[lane + 64 * i] = bad ? __builtin_nanf("") : 0.f;
     return;
   }
-  float z[P], p[P], u[P];
   float mx = -INF;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    const int e = lane + 64 * i;
-    z[i] = e < g.E ? g.logits[s * g.E + e] + (g.logit_bias ? g.logit_bias[e] : 0.f) : -INF;
+    z[i] += p[i];
     mx = fmaxf(mx, z[i]);
   }
   if (g.gating == 0) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    mx = wave_max(mx);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       p[i] = mx == -INF && z[i] == z[i] ? 0.f : expf(z[i] - mx);  // all -inf: no probability, no gradient
       sum += lane + 64 * i < g.E ? p[i] : 0.f;
     }
-    sum = wave_add(sum);
+    sum = group_sum<64>(sum);
     const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
 #pragma unroll
     for (int i = 0; i < P; ++i) p[i] *= inv;
@@ -187,20 +188,14 @@ __global__ __launch_bounds__(256) void k_router_backward(RouteGradArgs g) {
   const float pk = id >= 0 ? prob[wave][id] : 0.f;
   d *= g.scale;
   if (g.norm) {
-    const float total = wave_add(pk), dot = wave_add(d * pk);
+    const float total = group_sum<64>(pk), dot = group_sum<64>(d * pk);
     const bool low = total < 6.103515625e-5f;
     const float N = low ? 6.103515625e-5f : total;
     d = id >= 0 ? (d - (low ? 0.f : dot / N)) / N : 0.f;
   }
-  float gr[P];
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const int e = lane + 64 * i;
-    gr[i] = g.dprobs && e < g.E ? g.dprobs[e] : 0.f;
-  }
   for (int k = 0; k < g.K; ++k) {  // in order: an expert named twice gets both
-    const int ek = __shfl(id, k);
-    const float dk = __shfl(d, k);
+    const int ek = __builtin_amdgcn_readlane(id, k);
+    const float dk = readlane_f(d, k);
 #pragma unroll
     for (int i = 0; i < P; ++i) gr[i] += ek == lane + 64 * i ? dk : 0.f;
   }
@@ -208,7 +203,7 @@ __global__ __launch_bounds__(256) void k_router_backward(RouteGradArgs g) {
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < P; ++i) dot += p[i] * gr[i];
-    dot = wave_add(dot);
+    dot = group_sum<64>(dot);
 #pragma unroll
     for (int i = 0; i < P; ++i) gr[i] = p[i] * (gr[i] - dot);
   } else {
@@ -308,7 +303,7 @@ int zm_router_backward(const zm_router_spec *spec, const float *logits, const fl
   g.gating = spec->gating;
   g.norm = spec->weights_norm;
   g.scale = spec->weights_scale != 0.f ? spec->weights_scale : 1.f;
-  const dim3 grid((unsigned)(((int64_t)S + 3) / 4)), b(256);
+  const dim3 grid((unsigned)(((int64_t)S + ROUTE_WAVES - 1) / ROUTE_WAVES)), b(64 * ROUTE_WAVES);
   const hipStream_t st = (hipStream_t)stream;
   if (g.E <= 64) hipLaunchKernelGGL((k_router_backward<1>), grid, b, 0, st, g);
   else if (g.E <= 128) hipLaunchKernelGGL((k_router_backward<2>), grid, b, 0, st, g);

@@ -842,9 +842,7 @@ __global__ __launch_bounds__(256) void k_linear_rows(LinArgs g) {
 #pragma unroll
     for (int s = 0; s < S; ++s) acc[s] = __builtin_fmaf(to_f32(w[last]), to_f32(x[s * g.lda + last]), acc[s]);
 #pragma unroll
-  for (int s = 0; s < S; ++s)
-#pragma unroll
-    for (int q = 32; q; q >>= 1) acc[s] += __shfl_xor(acc[s], q);
+  for (int s = 0; s < S; ++s) acc[s] = group_sum<64>(acc[s]);
   if (WPR > 1) {
     if (!lane)
 #pragma unroll

@@ -37,9 +37,7 @@ struct NormArgs {
 template <int TPR, int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[N]) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1)
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], o);
+  for (int k = 0; k < N; ++k) v[k] = group_sum<64>(v[k]);
   if (TPR > 64) {
     const int wave = threadIdx.x >> 6, first = wave / (TPR / 64) * (TPR / 64);
     if (!(threadIdx.x & 63))
