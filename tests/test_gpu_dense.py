@@ -282,6 +282,14 @@ def test_linear_backward(S, I, O, xt, wt):
     check_linear_backward(S, I, O, xt, wt, ydt="f32", seed=31)
 
 
+@pytest.mark.parametrize("S,I,O", [(700, 264, 160), (700, 1000, 288), (1100, 2048, 152), (390, 136, 320), (2000, 128, 130)])
+def test_linear_narrow_w(S, I, O):
+    """f32 products whose w fills tiles of 160 rows better than tiles of 128."""
+    check_linear(S, I, O, "f32", "f32", "silu")
+    check_linear_backward(S, I, O, "f32", "f32")
+    check_linear_backward(S, I, O, "f32", "f32", "gelu")
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_linear_backward_activations(act):
     check_linear_backward(70, 96, 56, "f32", "bf16", act)

@@ -111,8 +111,9 @@ struct Plan {
 // the kernels of a product, by its rows and by whether its operands can be read 16 bytes at a time
 enum Kind { ROWS, FEW, TILES };
 
-// `products`: of terms, for each product of values; 1: 16-bit operands of one type, which go straight into LDS
-Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, bool vec, size_t most) {
+// `products`: of terms, for each product of values; 1: 16-bit operands of one type, which go straight into LDS;
+// `side`: Product's
+Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, int side, bool vec, size_t most) {
   const bool dma = products == 1;
   const int step = dma ? DMA_BK : 32;
   Plan p{};
@@ -145,10 +146,16 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, 
       };
       static const Tile dma_tiles[] = {{2, 256, 256, 1.9, 0}, {3, 256, 128, 1.04, 0}, {0, 128, 128, 0.75, 1.09}};
       static const Tile term_tiles[] = {{0, 128, 128, 1.0, 1.5}, {0, 128, 128, 1.2, 2.1}, {0, 128, 128, 1.3, 0}};
+      // w's side of a product may be narrow, as a router's is: 160 rows fill one tile of 160, and 62% of two of 128
+      // (4095 rows by w of 160 x 5120: 74 -> 56 us, its gradient by w 84 -> 67; w of 288 x 2048 89 -> 72 and 99 -> 83)
+      static const Tile wide_n[] = {{0, 128, 128, 1.3, 0}, {4, 128, 160, 1.8, 0}};
+      static const Tile wide_m[] = {{0, 128, 128, 1.3, 0}, {4, 160, 128, 1.8, 0}};
       const bool lds = dma && vec;  // (without 16-byte loads 16-bit operands go through registers too)
       const Tile *first = lds ? dma_tiles : term_tiles + (products <= 3 ? 0 : products <= 5 ? 1 : 2);
+      int tiles_of = lds ? 3 : 1;
+      if (products == 6 && vec && side) first = side > 0 ? wide_n : wide_m, tiles_of = 2;
       double best = 1e30;
-      for (const Tile *t = first; t < first + (lds ? 3 : 1); ++t) {
+      for (const Tile *t = first; t < first + tiles_of; ++t) {
         const int64_t tiles = ((M + t->bm - 1) / t->bm) * ((N + t->bn - 1) / t->bn);
         for (int64_t s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
           if (s > 1 && (s * plane > most || steps < 4 * s || tiles * s > 1024)) break;
@@ -199,13 +206,14 @@ struct Product {
   int a_type, b_type, planes;
   bool shaped;   // strides and widths allow 16-byte loads
   bool forward;  // the product has kernels for few rows
+  int side;      // w's rows are columns (1) or rows (-1) of the result, or neither (0)
   Kind kind(bool vec) const {
     if (!forward || N >= (1 << 26) || K >= (1 << 30)) return TILES;
     return M <= LIN_ROWS ? ROWS : vec && lin_few_rows(M, N) ? FEW : TILES;
   }
   Plan plan_for(bool vec, size_t most) const {
     const int f32_by = b_type == LIN_BF16 ? 3 : b_type == LIN_F16 ? 5 : 6;
-    return plan(kind(vec), M, N, K, planes, a_type == LIN_F32 ? f32_by : 1, vec, most);
+    return plan(kind(vec), M, N, K, planes, a_type == LIN_F32 ? f32_by : 1, side, vec, most);
   }
   // partial sums of at most 64 MB
   size_t space() const { return plan_for(shaped, 64 << 20).part; }
@@ -213,7 +221,7 @@ struct Product {
 };
 Product forward(const zm_linear_desc &d) {
   return {d.S, d.O, d.I, d.x_type, d.w_type, 1,
-          vec_shape(d.x_stride, d.I, d.x_type, true) && vec_shape(d.w_stride, d.I, d.w_type, true), true};
+          vec_shape(d.x_stride, d.I, d.x_type, true) && vec_shape(d.w_stride, d.I, d.w_type, true), true, 1};
 }
 // What the products of the backward pass take for dz: dy itself; behind an activation f32 in the workspace; next to
 // bf16, where it is not bf16 itself, three planes of bf16 terms there.
@@ -229,11 +237,11 @@ int dz_type(const zm_linear_desc &d) {
 int64_t dz_ld(const zm_linear_desc &d) { return dz_form(d) == DZ_DY ? d.y_stride : (d.O + 7) / 8 * 8; }
 Product by_x(const zm_linear_desc &d) {
   return {d.S, d.I, d.O, dz_type(d), d.w_type, 1,
-          vec_shape(dz_ld(d), d.O, dz_type(d), true) && vec_shape(d.w_stride, d.I, d.w_type, false), false};
+          vec_shape(dz_ld(d), d.O, dz_type(d), true) && vec_shape(d.w_stride, d.I, d.w_type, false), false, 0};
 }
 Product by_w(const zm_linear_desc &d) {
   return {d.O, d.I, d.S, dz_type(d), d.x_type, dz_form(d) == DZ_TERMS ? 3 : 1,
-          vec_shape(dz_ld(d), d.O, dz_type(d), false) && vec_shape(d.x_stride, d.I, d.x_type, false), false};
+          vec_shape(dz_ld(d), d.O, dz_type(d), false) && vec_shape(d.x_stride, d.I, d.x_type, false), false, -1};
 }
 
 // chunks of rows of the bias gradient: 32 rows each, at most 256

@@ -227,15 +227,14 @@ struct Operand {
   static constexpr int R = KC ? 1 : 4 / (int)sizeof(T);  // rows of a unit
   static constexpr int CH = BK / 8;
   static constexpr int UNITS = ROWS / R * CH;
-  static constexpr int UPT = UNITS > NTHR ? UNITS / NTHR : 1;
+  static constexpr int UPT = (UNITS + NTHR - 1) / NTHR;
   static constexpr int NW = KC ? 2 * (int)sizeof(T) : 8;  // words of a unit
   static constexpr int PLANE = ROWS * BK;                 // 16-bit values of a term plane
-  static_assert(UNITS % NTHR == 0 || UNITS < NTHR, "units split evenly over the threads");
 
   const T *base;  // the tile's first row
   int64_t ld;
   int rows;       // of the matrix, from the tile's first row
-  int first;      // the thread's first unit (where there are fewer units than threads some are loaded and stored twice)
+  int first;      // the thread (where units and threads do not match some units are loaded and stored twice)
   int off[UPT];   // bytes from the tile's first row and column (16-byte loads)
   struct Raw {    // a step of the tile as it came from memory: the thread's units
     uint32_t r[UPT][NW];
@@ -246,7 +245,7 @@ struct Operand {
     ld = ld_;
     base = (const T *)p + (KC ? row0 * ld : row0);
     rows = (int)(total - row0 < ROWS ? total - row0 : ROWS);
-    first = t % UNITS;
+    first = t;
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       int row, c;
@@ -256,6 +255,7 @@ struct Operand {
     }
   }
   __device__ __forceinline__ static void place(int u, int &row, int &c) {
+    if (UNITS % NTHR) u %= UNITS;
     if (KC) {
       row = u / CH;
       c = u % CH;
@@ -1028,7 +1028,7 @@ void lin_few_of(const LinArgs &g, hipStream_t st) {
 }
 
 // The launch of one kernel instance.  `tile`: 0 = 128 x 128, 1 = 32 x 128, for 16-bit operands with 16-byte loads
-// (`vec`) 2 = 256 x 256 and 3 = 256 x 128.
+// (`vec`) 2 = 256 x 256 and 3 = 256 x 128; for f32 by f32 4 = 160 x 128 (gradient by w) or 128 x 160 (forward).
 template <class TA, int NA, bool KCA, class TB, int NB, bool KCB>
 void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices)), b(512);
@@ -1043,6 +1043,13 @@ void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
     else if (tile == 3) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 128, 4, 2>), grid, b, 0, st, g);
     else hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 128, 128, 2, 4>), grid, b, 0, st, g);
   } else {
+    if constexpr (NA * NB == 9 && KCA == KCB) {
+      if (tile == 4) {
+        constexpr int BM = KCA ? 128 : 160, BN = KCA ? 160 : 128, WM = KCA ? 4 : 2;
+        hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, BM, BN, WM, 8 / WM, true>), grid, b, 0, st, g);
+        return;
+      }
+    }
     hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 4, true>), grid, b, 0, st, g);
   }
 }
