@@ -273,7 +273,8 @@ int zm_combine_backward(const float *dout, const float *y, int64_t y_tok, int64_
   g.S = S;
   g.K = K;
   g.H = H;
-  const bool vec = !(H & 3) && quad(dout) && (!dweights || (!(y_tok & 3) && !(y_route & 3) && quad(y))) && (!dy || quad(dy));
+  const bool vec = !(H & 3) && quad(dout) && (!dweights || (!(y_tok & 3) && !(y_route & 3) && quad(y))) &&
+                   (!dy || quad(dy));
   const dim3 grid((unsigned)((S * K + 3) / 4));
   if (vec) hipLaunchKernelGGL((k_combine_backward<4>), grid, dim3(256), 0, (hipStream_t)stream, g);
   else hipLaunchKernelGGL((k_combine_backward<1>), grid, dim3(256), 0, (hipStream_t)stream, g);

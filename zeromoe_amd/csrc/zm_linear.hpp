@@ -198,7 +198,8 @@ static __global__ __launch_bounds__(256) void k_parts_sum(const float *__restric
     if (dst) dst[k < n0 ? k : k - n0] = a;
   }
 }
-static inline void parts_sum(const float *part, int parts, int64_t n, int64_t n0, float *dst0, float *dst1, hipStream_t st) {
+static inline void parts_sum(const float *part, int parts, int64_t n, int64_t n0, float *dst0, float *dst1,
+                             hipStream_t st) {
   if (!(n & 3) && !((uintptr_t)part & 15))
     hipLaunchKernelGGL((k_parts_sum<4>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, part, parts, n, n0, dst0, dst1);
   else
@@ -579,7 +580,8 @@ constexpr int DMA_BK = 64;
 
 template <bool KC, int ROWS, int NTHR, int FR>
 struct DmaOperand {
-  static constexpr int BK = DMA_BK, PER = ROWS * BK / 8 / NTHR, WIDE = ROWS / 8;  // 16-byte chunks of a thread; of a row of k
+  static constexpr int BK = DMA_BK;
+  static constexpr int PER = ROWS * BK / 8 / NTHR, WIDE = ROWS / 8;  // 16-byte chunks of a thread; of a row of k
   static constexpr int BYTES = ROWS * BK * 2;
   const uint16_t *base;
   int64_t ld;
@@ -611,7 +613,7 @@ struct DmaOperand {
     const int lane = threadIdx.x & 63, fr = lane & 15, fc = lane >> 4;
     if constexpr (KC) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) at[s] = 2 * ((w0 + fr) * BK + ((4 * s + fc) ^ (fr >> 1)) * 8);  // (w0 is a multiple of 16)
+      for (int s = 0; s < 2; ++s) at[s] = 2 * ((w0 + fr) * BK + ((4 * s + fc) ^ (fr >> 1)) * 8);  // (w0: 16 n)
     } else {
       const int k = 8 * fc + (fr >> 2);
 #pragma unroll
@@ -635,7 +637,8 @@ struct DmaOperand {
     } else {
       typedef __attribute__((address_space(3))) v4s *lp;
       const uint32_t q = lds + at[i] + 64 * ROWS * s;
-      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 8 * ROWS));
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q),
+                hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 8 * ROWS));
       return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
@@ -1056,7 +1059,7 @@ void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
 
 // the products by what their operands are: forward (x, w), dx (dz, w), dw (dz, x)
 void lin_rows(int x_type, int w_type, const LinArgs &g, hipStream_t st);  // M <= LIN_ROWS, any alignment
-void lin_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);   // where lin_few_rows(), operands with 16-byte loads
+void lin_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);   // where lin_few_rows(), by 16-byte loads
 void lin_fwd(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dx(int x_type, int w_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
 void lin_dw(int x_type, int dz_type, const LinArgs &g, bool vec, int tile, hipStream_t st);

@@ -485,7 +485,8 @@ int zm_layer_norm_backward(int type, const void *dy, int64_t dy_stride, const vo
     return 0;
   }
   if (!dy || !x || !mean || !rstd) return fail("zm_layer_norm_backward: null pointer");
-  if (x_stride < 0 || dy_stride < 0 || (dx && rows > 1 && dx_stride < n)) return fail("zm_layer_norm_backward: bad stride");
+  if (x_stride < 0 || dy_stride < 0 || (dx && rows > 1 && dx_stride < n))
+    return fail("zm_layer_norm_backward: bad stride");
   const bool sums = dweight || dbias;
   if (sums && (!workspace || ((uintptr_t)workspace & 15) || workspace_size < zm_layer_norm_backward_workspace_size(rows, n)))
     return fail("zm_layer_norm_backward: a 16-byte aligned workspace of zm_layer_norm_backward_workspace_size() bytes is needed");
