@@ -290,6 +290,20 @@ def test_linear_narrow_w(S, I, O):
     check_linear_backward(S, I, O, "f32", "f32", "gelu")
 
 
+@pytest.mark.parametrize("S,I,O", [(2100, 40, 2600), (2093, 520, 2603), (2500, 8, 2500), (16493, 264, 157)])
+def test_linear_f32_more_tiles_than_cus(S, I, O):
+    """More tiles of 128 x 128 than CUs: tiles of one buffer, two on a CU, and tiles of 160 rows of w (the last)."""
+    check_linear(S, I, O, "f32", "f32")
+    check_linear(S, I, O, "f32", "f32", "gelu", bias=False, residual=False, seed=41)
+
+
+@pytest.mark.parametrize("S,I,O", [(2100, 2600, 40), (2093, 2604, 520), (2500, 2500, 8), (259, 16516, 156)])
+def test_linear_backward_f32_more_tiles_than_cus(S, I, O):
+    """The same for the gradients: one buffer by x, tiles of 160 rows by w (the last)."""
+    check_linear_backward(S, I, O, "f32", "f32")
+    check_linear_backward(S, I, O, "f32", "f32", "silu", seed=21)
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_linear_backward_activations(act):
     check_linear_backward(70, 96, 56, "f32", "bf16", act)

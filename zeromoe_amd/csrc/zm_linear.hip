@@ -139,30 +139,37 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, 
       z = std::max<int64_t>(1, std::min<int64_t>(z, (int64_t)(most / plane)));
     } else {
       // The cheapest tile and number of slices by what they measured: us of a step with one tile a CU and, where two
-      // fit, with two; and a join of the slices at 5 TB/s with 4 us to start.
+      // fit, with two; us to start and end a tile (half more for two together); and a join of the slices at 5 TB/s
+      // with 4 us to start.
       struct Tile {
         int kind, bm, bn;
-        double one, two;
+        double one, two, start;
       };
-      static const Tile dma_tiles[] = {{2, 256, 256, 1.9, 0}, {3, 256, 128, 1.04, 0}, {0, 128, 128, 0.75, 1.09}};
-      static const Tile term_tiles[] = {{0, 128, 128, 1.0, 1.5}, {0, 128, 128, 1.2, 2.1}, {0, 128, 128, 1.3, 0}};
+      static const Tile dma_tiles[] = {
+          {2, 256, 256, 1.9, 0, 0}, {3, 256, 128, 1.04, 0, 0}, {0, 128, 128, 0.75, 1.09, 0}};
+      static const Tile term_tiles[] = {
+          {0, 128, 128, 1.0, 1.5, 0}, {0, 128, 128, 1.2, 2.1, 0}, {0, 128, 128, 1.3, 0, 0}};
       // w's side of a product may be narrow, as a router's is: 160 rows fill one tile of 160, and 62% of two of 128
       // (4095 rows by w of 160 x 5120: 74 -> 56 us, its gradient by w 84 -> 67; w of 288 x 2048 89 -> 72 and 99 -> 83)
-      static const Tile wide_n[] = {{0, 128, 128, 1.3, 0}, {4, 128, 160, 1.8, 0}};
-      static const Tile wide_m[] = {{0, 128, 128, 1.3, 0}, {4, 160, 128, 1.8, 0}};
+      static const Tile wide_m[] = {{0, 128, 128, 1.43, 0, 5.5}, {4, 160, 128, 1.8, 0, 8}};
+      // with one buffer two tiles share a CU, and one's start and end lie under the other's products: short k and more
+      // tiles than CUs (gradient by x of 4095 x 5120 with k = 160: 70 -> 57 us, of 2048 x 4096 with k = 512 58 -> 54;
+      // alone on its CU it takes 111 us where two buffers take 98, 2048^3)
+      static const Tile wide_n[] = {
+          {0, 128, 128, 1.43, 0, 5.5}, {5, 128, 128, 1.65, 2.88, 5.5}, {4, 128, 160, 1.8, 0, 8}};
       const bool lds = dma && vec;  // (without 16-byte loads 16-bit operands go through registers too)
       const Tile *first = lds ? dma_tiles : term_tiles + (products <= 3 ? 0 : products <= 5 ? 1 : 2);
       int tiles_of = lds ? 3 : 1;
-      if (products == 6 && vec && side) first = side > 0 ? wide_n : wide_m, tiles_of = 2;
+      if (products == 6 && vec) first = side < 0 ? wide_m : wide_n, tiles_of = side > 0 ? 3 : 2;
       double best = 1e30;
       for (const Tile *t = first; t < first + tiles_of; ++t) {
         const int64_t tiles = ((M + t->bm - 1) / t->bm) * ((N + t->bn - 1) / t->bn);
         for (int64_t s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
           if (s > 1 && (s * plane > most || steps < 4 * s || tiles * s > 1024)) break;
           const int64_t n = tiles * s;
-          const double rounds = t->two ? n / 512 * t->two + (n % 512 > 256 ? t->two : n % 512 ? t->one : 0.0)
-                                       : (double)((n + 255) / 256) * t->one;
-          const double us = rounds * (double)((steps + s - 1) / s) + (s > 1 ? 4.0 + s * plane * 2 / 5e6 : 0.0);
+          const double k = (double)((steps + s - 1) / s), one = t->one * k + t->start, two = t->two * k + 1.5 * t->start;
+          double us = t->two ? n / 512 * two + (n % 512 > 256 ? two : n % 512 ? one : 0.0) : (n + 255) / 256 * one;
+          us += s > 1 ? 4.0 + s * plane * 2 / 5e6 : 0.0;
           if (us < best) {
             best = us;
             z = s;

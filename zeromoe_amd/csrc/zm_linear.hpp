@@ -455,9 +455,11 @@ struct Pairs {
 // deep in LDS: while one is multiplied, the next one, in registers, is split into terms and stored, and the one after
 // that is on its way from memory; one barrier a step.  The instruction's rows are the results' columns n, so that a
 // lane ends with 4 neighbouring n of one row m.  f32 by f32, 2048^3: 95 us, 181 TFLOP/s of f32 products (1085 of bf16
-// ones), against 103 us with one buffer, the splitting in front of the products and two workgroups a CU.
-template <class TA, int NA, bool KCA, class TB, int NB, bool KCB, int BM, int BN, int WM, int WN, bool VEC>
-__global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
+// ones).  With one buffer (BUFS) the splitting follows the products, one step is on its way, and two workgroups of f32
+// by f32 share a CU (where there are two: 4096 x 5120 by k = 64 42 -> 35 us; alone 98 -> 111, 2048^3).
+template <class TA, int NA, bool KCA, class TB, int NB, bool KCB, int BM, int BN, int WM, int WN, bool VEC,
+          int BUFS = 2>
+__global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinArgs g) {
   constexpr bool F16 = std::is_same<TA, _Float16>::value && std::is_same<TB, _Float16>::value && NA == 1 && NB == 1;
   constexpr int BK = NA * NB == 1 ? 64 : 32;
   constexpr int NTHR = 64 * WM * WN;
@@ -465,7 +467,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
   typedef Operand<TA, NA, KCA, BM, BK, NTHR, VEC> OA;
   typedef Operand<TB, NB, KCB, BN, BK, NTHR, VEC> OB;
   constexpr int LA = NA * BM * BK, LDS = LA + NB * BN * BK;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2][LDS];
+  __shared__ __attribute__((aligned(16))) uint16_t lds[BUFS][LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int tile = xcd_order(blockIdx.x, gridDim.x);
   const int per = g.tiles_m * g.tiles_n;
@@ -513,7 +515,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
         for (int t = 0; t < NB; ++t)
           fb[j][t] = *reinterpret_cast<const v8bf *>(from + LA + t * BN * BK + r * BK + chunk_at<BK>(r, 4 * s + fc) * 8);
       }
-      if (s == BK / 32 - 1) {
+      if (BUFS == 2 && s == BK / 32 - 1) {
         a.store(to, next.a);
         b.store(to + LA, next.b);
       }
@@ -535,7 +537,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
         }
     }
 
-    if (NA * NB > 1) {
+    if (BUFS == 1) {
+      __syncthreads();
+      a.store(to, next.a);
+      b.store(to + LA, next.b);
+    } else if (NA * NB > 1) {
       // the splitting into terms goes between the products, which leave the vector units three of four issues
 #pragma unroll
       for (int i = 0; i < FM * FN * NA * NB; ++i) {
@@ -547,14 +553,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear(LinArgs g) {
   };
   Raw p, q;
   load(p);
-  load(q);
+  if (BUFS == 2) load(q);
   a.store(lds[0], p.a);
   b.store(lds[0] + LA, p.b);
   __syncthreads();
   for (int64_t t = 0; t < steps; t += 2) {
-    step(lds[0], lds[1], q, p);
+    step(lds[0], lds[BUFS - 1], BUFS == 2 ? q : p, p);
     if (t + 1 >= steps) break;
-    step(lds[1], lds[0], p, q);
+    step(lds[BUFS - 1], lds[0], p, BUFS == 2 ? q : p);
   }
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -1031,7 +1037,8 @@ void lin_few_of(const LinArgs &g, hipStream_t st) {
 }
 
 // The launch of one kernel instance.  `tile`: 0 = 128 x 128, 1 = 32 x 128, for 16-bit operands with 16-byte loads
-// (`vec`) 2 = 256 x 256 and 3 = 256 x 128; for f32 by f32 4 = 160 x 128 (gradient by w) or 128 x 160 (forward).
+// (`vec`) 2 = 256 x 256 and 3 = 256 x 128; for f32 by f32 4 = 160 x 128 (gradient by w) or 128 x 160 (forward)
+// and 5 = 128 x 128 with one buffer (forward, gradient by x).
 template <class TA, int NA, bool KCA, class TB, int NB, bool KCB>
 void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices)), b(512);
@@ -1046,6 +1053,12 @@ void lin_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
     else if (tile == 3) hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 256, 128, 4, 2>), grid, b, 0, st, g);
     else hipLaunchKernelGGL((k_linear_dma<F16, KCA, KCB, 128, 128, 2, 4>), grid, b, 0, st, g);
   } else {
+    if constexpr (NA * NB == 9 && KCA) {
+      if (tile == 5) {
+        hipLaunchKernelGGL((k_linear<TA, NA, KCA, TB, NB, KCB, 128, 128, 2, 4, true, 1>), grid, b, 0, st, g);
+        return;
+      }
+    }
     if constexpr (NA * NB == 9 && KCA == KCB) {
       if (tile == 4) {
         constexpr int BM = KCA ? 128 : 160, BN = KCA ? 160 : 128, WM = KCA ? 4 : 2;
