@@ -1,0 +1,63 @@
+"""The dense operators where a formula taken as it stands loses its digits or its infinities: rows that one expert
+dominates, values next to a border, infinities and NaN.  Against the definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_dense import ACTS, PAIRS, TYPES, U, act64, close, gate64, half_step, rand, route_grad64, slope64, sum_tol
+
+pytestmark = pytest.mark.gpu
+
+GATINGS = ["softmax", "sigmoid", "sqrt_softplus"]
+
+
+# ---------------------------------------------------------------- gradient of the routing
+
+
+@pytest.mark.parametrize("gating", GATINGS)
+@pytest.mark.parametrize("S,E", [(1, 1), (4, 60), (565, 200), (33, 384), (7, 1024)])
+def test_one_renormalised_route_has_no_gradient(S, E, gating):
+    """Its weight is a constant, so the gradient is 0 and not the rounding of a difference."""
+    import zeromoe_amd as Z
+
+    logits, dw = rand(S, E, seed=1, scale=1.5), rand(S, 1, seed=2)
+    ids, w = Z.router(logits, 1, gating=gating, weights_norm=True, weights_scale=2.5)
+    k = dict(gating=gating, weights_norm=True, weights_scale=2.5)
+    assert (Z.router_backward(logits, ids, dw, **k) == 0).all()
+    # the same route among others that take no part, and one expert named by every route
+    wide = torch.full((S, min(E, 4)), -1, device="cuda", dtype=torch.int32)
+    wide[:, -1:] = ids
+    assert (Z.router_backward(logits, wide, rand(*wide.shape, seed=3), **k) == 0).all()
+    twice, d2 = ids.expand(S, min(E, 2)).contiguous(), rand(S, min(E, 2), seed=4)
+    # the two routes' results are each other's negative but for a few roundings of dw / N
+    p = gate64(logits.double(), gating).gather(1, ids.long())
+    assert (Z.router_backward(logits, twice, d2, **k).abs() <= 16 * U * 2.5 * d2.abs().sum(-1, keepdim=True) / p).all()
+    # what a balance loss adds stays
+    dp = rand(E, seed=5)
+    got = Z.router_backward(logits, ids, dw, dprobs=dp, **k)
+    want = route_grad64(logits, ids, torch.zeros_like(dw), gating, None, True, 2.5, dp)
+    p = gate64(logits.double(), gating)
+    close(got, want, U * (40 + 2 * math.sqrt(E)) * (dp.abs().double() + (p * dp.abs().double()).sum(-1, keepdim=True)) * p * 2 + 1e-37)
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("gating", GATINGS)
+def test_a_dominated_row_keeps_its_digits(gating, norm):
+    """One expert has nearly all of the weight: every result, its own among them, to within roundings of itself.
+
+    A result is a product and quotient of sums without cancellation (the dw below have none), each of up to E terms of
+    one sign and one size: 2 log2 E roundings of pairwise sums, exp's argument up to 20 (20 roundings), exp, log1p and
+    the divisions a few each: 100 roundings cover them."""
+    import zeromoe_amd as Z
+
+    for E, seed in ((12, 1), (200, 2), (1000, 3)):
+        chosen = torch.randperm(E, generator=torch.Generator().manual_seed(seed))[:4].int().cuda()
+        logits = torch.full((1, E), -19.0, device="cuda") - rand(1, E, seed=seed).abs().clamp(max=1)
+        logits[0, chosen.long()] = torch.tensor([1.25, -12.0, -13.0, -12.5], device="cuda")
+        ids, dw = chosen[None].contiguous(), torch.tensor([[0.3, -0.5, 0.7, 0.2]], device="cuda")
+        got = Z.router_backward(logits, ids, dw, gating=gating, weights_norm=norm)
+        want = route_grad64(logits, ids, dw, gating, None, norm, 0.0, None)
+        if norm or gating != "softmax":  # the others' are 0
+            want = torch.zeros_like(want).scatter_(1, ids.long(), want.gather(1, ids.long()))
+        close(got, want, 100 * U * want.abs())

@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_router_backward(RouteGradA
       if (lane + 64 * i < g.E) out[lane + 64 * i] = bad ? __builtin_nanf("") : 0.f;
     return;
   }
-  float mx = -INF;
+  float mx = -INF, p_most = 0.f;  // p_most: softmax's largest probability, that of z = mx
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     z[i] += p[i];
@@ -164,6 +164,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_router_backward(RouteGradA
     }
     sum = group_sum<64>(sum);
     const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+    p_most = inv;
 #pragma unroll
     for (int i = 0; i < P; ++i) p[i] *= inv;
   } else {
@@ -187,12 +188,44 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_router_backward(RouteGradA
   __builtin_amdgcn_wave_barrier();
   const float pk = id >= 0 ? prob[wave][id] : 0.f;
   d *= g.scale;
+  bool flat = false;  // the weights' sum is constant: sum_e p g is 0 over the routes
   if (g.norm) {
-    const float total = group_sum<64>(pk), dot = group_sum<64>(d * pk);
-    const bool low = total < 6.103515625e-5f;
-    const float N = low ? 6.103515625e-5f : total;
-    d = id >= 0 ? (d - (low ? 0.f : dot / N)) / N : 0.f;
+    const float total = group_sum<64>(pk);
+    flat = !(total < 6.103515625e-5f);
+    float N = 6.103515625e-5f, dot = 0.f;
+    if (flat) {
+      // Taking one route's d off all of them changes nothing here.  That of the largest p is taken: its own result, a
+      // difference of two nearly equal numbers where it is most of the sum (and 0 where it is all of it), is then made
+      // of the other routes alone.
+      const uint64_t valid = __ballot(id >= 0);
+      const uint64_t largest = __ballot(id >= 0 && pk == wave_max(id >= 0 ? pk : -INF));
+      d = id >= 0 ? d - readlane_f(d, __builtin_ctzll(largest ? largest : valid)) : 0.f;
+      dot = group_sum<64>(d * pk);
+      N = total;
+    }
+    d = id >= 0 ? (d - dot / N) / N : 0.f;
   }
+  // softmax: g - sum p g.  Where one p is more than half of the row, its g is taken off all of them first (sum p is 1),
+  // for the same reason; with no such p the sum of two nearly equal numbers does not arise.
+  auto centre = [&] {
+    if (p_most > 0.5f) {
+      float r = 0.f;
+      bool here = false;
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if (z[i] == mx) r = gr[i], here = true;
+      r = readlane_f(r, __builtin_ctzll(__ballot(here)));
+#pragma unroll
+      for (int i = 0; i < P; ++i) gr[i] -= r;
+    }
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) dot += p[i] * gr[i];
+    dot = group_sum<64>(dot);
+#pragma unroll
+    for (int i = 0; i < P; ++i) gr[i] -= dot;
+  };
+  if (g.gating == 0 && flat && g.dprobs) centre();
   for (int k = 0; k < g.K; ++k) {  // in order: an expert named twice gets both
     const int ek = __builtin_amdgcn_readlane(id, k);
     const float dk = readlane_f(d, k);
@@ -200,12 +233,9 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_router_backward(RouteGradA
     for (int i = 0; i < P; ++i) gr[i] += ek == lane + 64 * i ? dk : 0.f;
   }
   if (g.gating == 0) {
-    float dot = 0.f;
+    if (!flat) centre();
 #pragma unroll
-    for (int i = 0; i < P; ++i) dot += p[i] * gr[i];
-    dot = group_sum<64>(dot);
-#pragma unroll
-    for (int i = 0; i < P; ++i) gr[i] = p[i] * (gr[i] - dot);
+    for (int i = 0; i < P; ++i) gr[i] *= p[i];
   } else {
 #pragma unroll
     for (int i = 0; i < P; ++i) gr[i] *= g.gating == 1 ? p[i] * (1.0f - p[i]) : u[i];
