@@ -61,3 +61,26 @@ def test_a_dominated_row_keeps_its_digits(gating, norm):
         if norm or gating != "softmax":  # the others' are 0
             want = torch.zeros_like(want).scatter_(1, ids.long(), want.gather(1, ids.long()))
         close(got, want, 100 * U * want.abs())
+
+
+# ---------------------------------------------------------------- infinities and NaN in the gradients of a product
+
+
+@pytest.mark.parametrize("S,I,O", [(9, 264, 40), (200, 96, 133), (300, 512, 256)])
+@pytest.mark.parametrize("act,ydt", [("none", None), ("none", "f32"), ("silu", None), ("gelu", "f32")])
+@pytest.mark.parametrize("xt,wt", PAIRS)
+def test_a_gradient_that_overflowed_shows(xt, wt, act, ydt, S, I, O):
+    """An infinity and a NaN in dy reach the rows of dx, the rows of dw and the entries of dbias that are theirs, and no
+    others: a check for overflow sees them wherever it looks."""
+    import zeromoe_amd as Z
+
+    x, w = rand(S, I, seed=1, dtype=TYPES[xt]), rand(O, I, seed=2, scale=0.02, dtype=TYPES[wt])
+    yt = TYPES[ydt or xt]
+    dy, pre = rand(S, O, seed=3, scale=0.01, dtype=yt), None if act == "none" else rand(S, O, seed=4, dtype=yt)
+    dy[2, 5], dy[7, 30] = float("inf"), float("nan")
+    dx, dw, db = Z.linear_backward(dy, x, w, act=act, pre=pre)
+    rows, cols = torch.zeros(S, device="cuda", dtype=torch.bool), torch.zeros(O, device="cuda", dtype=torch.bool)
+    rows[[2, 7]] = cols[[5, 30]] = True
+    assert not dx[rows].isfinite().any() and dx[~rows].isfinite().all()
+    assert not dw[cols].isfinite().any() and dw[~cols].isfinite().all()
+    assert not db[cols].isfinite().any() and db[~cols].isfinite().all()

@@ -73,8 +73,10 @@ __global__ __launch_bounds__(256) void k_linear_dz(DzArgs g) {
             bf16 e[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-              e[j] = from_f32<bf16>(k ? r[j] : __builtin_amdgcn_fmed3f(r[j], -BF16_MOST, BF16_MOST));
-              r[j] -= to_f32(e[j]);
+              // an infinity or a NaN is the first term (the gradient by x may read no other), the rest is 0
+              const bool finite = fabsf(r[j]) <= F32_MOST;
+              e[j] = from_f32<bf16>(k || !finite ? r[j] : __builtin_amdgcn_fmed3f(r[j], -BF16_MOST, BF16_MOST));
+              r[j] = finite ? r[j] - to_f32(e[j]) : 0.f;
             }
             if constexpr (V == 4) __builtin_memcpy(__builtin_assume_aligned(d, 8), e, 8);
             else *d = e[0];

@@ -127,6 +127,7 @@ __device__ __forceinline__ float lin_act_slope(float z, int act) {
 // ============================================================ terms
 
 constexpr float BF16_MOST = 3.38953139e38f;  // largest finite bf16
+constexpr float F32_MOST = 3.40282347e38f;   // largest finite f32
 
 // v[8] as NT bf16 terms, without a branch.  T is what the values came from: an f32 past bf16's largest is cut to that
 // for its first term (it would round to infinity and leave inf - inf behind); an infinity ends as a NaN term.
