@@ -84,3 +84,25 @@ def test_a_gradient_that_overflowed_shows(xt, wt, act, ydt, S, I, O):
     assert not dx[rows].isfinite().any() and dx[~rows].isfinite().all()
     assert not dw[cols].isfinite().any() and dw[~cols].isfinite().all()
     assert not db[cols].isfinite().any() and db[~cols].isfinite().all()
+
+
+@pytest.mark.parametrize("act", ACTS[1:])
+@pytest.mark.parametrize("xt,wt", PAIRS)
+def test_a_nan_before_the_activation_shows(xt, wt, act):
+    """Its result is NaN, and so are the gradients that it takes part in."""
+    import zeromoe_amd as Z
+
+    S, I, O = 40, 72, 24
+    x, w = rand(S, I, seed=1, dtype=TYPES[xt]), rand(O, I, seed=2, dtype=TYPES[wt])
+    dy, pre = rand(S, O, seed=3, dtype=TYPES[xt]), rand(S, O, seed=4, dtype=TYPES[xt])
+    pre[11, 6] = float("nan")
+    dx, dw, db = Z.linear_backward(dy, x, w, act=act, pre=pre)
+    rows, cols = torch.arange(S, device="cuda") == 11, torch.arange(O, device="cuda") == 6
+    assert dx[rows].isnan().all() and dx[~rows].isfinite().all()
+    assert dw[cols].isnan().all() and dw[~cols].isfinite().all()
+    assert db[cols].isnan().all() and db[~cols].isfinite().all()
+    for n in (1, 7, 40):  # the forward pass, by its kernels for few rows and many
+        y = x[:n].clone()
+        y[0, 3] = float("nan")
+        y = Z.linear(y, w, act=act)
+        assert y[0].isnan().all() and y[1:].isfinite().all()

@@ -100,6 +100,7 @@ __device__ __forceinline__ float lin_act(float z, int act) {
   }
 }
 __device__ __forceinline__ float lin_act_slope(float z, int act) {
+  if (z != z) return z;  // (the clamps and comparisons below would make a number of it)
   switch (act) {
   case ACT_RELU: return z > 0.f ? 1.0f : 0.0f;
   case ACT_GELU: {
