@@ -106,3 +106,46 @@ def test_a_nan_before_the_activation_shows(xt, wt, act):
         y[0, 3] = float("nan")
         y = Z.linear(y, w, act=act)
         assert y[0].isnan().all() and y[1:].isfinite().all()
+
+
+# ---------------------------------------------------------------- layer norm
+
+
+@pytest.mark.parametrize("xt", list(TYPES))
+@pytest.mark.parametrize("n", [72, 264, 1000, 2047, 4096, 5120, 7168, 8192, 20000])
+def test_layer_norm_of_small_spreads_far_from_zero(n, xt):
+    """Constant rows whose sums are not whole numbers of f32, and spreads of a millionth of the mean.
+
+    A first mean is off by D standard deviations, D = (4 + 2 sqrt n) 2^-24 mean|x| rstd, and every difference from it is
+    exact to 2^-24 of itself; their own mean is off by (4 + 2 sqrt n) 2^-24 of their size, 1 + D.  So h is off by as much,
+    and 1 / rstd^2 by as much of 1 + D^2.  The saved mean is rounded once, 2^-24 of it, and the gradients' h with it."""
+    import zeromoe_amd as Z
+
+    noise = rand(6, n, seed=1)
+    x = torch.stack([torch.full((n,), 12345.6), torch.full((n,), 3000.7), torch.full((n,), -0.1)]).cuda()
+    x = torch.cat([x, 1e4 + 0.01 * noise[:1], -3e3 + 0.1 * noise[1:2], 50 + 1e-3 * noise[2:3], noise[3:]]).to(TYPES[xt])
+    gain, shift, eps = 1 + 0.2 * rand(n, seed=2), rand(n, seed=3), 1e-5
+    y, mean, rstd = Z.layer_norm(x, gain, shift, eps=eps, stats=True)
+    x64 = x.double()
+    m64 = x64.mean(-1, keepdim=True)
+    r64 = 1 / torch.sqrt(x64.var(-1, unbiased=False, keepdim=True) + eps)
+    h64 = (x64 - m64) * r64
+    k = U * (4 + 2 * math.sqrt(n))
+    D = k * x64.abs().mean(-1, keepdim=True) * r64
+    htol = 4 * k * (1 + h64.abs()) * (1 + D) ** 2
+    y64 = h64 * gain.double() + shift.double()
+    last = half_step(x.dtype) * y64.abs() + (2.0 ** -25 if xt == "f16" else 0)
+    close(y, y64, htol * gain.double().abs() + 2 * U * (y64.abs() + shift.double().abs()) + last)
+    close(mean, m64[:, 0], (U * m64.abs() + 2 * k * (1 + D) / r64)[:, 0])
+    close(rstd, r64[:, 0], (4 * k * (1 + D) ** 2 * r64)[:, 0])
+    dy = rand(x.shape[0], n, seed=4, dtype=x.dtype)
+    dx, dw, db = Z.layer_norm_backward(dy, x, mean, rstd, gain)
+    hb = htol + U * m64.abs() * r64
+    g = dy.double() * gain.double()
+    s1, s2 = g.mean(-1, keepdim=True), (g * h64).mean(-1, keepdim=True)
+    want = r64 * (g - s1 - h64 * s2)
+    a = g.abs().mean(-1, keepdim=True)
+    ah = (g.abs() * h64.abs()).mean(-1, keepdim=True)
+    tol = r64 * (8 * k * (1 + D) ** 2 * (g.abs() + a + h64.abs() * ah) + hb * (s2.abs() + a) + (h64.abs() + hb) * (g.abs() * hb).mean(-1, keepdim=True))
+    close(dx, want, tol + half_step(x.dtype) * want.abs() + (2.0 ** -25 if xt == "f16" else 0))
+    close(dw, (dy.double() * h64).sum(0), (dy.double().abs() * (hb + 8 * U * h64.abs())).sum(0) + 1e-37)

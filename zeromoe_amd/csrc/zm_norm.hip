@@ -7,8 +7,10 @@
 //   dweight_i = sum_r dy_ri h_ri,  dbias_i = sum_r dy_ri
 //
 // Bound by memory: x in and y out; x and dy in and dx out.  A row sits in the registers of one workgroup (or one
-// wave), so it is read once; the variance is taken around the mean, not from the sum of squares, so a mean far from
-// zero costs no digits.  All sums are f32.
+// wave), so it is read once.  All sums are f32.  The sum's rounding leaves a first mean off by some 2^-24 of the values'
+// size, which is many standard deviations where a row's mean is far larger than its spread; so the differences from
+// it are summed too (next to their squares): their mean corrects the differences and the variance.  What is left of the
+// error is 2^-24 of the differences.  The saved mean is rounded to f32 once.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -57,6 +59,13 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[1]) {
   float a[1] = {v};
   row_sums<TPR, 1>(a, red);
   return a[0];
+}
+// d[0] = sum of d and d[1] = sum of d^2 over a row, d the differences from a first mean: what is to be taken off them,
+// and 1 / sqrt(variance + eps)
+__device__ __forceinline__ void row_stats(const float (&d)[2], float n, float eps, float &delta, float &rstd) {
+  delta = d[0] / n;
+  const float var = d[1] / n - delta * delta;
+  rstd = 1.0f / sqrtf((var < 0.f ? 0.f : var) + eps);  // (a NaN stays one)
 }
 
 // 16 bytes of T as floats
@@ -132,7 +141,7 @@ __device__ __forceinline__ void load_vec(const float *p, int i, int n, float oth
 template <class T, int NT, int TPR, int C, bool ALIGNED>
 __global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
   constexpr int V = Pack<T>::V, RPB = NT / TPR;
-  __shared__ float red[2][2][NT / 64][1];
+  __shared__ float red[2][NT / 64][1], red2[2][NT / 64][2];
   const int t = threadIdx.x & (TPR - 1);
   float w[C][V], b[C][V];
 #pragma unroll
@@ -165,28 +174,30 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int j = 0; j < V; ++j) sum += v[c][j];
-    const float mean = row_sum<TPR>(sum, red[par][0]) / n;
-    float sq = 0.f;
+    const float mean = row_sum<TPR>(sum, red[par]) / n;
+    float d[2] = {0.f, 0.f}, delta, rstd;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int i = (t + TPR * c) * V;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         v[c][j] = (ALIGNED ? i : i + j) < g.n ? v[c][j] - mean : 0.f;
-        sq = __builtin_fmaf(v[c][j], v[c][j], sq);
+        d[0] += v[c][j];
+        d[1] = __builtin_fmaf(v[c][j], v[c][j], d[1]);
       }
     }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, red[par][1]) / n + g.eps);
+    row_sums<TPR, 2>(d, red2[par]);
+    row_stats(d, n, g.eps, delta, rstd);
     T *y = (T *)g.y + row * g.ldy;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int i = (t + TPR * c) * V;
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[c][j] = __builtin_fmaf(v[c][j] * rstd, w[c][j], b[c][j]);
+      for (int j = 0; j < V; ++j) v[c][j] = __builtin_fmaf((v[c][j] - delta) * rstd, w[c][j], b[c][j]);
       store_pack<T, ALIGNED>(y, i, g.n, v[c]);
     }
     if (!t) {
-      if (g.mean) g.mean[row] = mean;
+      if (g.mean) g.mean[row] = mean + delta;
       if (g.rstd) g.rstd[row] = rstd;
     }
   }
@@ -195,25 +206,27 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs g) {
 // Rows too long for registers: read three times (the later ones from L2).
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_any(NormArgs g) {
-  __shared__ float red[2][4][1];
+  __shared__ float red[4][1], red2[4][2];
   const int64_t row = blockIdx.x;
   const T *x = (const T *)g.x + row * g.ldx;
   float sum = 0.f;
   for (int i = threadIdx.x; i < g.n; i += 256) sum += to_f32(x[i]);
-  const float mean = row_sum<256>(sum, red[0]) / (float)g.n;
-  float sq = 0.f;
+  const float mean = row_sum<256>(sum, red) / (float)g.n;
+  float s[2] = {0.f, 0.f}, delta, rstd;
   for (int i = threadIdx.x; i < g.n; i += 256) {
     const float d = to_f32(x[i]) - mean;
-    sq += d * d;
+    s[0] += d;
+    s[1] += d * d;
   }
-  const float rstd = 1.0f / sqrtf(row_sum<256>(sq, red[1]) / (float)g.n + g.eps);
+  row_sums<256, 2>(s, red2);
+  row_stats(s, (float)g.n, g.eps, delta, rstd);
   T *y = (T *)g.y + row * g.ldy;
   for (int i = threadIdx.x; i < g.n; i += 256) {
-    const float h = (to_f32(x[i]) - mean) * rstd;
+    const float h = (to_f32(x[i]) - mean - delta) * rstd;
     y[i] = from_f32<T>(h * (g.weight ? g.weight[i] : 1.0f) + (g.bias ? g.bias[i] : 0.0f));
   }
   if (!threadIdx.x) {
-    if (g.mean) g.mean[row] = mean;
+    if (g.mean) g.mean[row] = mean + delta;
     if (g.rstd) g.rstd[row] = rstd;
   }
 }
