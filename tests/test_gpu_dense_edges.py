@@ -149,3 +149,19 @@ def test_layer_norm_of_small_spreads_far_from_zero(n, xt):
     tol = r64 * (8 * k * (1 + D) ** 2 * (g.abs() + a + h64.abs() * ah) + hb * (s2.abs() + a) + (h64.abs() + hb) * (g.abs() * hb).mean(-1, keepdim=True))
     close(dx, want, tol + half_step(x.dtype) * want.abs() + (2.0 ** -25 if xt == "f16" else 0))
     close(dw, (dy.double() * h64).sum(0), (dy.double().abs() * (hb + 8 * U * h64.abs())).sum(0) + 1e-37)
+
+
+@pytest.mark.parametrize("n", [1, 7, 72, 100, 264, 2000, 4100])
+def test_layer_norm_backward_of_huge_constant_rows(n):
+    """Rows that are finite, and so are their gradients by the formula: h is 0, dx = rstd (g - mean g)."""
+    import zeromoe_amd as Z
+
+    dy = rand(4, n, seed=1, scale=1e-3)
+    x = torch.tensor([1e38 / n, -3e38 / n, 1e37 / n, 2.0], device="cuda")[:, None].expand(4, n).contiguous()
+    rstd = torch.full((4,), 1e3 * n, device="cuda")
+    dx, dw, db = Z.layer_norm_backward(dy, x, x[:, 0], rstd)
+    g = dy.double()
+    mean = g.mean(-1, keepdim=True)
+    close(dx, rstd.double()[:, None] * (g - mean), rstd.double()[:, None] * (sum_tol(n, g.abs().mean(-1, keepdim=True)) + 4 * U * (g.abs() + mean.abs())))
+    assert (dw == 0).all()
+    close(db, g.sum(0), sum_tol(4, g.abs().sum(0)))

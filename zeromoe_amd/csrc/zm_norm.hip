@@ -278,9 +278,11 @@ __global__ __launch_bounds__(NT) void k_norm_backward(NormArgs g) {
       float xv[V], gv[V];
       unpack<T>(rx[c], xv);
       unpack<T>(rg[c], gv);
+      const int i = (t + TPR * c) * V;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float h = (xv[j] - mean) * rstd;  // past n: dy is 0, so nothing is added
+        // past n dy is 0, and h too: mean rstd may be past f32's largest where the row's own h are not
+        const float h = (xv[j] - mean) * ((ALIGNED ? i : i + j) < g.n ? rstd : 0.f);
         const float gw = gv[j] * w[c][j];
         dw[c][j] = __builtin_fmaf(gv[j], h, dw[c][j]);
         db[c][j] += gv[j];
