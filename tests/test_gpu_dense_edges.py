@@ -165,3 +165,29 @@ def test_layer_norm_backward_of_huge_constant_rows(n):
     close(dx, rstd.double()[:, None] * (g - mean), rstd.double()[:, None] * (sum_tol(n, g.abs().mean(-1, keepdim=True)) + 4 * U * (g.abs() + mean.abs())))
     assert (dw == 0).all()
     close(db, g.sum(0), sum_tol(4, g.abs().sum(0)))
+
+
+@pytest.mark.parametrize("S,I,O", [(3, 64, 40), (40, 264, 100), (130, 512, 257), (600, 1000, 160), (2048, 256, 96)])
+@pytest.mark.parametrize("act,ydt", [("none", "f32"), ("gelu", None), ("silu", "f32")])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_a_16_bit_dx_keeps_sixteen_bits_of_dz(t, act, ydt, S, I, O):
+    """A gradient whose rows sum to about zero times a w whose rows are alike: the sum cancels, and what dz has lost
+    before it shows.  Two bf16 terms of dz leave out 2^-16 of |dz w| at most."""
+    import zeromoe_amd as Z
+
+    dtype, yt = TYPES[t], TYPES[ydt or t]
+    x = rand(S, I, seed=1, dtype=dtype)
+    w = (1.0 + 0.05 * rand(O, I, seed=2)).to(dtype)
+    pre = None if act == "none" else rand(S, O, seed=4, scale=1.5, dtype=yt)
+    slope = 1.0 if act == "none" else slope64(pre.double(), act)
+    dz = rand(S, O, seed=3).double()
+    # dz with a sum of zero: dy is that over the slope, where there is one to divide by
+    dz = dz - dz.mean(-1, keepdim=True)
+    dy = dz if act == "none" else dz / torch.where(slope.abs() < 0.05, torch.full_like(slope, 0.05), slope)
+    dy = dy.to(yt)
+    dx = Z.linear_backward(dy, x, w, act=act, pre=pre, need_dw=False, need_dbias=False)[0]
+    dz = dy.double() * slope
+    want = dz @ w.double()
+    absdot = (dz.abs() + (16 * U * dy.double().abs() if act != "none" else 0)) @ w.double().abs()
+    small = 2.0 ** -25 if t == "f16" else 0
+    close(dx, want, sum_tol(O, absdot) + (2.0 ** -16 + (16 * U if act != "none" else 0)) * absdot + half_step(dtype) * want.abs() + small)

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void k_linear_dz(DzArgs g) {
             bf16 e[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-              // an infinity or a NaN is the first term (the gradient by x may read no other), the rest is 0
+              // an infinity or a NaN is the first term, the rest is 0
               const bool finite = fabsf(r[j]) <= F32_MOST;
               e[j] = from_f32<bf16>(k || !finite ? r[j] : __builtin_amdgcn_fmed3f(r[j], -BF16_MOST, BF16_MOST));
               r[j] = finite ? r[j] - to_f32(e[j]) : 0.f;
@@ -213,6 +213,7 @@ bool vec_at(const void *p) { return !((uintptr_t)p & 15); }
 struct Product {
   int64_t M, N, K;
   int a_type, b_type, planes;
+  int64_t plane; // values from one plane of a to the next
   bool shaped;   // strides and widths allow 16-byte loads
   bool forward;  // the product has kernels for few rows
   int side;      // w's rows are columns (1) or rows (-1) of the result, or neither (0)
@@ -229,7 +230,7 @@ struct Product {
   Plan planned(bool vec) const { return plan_for(vec, vec == shaped ? 64 << 20 : space()); }
 };
 Product forward(const zm_linear_desc &d) {
-  return {d.S, d.O, d.I, d.x_type, d.w_type, 1,
+  return {d.S, d.O, d.I, d.x_type, d.w_type, 1, 0,
           vec_shape(d.x_stride, d.I, d.x_type, true) && vec_shape(d.w_stride, d.I, d.w_type, true), true, 1};
 }
 // What the products of the backward pass take for dz: dy itself; behind an activation f32 in the workspace; next to
@@ -245,11 +246,11 @@ int dz_type(const zm_linear_desc &d) {
 }
 int64_t dz_ld(const zm_linear_desc &d) { return dz_form(d) == DZ_DY ? d.y_stride : (d.O + 7) / 8 * 8; }
 Product by_x(const zm_linear_desc &d) {
-  return {d.S, d.I, d.O, dz_type(d), d.w_type, 1,
+  return {d.S, d.I, d.O, dz_type(d), d.w_type, dz_form(d) == DZ_TERMS ? 2 : 1, d.S * dz_ld(d),
           vec_shape(dz_ld(d), d.O, dz_type(d), true) && vec_shape(d.w_stride, d.I, d.w_type, false), false, 0};
 }
 Product by_w(const zm_linear_desc &d) {
-  return {d.O, d.I, d.S, dz_type(d), d.x_type, dz_form(d) == DZ_TERMS ? 3 : 1,
+  return {d.O, d.I, d.S, dz_type(d), d.x_type, dz_form(d) == DZ_TERMS ? 3 : 1, d.S * dz_ld(d),
           vec_shape(dz_ld(d), d.O, dz_type(d), false) && vec_shape(d.x_stride, d.I, d.x_type, false), false, -1};
 }
 
@@ -311,7 +312,7 @@ LinArgs product(const Product &q, const void *a, int64_t lda, const void *b, int
   g.N = q.N;
   g.K = q.K;
   g.planes = q.planes;
-  g.plane = q.planes > 1 ? q.K * lda : 0;
+  g.plane = q.plane;
   g.tiles_m = p.tiles_m;
   g.tiles_n = p.tiles_n;
   g.slices = p.slices;

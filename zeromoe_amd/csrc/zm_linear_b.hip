@@ -1,8 +1,9 @@
 // zm_linear_b.hip -- products of the gradient by x: dz [S][O] by w [O][I], k = O contiguous in dz, rows in w.
 //
 // The result has x's type.  Where that is 16 bits and dz is not (behind an activation, or from an f32 result), dz enters
-// with fewer terms: for bf16 its first bf16 term alone (its rounding, 2^-9, is the result's own), for f16 two of them
-// (2^-17 against the result's 2^-12; one f16 term could overflow or lose small gradients).
+// with two bf16 terms, 16 bits: what they leave out is 2^-16 of |dz w|, next to the result's own rounding of 2^-8 (bf16)
+// or 2^-11 (f16).  One term, 2^-8 of |dz w|, would be more than the result's rounding wherever the sum cancels (and one
+// f16 term could overflow or lose small gradients).
 #include <hip/hip_runtime.h>
 
 #include "zm_linear.hpp"
