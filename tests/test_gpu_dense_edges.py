@@ -191,3 +191,25 @@ def test_a_16_bit_dx_keeps_sixteen_bits_of_dz(t, act, ydt, S, I, O):
     absdot = (dz.abs() + (16 * U * dy.double().abs() if act != "none" else 0)) @ w.double().abs()
     small = 2.0 ** -25 if t == "f16" else 0
     close(dx, want, sum_tol(O, absdot) + (2.0 ** -16 + (16 * U if act != "none" else 0)) * absdot + half_step(dtype) * want.abs() + small)
+
+
+# ---------------------------------------------------------------- slopes
+
+
+def test_slope_of_a_saturated_sigmoid():
+    """sigmoid'(z) = sigmoid(z) sigmoid(-z) to within roundings of itself, also where sigmoid(z) is 1 in f32: exp of an
+    exact argument to two steps, a sum, a division and three products: 16 roundings cover them."""
+    import zeromoe_amd as Z
+
+    z = torch.cat([torch.linspace(-60, 60, 481), torch.tensor([16.6, 17.0, 25.0, 80.0])]).cuda()
+    slope = torch.sigmoid(z.double()) * torch.sigmoid(-z.double())
+    dy = rand(1, z.numel(), seed=1)
+    x, w = torch.zeros(1, 4, device="cuda"), torch.zeros(z.numel(), 4, device="cuda")
+    db = Z.linear_backward(dy, x, w, act="sigmoid", pre=z[None])[2]
+    want = dy[0].double() * slope
+    close(db, want, 16 * U * want.abs())
+    # as a gating: 97 rows of five experts, all of them routed
+    logits = z.view(97, 5)
+    ids, dw = torch.arange(5, device="cuda", dtype=torch.int32).expand(97, 5).contiguous(), rand(97, 5, seed=2)
+    want = dw.double() * slope.view(97, 5)
+    close(Z.router_backward(logits, ids, dw, gating="sigmoid"), want, 16 * U * want.abs())

@@ -8,7 +8,7 @@
 //   weights[k] = c p[e_k] / N,  N = max(sum_j p[e_j], 2^-14) where weights are normalised, else 1
 //   d_k = c dweights[k], less c sum_j dweights[j] p[e_j] / N where N is the sum; all over N
 //   g[e] = sum of d_k over the k with e_k = e, plus dprobs[e]
-//   softmax: dlogits = p (g - sum_e p g);  sigmoid: g p (1 - p);  sqrt-softplus: g sigmoid(z) / (2 p)
+//   softmax: dlogits = p (g - sum_e p g);  sigmoid: g sigmoid(z) sigmoid(-z);  sqrt-softplus: g sigmoid(z) / (2 p)
 // Routes with a negative id take no part: their row of y is not read.
 #include <hip/hip_runtime.h>
 
@@ -171,12 +171,13 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_router_backward(RouteGradA
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const float a = z[i];
-      const float q = 1.0f / (1.0f + expf(-a));
+      const float e = expf(-fabsf(a)), r = 1.0f / (1.0f + e), q = a < 0.f ? e * r : r;  // q: sigmoid
       if (g.gating == 1) {
         p[i] = q;
+        u[i] = e * r * r;  // (p (1 - p) has no digits left where p is near 1)
       } else {
         // far below zero softplus(z) is e^z to within f32, and its square root's slope half of that root
-        p[i] = a < -17.f ? expf(0.5f * a) : sqrtf(fmaxf(a, 0.f) + log1pf(expf(-fabsf(a))));
+        p[i] = a < -17.f ? expf(0.5f * a) : sqrtf(fmaxf(a, 0.f) + log1pf(e));
         u[i] = a < -17.f ? 0.5f * p[i] : q / (2.0f * p[i]);
       }
     }
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_router_backward(RouteGradA
     for (int i = 0; i < P; ++i) gr[i] *= p[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < P; ++i) gr[i] *= g.gating == 1 ? p[i] * (1.0f - p[i]) : u[i];
+    for (int i = 0; i < P; ++i) gr[i] *= u[i];
   }
 #pragma unroll
   for (int i = 0; i < P; ++i)

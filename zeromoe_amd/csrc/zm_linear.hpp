@@ -118,8 +118,8 @@ __device__ __forceinline__ float lin_act_slope(float z, int act) {
     return g * (1.0f + zc * (1.0f - g));
   }
   case ACT_SIGMOID: {
-    const float g = 1.0f / (1.0f + expf(-z));
-    return g * (1.0f - g);
+    const float e = expf(-fabsf(z)), r = 1.0f / (1.0f + e);
+    return e * r * r;  // sigmoid(z) sigmoid(-z): g (1 - g) has no digits left where g is near 1
   }
   default: return 1.0f;
   }
