@@ -342,8 +342,8 @@ int zm_expert_bad_counts(zm_expert_scratch *s, int32_t counts[2], int reset);
  *   x F32 with w F32, F16 or BF16; x F16 with w F16; x BF16 with w BF16
  *   y, residual and pre: F32 or x's type;  bias F32 [O]
  * f32 operands keep their 24 bits (they enter as sums of bf16 terms; below
- * 2^-110 what is left of a value after 2^-133 is lost); results are rounded once.  A row or column with an infinity or NaN gives non-finite
- * results.  pre (optional) receives x . w^T + bias for the backward pass.
+ * 2^-110 what is left of a value after 2^-133 is lost); results are rounded
+ * once.  Infinities and NaN give what the formula gives.  pre (optional) receives x . w^T + bias for the backward pass.
  * residual (optional) may be y itself.  S may be 0. */
 enum {
   ZM_ACT_NONE = 0,

@@ -213,3 +213,90 @@ def test_slope_of_a_saturated_sigmoid():
     ids, dw = torch.arange(5, device="cuda", dtype=torch.int32).expand(97, 5).contiguous(), rand(97, 5, seed=2)
     want = dw.double() * slope.view(97, 5)
     close(Z.router_backward(logits, ids, dw, gating="sigmoid"), want, 16 * U * want.abs())
+
+
+# ---------------------------------------------------------------- infinities in a product
+
+
+def products64(a, b):
+    """a b^T value by value (a library product may pad with zeros, and 0 inf is NaN)."""
+    return torch.stack([(a.double() * row.double()).sum(-1) for row in b], -1)
+
+
+def same(got, want, tol):
+    """Infinities and NaN where the formula has them; elsewhere within the tolerance."""
+    assert torch.equal(got.isnan(), want.isnan())
+    inf = want.isinf()
+    assert torch.equal(got.isinf(), inf) and (got[inf].double() == want[inf]).all()
+    ok = want.isfinite()
+    close(got[ok], want[ok], tol[ok])
+
+
+@pytest.mark.parametrize("I,O", [(72, 24), (520, 133), (2056, 40), (4100, 600)])
+@pytest.mark.parametrize("S", [2, 5, 24, 100, 300])
+@pytest.mark.parametrize("xt,wt", PAIRS)
+def test_infinities_go_by_the_formula(xt, wt, S, I, O):
+    """Whatever kernel the number of rows brings: an infinity times a weight is one of its sign, times zero NaN, and two
+    of both signs are NaN."""
+    import zeromoe_amd as Z
+
+    inf = float("inf")
+    x, w = rand(S, I, seed=1, dtype=TYPES[xt]), rand(O, I, seed=2, scale=0.05, dtype=TYPES[wt])
+    b = rand(O, seed=3)
+    x[0, 9] = inf
+    x[1, 3], x[1, I - 1] = -inf, inf
+    x[S - 1, 5] = -inf
+    w[4, 5] = w[7, 9] = 0.0  # times an infinity
+    w[11, 20], w[12, 21] = inf, float("nan")
+    xf, wf = torch.where(x.isfinite(), x, torch.zeros_like(x)), torch.where(w.isfinite(), w, torch.zeros_like(w))
+    tol = sum_tol(I, xf.double().abs() @ wf.double().abs().t() + b.double().abs())
+    want = products64(x, w) + b.double()
+    y, pre = Z.linear(x, w, bias=b, act="relu", out_dtype=torch.float32, save_pre=True)
+    same(pre, want, tol)
+    same(y, torch.where(want.isnan(), want, want.clamp(min=0)), tol)
+    p = torch.sigmoid(want)  # of an infinity 0 or 1
+    same(Z.linear(x, w, bias=b, act="sigmoid", out_dtype=torch.float32), p, tol + 8 * U)
+
+
+@pytest.mark.parametrize("S,I,O", [(3, 72, 40), (40, 264, 133), (300, 520, 72), (130, 1000, 640)])
+@pytest.mark.parametrize("act,ydt", [("none", None), ("none", "f32"), ("silu", None)])
+@pytest.mark.parametrize("xt,wt", PAIRS)
+def test_infinities_in_gradients_go_by_the_formula(xt, wt, act, ydt, S, I, O):
+    import zeromoe_amd as Z
+
+    inf, yt = float("inf"), TYPES[ydt or xt]
+    x, w = rand(S, I, seed=1, dtype=TYPES[xt]), rand(O, I, seed=2, scale=0.05, dtype=TYPES[wt])
+    dy, pre = rand(S, O, seed=3, dtype=yt), None if act == "none" else rand(S, O, seed=4, dtype=yt)
+    dy[0, 9], dy[1, 3], dy[1, O - 1] = inf, -inf, inf
+    w[9, 5] = x[0, 6] = 0.0
+    w[11, 20], x[S - 1, 30] = inf, -inf
+    slope = 1.0 if act == "none" else slope64(pre.double(), act)
+    dz = dy.double() * slope
+    z, xf, wf = (torch.where(t.isfinite(), t, torch.zeros_like(t)).double() for t in (dz, x, w))
+    # silu' = g (1 + z (1 - g)), |z| up to 4.5 here: g is off by up to 3 roundings (exp's of e^-z, the sum's, the
+    # quotient's), so z (1 - g) by 3 |z| and its own, and the slope by up to 16 2^-24 of 1, not of itself: it passes
+    # through 0 at z = -1.28.  dz is off by as much of |dy|, whatever is left of the sum
+    off = (16 * U if act != "none" else 0.0) * torch.where(dy.isfinite(), dy, torch.zeros_like(dy)).double().abs()
+    dx, dw, db = Z.linear_backward(dy, x, w, act=act, pre=pre)
+    t = z.abs() @ wf.abs()
+    want = products64(dz, w.t())
+    small = 2.0 ** -25 if xt == "f16" else 0
+    same(dx, want, sum_tol(O, t) + 2.0 ** -16 * t + off @ wf.abs() + half_step(dx.dtype) * (z @ wf).abs() + small)
+    t = z.abs().t() @ xf.abs()
+    same(dw, products64(dz.t(), x.t()), sum_tol(S, t) + off.t() @ xf.abs() + half_step(torch.float32) * t)
+    same(db, dz.sum(0), sum_tol(S, z.abs().sum(0)) + off.sum(0))
+
+
+def test_sums_whose_terms_overflow():
+    """Products of terms may pass f32's largest where the products of values and their sum do not."""
+    import zeromoe_amd as Z
+
+    for S in (2, 40, 200):
+        x = torch.zeros(S, 64, device="cuda")
+        x[:, 3], x[:, 8] = 2.0 ** 127 * 1.99, 1.0
+        w = torch.zeros(24, 64, device="cuda")
+        w[:, 3] = torch.linspace(0.9, 1.0048, 24)  # up to a hair below 2^128
+        y = Z.linear(x, w)
+        want = products64(x, w)
+        assert (want < 2.0 ** 128).all()
+        close(y, want, 2 * U * want.abs())

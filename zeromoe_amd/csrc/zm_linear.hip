@@ -73,10 +73,10 @@ __global__ __launch_bounds__(256) void k_linear_dz(DzArgs g) {
             bf16 e[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-              // an infinity or a NaN is the first term, the rest is 0
-              const bool finite = fabsf(r[j]) <= F32_MOST;
-              e[j] = from_f32<bf16>(k || !finite ? r[j] : __builtin_amdgcn_fmed3f(r[j], -BF16_MOST, BF16_MOST));
-              r[j] = finite ? r[j] - to_f32(e[j]) : 0.f;
+              // an infinity or a NaN is the first term (what follows it is NaN)
+              const float most = __builtin_amdgcn_fmed3f(r[j], -BF16_MOST, BF16_MOST);
+              e[j] = from_f32<bf16>(k || !(fabsf(r[j]) <= F32_MOST) ? r[j] : most);
+              r[j] -= to_f32(e[j]);
             }
             if constexpr (V == 4) __builtin_memcpy(__builtin_assume_aligned(d, 8), e, 8);
             else *d = e[0];
@@ -213,10 +213,11 @@ bool vec_at(const void *p) { return !((uintptr_t)p & 15); }
 struct Product {
   int64_t M, N, K;
   int a_type, b_type, planes;
-  int64_t plane; // values from one plane of a to the next
-  bool shaped;   // strides and widths allow 16-byte loads
-  bool forward;  // the product has kernels for few rows
-  int side;      // w's rows are columns (1) or rows (-1) of the result, or neither (0)
+  int64_t plane;    // values from one plane of a to the next
+  bool shaped;      // strides and widths allow 16-byte loads
+  bool a_kc, b_kc;  // k contiguous in a and in b, else rows
+  bool forward;     // the product has kernels for few rows
+  int side;         // w's rows are columns (1) or rows (-1) of the result, or neither (0)
   Kind kind(bool vec) const {
     if (!forward || N >= (1 << 26) || K >= (1 << 30)) return TILES;
     return M <= LIN_ROWS ? ROWS : vec && lin_few_rows(M, N) ? FEW : TILES;
@@ -231,7 +232,7 @@ struct Product {
 };
 Product forward(const zm_linear_desc &d) {
   return {d.S, d.O, d.I, d.x_type, d.w_type, 1, 0,
-          vec_shape(d.x_stride, d.I, d.x_type, true) && vec_shape(d.w_stride, d.I, d.w_type, true), true, 1};
+          vec_shape(d.x_stride, d.I, d.x_type, true) && vec_shape(d.w_stride, d.I, d.w_type, true), true, true, true, 1};
 }
 // What the products of the backward pass take for dz: dy itself; behind an activation f32 in the workspace; next to
 // bf16, where it is not bf16 itself, three planes of bf16 terms there.
@@ -247,11 +248,11 @@ int dz_type(const zm_linear_desc &d) {
 int64_t dz_ld(const zm_linear_desc &d) { return dz_form(d) == DZ_DY ? d.y_stride : (d.O + 7) / 8 * 8; }
 Product by_x(const zm_linear_desc &d) {
   return {d.S, d.I, d.O, dz_type(d), d.w_type, dz_form(d) == DZ_TERMS ? 2 : 1, d.S * dz_ld(d),
-          vec_shape(dz_ld(d), d.O, dz_type(d), true) && vec_shape(d.w_stride, d.I, d.w_type, false), false, 0};
+          vec_shape(dz_ld(d), d.O, dz_type(d), true) && vec_shape(d.w_stride, d.I, d.w_type, false), true, false, false, 0};
 }
 Product by_w(const zm_linear_desc &d) {
   return {d.O, d.I, d.S, dz_type(d), d.x_type, dz_form(d) == DZ_TERMS ? 3 : 1, d.S * dz_ld(d),
-          vec_shape(dz_ld(d), d.O, dz_type(d), false) && vec_shape(d.x_stride, d.I, d.x_type, false), false, -1};
+          vec_shape(dz_ld(d), d.O, dz_type(d), false) && vec_shape(d.x_stride, d.I, d.x_type, false), false, false, false, -1};
 }
 
 // chunks of rows of the bias gradient: 32 rows each, at most 256
@@ -318,6 +319,11 @@ LinArgs product(const Product &q, const void *a, int64_t lda, const void *b, int
   g.slices = p.slices;
   g.kslice = p.kslice;
   g.part = part;
+  g.terms = q.a_type == LIN_F32 || q.planes > 1;
+  g.a_kc = q.a_kc;
+  g.b_kc = q.b_kc;
+  g.a_type = q.a_type;
+  g.b_type = q.b_type;
   return g;
 }
 

@@ -99,8 +99,7 @@ __device__ __forceinline__ float lin_act(float z, int act) {
   default: return z;
   }
 }
-__device__ __forceinline__ float lin_act_slope(float z, int act) {
-  if (z != z) return z;  // (the clamps and comparisons below would make a number of it)
+__device__ __forceinline__ float lin_slope_of_number(float z, int act) {
   switch (act) {
   case ACT_RELU: return z > 0.f ? 1.0f : 0.0f;
   case ACT_GELU: {
@@ -123,6 +122,11 @@ __device__ __forceinline__ float lin_act_slope(float z, int act) {
   }
   default: return 1.0f;
   }
+}
+// (the clamps and comparisons above would make a number of a NaN)
+__device__ __forceinline__ float lin_act_slope(float z, int act) {
+  const float s = lin_slope_of_number(z, act);
+  return z == z ? s : z;
 }
 
 // ============================================================ terms
@@ -381,6 +385,9 @@ struct LinArgs {
   int64_t kslice;  // k of a slice; k_linear, k_linear_dma: steps of a slice
   float *part;     // [slices][M][N] when slices > 1
   LinEpilogue e;
+  bool terms;      // values enter as sums of terms: what follows says how they lie, for lin_again()
+  bool a_kc, b_kc; // k contiguous, else rows
+  int a_type, b_type;
 };
 
 __device__ __forceinline__ float lin_finish1(const LinEpilogue &e, int64_t m, int64_t n, float z) {
@@ -406,6 +413,64 @@ __device__ __forceinline__ void lin_finish4(const LinEpilogue &e, int64_t m, int
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (n + j < N) lin_store(e.y, e.type, (size_t)(m * e.ldy + n + j), lin_finish1(e, m, n + j, z[j]));
+}
+
+__device__ __forceinline__ bool lin_finite(float v) { return fabsf(v) <= F32_MOST; }
+// One sum again from the values themselves.  An infinity times a sum of terms is a sum of infinities of both signs or of
+// zero times one, so NaN stands where the formula may have an infinity, and terms' products may pass f32's largest where
+// their sum does not.  A sum that is not finite is taken again in f32, value by value: what an infinity gives does not go
+// by the number of rows or by the kernel.  Finite sums cost nothing (2048^3 in f32: 121 us, as before); with an infinity
+// in every row all of them are taken again, 16 ms; behind a NaN, where the sum stays one, 0.14 ms.
+__device__ __forceinline__ float lin_again(const LinArgs &g, int64_t m, int64_t n) {
+  const int64_t ak = g.a_kc ? 1 : g.lda, bk = g.b_kc ? 1 : g.ldb;
+  size_t ia = (size_t)(g.a_kc ? m * g.lda : m), ib = (size_t)(g.b_kc ? n * g.ldb : n);
+  float s = 0.f;
+  for (int64_t k = 0; k < g.K && s == s; k += 4, ia += 4 * ak, ib += 4 * bk) {
+    float a[4], b[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool in = k + u < g.K;
+      a[u] = in ? lin_load(g.a, g.a_type, ia + u * ak) : 0.f;
+      for (int p = 1; p < g.planes && lin_finite(a[u]); ++p)  // (an infinity or a NaN is its first term)
+        a[u] += in ? lin_load(g.a, g.a_type, ia + u * ak + p * g.plane) : 0.f;
+      b[u] = in ? lin_load(g.b, g.b_type, ib + u * bk) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s = __builtin_fmaf(a[u], b[u], s);
+  }
+  return s;
+}
+// sums of row m, columns n .. n + 3: those that are not finite again
+__device__ __forceinline__ void lin_repair(const LinArgs &g, int64_t m, int64_t n, v4f &v) {
+  if (m >= g.M || lin_finite((fabsf(v.x) + fabsf(v.y)) + (fabsf(v.z) + fabsf(v.w)))) return;
+#pragma unroll 1
+  for (int q = 0; q < 4; ++q) {
+    const float x = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
+    if (lin_finite(x) || n + q >= g.N) continue;
+    const float y = lin_again(g, m, n + q);
+    v.x = q == 0 ? y : v.x;
+    v.y = q == 1 ? y : v.y;
+    v.z = q == 2 ? y : v.z;
+    v.w = q == 3 ? y : v.w;
+  }
+}
+// the same for a wave's fragments, where there is one slice (else the slices' join does it); at(i, 0), at(j, 1): their m
+// and n; TERMS: whether the kernel's operands may come as terms
+template <bool TERMS, int FM, int FN, class At>
+__device__ __forceinline__ void lin_repair_all(const LinArgs &g, v4f (&acc)[FM][FN], const At &at) {
+  if (!TERMS || !g.terms || g.slices > 1) return;
+  float most = 0.f;  // (a sum past f32's largest is looked at again value by value)
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) most += fabsf(acc[i][j][q]);
+  if (__ballot(!lin_finite(most)) == 0) return;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) lin_repair(g, at(i, 0), at(j, 1), acc[i][j]);
 }
 
 // four sums of slice z: into its plane, or finished where there is one slice
@@ -564,6 +629,7 @@ __global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinA
     if (t + 1 >= steps) break;
     step(lds[BUFS - 1], lds[0], p, BUFS == 2 ? q : p);
   }
+  lin_repair_all<(NA * NB > 1 || !KCB), FM, FN>(g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -751,6 +817,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
   }
   wait_vm<0>();  // (what was asked for past the end writes zeros: not into another workgroup's LDS)
   const int fr = lane & 15, fc = lane >> 4;
+  lin_repair_all<!KCB, FM, FN>(g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -798,7 +865,9 @@ static __global__ __launch_bounds__(256) void k_linear_join(LinArgs g) {
 #pragma unroll
     for (int k = 1; k < G; ++k) v += red[k][threadIdx.x];
   }
-  if (in) lin_finish4(g.e, m, n, g.N, v);
+  if (!in) return;
+  if (g.terms) lin_repair(g, m, n, v);
+  lin_finish4(g.e, m, n, g.N, v);
 }
 static inline void lin_join(const LinArgs &g, hipStream_t st) {
   const int64_t quads = g.M * ((g.N + 3) / 4);
@@ -1013,6 +1082,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
     if (k + 2 * KS < ke) load(p, k + 2 * KS);
     step(q, lds[1]);
   }
+  lin_repair_all<(NX * NW > 1), MT, NF>(g, acc, [&](int i, int n) { return n ? n1 + 16 * i + 4 * fc : m0 + 16 * i + fr; });
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
