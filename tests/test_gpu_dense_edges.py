@@ -300,3 +300,35 @@ def test_sums_whose_terms_overflow():
         want = products64(x, w)
         assert (want < 2.0 ** 128).all()
         close(y, want, 2 * U * want.abs())
+
+
+# ---------------------------------------------------------------- arguments
+
+
+def test_a_gradient_does_not_end_silently():
+    """In grad mode a tensor that requires a gradient is refused by every call that takes it; under no_grad it is taken."""
+    import zeromoe_amd as Z
+
+    x, w, b, y3, wt = rand(4, 16), rand(8, 16), rand(8), rand(4, 2, 16), rand(4, 2)
+    dy, r = rand(4, 8), rand(4, 8)
+    ids = torch.zeros(4, 2, device="cuda", dtype=torch.int32)
+    _, mean, rstd = Z.layer_norm(x, stats=True)
+    calls = [(Z.linear, dict(x=x, w=w, bias=b, residual=r)), (Z.linear_backward, dict(dy=dy, x=x, w=w, act="silu", pre=r)),
+             (Z.layer_norm, dict(x=x, weight=x[0].clone(), bias=x[1].clone())),
+             (Z.layer_norm_backward, dict(dy=x.clone(), x=x, mean=mean, rstd=rstd, weight=x[0].clone())),
+             (Z.combine, dict(y=y3, weights=wt, residual=x)), (Z.combine_backward, dict(dout=x, y=y3, weights=wt, need_dy=True)),
+             (Z.router_backward, dict(logits=r, ids=ids, dweights=wt, logit_bias=b, dprobs=b.clone()))]
+    for f, args in calls:
+        want = f(**args)
+        want = want if isinstance(want, tuple) else (want,)
+        for name, t in args.items():
+            if not isinstance(t, torch.Tensor) or t is ids:
+                continue
+            p = dict(args, **{name: t.clone().requires_grad_()})
+            with pytest.raises(ValueError, match="requires a gradient"):
+                f(**p)
+            with pytest.raises(ValueError, match="requires a gradient"):
+                f(**p, stream=torch.cuda.Stream())
+            with torch.no_grad():
+                got = f(**p)
+            assert all(torch.equal(u, v) and not u.requires_grad for u, v in zip(got if isinstance(got, tuple) else (got,), want))

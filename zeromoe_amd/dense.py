@@ -3,7 +3,8 @@ its epilogue, the layer norm, the weighted sum of the experts' rows, and their g
 
 Device tensors in, device tensors out, on the current stream or on `stream`; outputs and workspaces come from torch's
 allocator for that stream, so a call may be captured into a graph.  Gradients are calls of their own: nothing here is
-recorded by autograd."""
+recorded by autograd, so a tensor that requires a gradient is refused unless torch.no_grad() (or a Function of the
+caller's around a pair of calls) says that none is expected."""
 from __future__ import annotations
 
 from typing import Optional
@@ -30,6 +31,17 @@ def _index(t: torch.Tensor, who: str) -> int:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{who}: device tensors are needed")
     return t.get_device()
+
+
+_grad_mode = torch.is_grad_enabled
+
+
+def _recorded(who: str, *tensors):
+    """Refuses, in grad mode, tensors whose gradient would silently end here."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{who}: an argument requires a gradient, which is not recorded here: call it under "
+                             "torch.no_grad() and take the gradient from its own call, or pass the tensor detached")
 
 
 def _there(fn, d: int, stream, *args):
@@ -111,6 +123,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias=None, act: str = "none", resid
     d = _index(x, "linear")
     if stream is not None or d != _device():
         return _there(linear, d, stream, x, w, bias, act, residual, out, out_dtype, save_pre)
+    if _grad_mode():
+        _recorded("linear", x, w, bias, residual, out)
     st = _raw_stream(d)
     _linear_types(d, x, w)
     S, I = x.shape
@@ -141,6 +155,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str
     d = _index(dy, "linear_backward")
     if stream is not None or d != _device():
         return _there(linear_backward, d, stream, dy, x, w, act, pre, need_dx, need_dw, need_dbias)
+    if _grad_mode():
+        _recorded("linear_backward", dy, x, w, pre)
     st = _raw_stream(d)
     _linear_types(d, x, w)
     S, I = x.shape
@@ -182,6 +198,8 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=N
     d = _index(x, "layer_norm")
     if stream is not None or d != _device():
         return _there(layer_norm, d, stream, x, weight, bias, eps, out, stats)
+    if _grad_mode():
+        _recorded("layer_norm", x, weight, bias, out)
     st = _raw_stream(d)
     _norm_rows(d, x)
     rows, n = x.shape
@@ -203,6 +221,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     d = _index(dy, "layer_norm_backward")
     if stream is not None or d != _device():
         return _there(layer_norm_backward, d, stream, dy, x, mean, rstd, weight, need_dx, need_dweight, need_dbias)
+    if _grad_mode():
+        _recorded("layer_norm_backward", dy, x, mean, rstd, weight)
     st = _raw_stream(d)
     _norm_rows(d, x)
     rows, n = x.shape
@@ -234,6 +254,8 @@ def combine(y: torch.Tensor, weights: torch.Tensor, ids=None, residual=None, out
     d = _index(y, "combine")
     if stream is not None or d != _device():
         return _there(combine, d, stream, y, weights, ids, residual, out)
+    if _grad_mode():
+        _recorded("combine", y, weights, residual, out)
     st = _raw_stream(d)
     y = _routes(y)
     S, K, H = y.shape
@@ -258,6 +280,8 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, weights=None, ids=None
     d = _index(dout, "combine_backward")
     if stream is not None or d != _device():
         return _there(combine_backward, d, stream, dout, y, weights, ids, need_dy)
+    if _grad_mode():
+        _recorded("combine_backward", dout, y, weights)
     st = _raw_stream(d)
     y = _routes(y)
     S, K, H = y.shape
@@ -287,6 +311,8 @@ def router_backward(logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Ten
     if stream is not None or d != _device():
         return _there(router_backward, d, stream, logits, ids, dweights, gating, logit_bias, weights_norm, weights_scale,
                       dprobs)
+    if _grad_mode():
+        _recorded("router_backward", logits, dweights, logit_bias, dprobs)
     st = _raw_stream(d)
     if logits.dim() != 2 or logits.dtype != _F32 or ids.dim() != 2:
         raise ValueError("logits (S, E) float32 and ids (S, K) are needed")
