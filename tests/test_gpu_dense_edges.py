@@ -332,3 +332,18 @@ def test_a_gradient_does_not_end_silently():
             with torch.no_grad():
                 got = f(**p)
             assert all(torch.equal(u, v) and not u.requires_grad for u, v in zip(got if isinstance(got, tuple) else (got,), want))
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Not taken for what their lower 32 bits say."""
+    import zeromoe_amd as Z
+
+    n = (1 << 32) + 1
+    one, i32 = torch.zeros(1, 1, device="cuda"), torch.zeros(1, 1, device="cuda", dtype=torch.int32)
+    for f in (lambda: Z.router_backward(one.expand(n, 1), i32.expand(n, 1), one.expand(n, 1)),
+              lambda: Z.combine(one.view(1, 1, 1).expand(1, 1, n), one),
+              lambda: Z.combine(one.view(1, 1, 1).expand(1, n, 1), one.expand(1, n)),
+              lambda: Z.router_backward(one.expand(1, n), i32, one),
+              lambda: Z.combine_backward(one.expand(1, n), one.view(1, 1, 1).expand(1, 1, n))):
+        with pytest.raises(ValueError, match="too large"):
+            f()

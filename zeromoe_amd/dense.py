@@ -66,6 +66,9 @@ def _need(t: torch.Tensor, what: str, d: int, dtypes, shape) -> torch.Tensor:
     return t
 
 
+_COUNTS = 1 << 31  # sizes from here on do not fit the C calls' 32-bit counts, which would take them for others
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` with contiguous columns; rows keep their stride."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
@@ -244,6 +247,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
 def _routes(y):
     if y.dim() != 3 or y.dtype != _F32:
         raise ValueError(f"y (S, K, H) float32 is needed, not {tuple(y.shape)} {y.dtype}")
+    if y.shape[1] >= _COUNTS or y.shape[2] >= _COUNTS:
+        raise ValueError(f"y of {tuple(y.shape)} is too large")
     return _rows(y)
 
 
@@ -316,9 +321,11 @@ def router_backward(logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Ten
     st = _raw_stream(d)
     if logits.dim() != 2 or logits.dtype != _F32 or ids.dim() != 2:
         raise ValueError("logits (S, E) float32 and ids (S, K) are needed")
-    logits = _flat(logits)
     S, E = logits.shape
     K = ids.shape[1]
+    if S >= _COUNTS or E >= _COUNTS or K >= _COUNTS:
+        raise ValueError(f"logits of {tuple(logits.shape)} or ids of {tuple(ids.shape)} are too large")
+    logits = _flat(logits)
     ids = _flat(_need(ids, "ids", d, _I32S, (S, K)))
     dweights = _flat(_need(dweights, "dweights", d, _F32S, (S, K)))
     logit_bias, dprobs = _vector(logit_bias, "logit_bias", d, E), _vector(dprobs, "dprobs", d, E)
