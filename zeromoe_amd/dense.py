@@ -36,12 +36,9 @@ def _index(t: torch.Tensor, who: str) -> int:
 _grad_mode = torch.is_grad_enabled
 
 
-def _recorded(who: str, *tensors):
-    """Refuses, in grad mode, tensors whose gradient would silently end here."""
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            raise ValueError(f"{who}: an argument requires a gradient, which is not recorded here: call it under "
-                             "torch.no_grad() and take the gradient from its own call, or pass the tensor detached")
+def _not_recorded(who: str):
+    raise ValueError(f"{who}: an argument requires a gradient, which is not recorded here: call it under torch.no_grad() "
+                     "and take the gradient from its own call, or pass the tensor detached")
 
 
 def _there(fn, d: int, stream, *args):
@@ -126,8 +123,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias=None, act: str = "none", resid
     d = _index(x, "linear")
     if stream is not None or d != _device():
         return _there(linear, d, stream, x, w, bias, act, residual, out, out_dtype, save_pre)
-    if _grad_mode():
-        _recorded("linear", x, w, bias, residual, out)
+    if _grad_mode() and (x.requires_grad or w.requires_grad or bias is not None and bias.requires_grad
+                         or residual is not None and residual.requires_grad or out is not None and out.requires_grad):
+        _not_recorded("linear")
     st = _raw_stream(d)
     _linear_types(d, x, w)
     S, I = x.shape
@@ -158,8 +156,9 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str
     d = _index(dy, "linear_backward")
     if stream is not None or d != _device():
         return _there(linear_backward, d, stream, dy, x, w, act, pre, need_dx, need_dw, need_dbias)
-    if _grad_mode():
-        _recorded("linear_backward", dy, x, w, pre)
+    if _grad_mode() and (dy.requires_grad or x.requires_grad or w.requires_grad
+                         or pre is not None and pre.requires_grad):
+        _not_recorded("linear_backward")
     st = _raw_stream(d)
     _linear_types(d, x, w)
     S, I = x.shape
@@ -201,8 +200,9 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=N
     d = _index(x, "layer_norm")
     if stream is not None or d != _device():
         return _there(layer_norm, d, stream, x, weight, bias, eps, out, stats)
-    if _grad_mode():
-        _recorded("layer_norm", x, weight, bias, out)
+    if _grad_mode() and (x.requires_grad or weight is not None and weight.requires_grad
+                         or bias is not None and bias.requires_grad or out is not None and out.requires_grad):
+        _not_recorded("layer_norm")
     st = _raw_stream(d)
     _norm_rows(d, x)
     rows, n = x.shape
@@ -224,8 +224,9 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     d = _index(dy, "layer_norm_backward")
     if stream is not None or d != _device():
         return _there(layer_norm_backward, d, stream, dy, x, mean, rstd, weight, need_dx, need_dweight, need_dbias)
-    if _grad_mode():
-        _recorded("layer_norm_backward", dy, x, mean, rstd, weight)
+    if _grad_mode() and (dy.requires_grad or x.requires_grad or mean.requires_grad or rstd.requires_grad
+                         or weight is not None and weight.requires_grad):
+        _not_recorded("layer_norm_backward")
     st = _raw_stream(d)
     _norm_rows(d, x)
     rows, n = x.shape
@@ -259,8 +260,9 @@ def combine(y: torch.Tensor, weights: torch.Tensor, ids=None, residual=None, out
     d = _index(y, "combine")
     if stream is not None or d != _device():
         return _there(combine, d, stream, y, weights, ids, residual, out)
-    if _grad_mode():
-        _recorded("combine", y, weights, residual, out)
+    if _grad_mode() and (y.requires_grad or weights.requires_grad or residual is not None and residual.requires_grad
+                         or out is not None and out.requires_grad):
+        _not_recorded("combine")
     st = _raw_stream(d)
     y = _routes(y)
     S, K, H = y.shape
@@ -285,8 +287,8 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, weights=None, ids=None
     d = _index(dout, "combine_backward")
     if stream is not None or d != _device():
         return _there(combine_backward, d, stream, dout, y, weights, ids, need_dy)
-    if _grad_mode():
-        _recorded("combine_backward", dout, y, weights)
+    if _grad_mode() and (dout.requires_grad or y.requires_grad or weights is not None and weights.requires_grad):
+        _not_recorded("combine_backward")
     st = _raw_stream(d)
     y = _routes(y)
     S, K, H = y.shape
@@ -316,8 +318,10 @@ def router_backward(logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Ten
     if stream is not None or d != _device():
         return _there(router_backward, d, stream, logits, ids, dweights, gating, logit_bias, weights_norm, weights_scale,
                       dprobs)
-    if _grad_mode():
-        _recorded("router_backward", logits, dweights, logit_bias, dprobs)
+    if _grad_mode() and (logits.requires_grad or dweights.requires_grad
+                         or logit_bias is not None and logit_bias.requires_grad
+                         or dprobs is not None and dprobs.requires_grad):
+        _not_recorded("router_backward")
     st = _raw_stream(d)
     if logits.dim() != 2 or logits.dtype != _F32 or ids.dim() != 2:
         raise ValueError("logits (S, E) float32 and ids (S, K) are needed")
