@@ -327,8 +327,8 @@ int zm_expert_bad_counts(zm_expert_scratch *s, int32_t counts[2], int reset);
  * What a block has next to its routed experts, with the gradients of a step
  * that trains the router and the norm over frozen quantized experts: the
  * unquantized matrix product (router, shared expert, attention output), the
- * layer norm, the weighted sum of the experts' rows and the gradient of the
- * routing.  No counterpart among the reference's kernels; the products of
+ * layer norm (with mean and bias; an RMS norm is not here), the weighted sum of
+ * the experts' rows and the gradient of the routing.  No counterpart among the reference's kernels; the products of
  * quantized weights are zm_f32_matmul and zm_mul_mat_id.
  *
  * Types are F32, F16 and BF16; all sums are f32 in a fixed order, so a call
@@ -342,8 +342,8 @@ int zm_expert_bad_counts(zm_expert_scratch *s, int32_t counts[2], int reset);
  *   x F32 with w F32, F16 or BF16; x F16 with w F16; x BF16 with w BF16
  *   y, residual and pre: F32 or x's type;  bias F32 [O]
  * f32 operands keep their 24 bits (they enter as sums of bf16 terms; below
- * 2^-110 what is left of a value after 2^-133 is lost); results are rounded
- * once.  Infinities and NaN give what the formula gives.  pre (optional) receives x . w^T + bias for the backward pass.
+ * 2^-110 what is left of a value after 2^-133 is lost), a product of two of them
+ * is off by 2^-23 of itself at most; results are rounded once.  Infinities and NaN give what the formula gives.  pre (optional) receives x . w^T + bias for the backward pass.
  * residual (optional) may be y itself.  S may be 0. */
 enum {
   ZM_ACT_NONE = 0,
@@ -365,16 +365,18 @@ int zm_linear(const zm_linear_desc *desc, const void *x, const void *w, const fl
 /* Gradients by dy [S][O]: dz = dy act'(pre), dx = dz w [S][I] of x's type,
  * dw = dz^T x [O][I] f32, dbias = sum_s dz [O] f32; each is skipped when NULL,
  * contiguous otherwise (the residual's gradient is dy).  pre is needed with an
- * activation.  With S == 0 dw and dbias are zero.  x is read for dw alone, w
- * for dx alone. */
+ * activation.  dz is f32; next to a 16-bit x dx takes 16 bits of it (2^-16 of
+ * |dz| |w|, before the result's own rounding), unless it is a dy of x's type.
+ * With S == 0 dw and dbias are zero.  x is read for dw alone, w for dx alone. */
 size_t zm_linear_backward_workspace_size(const zm_linear_desc *desc);
 int zm_linear_backward(const zm_linear_desc *desc, const void *dy, const void *x, const void *w, const void *pre,
                        void *dx, float *dw, float *dbias, void *workspace, size_t workspace_size, void *stream);
 
 /* y[r] = (x[r] - mean_r) rstd_r weight + bias over rows of n values,
  * rstd = 1 / sqrt(variance + eps); x and y of `type`, weight and bias F32 [n]
- * (NULL: 1 and 0); mean and rstd F32 [rows] (optional) for the backward pass.
- * y may be x. */
+ * (NULL: 1 and 0); mean and rstd F32 [rows] (optional) for the backward pass,
+ * each rounded to f32 once: y itself does not lose by a mean far larger than the
+ * spread, h in the backward pass is off by 2^-24 |mean| rstd.  y may be x. */
 int zm_layer_norm(int type, const void *x, int64_t x_stride, const float *weight, const float *bias, float eps,
                   int64_t rows, int64_t n, void *y, int64_t y_stride, float *mean, float *rstd, void *stream);
 /* dx [rows][n] of `type`, dweight and dbias F32 [n], each skipped when NULL.
@@ -401,7 +403,7 @@ int zm_combine_backward(const float *dout, const float *y, int64_t y_tok, int64_
 
 /* Gradient of zm_router's weights by its logits, the selection held fixed:
  * dlogits [S][E] from dweights [S][K].  ids are expert ids, those zm_router
- * gives without a slot table (an expert named twice counts twice); a negative
+ * gives without a slot table or a mask (an expert named twice counts twice); a negative
  * one takes no part, a row of them alone (padding) has a zero gradient, and an
  * id >= n_experts gives a NaN row.  dprobs [E] (optional) is added to the
  * gradient of every token's gate probabilities (a balance loss on their mean;

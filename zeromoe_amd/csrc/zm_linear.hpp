@@ -7,9 +7,10 @@
 //   v = t0 + t1 + t2,  t0 = bf16(v), t1 = bf16(v - t0), t2 = bf16(v - t0 - t1)
 // (3 x 8 significant bits cover the 24 of f32; the differences are exact), an f16
 // value as two (11 bits), a bf16 value as one.  A product of two sums keeps the
-// term pairs (i, j) with i + j <= 2 (each next pair is 2^-9 smaller with
-// round-to-nearest terms; what is left out is below 2^-26 of |a||b|): 6 bf16
-// products for f32 x f32, 5 for f32 x f16, 3 for f32 x bf16, accumulated in f32.
+// term pairs (i, j) with i + j <= 2: 6 bf16 products for f32 x f32, 5 for
+// f32 x f16, 3 for f32 x bf16, accumulated in f32.  A term is at most 2^-8 of the
+// one before it, so the pairs left out, (1, 2) and (2, 1), are at most 2^-23 of
+// |a||b| (2^-24.2 in 2e7 products of values from [1, 2)).
 // bf16 x bf16 and f16 x f16 are one product in their own type.
 #pragma once
 
@@ -419,8 +420,9 @@ __device__ __forceinline__ bool lin_finite(float v) { return fabsf(v) <= F32_MOS
 // One sum again from the values themselves.  An infinity times a sum of terms is a sum of infinities of both signs or of
 // zero times one, so NaN stands where the formula may have an infinity, and terms' products may pass f32's largest where
 // their sum does not.  A sum that is not finite is taken again in f32, value by value: what an infinity gives does not go
-// by the number of rows or by the kernel.  Finite sums cost nothing (2048^3 in f32: 121 us, as before); with an infinity
-// in every row all of them are taken again, 16 ms; behind a NaN, where the sum stays one, 0.14 ms.
+// by the number of rows or by the kernel.  Finite sums cost a check (2048^3 in f32: 108 us with and without it); with an
+// infinity in every row all of them are taken again, 16 ms (512 x 4096 x 4096, f32 by bf16: 32); behind a NaN, where the
+// sum stays one, 0.14 ms.
 __device__ __forceinline__ float lin_again(const LinArgs &g, int64_t m, int64_t n) {
   const int64_t ak = g.a_kc ? 1 : g.lda, bk = g.b_kc ? 1 : g.ldb;
   size_t ia = (size_t)(g.a_kc ? m * g.lda : m), ib = (size_t)(g.b_kc ? n * g.ldb : n);
@@ -512,11 +514,8 @@ struct LinSteps {
   }
 };
 
-// The term pairs of a product: (0,0) first, then those 2^-9, 2^-18 smaller
-template <int NA, int NB>
-struct Pairs {
-  static constexpr int MOST = 2;  // i + j
-};
+// The term pairs (i, j) of a product: (0, 0) first, then those 2^-8 and 2^-16 smaller, up to this i + j
+constexpr int PAIRS_MOST = 2;
 
 // One workgroup: BM x BN results over one slice of k; WM x WN waves of 16 x 16 matrix instructions.  Two steps of BK
 // deep in LDS: while one is multiplied, the next one, in registers, is split into terms and stored, and the one after
@@ -590,7 +589,7 @@ __global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinA
       for (int ta = 0; ta < NA; ++ta)
 #pragma unroll
         for (int tb = 0; tb < NB; ++tb) {
-          if (ta + tb > Pairs<NA, NB>::MOST) continue;
+          if (ta + tb > PAIRS_MOST) continue;
 #pragma unroll
           for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -1060,7 +1059,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
           const v8bf tx = *reinterpret_cast<const v8bf *>(to + a * PLANE + r * KS + chunk_at<KS>(r, 4 * h + fc) * 8);
 #pragma unroll
           for (int b = 0; b < NW; ++b) {
-            if (a + b > Pairs<NX, NW>::MOST) continue;
+            if (a + b > PAIRS_MOST) continue;
 #pragma unroll
             for (int j = 0; j < NF; ++j) {
               if constexpr (F16)

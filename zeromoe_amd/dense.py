@@ -152,7 +152,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str
                     need_dx: bool = True, need_dw: bool = True, need_dbias: bool = True, stream=None):
     """(dx, dw, dbias) of linear() for dy (S, O), its gradient by the result: dx (S, I) of x's type, dw (O, I) and
     dbias (O) float32; None in the place of one that is not needed.  The residual's gradient is dy itself.  pre: what
-    linear(save_pre=True) returned, needed with an activation.  (zm_linear_backward)"""
+    linear(save_pre=True) returned, needed with an activation.  Behind an activation, or from a float32 dy, a 16-bit dx
+    takes 16 bits of dy act'(pre).  (zm_linear_backward)"""
     d = _index(dy, "linear_backward")
     if stream is not None or d != _device():
         return _there(linear_backward, d, stream, dy, x, w, act, pre, need_dx, need_dw, need_dbias)
@@ -311,7 +312,7 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, weights=None, ids=None
 def router_backward(logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Tensor, gating="softmax",
                     logit_bias=None, weights_norm: bool = False, weights_scale: float = 0.0, dprobs=None, stream=None):
     """The gradient of router()'s weights by its logits (S, E) float32, the selection held fixed: ids (S, K) int32 are
-    expert ids (router() without a slot table), dweights (S, K).  A negative id takes no part; a row of them alone has
+    expert ids (router() without a slot table or a mask), dweights (S, K).  A negative id takes no part; a row of them alone has
     a zero gradient.  dprobs (E): added to the gradient of every routed token's gate probabilities, as a balance loss
     on their mean has it.  The gradient by logit_bias is the result's sum over the tokens.  (zm_router_backward)"""
     d = _index(logits, "router_backward")
