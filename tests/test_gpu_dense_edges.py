@@ -347,3 +347,107 @@ def test_sizes_past_32_bits_are_refused():
               lambda: Z.combine_backward(one.expand(1, n), one.view(1, 1, 1).expand(1, 1, n))):
         with pytest.raises(ValueError, match="too large"):
             f()
+
+
+# ---------------------------------------------------------------- allowed calls that are not the usual ones
+
+
+@pytest.mark.parametrize("xt,wt", PAIRS)
+@pytest.mark.parametrize("S,I,O", [(1, 264, 72), (5, 72, 40), (50, 264, 72), (300, 72, 264), (257, 1000, 40)])
+def test_linear_backward_of_strided_rows_on_any_address(xt, wt, S, I, O):
+    """dy, x, w and pre as columns of wider buffers, on even and odd addresses: the results of contiguous copies, but for
+    the order of sums that another kernel has; and the neighbours of nothing are read as values."""
+    import zeromoe_amd as Z
+
+    def view(n, width, off, pad, seed, dtype, scale=1.0):
+        b = torch.full((n * (width + pad) + 16,), float("nan"), device="cuda", dtype=dtype)
+        v = b[off:off + n * (width + pad)].view(n, width + pad)[:, :width]
+        return v.copy_(rand(n, width, seed=seed, dtype=dtype, scale=scale))
+
+    for off, pad in ((0, 8), (1, 3), (4, 4), (1, 8)):
+        for act, ydt in (("none", None), ("silu", None), ("gelu_tanh", "f32")):
+            yt = TYPES[ydt or xt]
+            x, w = view(S, I, off, pad, 1, TYPES[xt]), view(O, I, off, pad, 2, TYPES[wt], 0.05)
+            dy, pre = view(S, O, off, pad, 3, yt, 0.1), view(S, O, off, pad + 8, 4, yt)
+            dx, dw, db = Z.linear_backward(dy, x, w, act=act, pre=pre)
+            slope = 1.0 if act == "none" else slope64(pre.double(), act)
+            dz = dy.double() * slope
+            offs = (16 * U if act != "none" else 0.0) * dy.double().abs()  # the slope's own roundings, of 1
+            t = dz.abs() @ w.double().abs()
+            want = dz @ w.double()
+            close(dx, want, sum_tol(O, t) + (2.0 ** -16 if xt != "f32" else 0) * t + offs @ w.double().abs()
+                  + half_step(dx.dtype) * want.abs() + (2.0 ** -25 if xt == "f16" else 0))
+            t = dz.abs().t() @ x.double().abs()
+            close(dw, dz.t() @ x.double(), sum_tol(S, t) + offs.t() @ x.double().abs() + U * t)
+            close(db, dz.sum(0), sum_tol(S, dz.abs().sum(0)) + offs.sum(0))
+
+
+@pytest.mark.parametrize("xt,wt", PAIRS)
+@pytest.mark.parametrize("S", [1, 3, 20, 130, 700])
+def test_linear_strided_residual_pre_and_repeated_weight_rows(S, xt, wt):
+    import zeromoe_amd as Z
+
+    I, O = 2056, 72
+    x, w = rand(S, I, seed=1, dtype=TYPES[xt]), rand(1, I, seed=2, scale=0.02, dtype=TYPES[wt]).expand(O, I)
+    for dtype in {TYPES[xt], torch.float32}:
+        for off, pad in ((0, 8), (3, 5)):
+            r = rand(S, O + off + pad, seed=3, dtype=dtype)[:, off:off + O]
+            y, pre = Z.linear(x, w, residual=r, act="relu", out_dtype=dtype, save_pre=True)
+            y2, pre2 = Z.linear(x, w.contiguous(), residual=r.contiguous(), act="relu", out_dtype=dtype, save_pre=True)
+            z = x.double() @ w.double().t()
+            tol = sum_tol(I, x.double().abs() @ w.double().abs().t())
+            for p, q in ((pre, y), (pre2, y2)):
+                small = 2.0 ** -25 if dtype == torch.float16 else 0
+                close(p, z, tol + half_step(dtype) * z.abs() + small)
+                want = z.clamp(min=0) + r.double()
+                close(q, want, tol + 2 * U * r.double().abs() + half_step(dtype) * want.abs() + small)
+
+
+@pytest.mark.parametrize("xt", list(TYPES))
+@pytest.mark.parametrize("n", [5, 64, 257, 1024, 4100, 8192, 20000])
+def test_layer_norm_gradient_over_its_operands(n, xt):
+    """dx in the place of dy, and of x, as the C call allows."""
+    import zeromoe_amd as Z
+    from zeromoe_amd._lib import check, lib
+
+    rows, code = 700, {"f32": 0, "f16": 1, "bf16": 30}[xt]
+    x, dy, gain = rand(rows, n, seed=1, dtype=TYPES[xt]), rand(rows, n, seed=2, dtype=TYPES[xt]), rand(n, seed=3)
+    _, mean, rstd = Z.layer_norm(x, gain, stats=True)
+    want = Z.layer_norm_backward(dy, x, mean, rstd, gain)
+    ws = torch.empty(lib().zm_layer_norm_backward_workspace_size(rows, n), device="cuda", dtype=torch.uint8)
+    st = torch.cuda.current_stream().cuda_stream
+    for over in ("dy", "x"):
+        a, b = dy.clone(), x.clone()
+        d, dw, db = a if over == "dy" else b, torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+        check(lib().zm_layer_norm_backward(code, a.data_ptr(), n, b.data_ptr(), n, gain.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                           rows, n, d.data_ptr(), n, dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws.numel(), st), "ln")
+        for got, w in zip((d, dw, db), want):
+            assert torch.equal(got, w)
+    x2 = x.clone()
+    y, m2, r2 = Z.layer_norm(x2, gain, stats=True, out=x2)
+    assert y is x2 and torch.equal(m2, mean) and torch.equal(r2, rstd) and torch.equal(y, Z.layer_norm(x, gain))
+
+
+def test_combine_gradient_without_its_rows():
+    """dy alone reads no y, and dweights alone no weights."""
+    from zeromoe_amd._lib import check, lib
+
+    S, K, H = 9, 3, 68
+    d, w, st = rand(S, H, seed=1), rand(S, K, seed=2), torch.cuda.current_stream().cuda_stream
+    ids = torch.randint(-1, 2, (S, K), device="cuda", dtype=torch.int32, generator=torch.Generator("cuda").manual_seed(3))
+    dy = torch.empty(S, K, H, device="cuda")
+    check(lib().zm_combine_backward(d.data_ptr(), None, 0, 0, w.data_ptr(), ids.data_ptr(), S, K, H, None, dy.data_ptr(), st), "dy")
+    assert torch.equal(dy, torch.where((ids >= 0)[:, :, None], w[:, :, None] * d[:, None], torch.zeros_like(dy)))
+
+
+def test_combine_of_most_routes_and_single_columns():
+    import zeromoe_amd as Z
+
+    for S, K, H in ((3, 64, 1), (1, 64, 260), (5, 33, 3)):
+        y, w, d = rand(S, K, H, seed=1), rand(S, K, seed=2), rand(S, H, seed=3)
+        off = torch.full((S, K), -1, device="cuda", dtype=torch.int32)
+        close(Z.combine(y, w), (w.double()[:, :, None] * y.double()).sum(1), sum_tol(2 * K, (w[:, :, None] * y).abs().double().sum(1)))
+        assert torch.equal(Z.combine(y, w, ids=off, residual=d), d) and (Z.combine(y, w, ids=off) == 0).all()
+        assert (Z.combine_backward(d, y, ids=off) == 0).all()
+        t = y.transpose(0, 1).contiguous().transpose(0, 1)  # routes outermost, as one expert after the other leaves them
+        assert torch.equal(Z.combine(t, w), Z.combine(y, w)) and torch.equal(Z.combine_backward(d, t), Z.combine_backward(d, y))
