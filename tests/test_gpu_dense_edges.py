@@ -451,3 +451,32 @@ def test_combine_of_most_routes_and_single_columns():
         assert (Z.combine_backward(d, y, ids=off) == 0).all()
         t = y.transpose(0, 1).contiguous().transpose(0, 1)  # routes outermost, as one expert after the other leaves them
         assert torch.equal(Z.combine(t, w), Z.combine(y, w)) and torch.equal(Z.combine_backward(d, t), Z.combine_backward(d, y))
+
+
+@pytest.mark.parametrize("gating", GATINGS)
+@pytest.mark.parametrize("K", [2, 5, 8, 17, 40, 64])
+def test_a_dominated_row_wherever_its_routes_stand(gating, K):
+    """The dominating route at every place of a row, others left out before and behind it: within roundings as above."""
+    import zeromoe_amd as Z
+
+    E = 128
+    g = torch.Generator().manual_seed(K)
+    ids = torch.stack([torch.randperm(E, generator=g)[:K] for _ in range(K)]).int()
+    logits = torch.full((K, E), -19.0)
+    logits.scatter_(1, ids.long(), -12.0 - torch.rand(K, K, generator=g))
+    at = torch.arange(K)
+    logits[at, ids[at, at].long()] = 1.25
+    left = torch.rand(K, K, generator=g) < 0.3
+    left[at, at] = False
+    ids[left] = -1
+    dw = 0.1 + torch.rand(K, K, generator=g)
+    dw[at, at] = -0.4  # sum of (d - d0) p: no cancellation
+    ids, logits, dw = ids.cuda(), logits.cuda(), dw.cuda()
+    got = Z.router_backward(logits, ids, dw, gating=gating, weights_norm=True)
+    want = route_grad64(logits, ids, dw, gating, None, True, 0.0, None)
+    on = torch.zeros(K, E + 1, device="cuda", dtype=torch.bool).scatter_(1, torch.where(ids < 0, torch.full_like(ids, E), ids).long(), True)[:, :E]
+    alone = (ids >= 0).sum(-1, keepdim=True) == 1
+    want = torch.where(on & ~alone, want, torch.zeros_like(want))
+    # d' - sum d' p / N: for sqrt-softplus the others' p add to a tenth of N and more; the difference keeps at least a
+    # quarter of its larger part
+    close(got, want, 4 * 100 * U * want.abs())

@@ -198,9 +198,10 @@ __global__ __launch_bounds__(64 * ROUTE_WAVES) void k_router_backward(RouteGradA
       // Taking one route's d off all of them changes nothing here.  That of the largest p is taken: its own result, a
       // difference of two nearly equal numbers where it is most of the sum (and 0 where it is all of it), is then made
       // of the other routes alone.
-      const uint64_t valid = __ballot(id >= 0);
-      const uint64_t largest = __ballot(id >= 0 && pk == wave_max(id >= 0 ? pk : -INF));
-      d = id >= 0 ? d - readlane_f(d, __builtin_ctzll(largest ? largest : valid)) : 0.f;
+      const float top = wave_max(id >= 0 ? pk : -INF);  // (by all lanes, whether they have a route or not)
+      const uint64_t valid = __ballot(id >= 0), largest = __ballot(id >= 0 && pk == top);
+      const float d0 = readlane_f(d, __builtin_ctzll(largest ? largest : valid));
+      d = id >= 0 ? d - d0 : 0.f;
       dot = group_sum<64>(d * pk);
       N = total;
     }
