@@ -343,8 +343,9 @@ int zm_expert_bad_counts(zm_expert_scratch *s, int32_t counts[2], int reset);
  *   y, residual and pre: F32 or x's type;  bias F32 [O]
  * f32 operands keep their 24 bits (they enter as sums of bf16 terms; below
  * 2^-110 what is left of a value after 2^-133 is lost), a product of two of them
- * is off by 2^-23 of itself at most; results are rounded once.  Infinities and NaN give what the formula gives.  pre (optional) receives x . w^T + bias for the backward pass.
- * residual (optional) may be y itself.  S may be 0. */
+ * is off by 2^-23 of itself at most; results are rounded once.  Infinities and
+ * NaN give what the formula gives.  pre (optional) receives x . w^T + bias for
+ * the backward pass.  residual (optional) may be y itself.  S may be 0. */
 enum {
   ZM_ACT_NONE = 0,
   ZM_ACT_RELU = 1,

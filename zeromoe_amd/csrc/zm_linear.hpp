@@ -628,7 +628,8 @@ __global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinA
     if (t + 1 >= steps) break;
     step(lds[BUFS - 1], lds[0], p, BUFS == 2 ? q : p);
   }
-  lin_repair_all<(NA * NB > 1 || !KCB), FM, FN>(g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
+  lin_repair_all<(NA * NB > 1 || !KCB), FM, FN>(
+      g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -816,7 +817,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
   }
   wait_vm<0>();  // (what was asked for past the end writes zeros: not into another workgroup's LDS)
   const int fr = lane & 15, fc = lane >> 4;
-  lin_repair_all<!KCB, FM, FN>(g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
+  lin_repair_all<!KCB, FM, FN>(
+      g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll

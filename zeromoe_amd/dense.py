@@ -312,9 +312,10 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, weights=None, ids=None
 def router_backward(logits: torch.Tensor, ids: torch.Tensor, dweights: torch.Tensor, gating="softmax",
                     logit_bias=None, weights_norm: bool = False, weights_scale: float = 0.0, dprobs=None, stream=None):
     """The gradient of router()'s weights by its logits (S, E) float32, the selection held fixed: ids (S, K) int32 are
-    expert ids (router() without a slot table or a mask), dweights (S, K).  A negative id takes no part; a row of them alone has
-    a zero gradient.  dprobs (E): added to the gradient of every routed token's gate probabilities, as a balance loss
-    on their mean has it.  The gradient by logit_bias is the result's sum over the tokens.  (zm_router_backward)"""
+    expert ids (router() without a slot table or a mask), dweights (S, K).  A negative id takes no part; a row of them
+    alone has a zero gradient.  dprobs (E): added to the gradient of every routed token's gate probabilities, as a
+    balance loss on their mean has it.  The gradient by logit_bias is the result's sum over the tokens.
+    (zm_router_backward)"""
     d = _index(logits, "router_backward")
     if stream is not None or d != _device():
         return _there(router_backward, d, stream, logits, ids, dweights, gating, logit_bias, weights_norm, weights_scale,
