@@ -373,6 +373,31 @@ size_t zm_linear_backward_workspace_size(const zm_linear_desc *desc);
 int zm_linear_backward(const zm_linear_desc *desc, const void *dy, const void *x, const void *w, const void *pre,
                        void *dx, float *dw, float *dbias, void *workspace, size_t workspace_size, void *stream);
 
+/* y[s] = act(x[s] . w_gate^T + b_gate) (x[s] . w_up^T + b_up): the gated half of a
+ * feed-forward block (its other half is zm_linear), x [S][I], w_gate and w_up [F][I]
+ * of one type and stride, b_gate and b_up F32 [F] (optional, each).  Types,
+ * activations, infinities and sums as zm_linear's; both factors stay f32 until the
+ * product is rounded.  gate and up (optional, together) receive the factors before
+ * the activation for the backward pass, in y's type.  S may be 0. */
+typedef struct zm_glu_desc {
+  int32_t x_type, w_type, y_type; /* y_type: of y, gate, up and dy */
+  int32_t act;
+  int64_t S, I, F;
+  int64_t x_stride, w_stride, y_stride, gate_stride, up_stride; /* y_stride: of y and dy */
+} zm_glu_desc;
+size_t zm_glu_workspace_size(const zm_glu_desc *desc);
+int zm_glu(const zm_glu_desc *desc, const void *x, const void *w_gate, const void *w_up, const float *b_gate,
+           const float *b_up, void *y, void *gate, void *up, void *workspace, size_t workspace_size, void *stream);
+/* Gradients by dy [S][F]: dg = dy up act'(gate), du = dy act(gate), dx = dg w_gate +
+ * du w_up [S][I] of x's type, dw = {dg^T x, du^T x} F32 [2][F][I], db = sums of dg and
+ * of du over s, F32 [2][F]; each is skipped when NULL, contiguous otherwise.  dg and
+ * du are f32; next to a 16-bit x dx takes 16 bits of them.  With S == 0 dw and db
+ * are zero.  x is read for dw alone, the weights for dx alone. */
+size_t zm_glu_backward_workspace_size(const zm_glu_desc *desc);
+int zm_glu_backward(const zm_glu_desc *desc, const void *dy, const void *x, const void *w_gate, const void *w_up,
+                    const void *gate, const void *up, void *dx, float *dw, float *db, void *workspace,
+                    size_t workspace_size, void *stream);
+
 /* y[r] = (x[r] - mean_r) rstd_r weight + bias over rows of n values,
  * rstd = 1 / sqrt(variance + eps); x and y of `type`, weight and bias F32 [n]
  * (NULL: 1 and 0); mean and rstd F32 [rows] (optional) for the backward pass,

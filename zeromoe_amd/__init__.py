@@ -30,8 +30,8 @@ Torch is used only for device memory and the current stream.
 """
 from __future__ import annotations
 
-from .dense import (combine, combine_backward, layer_norm, layer_norm_backward, linear, linear_backward,
-                    router_backward)
+from .dense import (combine, combine_backward, glu, glu_backward, layer_norm, layer_norm_backward, linear,
+                    linear_backward, router_backward)
 from .ops import (GGML_TYPES, ColdLane, ExpertExecutor, MoELayer, block_dots, bucket, builtin_iq2xxs_grid, builtin_iq3xxs_grid,
                   builtin_iq4nl_table,                   f32_matmul,
                   glm5next_router_topk, init, moe_unpack, mul_mat_id, mul_mat_id_f32, quantize_q8_K, router, row_size,
@@ -42,4 +42,4 @@ __all__ = ["GGML_TYPES", "ColdLane", "ExpertExecutor", "MoELayer", "block_dots",
            "glm5next_router_topk", "init", "moe_unpack", "mul_mat_id", "mul_mat_id_f32", "quantize_q8_K", "router", "row_size",
            "scatter_accum", "set_iq2xxs_grid", "set_iq3xxs_grid", "set_iq4nl_table", "swiglu",
            "combine", "combine_backward", "layer_norm", "layer_norm_backward", "linear", "linear_backward",
-           "router_backward"]
+           "router_backward", "glu", "glu_backward"]

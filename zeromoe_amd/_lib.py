@@ -54,6 +54,11 @@ class ZmLinearDesc(C.Structure):
                 ("x_stride", I64), ("w_stride", I64), ("y_stride", I64), ("res_stride", I64), ("pre_stride", I64)]
 
 
+class ZmGluDesc(C.Structure):
+    _fields_ = [("x_type", I32), ("w_type", I32), ("y_type", I32), ("act", I32), ("S", I64), ("I", I64), ("F", I64),
+                ("x_stride", I64), ("w_stride", I64), ("y_stride", I64), ("gate_stride", I64), ("up_stride", I64)]
+
+
 _MM = (None, [P, P, P, I, I, I])
 _MMS = (None, [P, P, P, I, I, I, P])
 _XS = C.POINTER(ZmExpertScratch)
@@ -115,6 +120,10 @@ SIGNATURES = {
     "zm_linear": (I, [C.POINTER(ZmLinearDesc), P, P, P, P, P, P, P, SZ, P]),
     "zm_linear_backward_workspace_size": (SZ, [C.POINTER(ZmLinearDesc)]),
     "zm_linear_backward": (I, [C.POINTER(ZmLinearDesc), P, P, P, P, P, P, P, P, SZ, P]),
+    "zm_glu_workspace_size": (SZ, [C.POINTER(ZmGluDesc)]),
+    "zm_glu": (I, [C.POINTER(ZmGluDesc), P, P, P, P, P, P, P, P, P, SZ, P]),
+    "zm_glu_backward_workspace_size": (SZ, [C.POINTER(ZmGluDesc)]),
+    "zm_glu_backward": (I, [C.POINTER(ZmGluDesc), P, P, P, P, P, P, P, P, P, P, SZ, P]),
     "zm_layer_norm": (I, [I, P, I64, P, P, F, I64, I64, P, I64, P, P, P]),
     "zm_layer_norm_backward_workspace_size": (SZ, [I64, I64]),
     "zm_layer_norm_backward": (I, [I, P, I64, P, I64, P, P, P, I64, I64, P, I64, P, P, P, SZ, P]),

@@ -100,6 +100,12 @@ __device__ __forceinline__ float lin_act(float z, int act) {
   default: return z;
   }
 }
+// act(z) as a factor: both gelus keep their digits where they are small (1 + erf and 1 + tanh have none left there)
+__device__ __forceinline__ float factor_act(float z, int act) {
+  if (act == ACT_GELU) return 0.5f * z * erfcf(z * -0.70710678118654752f);
+  if (act == ACT_GELU_TANH) return z / (1.0f + expf(-1.5957691216057307f * (z + 0.044715f * z * z * z)));
+  return lin_act(z, act);
+}
 __device__ __forceinline__ float lin_slope_of_number(float z, int act) {
   switch (act) {
   case ACT_RELU: return z > 0.f ? 1.0f : 0.0f;
@@ -213,6 +219,16 @@ static inline void parts_sum(const float *part, int parts, int64_t n, int64_t n0
     hipLaunchKernelGGL((k_parts_sum<1>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, part, parts, n, n0, dst0, dst1);
 }
 
+// ============================================================ two weights
+//
+// The gated product of zm_glu multiplies x by two weights of F rows each, and needs both sums of a column in one lane.
+// Its product takes them as one weight of 2 F rows, 16 of the first matrix and 16 of the second in turn (LIN_PAIR), so
+// that neighbouring fragments of a wave are the two factors of the same columns.  Its gradient by x is a sum of two
+// products, of dg by the first and du by the second weight: planes of `a` over k, one b behind the other (LIN_SUM).
+enum { LIN_ONE = 0, LIN_PAIR = 1, LIN_SUM = 2 };
+__host__ __device__ __forceinline__ constexpr int64_t pair_row(int64_t n) { return (n >> 5) * 16 + (n & 15); }
+__host__ __device__ __forceinline__ constexpr int64_t pair_column(int64_t f) { return (f >> 4) * 32 + (f & 15); }
+
 // ============================================================ operands
 //
 // A tile of ROWS rows (m or n) x BK columns (k) goes from global memory through registers into LDS, one plane per term:
@@ -230,7 +246,7 @@ __device__ __forceinline__ int chunk_at(int row, int c) {
   return c ^ (((row >> 2) ^ (row >> 4)) & 3);
 }
 
-template <class T, int NT, bool KC, int ROWS, int BK, int NTHR, bool VEC>
+template <class T, int NT, bool KC, int ROWS, int BK, int NTHR, bool VEC, bool PAIR = false>
 struct Operand {
   static constexpr int R = KC ? 1 : 4 / (int)sizeof(T);  // rows of a unit
   static constexpr int CH = BK / 8;
@@ -248,17 +264,27 @@ struct Operand {
     uint32_t r[UPT][NW];
   };
 
-  // `row0`: the tile's first row; `total`: rows of the matrix
-  __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t total, int t) {
+  // the row of its matrix, from the tile's first, that row `row` of the tile is
+  __device__ __forceinline__ static int mine(int row) { return PAIR ? (int)pair_row(row) : row; }
+  // `row0`: the tile's first row; `total`: rows of the matrix (PAIR: of both, `p` and `p2`; a wave reads one of them)
+  __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t total, int t,
+                                       const void *p2 = nullptr) {
     ld = ld_;
+    if constexpr (PAIR) {
+      static_assert(KC && UNITS % NTHR == 0 && NTHR / CH % 32 == 0 && 64 / CH <= 16, "a wave's rows are of one matrix");
+      row0 >>= 1;
+      total >>= 1;
+      if (uniform(t >> 6) * (64 / CH) & 16) p = p2;
+    }
+    constexpr int MOST = PAIR ? ROWS / 2 : ROWS;
     base = (const T *)p + (KC ? row0 * ld : row0);
-    rows = (int)(total - row0 < ROWS ? total - row0 : ROWS);
+    rows = (int)(total - row0 < MOST ? total - row0 : MOST);
     first = t;
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       int row, c;
       place(first + i * NTHR, row, c);
-      if (KC) off[i] = (min(row, rows - 1) * (int)ld + 8 * c) * (int)sizeof(T);
+      if (KC) off[i] = (min(mine(row), rows - 1) * (int)ld + 8 * c) * (int)sizeof(T);
       else off[i] = (8 * c * (int)ld + min(row, rows - R)) * (int)sizeof(T);
     }
   }
@@ -296,7 +322,7 @@ struct Operand {
       } else if (left == BK && (KC || rows >= R)) {
         // any alignment: memory takes it, the whole step exists
         if constexpr (KC) {
-          __builtin_memcpy(to.r[i], at + (int64_t)min(row, rows - 1) * ld + 8 * c, sizeof(to.r[i]));
+          __builtin_memcpy(to.r[i], at + (int64_t)min(mine(row), rows - 1) * ld + 8 * c, sizeof(to.r[i]));
         } else {
           const T *p = at + (int64_t)8 * c * ld + min(row, rows - R);
 #pragma unroll
@@ -306,7 +332,7 @@ struct Operand {
           }
         }
       } else if constexpr (KC) {
-        const T *p = at + (int64_t)min(row, rows - 1) * ld + 8 * c;
+        const T *p = at + (int64_t)min(mine(row), rows - 1) * ld + 8 * c;
         T e[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = 8 * c + j < left ? p[j] : from_f32<T>(0.f);
@@ -373,6 +399,9 @@ struct LinEpilogue {
   const float *bias;   // [N] or null
   int64_t ldy, ldr, ldp;
   int type, act;
+  // LIN_PAIR: y = act(z) u; pre is z, up is u (stride ldr, of the same type, with pre or null), bias2 is u's
+  void *up;
+  const float *bias2;
 };
 
 struct LinArgs {
@@ -389,7 +418,22 @@ struct LinArgs {
   bool terms;      // values enter as sums of terms: what follows says how they lie, for lin_again()
   bool a_kc, b_kc; // k contiguous, else rows
   int a_type, b_type;
+  int form;        // LIN_ONE, LIN_PAIR, LIN_SUM: N is 2 F up to the next 32 in LIN_PAIR
+  const void *b2;  // the second weight, of b's stride
+  int64_t F;       // LIN_PAIR: rows of each weight
+  int half;        // LIN_SUM: planes of a before those that go with b2, which start K values on in each row
+  int64_t b_skip;  // LIN_SUM: values from b to b2
 };
+// values from a's (b's) first plane to plane p
+template <int FORM>
+__device__ __forceinline__ int64_t a_skip(const LinArgs &g, int p) {
+  if (FORM == LIN_SUM && p >= g.half) return (p - g.half) * g.plane + g.K;
+  return p * g.plane;
+}
+template <int FORM>
+__device__ __forceinline__ int64_t b_skip(const LinArgs &g, int p) {
+  return FORM == LIN_SUM && p >= g.half ? g.b_skip : 0;
+}
 
 __device__ __forceinline__ float lin_finish1(const LinEpilogue &e, int64_t m, int64_t n, float z) {
   if (e.bias) z += e.bias[n];
@@ -416,6 +460,34 @@ __device__ __forceinline__ void lin_finish4(const LinEpilogue &e, int64_t m, int
     if (n + j < N) lin_store(e.y, e.type, (size_t)(m * e.ldy + n + j), lin_finish1(e, m, n + j, z[j]));
 }
 
+// LIN_PAIR: the sums z and u of row m, columns f .. f + 3 of which those below F exist
+__device__ __forceinline__ float lin_finish_pair1(const LinEpilogue &e, int64_t m, int64_t f, float z, float u) {
+  if (e.bias) z += e.bias[f];
+  if (e.bias2) u += e.bias2[f];
+  if (e.pre) {
+    lin_store(e.pre, e.type, (size_t)(m * e.ldp + f), z);
+    lin_store(e.up, e.type, (size_t)(m * e.ldr + f), u);
+  }
+  return factor_act(z, e.act) * u;
+}
+__device__ __forceinline__ void lin_finish_pair(const LinEpilogue &e, int64_t m, int64_t f, int64_t F, v4f z, v4f u) {
+  if (f + 4 <= F) {
+    if (e.bias) z += *reinterpret_cast<const v4fu *>(e.bias + f);
+    if (e.bias2) u += *reinterpret_cast<const v4fu *>(e.bias2 + f);
+    if (e.pre) {
+      lin_store4(e.pre, e.type, (size_t)(m * e.ldp + f), z);
+      lin_store4(e.up, e.type, (size_t)(m * e.ldr + f), u);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] = factor_act(z[j], e.act) * u[j];
+    lin_store4(e.y, e.type, (size_t)(m * e.ldy + f), z);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (f + j < F) lin_store(e.y, e.type, (size_t)(m * e.ldy + f + j), lin_finish_pair1(e, m, f + j, z[j], u[j]));
+}
+
 __device__ __forceinline__ bool lin_finite(float v) { return fabsf(v) <= F32_MOST; }
 // One sum again from the values themselves.  An infinity times a sum of terms is a sum of infinities of both signs or of
 // zero times one, so NaN stands where the formula may have an infinity, and terms' products may pass f32's largest where
@@ -425,22 +497,32 @@ __device__ __forceinline__ bool lin_finite(float v) { return fabsf(v) <= F32_MOS
 // sum stays one, 0.14 ms.
 __device__ __forceinline__ float lin_again(const LinArgs &g, int64_t m, int64_t n) {
   const int64_t ak = g.a_kc ? 1 : g.lda, bk = g.b_kc ? 1 : g.ldb;
-  size_t ia = (size_t)(g.a_kc ? m * g.lda : m), ib = (size_t)(g.b_kc ? n * g.ldb : n);
+  const int planes = g.form == LIN_SUM ? g.half : g.planes;
+  const void *from = g.form == LIN_PAIR && (n & 16) ? g.b2 : g.b;
+  if (g.form == LIN_PAIR) n = pair_row(n);
   float s = 0.f;
-  for (int64_t k = 0; k < g.K && s == s; k += 4, ia += 4 * ak, ib += 4 * bk) {
-    float a[4], b[4];
+  for (int h = 0; h < (g.form == LIN_SUM ? 2 : 1); ++h) {
+    size_t ia = (size_t)(g.a_kc ? m * g.lda : m) + (h ? g.K : 0), ib = (size_t)(g.b_kc ? n * g.ldb : n);
+    if (h) from = g.b2;
+    for (int64_t k = 0; k < g.K && s == s; k += 4, ia += 4 * ak, ib += 4 * bk) {
+      float a[4], b[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bool in = k + u < g.K;
-      a[u] = in ? lin_load(g.a, g.a_type, ia + u * ak) : 0.f;
-      for (int p = 1; p < g.planes && lin_finite(a[u]); ++p)  // (an infinity or a NaN is its first term)
-        a[u] += in ? lin_load(g.a, g.a_type, ia + u * ak + p * g.plane) : 0.f;
-      b[u] = in ? lin_load(g.b, g.b_type, ib + u * bk) : 0.f;
+      for (int u = 0; u < 4; ++u) {
+        const bool in = k + u < g.K;
+        a[u] = in ? lin_load(g.a, g.a_type, ia + u * ak) : 0.f;
+        for (int p = 1; p < planes && lin_finite(a[u]); ++p)  // (an infinity or a NaN is its first term)
+          a[u] += in ? lin_load(g.a, g.a_type, ia + u * ak + p * g.plane) : 0.f;
+        b[u] = in ? lin_load(from, g.b_type, ib + u * bk) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s = __builtin_fmaf(a[u], b[u], s);
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) s = __builtin_fmaf(a[u], b[u], s);
   }
   return s;
+}
+// whether column n of the product is one of the result
+__device__ __forceinline__ bool lin_column(const LinArgs &g, int64_t n) {
+  return g.form == LIN_PAIR ? pair_row(n) < g.F : n < g.N;
 }
 // sums of row m, columns n .. n + 3: those that are not finite again
 __device__ __forceinline__ void lin_repair(const LinArgs &g, int64_t m, int64_t n, v4f &v) {
@@ -448,7 +530,7 @@ __device__ __forceinline__ void lin_repair(const LinArgs &g, int64_t m, int64_t 
 #pragma unroll 1
   for (int q = 0; q < 4; ++q) {
     const float x = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
-    if (lin_finite(x) || n + q >= g.N) continue;
+    if (lin_finite(x) || !lin_column(g, n + q)) continue;
     const float y = lin_again(g, m, n + q);
     v.x = q == 0 ? y : v.x;
     v.y = q == 1 ? y : v.y;
@@ -489,6 +571,28 @@ __device__ __forceinline__ void lin_result(const LinArgs &g, int z, int64_t m, i
   }
 }
 
+// the sums of a wave's fragments, lane (fr, fc): row m0 + 16 i + fr, columns n0 + 16 j + 4 fc .. + 3
+template <int FORM, int FM, int FN>
+__device__ __forceinline__ void lin_results(const LinArgs &g, int z, int64_t m0, int64_t n0, int fr, int fc,
+                                            const v4f (&acc)[FM][FN]) {
+  if constexpr (FORM == LIN_PAIR) {
+    static_assert(FN % 2 == 0, "both factors of a column in one wave");
+    if (g.slices == 1) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; j += 2)
+          if (m0 + 16 * i + fr < g.M)
+            lin_finish_pair(g.e, m0 + 16 * i + fr, pair_row(n0 + 16 * j + 4 * fc), g.F, acc[i][j], acc[i][j + 1]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) lin_result(g, z, m0 + 16 * i + fr, n0 + 16 * j + 4 * fc, acc[i][j]);
+}
+
 // Workgroup -> tile.  Workgroups go to the 8 XCDs in turn; each XCD takes a run
 // of neighbouring tiles instead, so that the operands they share meet in its L2.
 __device__ __forceinline__ int xcd_order(int b, int n) {
@@ -524,14 +628,14 @@ constexpr int PAIRS_MOST = 2;
 // ones).  With one buffer (BUFS) the splitting follows the products, one step is on its way, and two workgroups of f32
 // by f32 share a CU (where there are two: 4096 x 5120 by k = 64 42 -> 35 us; alone 98 -> 111, 2048^3).
 template <class TA, int NA, bool KCA, class TB, int NB, bool KCB, int BM, int BN, int WM, int WN, bool VEC,
-          int BUFS = 2>
+          int BUFS = 2, int FORM = LIN_ONE>
 __global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinArgs g) {
   constexpr bool F16 = std::is_same<TA, _Float16>::value && std::is_same<TB, _Float16>::value && NA == 1 && NB == 1;
   constexpr int BK = NA * NB == 1 ? 64 : 32;
   constexpr int NTHR = 64 * WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   typedef Operand<TA, NA, KCA, BM, BK, NTHR, VEC> OA;
-  typedef Operand<TB, NB, KCB, BN, BK, NTHR, VEC> OB;
+  typedef Operand<TB, NB, KCB, BN, BK, NTHR, VEC, FORM == LIN_PAIR> OB;
   constexpr int LA = NA * BM * BK, LDS = LA + NB * BN * BK;
   __shared__ __attribute__((aligned(16))) uint16_t lds[BUFS][LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -542,7 +646,7 @@ __global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinA
   OA a;
   OB b;
   a.init(g.a, g.lda, m0, g.M, tid);
-  b.init(g.b, g.ldb, n0, g.N, tid);
+  b.init(g.b, g.ldb, n0, FORM == LIN_PAIR ? 2 * g.F : g.N, tid, g.b2);
   v4f acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -558,8 +662,8 @@ __global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinA
   };
   auto load = [&](Raw &to) {  // zeros behind the last step
     const int left = at.left > 0 ? (int)min(g.K - at.k, (int64_t)BK) : 0;
-    a.load(to.a, at.k, left, at.p * g.plane);
-    b.load(to.b, at.k, left, 0);
+    a.load(to.a, at.k, left, a_skip<FORM>(g, at.p));
+    b.load(to.b, at.k, left, b_skip<FORM>(g, at.p));
     at.next(BK);
   };
   auto step = [&](const uint16_t *from, uint16_t *to, const Raw &next, Raw &after) {
@@ -630,10 +734,7 @@ __global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinA
   }
   lin_repair_all<(NA * NB > 1 || !KCB), FM, FN>(
       g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) lin_result(g, z, m0 + wm + 16 * i + fr, n0 + wn + 16 * j + 4 * fc, acc[i][j]);
+  lin_results<FORM>(g, z, m0 + wm, n0 + wn, fr, fc, acc);
 }
 
 // ============================================================ 16-bit operands, large
@@ -652,7 +753,7 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 constexpr int DMA_BK = 64;
 
-template <bool KC, int ROWS, int NTHR, int FR>
+template <bool KC, int ROWS, int NTHR, int FR, bool PAIR = false>
 struct DmaOperand {
   static constexpr int BK = DMA_BK;
   static constexpr int PER = ROWS * BK / 8 / NTHR, WIDE = ROWS / 8;  // 16-byte chunks of a thread; of a row of k
@@ -674,14 +775,23 @@ struct DmaOperand {
     }
   }
   // `w0`: the wave's first row of the tile
-  __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t total, int w0) {
+  __device__ __forceinline__ void init(const void *p, int64_t ld_, int64_t row0, int64_t total, int w0,
+                                       const void *p2 = nullptr) {
     ld = ld_;
+    if constexpr (PAIR) {  // (a wave asks for 8 rows at a time, NTHR / 8 apart)
+      static_assert(KC && NTHR / 8 % 32 == 0, "a wave's rows are of one matrix");
+      row0 >>= 1;
+      total >>= 1;
+      if (uniform(threadIdx.x >> 6) & 2) p = p2;
+    }
+    constexpr int MOST = PAIR ? ROWS / 2 : ROWS;
     base = (const uint16_t *)p + (KC ? row0 * ld : row0);
-    const int rows = (int)(total - row0 < ROWS ? total - row0 : ROWS);
+    const int rows = (int)(total - row0 < MOST ? total - row0 : MOST);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       int r, c;
       place(i, r, c);
+      if (PAIR) r = (int)pair_row(r);
       off[i] = 2 * (KC ? min(r, rows - 1) * (int)ld + 8 * c : r * (int)ld + min(c, rows - 8));
     }
     const int lane = threadIdx.x & 63, fr = lane & 15, fc = lane >> 4;
@@ -718,11 +828,11 @@ struct DmaOperand {
   }
 };
 
-template <bool F16, bool KCA, bool KCB, int BM, int BN, int WM, int WN>
+template <bool F16, bool KCA, bool KCB, int BM, int BN, int WM, int WN, int FORM = LIN_ONE>
 __global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
   constexpr int NTHR = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   typedef DmaOperand<KCA, BM, NTHR, FM> OA;
-  typedef DmaOperand<KCB, BN, NTHR, FN> OB;
+  typedef DmaOperand<KCB, BN, NTHR, FN, FORM == LIN_PAIR> OB;
   constexpr int BYTES = OA::BYTES + OB::BYTES;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BYTES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -736,7 +846,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
   OA a;
   OB b;
   a.init(g.a, g.lda, m0, g.M, wm);
-  b.init(g.b, g.ldb, n0, g.N, wn);
+  b.init(g.b, g.ldb, n0, FORM == LIN_PAIR ? 2 * g.F : g.N, wn, g.b2);
   v4f acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -751,7 +861,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
     left = at.left > 0 ? (int)min(g.K - at.k, (int64_t)DMA_BK) : 0;
   };
   auto load = [&](uint32_t to) {
-    const v4u_t ra = a.source(at.k, at.p * g.plane), rb = b.source(at.k, 0);
+    const v4u_t ra = a.source(at.k, a_skip<FORM>(g, at.p)), rb = b.source(at.k, b_skip<FORM>(g, at.p));
 #pragma unroll
     for (int i = 0; i < OA::PER; ++i) a.ask(ra, to, i, left);
 #pragma unroll
@@ -798,7 +908,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
       __builtin_amdgcn_sched_barrier(0);
     }
     wait_barrier<0>();
-    const v4u_t ra = a.source(at.k, at.p * g.plane), rb = b.source(at.k, 0);
+    const v4u_t ra = a.source(at.k, a_skip<FORM>(g, at.p)), rb = b.source(at.k, b_skip<FORM>(g, at.p));
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       row(i, a1[i], b1);
@@ -819,10 +929,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
   const int fr = lane & 15, fc = lane >> 4;
   lin_repair_all<!KCB, FM, FN>(
       g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) lin_result(g, z, m0 + wm + 16 * i + fr, n0 + wn + 16 * j + 4 * fc, acc[i][j]);
+  lin_results<FORM>(g, z, m0 + wm, n0 + wn, fr, fc, acc);
 }
 
 // Results of the k slices added in order (the same bits on every call), then the epilogue.  G threads share four
@@ -991,7 +1098,7 @@ constexpr int FEW_ROWS = 64;
 // under f32 rows, 128 rows 27.1 -> 24.5, 256 rows 31.8 -> 31.1
 inline bool lin_few_rows(int64_t M, int64_t N) { return M <= 128 || (M <= 384 && N <= 512); }
 constexpr int FEW_UNIT = 128;  // a slice is a multiple of it: one unit of a 16-bit w, two of an f32 one
-template <class TX, int NX, class TW, int NW, int MT, int NF, int WAVES>
+template <class TX, int NX, class TW, int NW, int MT, int NF, int WAVES, int FORM = LIN_ONE>
 __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
   constexpr bool F16 = std::is_same<TX, _Float16>::value && NX == 1;
   constexpr int KS = sizeof(TW) == 2 ? FEW_UNIT : FEW_UNIT / 2, CH = KS / 8, ROWS = 16 * MT;
@@ -1006,11 +1113,16 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
   const int64_t kb = z * g.kslice, ke = min(g.K, kb + g.kslice);
   const int rows = (int)min(g.M - m0, (int64_t)ROWS);
   // bytes from the workgroup's first column, and from its first row of x
-  const TW *w = (const TW *)g.b + n0 * g.ldb;
+  const TW *w = (const TW *)g.b + (FORM == LIN_PAIR ? n0 / 2 : n0) * g.ldb;
+  const TW *w2 = FORM == LIN_PAIR ? (const TW *)g.b2 + n0 / 2 * g.ldb : w;
   const TX *x = (const TX *)g.a + m0 * g.lda;
   int wo[NF], xo[UX];
 #pragma unroll
-  for (int j = 0; j < NF; ++j) wo[j] = (int)((min(n1 + 16 * j + fr, g.N - 1) - n0) * g.ldb + 8 * fc) * (int)sizeof(TW);
+  for (int j = 0; j < NF; ++j) {
+    const int64_t n = n1 + 16 * j + fr;
+    const int64_t row = FORM == LIN_PAIR ? min(pair_row(n), g.F - 1) - n0 / 2 : min(n, g.N - 1) - n0;
+    wo[j] = (int)(row * g.ldb + 8 * fc) * (int)sizeof(TW);
+  }
 #pragma unroll
   for (int u = 0; u < UX; ++u) {
     const int q = threadIdx.x + THREADS * u, r = q / CH, c = q % CH;
@@ -1027,14 +1139,15 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
   };
   auto load = [&](Unit &t, int64_t k) {
     const int left = (int)min(ke - k, (int64_t)KS);
-    const rsrc_t rx = buf_at(x + k), rw = buf_at(w + k);
+    const rsrc_t rx = buf_at(x + k), rw = buf_at(w + k), rw2 = buf_at(w2 + k);
 #pragma unroll
     for (int u = 0; u < UX; ++u) t.x[u] = load8<TX>(rx, 8 * ((threadIdx.x + THREADS * u) % CH) < left ? xo[u] : OOR);
 #pragma unroll
     for (int h = 0; h < KS / 32; ++h)
 #pragma unroll
       for (int j = 0; j < NF; ++j)
-        t.w[h][j] = load8<TW>(rw, 32 * h + 8 * fc < left ? wo[j] + 32 * h * (int)sizeof(TW) : OOR);
+        t.w[h][j] = load8<TW>(FORM == LIN_PAIR && j % 2 ? rw2 : rw,
+                              32 * h + 8 * fc < left ? wo[j] + 32 * h * (int)sizeof(TW) : OOR);
   };
   // x's terms into `to` (which the waves have left behind a barrier ago), then the unit's products
   auto step = [&](Unit &t, uint16_t *to) {
@@ -1084,10 +1197,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
     step(q, lds[1]);
   }
   lin_repair_all<(NX * NW > 1), MT, NF>(g, acc, [&](int i, int n) { return n ? n1 + 16 * i + 4 * fc : m0 + 16 * i + fr; });
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NF; ++j) lin_result(g, z, m0 + 16 * i + fr, n1 + 16 * j + 4 * fc, acc[i][j]);
+  lin_results<FORM>(g, z, m0, n1, fr, fc, acc);
 }
 
 // columns of a workgroup (one wave each 16 of them): 64 where w is narrow, so that more of them share its reading, else
@@ -1108,6 +1218,191 @@ void lin_few_of(const LinArgs &g, hipStream_t st) {
   else if (g.M <= 32) lin_few_launch<TX, NX, TW, NW, 2>(g, st);
   else lin_few_launch<TX, NX, TW, NW, 4>(g, st);
 }
+
+// ============================================================ two weights: few rows, joins, launches
+
+// LIN_PAIR for up to four rows, as k_linear_rows: WPR waves read a row of each weight, four loads of each in flight.
+template <class TX, class TW, int S, int WPR>
+__global__ __launch_bounds__(256) void k_pair_rows(LinArgs g) {
+  constexpr int V = 16 / (int)sizeof(TW), U = 4;
+  __shared__ float red[2][4][S];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t f = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  if (WPR == 1 && f >= g.F) return;
+  const TW *w[2] = {(const TW *)g.b + f * g.ldb, (const TW *)g.b2 + f * g.ldb};
+  const TX *x = (const TX *)g.a;
+  float acc[2][S] = {};
+  const int K = (int)g.K, first = ((WPR == 1 ? 0 : wave * 64) + lane) * V, step = 64 * WPR * V;
+  typedef v4u v4uu __attribute__((aligned(2)));
+  for (int k0 = first; k0 + V <= K; k0 += U * step) {
+    v4u rw[2][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * step;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        rw[h][u] = k + V <= K ? __builtin_nontemporal_load(reinterpret_cast<const v4uu *>(w[h] + k)) : v4u{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * step;
+      if (k + V > K) break;
+      TW e[2][V];
+      __builtin_memcpy(e[0], &rw[0][u], 16);
+      __builtin_memcpy(e[1], &rw[1][u], 16);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        TX v[V];
+        __builtin_memcpy(v, x + s * g.lda + k, sizeof(v));
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[h][s] = __builtin_fmaf(to_f32(e[h][j]), to_f32(v[j]), acc[h][s]);
+      }
+    }
+  }
+  const int last = K / V * V + lane;
+  if (last < K && (WPR == 1 || wave == 0))
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        acc[h][s] = __builtin_fmaf(to_f32(w[h][last]), to_f32(x[s * g.lda + last]), acc[h][s]);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int s = 0; s < S; ++s) acc[h][s] = group_sum<64>(acc[h][s]);
+  if (WPR > 1) {
+    if (!lane)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int s = 0; s < S; ++s) red[h][wave][s] = acc[h][s];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < S; ++s) acc[h][s] = (red[h][0][s] + red[h][1][s]) + (red[h][2][s] + red[h][3][s]);
+  }
+  float z = acc[0][0], u = acc[1][0];
+#pragma unroll
+  for (int s = 1; s < S; ++s) z = lane == s ? acc[0][s] : z, u = lane == s ? acc[1][s] : u;
+  if (lane < S) lin_store(g.e.y, g.e.type, (size_t)(lane * g.e.ldy + f), lin_finish_pair1(g.e, lane, f, z, u));
+}
+
+// the slices' sums of both factors, as k_linear_join adds them, then act(z) u
+template <int G>
+static __global__ __launch_bounds__(256) void k_pair_join(LinArgs g) {
+  constexpr int Q = 256 / G;
+  __shared__ v4f red[2][G][Q];
+  const int64_t nq = (g.F + 3) / 4, q = (int64_t)blockIdx.x * Q + threadIdx.x % Q;
+  const int first = threadIdx.x / Q;
+  const bool in = q < g.M * nq;
+  const int64_t m = q / nq, f = (q - m * nq) * 4, n = pair_column(f);
+  v4f v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  const size_t plane = (size_t)g.M * g.N;
+  const float *p = g.part + (size_t)m * g.N + n;  // (N is a multiple of 32: whole packs)
+  if (in) {
+    for (int z0 = first; z0 < g.slices; z0 += 4 * G) {
+      v4f t[2][4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          t[h][u] = z0 + u * G < g.slices ? *reinterpret_cast<const v4f *>(p + (z0 + u * G) * plane + 16 * h)
+                                          : v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[h] += t[h][u];
+    }
+  }
+  if (G > 1) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) red[h][first][threadIdx.x % Q] = v[h];
+    __syncthreads();
+    if (first) return;
+#pragma unroll
+    for (int k = 1; k < G; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[h] += red[h][k][threadIdx.x];
+  }
+  if (!in) return;
+  if (g.terms) {
+    lin_repair(g, m, n, v[0]);
+    lin_repair(g, m, n + 16, v[1]);
+  }
+  lin_finish_pair(g.e, m, f, g.F, v[0], v[1]);
+}
+static inline void pair_join(const LinArgs &g, hipStream_t st) {
+  const int64_t quads = g.M * ((g.F + 3) / 4);
+  if (g.slices > 8 && quads < (1 << 26))
+    hipLaunchKernelGGL((k_pair_join<16>), dim3((unsigned)((quads + 15) / 16)), dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((k_pair_join<1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, g);
+}
+
+template <class TX, class TW, int S>
+void pair_rows_launch(const LinArgs &g, hipStream_t st) {
+  if (g.F >= 2048) hipLaunchKernelGGL((k_pair_rows<TX, TW, S, 1>), dim3((unsigned)((g.F + 3) / 4)), dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((k_pair_rows<TX, TW, S, 4>), dim3((unsigned)g.F), dim3(256), 0, st, g);
+}
+template <class TX, class TW>
+void pair_rows_of(const LinArgs &g, hipStream_t st) {
+  switch (g.M) {
+  case 1: pair_rows_launch<TX, TW, 1>(g, st); break;
+  case 2: pair_rows_launch<TX, TW, 2>(g, st); break;
+  case 3: pair_rows_launch<TX, TW, 3>(g, st); break;
+  default: pair_rows_launch<TX, TW, 4>(g, st); break;
+  }
+}
+// columns of the product of a workgroup: each wave takes 16 of each factor
+inline int few_pair_columns(int64_t M, int64_t N) { return M <= 32 && N < 4096 ? 128 : 256; }
+template <class TX, int NX, class TW, int NW, int MT>
+void pair_few_launch(const LinArgs &g, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices));
+  if (few_pair_columns(g.M, g.N) == 128)
+    hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, MT, 2, 4, LIN_PAIR>), grid, dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((k_linear_few<TX, NX, TW, NW, MT, 2, 8, LIN_PAIR>), grid, dim3(512), 0, st, g);
+}
+template <class TX, int NX, class TW, int NW>
+void pair_few_of(const LinArgs &g, hipStream_t st) {
+  if (g.M <= 16) pair_few_launch<TX, NX, TW, NW, 1>(g, st);
+  else if (g.M <= 32) pair_few_launch<TX, NX, TW, NW, 2>(g, st);
+  else pair_few_launch<TX, NX, TW, NW, 4>(g, st);
+}
+
+// Tiles with two weights, as lin_launch: LIN_PAIR (k contiguous in both operands) or LIN_SUM (rows in the weights).
+template <int FORM, class TA, int NA, class TB, int NB>
+void two_launch(const LinArgs &g, bool vec, int tile, hipStream_t st) {
+  constexpr bool KCB = FORM == LIN_PAIR;
+  const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.slices)), b(512);
+  if (tile == 1) {
+    if (vec) hipLaunchKernelGGL((k_linear<TA, NA, true, TB, NB, KCB, 32, 128, 2, 4, true, 2, FORM>), grid, b, 0, st, g);
+    else hipLaunchKernelGGL((k_linear<TA, NA, true, TB, NB, KCB, 32, 128, 2, 4, false, 2, FORM>), grid, b, 0, st, g);
+  } else if (!vec) {
+    hipLaunchKernelGGL((k_linear<TA, NA, true, TB, NB, KCB, 128, 128, 2, 4, false, 2, FORM>), grid, b, 0, st, g);
+  } else if constexpr (std::is_same<TA, TB>::value && sizeof(TA) == 2) {
+    constexpr bool F16 = std::is_same<TA, _Float16>::value;
+    if (tile == 2) hipLaunchKernelGGL((k_linear_dma<F16, true, KCB, 256, 256, 2, 4, FORM>), grid, b, 0, st, g);
+    else if (tile == 3) hipLaunchKernelGGL((k_linear_dma<F16, true, KCB, 256, 128, 4, 2, FORM>), grid, b, 0, st, g);
+    else hipLaunchKernelGGL((k_linear_dma<F16, true, KCB, 128, 128, 2, 4, FORM>), grid, b, 0, st, g);
+  } else {
+    if constexpr (NA * NB == 9) {
+      if (tile == 5) {
+        hipLaunchKernelGGL((k_linear<TA, NA, true, TB, NB, KCB, 128, 128, 2, 4, true, 1, FORM>), grid, b, 0, st, g);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((k_linear<TA, NA, true, TB, NB, KCB, 128, 128, 2, 4, true, 2, FORM>), grid, b, 0, st, g);
+  }
+}
+void pair_rows(int x_type, int w_type, const LinArgs &g, hipStream_t st);
+void pair_few(int x_type, int w_type, const LinArgs &g, hipStream_t st);
+void pair_fwd(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
+void pair_dx(int x_type, int w_type, const LinArgs &g, bool vec, int tile, hipStream_t st);
+
+// ============================================================ launches
 
 // The launch of one kernel instance.  `tile`: 0 = 128 x 128, 1 = 32 x 128, for 16-bit operands with 16-byte loads
 // (`vec`) 2 = 256 x 256 and 3 = 256 x 128; for f32 by f32 4 = 160 x 128 (gradient by w) or 128 x 160 (forward)

@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import ZmLinearDesc, check, lib
+from ._lib import ZmGluDesc, ZmLinearDesc, check, lib
 from .ops import _spec
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
@@ -183,6 +183,87 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str
     check(L.zm_linear_backward(desc, dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db),
                                _ptr(ws), 0 if ws is None else ws.numel(), st), "zm_linear_backward")
     return dx, dw, db
+
+
+def _glu_weights(d, x, w_gate, w_up):
+    _linear_types(d, x, w_gate)
+    _need(w_up, "w_up", d, (w_gate.dtype,), w_gate.shape)
+    F, I = w_gate.shape
+    if w_up.stride(1) != 1 and I != 1:
+        raise ValueError("w_up needs contiguous columns")
+    if w_up.stride(0) != w_gate.stride(0) and F != 1:
+        raise ValueError(f"w_gate and w_up need rows of one stride, not {w_gate.stride(0)} and {w_up.stride(0)}")
+
+
+def glu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate=None, b_up=None, act: str = "silu", out=None,
+        out_dtype=None, save: bool = False, stream=None):
+    """act(x w_gate^T + b_gate) * (x w_up^T + b_up), the gated half of a feed-forward block in one product: x (S, I),
+    w_gate and w_up (F, I) of one type and stride, b_gate and b_up (F) float32, each optional; types and activations as
+    linear()'s.  save: also returns both factors before the activation, (S, F) each in the result's type, for
+    glu_backward.  `out` overlaps no operand.  (zm_glu)"""
+    d = _index(x, "glu")
+    if stream is not None or d != _device():
+        return _there(glu, d, stream, x, w_gate, w_up, b_gate, b_up, act, out, out_dtype, save)
+    if _grad_mode() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                         or b_gate is not None and b_gate.requires_grad or b_up is not None and b_up.requires_grad
+                         or out is not None and out.requires_grad):
+        _not_recorded("glu")
+    st = _raw_stream(d)
+    _glu_weights(d, x, w_gate, w_up)
+    S, I = x.shape
+    F = w_gate.shape[0]
+    x = _rows(x)
+    dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+    if dtype != _F32 and dtype != x.dtype:
+        raise ValueError(f"the result is float32 or {x.dtype}, not {dtype}")
+    y = x.new_empty((S, F), dtype=dtype) if out is None else _out(out, "out", d, dtype, (S, F))
+    b_gate, b_up = _vector(b_gate, "b_gate", d, F), _vector(b_up, "b_up", d, F)
+    gate = up = None
+    if save:
+        gate, up = x.new_empty((S, F), dtype=dtype), x.new_empty((S, F), dtype=dtype)
+    desc = ZmGluDesc(_TYPES[x.dtype], _TYPES[w_gate.dtype], _TYPES[dtype], _act(act), S, I, F, x.stride(0),
+                     w_gate.stride(0), y.stride(0), F, F)
+    L = lib()
+    ws = _space(L.zm_glu_workspace_size(desc), x)
+    check(L.zm_glu(desc, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _ptr(b_gate), _ptr(b_up), y.data_ptr(),
+                   _ptr(gate), _ptr(up), _ptr(ws), 0 if ws is None else ws.numel(), st), "zm_glu")
+    return (y, gate, up) if save else y
+
+
+def glu_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor,
+                 up: torch.Tensor, act: str = "silu", need_dx: bool = True, need_dw: bool = True, need_db: bool = True,
+                 stream=None):
+    """(dx, dw_gate, dw_up, db_gate, db_up) of glu() for dy (S, F), its gradient by the result, with the factors gate and
+    up that glu(save=True) returned, all three of one type: dx (S, I) of x's type, the weights' (F, I) and the biases'
+    (F) float32; None in the place of those that are not needed.  A 16-bit dx takes 16 bits of the factors' gradients.
+    (zm_glu_backward)"""
+    d = _index(dy, "glu_backward")
+    if stream is not None or d != _device():
+        return _there(glu_backward, d, stream, dy, x, w_gate, w_up, gate, up, act, need_dx, need_dw, need_db)
+    if _grad_mode() and (dy.requires_grad or x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                         or gate.requires_grad or up.requires_grad):
+        _not_recorded("glu_backward")
+    st = _raw_stream(d)
+    _glu_weights(d, x, w_gate, w_up)
+    S, I = x.shape
+    F = w_gate.shape[0]
+    x = _rows(x)
+    dy = _rows(_need(dy, "dy", d, (_F32, x.dtype), (S, F)))
+    gate = _rows(_need(gate, "gate", d, (dy.dtype,), (S, F)))
+    up = _rows(_need(up, "up", d, (dy.dtype,), (S, F)))
+    dx = x.new_empty((S, I)) if need_dx else None
+    dw = x.new_empty((2, F, I), dtype=_F32) if need_dw else None
+    db = x.new_empty((2, F), dtype=_F32) if need_db else None
+    desc = ZmGluDesc(_TYPES[x.dtype], _TYPES[w_gate.dtype], _TYPES[dy.dtype], _act(act), S, I, F, x.stride(0),
+                     w_gate.stride(0), dy.stride(0), gate.stride(0), up.stride(0))
+    L = lib()
+    ws = _space(L.zm_glu_backward_workspace_size(desc), x)
+    check(L.zm_glu_backward(desc, dy.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), gate.data_ptr(),
+                            up.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), 0 if ws is None else ws.numel(), st),
+          "zm_glu_backward")
+    dw_gate, dw_up = (None, None) if dw is None else dw.unbind(0)
+    db_gate, db_up = (None, None) if db is None else db.unbind(0)
+    return dx, dw_gate, dw_up, db_gate, db_up
 
 
 def _norm_rows(d, x):
