@@ -439,6 +439,54 @@ int zm_combine_backward(const float *dout, const float *y, int64_t y_tok, int64_
 int zm_router_backward(const zm_router_spec *spec, const float *logits, const float *logit_bias, const int32_t *ids,
                        const float *dweights, const float *dprobs, int S, float *dlogits, void *stream);
 
+/* Low-rank adapters beside a projection that all tokens share:
+ * y[s] = residual[s] + scale[e] (x[s] . a[e]^T) . b[e]^T, e = ids[s], x [S][I], a [n][R][I], b [n][O][R] (a
+ * token's request names its adapter; adapters of a smaller rank are filled up with zeros).  Types as
+ * zm_linear's, the adapters in the place of w; y and residual F32 or of x's type; scale F32 [n] (NULL: 1).
+ * e < 0: no adapter, y is the residual (zeros without one); e >= n: a NaN row.  v (optional, F32 [S][R])
+ * receives x[s] . a[e]^T for the backward pass, 0 or NaN for those.  n <= 512, R <= 256, S < 2^24.  residual
+ * (optional) may be y itself, of y's stride.  Columns are contiguous, the other strides are in elements.
+ * Among f32 operands an infinity may come out as a NaN of its row.  S may be 0. */
+typedef struct zm_lora_desc {
+  int32_t x_type, w_type, y_type; /* y_type: of y, residual and dy */
+  int32_t n, R;
+  int64_t S, I, O;
+  int64_t x_stride, y_stride, res_stride;                   /* y_stride: of y and dy */
+  int64_t a_stride, a_adapter, b_stride, b_adapter;         /* of rows, and from one adapter to the next */
+} zm_lora_desc;
+size_t zm_lora_workspace_size(const zm_lora_desc *desc);
+int zm_lora(const zm_lora_desc *desc, const void *x, const void *a, const void *b, const int32_t *ids, const float *scale,
+            const void *residual, void *y, float *v, void *workspace, size_t workspace_size, void *stream);
+/* Gradients by dy [S][O]: u[s] = dy[s] . b[e], dx[s] = scale[e] u[s] . a[e] [S][I] of x's type (zeros for e < 0,
+ * NaN for e >= n), da[e] = scale[e] sum of u[s]^T x[s] over e's tokens, F32 [n][R][I], db[e] = scale[e] sum of
+ * dy[s]^T v[s], F32 [n][O][R] (zeros where an adapter has no token), each skipped when NULL, contiguous
+ * otherwise; the residual's gradient is dy.  u is f32.  v as zm_lora left it, read for db alone; x is read for
+ * da alone.  With S == 0 da and db are zero. */
+size_t zm_lora_backward_workspace_size(const zm_lora_desc *desc);
+int zm_lora_backward(const zm_lora_desc *desc, const void *dy, const void *x, const void *a, const void *b, const int32_t *ids,
+                     const float *scale, const float *v, void *dx, float *da, float *db, void *workspace,
+                     size_t workspace_size, void *stream);
+
+/* Gradients of a whole step: contiguous arrays of F32, F16 or BF16, any number
+ * of them.  The list is read before the call returns (host memory).
+ *   norm = sqrt(sum of all squares), in f64 until it is rounded to F32 once
+ *   c = min(1, max_norm / (norm + eps)), out = c g
+ * out may be data itself (of the same type); a c of 1 then leaves it untouched.
+ * Otherwise no result overlaps a gradient or another result (checked).  A norm
+ * that is infinite or NaN gives what the formula gives: gradients of 0 and NaN.
+ * norm (device memory) may be NULL in zm_grad_clip.  zm_grad_norm reads data, n
+ * and type alone. */
+typedef struct zm_grad {
+  const void *data;
+  void *out;
+  int64_t n;
+  int32_t type, out_type;
+} zm_grad;
+size_t zm_grad_norm_workspace_size(int64_t count); /* of both */
+int zm_grad_norm(const zm_grad *grads, int64_t count, float *norm, void *workspace, size_t workspace_size, void *stream);
+int zm_grad_clip(const zm_grad *grads, int64_t count, double max_norm, double eps, float *norm, void *workspace,
+                 size_t workspace_size, void *stream);
+
 /* ---------------------------------------------------------------- expert records
  *
  * Device-local unpack of expert-major transfer records [gate | up | down]

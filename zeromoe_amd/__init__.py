@@ -32,6 +32,8 @@ from __future__ import annotations
 
 from .dense import (combine, combine_backward, glu, glu_backward, layer_norm, layer_norm_backward, linear,
                     linear_backward, router_backward)
+from .grads import clip_grad_norm, grad_norm
+from .lora import lora, lora_backward
 from .ops import (GGML_TYPES, ColdLane, ExpertExecutor, MoELayer, block_dots, bucket, builtin_iq2xxs_grid, builtin_iq3xxs_grid,
                   builtin_iq4nl_table,                   f32_matmul,
                   glm5next_router_topk, init, moe_unpack, mul_mat_id, mul_mat_id_f32, quantize_q8_K, router, row_size,
@@ -42,4 +44,5 @@ __all__ = ["GGML_TYPES", "ColdLane", "ExpertExecutor", "MoELayer", "block_dots",
            "glm5next_router_topk", "init", "moe_unpack", "mul_mat_id", "mul_mat_id_f32", "quantize_q8_K", "router", "row_size",
            "scatter_accum", "set_iq2xxs_grid", "set_iq3xxs_grid", "set_iq4nl_table", "swiglu",
            "combine", "combine_backward", "layer_norm", "layer_norm_backward", "linear", "linear_backward",
-           "router_backward", "glu", "glu_backward"]
+           "router_backward", "glu", "glu_backward", "grad_norm", "clip_grad_norm", "lora",
+           "lora_backward"]

@@ -54,6 +54,12 @@ class ZmLinearDesc(C.Structure):
                 ("x_stride", I64), ("w_stride", I64), ("y_stride", I64), ("res_stride", I64), ("pre_stride", I64)]
 
 
+class ZmLoraDesc(C.Structure):
+    _fields_ = [("x_type", I32), ("w_type", I32), ("y_type", I32), ("n", I32), ("R", I32), ("S", I64), ("I", I64), ("O", I64),
+                ("x_stride", I64), ("y_stride", I64), ("res_stride", I64), ("a_stride", I64), ("a_adapter", I64),
+                ("b_stride", I64), ("b_adapter", I64)]
+
+
 class ZmGluDesc(C.Structure):
     _fields_ = [("x_type", I32), ("w_type", I32), ("y_type", I32), ("act", I32), ("S", I64), ("I", I64), ("F", I64),
                 ("x_stride", I64), ("w_stride", I64), ("y_stride", I64), ("gate_stride", I64), ("up_stride", I64)]
@@ -130,6 +136,13 @@ SIGNATURES = {
     "zm_combine": (I, [P, I64, I64, P, P, P, I64, I, I, P, P]),
     "zm_combine_backward": (I, [P, P, I64, I64, P, P, I64, I, I, P, P, P]),
     "zm_router_backward": (I, [C.POINTER(ZmRouterSpec), P, P, P, P, P, I, P, P]),
+    "zm_lora_workspace_size": (SZ, [C.POINTER(ZmLoraDesc)]),
+    "zm_lora": (I, [C.POINTER(ZmLoraDesc), P, P, P, P, P, P, P, P, P, SZ, P]),
+    "zm_lora_backward_workspace_size": (SZ, [C.POINTER(ZmLoraDesc)]),
+    "zm_lora_backward": (I, [C.POINTER(ZmLoraDesc), P, P, P, P, P, P, P, P, P, P, P, SZ, P]),
+    "zm_grad_norm_workspace_size": (SZ, [I64]),
+    "zm_grad_norm": (I, [C.c_char_p, I64, P, P, SZ, P]),  # (the list as packed bytes)
+    "zm_grad_clip": (I, [C.c_char_p, I64, C.c_double, C.c_double, P, P, SZ, P]),
     "zm_cold_lane_create": (P, [C.POINTER(ZmColdLaneDesc)]),
     "zm_cold_lane_destroy": (None, [P]),
     "zm_cold_lane_fork": (I, [P, P, P, P, I, P]),
