@@ -16,7 +16,7 @@ SOURCES = ("zm_api.hip", "zm_dec_a.hip", "zm_dec_b.hip", "zm_mmq_a.hip", "zm_mmq
            "zm_mmq_d.hip", "zm_exec.hip", "zm_pack.hip", "zm_lane.hip", "zm_linear.hip", "zm_linear_a.hip", "zm_linear_b.hip",
            "zm_linear_c.hip", "zm_linear_d.hip", "zm_glu.hip", "zm_glu_a.hip", "zm_glu_b.hip", "zm_glu_c.hip",
            "zm_norm.hip", "zm_combine.hip", "zm_grads.hip", "zm_lora.hip",
-           "zm_lora_a.hip", "zm_lora_b.hip")
+           "zm_lora_a.hip", "zm_lora_b.hip", "zm_lora_c.hip")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 # -ffp-contract=off: the quantizer, router and SwiGLU are bit-reproducible

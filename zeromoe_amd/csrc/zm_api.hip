@@ -460,14 +460,6 @@ int check_router(const zm_router_spec &spec) {
 
 // ====================================================================== C ABI
 
-namespace zm {
-void bucket_tokens(const int32_t *ids, int S, int E, int tok, int32_t *counts, int32_t *offs, int32_t *pairs,
-                   int32_t *active, int32_t *n_active, int32_t *items, int32_t *n_items, hipStream_t stream) {
-  const BucketArgs a{ids, 1, 1, S, E, counts, offs, pairs, active, n_active, items, n_items, tok};
-  hipLaunchKernelGGL(k_bucket, dim3(1), dim3(1024), 0, stream, a);
-}
-}  // namespace zm
-
 extern "C" {
 
 const char *zm_last_error(void) { return g_err; }

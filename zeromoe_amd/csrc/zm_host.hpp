@@ -17,10 +17,6 @@ int device_grid(const uint64_t **grid);
 int device_table(int type, const uint64_t **table);
 // one more executed MUL_MAT_ID hook launch (zm_mul_mat_id_launches)
 void count_mmid_launch();
-// S tokens bucketed by ids [S] below E <= 512 (others take no part) by one launch: counts [E], offs [E + 1], pairs [S],
-// and items (mmq_item) of up to `tok` tokens of one id, at most S / tok + min(S, E) of them; active [E] and n_active too
-void bucket_tokens(const int32_t *ids, int S, int E, int tok, int32_t *counts, int32_t *offs, int32_t *pairs,
-                   int32_t *active, int32_t *n_active, int32_t *items, int32_t *n_items, hipStream_t stream);
 
 }  // namespace zm
 

@@ -17,15 +17,13 @@ int check_lora(const zm_lora_desc *d, const char *who) {
     return fail("%s: 16-bit activations need adapters of their own type", who);
   if (d->y_type != ZM_TYPE_F32 && d->y_type != d->x_type)
     return fail("%s: the result is F32 or of the activations' type", who);
-  if (d->n <= 0 || d->n > BUCKET_MAX_E) return fail("%s: 1 to %d adapters, not %d", who, BUCKET_MAX_E, d->n);
+  if (d->n <= 0 || d->n > LORA_MOST_N) return fail("%s: 1 to %d adapters, not %d", who, LORA_MOST_N, d->n);
   if (d->R <= 0 || d->R > LORA_MOST_R) return fail("%s: a rank of 1 to %d, not %d", who, LORA_MOST_R, d->R);
-  if (d->S < 0 || d->S >= MMQ_MAX_PAIRS) return fail("%s: S from 0 to 2^24 is needed", who);
+  if (d->S < 0 || d->S >= 1 << 24) return fail("%s: S from 0 to 2^24 is needed", who);
   if (d->I <= 0 || d->O <= 0 || d->I >= 1 << 30 || d->O >= 1 << 30) return fail("%s: I and O from 1 to 2^30 are needed", who);
   if (d->x_stride < 0 || d->y_stride < 0 || d->res_stride < 0 || d->a_stride < 0 || d->b_stride < 0 || d->a_adapter < 0 ||
       d->b_adapter < 0)
     return fail("%s: negative stride", who);
-  if ((d->S / LORA_TOKENS + d->n) * ((std::max(d->I, d->O) + 255) / 256) >= 1 << 26)
-    return fail("%s: S x I or S x O too large for one launch", who);
   return 0;
 }
 
@@ -37,44 +35,26 @@ int64_t slices_of(int64_t n, int64_t want, int64_t K, int64_t unit, int64_t most
   return std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want / std::max<int64_t>(n, 1), most), K / unit));
 }
 
-struct Shrink {
-  int slices, chunks;
-  int64_t kslice;
-  size_t part;  // bytes
-};
-Shrink shrink_of(const zm_lora_desc &d, int64_t K) {
-  Shrink p;
-  p.chunks = (d.R + lora_r_of(d.R) - 1) / lora_r_of(d.R);
-  const int64_t z = slices_of(most_items(d) * p.chunks, 1024, K, 256, 16);
-  p.kslice = ((K + z - 1) / z + 255) / 256 * 256;
-  p.slices = (int)((K + p.kslice - 1) / p.kslice);
-  p.part = align256((size_t)p.slices * d.S * d.R * 4);
-  return p;
-}
 // slices of an adapter's tokens for its gradient of N columns; their sums take at most 64 MB
 int sums_slices(const zm_lora_desc &d, int64_t N) {
   const int64_t groups = (N + 63) / 64 * ((d.R + lora_r_of(d.R) - 1) / lora_r_of(d.R)) * d.n;
-  return (int)slices_of(groups, 512, d.S / d.n, 128, (64 << 20) / (4 * N * d.R * d.n));
+  return (int)slices_of(groups, 512, d.S / d.n, 256, (64 << 20) / (4 * N * d.R * d.n));
 }
 size_t sums_space(const zm_lora_desc &d, int64_t N) {
   const int z = sums_slices(d, N);
   return z > 1 ? align256((size_t)z * d.n * d.R * N * 4) : 0;
 }
 
-// Workspace: the buckets | v or u of each slice | (backward) u, and one gradient's sums.
+// Workspace: the items | (backward) u, and the slices' sums of each gradient.
 struct Space {
-  size_t buckets, part, u, sums, total;
+  size_t items, u, total;
 };
-size_t bucket_bytes(const zm_lora_desc &d) { return align256((3 * d.n + 3 + d.S + most_items(d)) * 4); }
+size_t item_bytes(const zm_lora_desc &d) { return align256((2 * d.n + 1 + (LORA_TOKENS + 1) * most_items(d)) * 4); }
 Space space_of(const zm_lora_desc &d, bool backward) {
   Space s{};
-  s.buckets = bucket_bytes(d);
-  s.part = shrink_of(d, backward ? d.O : d.I).part;
-  if (backward) {
-    s.u = align256((size_t)d.S * d.R * 4);
-    s.sums = std::max(sums_space(d, d.I), sums_space(d, d.O));
-  }
-  s.total = s.buckets + s.part + s.u + s.sums;
+  s.items = item_bytes(d);
+  if (backward) s.u = align256((size_t)d.S * d.R * 4);
+  s.total = s.items + s.u + (backward ? sums_space(d, d.I) + sums_space(d, d.O) : 0);
   return s;
 }
 
@@ -84,73 +64,45 @@ bool few_tokens(const zm_lora_desc &d) {
   return d.S <= 4096 && a <= 1 << 20 && d.S * ((d.O + 511) / 512) * a <= 64 << 20;
 }
 
-LoraArgs buckets(const zm_lora_desc &d, const int32_t *ids, const float *scale, uint8_t *ws, hipStream_t st) {
+LoraArgs items(const zm_lora_desc &d, const int32_t *ids, const float *scale, uint8_t *ws, hipStream_t st) {
   LoraArgs g{};
   g.R = d.R;
   g.S = (int)d.S;
   g.n = d.n;
   g.ids = ids;
   g.scale = scale;
+  g.rest = (int)most_items(d);
   int32_t *p = (int32_t *)ws;
-  int32_t *counts = p, *offs = p + d.n, *active = p + 2 * d.n + 1, *n_active = active + d.n, *n_items = n_active + 1;
-  int32_t *pairs = n_items + 1, *items = pairs + d.S;
-  bucket_tokens(ids, (int)d.S, d.n, LORA_TOKENS, counts, offs, pairs, active, n_active, items, n_items, st);
-  g.counts = counts;
-  g.offs = offs;
-  g.pairs = pairs;
-  g.items = items;
-  g.n_items = n_items;
+  const int64_t most = most_items(d);
+  g.it.tokens = p;
+  g.it.item_e = p + LORA_TOKENS * most;
+  g.it.counts = g.it.item_e + most;
+  g.it.first = g.it.counts + d.n;
+  g.it.n_items = g.it.first + d.n;
+  hipLaunchKernelGGL(k_lora_items, dim3(1), dim3(1024), 0, st, ids, (int)d.S, (int)d.n, g.it);
   return g;
 }
-// x by the matrices m over K, into the slices' parts of v
-void shrink(const zm_lora_desc &d, LoraArgs g, const void *x, int x_type, int64_t ldx, const void *m, int64_t ldm,
-            int64_t adapter, int64_t K, bool kc, float *part, hipStream_t st) {
-  const Shrink p = shrink_of(d, K);
-  g.x = x;
-  g.ldx = ldx;
+// the workgroups of k_lora: one an item, and one for 64 tokens to look for those without an adapter
+int groups_of(const zm_lora_desc &d) { return (int)(most_items(d) + (d.S + 63) / 64); }
+LoraSumArgs sums_args(const zm_lora_desc &d, const float *a, const void *m, int64_t ldm, int64_t N, const float *scale,
+                      float *dst, float *space) {
+  LoraSumArgs g{};
+  g.a = a;
   g.m = m;
   g.ldm = ldm;
-  g.adapter = adapter;
-  g.K = K;
-  g.slices = p.slices;
-  g.chunks = p.chunks;
-  g.kslice = p.kslice;
-  g.part = part;
-  lora_shrink(x_type, d.w_type, kc, g, (int)(most_items(d) * p.slices * p.chunks), st);
-}
-// the slices' sums (kept in v, unless null) by the matrices m, N columns of y
-void expand(const zm_lora_desc &d, LoraArgs g, const float *part, int slices, float *v, const void *m, int64_t ldm,
-            int64_t adapter, int64_t N, bool kc, const void *res, int64_t ldr, void *y, int64_t ldy, int type,
-            hipStream_t st) {
-  g.part = (float *)part;
-  g.slices = slices;
-  g.v = v;
-  g.m = m;
-  g.ldm = ldm;
-  g.adapter = adapter;
   g.N = N;
-  g.res = res;
-  g.ldr = ldr;
-  g.y = y;
-  g.ldy = ldy;
-  g.type = type;
-  g.chunks = (int)((N + 255) / 256);
-  g.rest = (int)most_items(d);
-  lora_expand(d.w_type, kc, g, (int)((g.rest + (d.S + 63) / 64) * g.chunks), st);
-}
-// dst [n][R][N], or [n][N][R] (by_r): the sums over each adapter's tokens of a's and m's rows
-void sums(const zm_lora_desc &d, LoraArgs g, const float *a, const void *m, int m_type, int64_t ldm, int64_t N, bool by_r,
-          float *dst, float *space, hipStream_t st) {
-  g.v = (float *)a;
-  g.x = m;
-  g.ldx = ldm;
-  g.N = N;
-  g.chunks = (d.R + lora_r_of(d.R) - 1) / lora_r_of(d.R);
+  g.R = d.R;
+  g.n = d.n;
   g.slices = sums_slices(d, N);
-  g.y = g.slices > 1 ? space : dst;
-  lora_sums(m_type, by_r, g, (int)((N + 63) / 64 * g.chunks * g.slices * d.n), st);
-  const int64_t all = (int64_t)d.n * d.R * N;
-  if (g.slices > 1) parts_sum(space, g.slices, all, all, dst, nullptr, st);
+  g.chunks = (d.R + lora_r_of(d.R) - 1) / lora_r_of(d.R);
+  g.scale = scale;
+  g.out = g.slices > 1 ? space : dst;
+  return g;
+}
+unsigned sums_groups(const LoraSumArgs &g) { return (unsigned)((g.N + 63) / 64 * g.chunks * g.slices * g.n); }
+void join_sums(const LoraSumArgs &g, float *dst, hipStream_t st) {
+  const int64_t all = (int64_t)g.n * g.R * g.N;
+  if (g.slices > 1) parts_sum(g.out, g.slices, all, all, dst, nullptr, st);
 }
 
 int check_space(void *ws, size_t size, size_t need, const char *who) {
@@ -183,12 +135,23 @@ int zm_lora(const zm_lora_desc *d, const void *x, const void *a, const void *b, 
   }
   const Space s = space_of(*d, false);
   if (check_space(workspace, workspace_size, s.total, "zm_lora")) return -1;
-  uint8_t *ws = (uint8_t *)workspace;
-  float *part = (float *)(ws + s.buckets);
-  const LoraArgs g = buckets(*d, ids, scale, ws, st);
-  shrink(*d, g, x, d->x_type, d->x_stride, a, d->a_stride, d->a_adapter, d->I, true, part, st);
-  expand(*d, g, part, shrink_of(*d, d->I).slices, v, b, d->b_stride, d->b_adapter, d->O, true, residual, d->res_stride, y,
-         d->y_stride, d->y_type, st);
+  LoraArgs g = items(*d, ids, scale, (uint8_t *)workspace, st);
+  g.x = x;
+  g.ldx = d->x_stride;
+  g.m = a;
+  g.ldm = d->a_stride;
+  g.m_adapter = d->a_adapter;
+  g.K = d->I;
+  g.l = b;
+  g.ldl = d->b_stride;
+  g.l_adapter = d->b_adapter;
+  g.N = d->O;
+  g.res = residual;
+  g.ldr = d->res_stride;
+  g.y = y;
+  g.ldy = d->y_stride;
+  g.v = v;
+  lora_forward(d->x_type, d->w_type, d->y_type, g, groups_of(*d), st);
   return launched();
 }
 
@@ -212,19 +175,31 @@ int zm_lora_backward(const zm_lora_desc *d, const void *dy, const void *x, const
   const Space s = space_of(*d, true);
   if (check_space(workspace, workspace_size, s.total, "zm_lora_backward")) return -1;
   uint8_t *ws = (uint8_t *)workspace;
-  float *part = (float *)(ws + s.buckets), *u = (float *)(ws + s.buckets + s.part), *space = (float *)((uint8_t *)u + s.u);
-  const LoraArgs g = buckets(*d, ids, scale, ws, st);
+  float *u = (float *)(ws + s.items), *sa = (float *)(ws + s.items + s.u), *sb = sa + sums_space(*d, d->I) / 4;
+  LoraArgs g = items(*d, ids, scale, ws, st);
   if (dx || da) {
-    const int slices = shrink_of(*d, d->O).slices;
-    shrink(*d, g, dy, d->y_type, d->y_stride, b, d->b_stride, d->b_adapter, d->O, false, part, st);
-    if (slices == 1) u = part;
-    if (dx)
-      expand(*d, g, part, slices, da && slices > 1 ? u : nullptr, a, d->a_stride, d->a_adapter, d->I, false, nullptr, 0, dx,
-             d->I, d->x_type, st);
-    else if (slices > 1) parts_sum(part, slices, d->S * d->R, d->S * d->R, u, nullptr, st);
+    g.x = dy;
+    g.ldx = d->y_stride;
+    g.m = b;
+    g.ldm = d->b_stride;
+    g.m_adapter = d->b_adapter;
+    g.K = d->O;
+    g.l = a;
+    g.ldl = d->a_stride;
+    g.l_adapter = d->a_adapter;
+    g.N = dx ? d->I : 0;
+    g.y = dx;
+    g.ldy = d->I;
+    g.v = da ? u : nullptr;
+    lora_backward(d->y_type, d->w_type, d->x_type, g, groups_of(*d), st);
   }
-  if (da) sums(*d, g, u, x, d->x_type, d->x_stride, d->I, false, da, space, st);
-  if (db) sums(*d, g, v, dy, d->y_type, d->y_stride, d->O, true, db, space, st);
+  if (da || db) {
+    const LoraSumArgs ga = sums_args(*d, u, x, d->x_stride, d->I, scale, da, sa);
+    const LoraSumArgs gb = sums_args(*d, v, dy, d->y_stride, d->O, scale, db, sb);
+    lora_sums(d->x_type, d->y_type, g.it, ga, da ? sums_groups(ga) : 0, gb, db ? sums_groups(gb) : 0, st);
+    if (da) join_sums(ga, da, st);
+    if (db) join_sums(gb, db, st);
+  }
   return launched();
 }
 

@@ -3,14 +3,17 @@
 //   y[s] = residual[s] + c[e] (x[s] A[e]^T) B[e]^T,  e = ids[s],  A [n][R][I], B [n][O][R]
 //
 // and the gradients by x, A and B.  R is small (16 of thousands), so all of it is bound by reading x and the named
-// adapters and by reading and writing y: 2 R operations a value.  Two products of one shape each carry both directions:
+// adapters and by reading and writing y: 2 R operations a value.  One kernel carries both directions, a product over the
+// long axis and one over the short axis with v between them in LDS, where it stays f32 and enters as three bf16 terms
+// (zm_linear.hpp):
 //
-//   shrink  v[s][r] = sum_k x[s][k] M(r, k)            M = A, k contiguous; backward x = dy, M(r, k) = B[k][r]
-//   expand  y[s][o] = residual + c sum_r v[s][r] M(o, r)  M = B, r contiguous; backward M(o, r) = A[r][o]
+//   v[s][r] = sum_k x[s][k] M(r, k)                 M = A, k contiguous; backward x = dy, M(r, k) = B[k][r]
+//   y[s][o] = residual + c sum_r v[s][r] L(o, r)    L = B, r contiguous; backward L(o, r) = A[r][o]
 //
-// and the adapters' gradients are one of a third: sum over an adapter's tokens of c a[s][r] m[s][j] (a = u, m = x for dA,
-// a = v, m = dy for dB).  Tokens are bucketed by adapter first (k_bucket: a stable order, so sums have a fixed order);
-// an item is up to 64 tokens of one adapter.  v stays f32, and enters products as three bf16 terms (zm_linear.hpp).
+// and the adapters' gradients are sums over an adapter's tokens of c a[s][r] m[s][j] (a = u, m = x for dA, a = v, m = dy
+// for dB).  Tokens are sorted by adapter first (a stable order, so sums have a fixed order) into items of up to 32 tokens
+// of one adapter.  (Two kernels with v in memory, the long axis in slices, took 50 + 58 us where the one takes LORA_US:
+// 8192 x 7168 x 2048, R 64, bf16.)
 //
 // The matrix instructions (16 x 16, 32 of the summed index) take 8 consecutive values of that index a lane: lane (fr, fc)
 // row fr, values 8 fc ..  Where memory has the rows contiguous instead (B in the backward pass, and all operands of a sum
@@ -18,89 +21,227 @@
 // NF fr + h belong to fragment h.
 #pragma once
 
-#include "zm_kernels.hpp"
 #include "zm_linear.hpp"
 
 namespace zm {
 
-constexpr int LORA_TOKENS = 64;  // of an item
-constexpr int LORA_MOST_R = 256;
+constexpr int LORA_TOKENS = 32;  // of an item
+constexpr int LORA_MOST_R = 256, LORA_MOST_N = 512;
 
+// The items: adapter e's tokens lie at tokens[32 first[e] ..], counts[e] of them, in ascending order, -1 behind them up to
+// the next item; item i is of adapter item_e[i].
+struct LoraItems {
+  int32_t *counts, *first, *item_e, *tokens, *n_items;  // [n], [n], [items], [items][32], one
+};
 struct LoraArgs {
-  const void *x, *m;       // shrink: rows and matrices; expand: matrices; sums: rows
-  int64_t ldx, ldm, adapter;  // strides of x's rows, of m's rows and from one adapter to the next
-  int64_t K, N;            // shrink: the summed index; expand, sums: columns of the result
+  const void *x, *m, *l;  // rows, the matrices of the long axis and those of the short one
+  int64_t ldx, ldm, ldl;  // strides of their rows
+  int64_t m_adapter, l_adapter;
+  int64_t K, N;           // the long axis, and columns of the result (0: v alone)
   int R, S, n;
-  const int32_t *counts, *offs, *pairs, *items, *n_items, *ids;
-  int slices, chunks;      // shrink: slices of k and chunks of r; expand: chunks of columns; sums: slices of tokens
-  int64_t kslice;
-  float *part;             // shrink writes, expand adds [slices][S][R]
-  float *v;                // expand: the sums of the slices, or null; sums: a [S][R]
-  const float *scale;      // [n] or null
-  const void *res;         // expand: [S][ldr] of `type`, or null
+  LoraItems it;
+  const int32_t *ids;
+  float *v;               // [S][R], or null
+  const float *scale;     // [n] or null
+  const void *res;        // [S][ldr] or null
   void *y;
   int64_t ldr, ldy;
-  int type;
-  int rest;                // expand: the first workgroup that looks for tokens without an adapter
+  int rest;               // the first workgroup that looks for tokens without an adapter
 };
 
+// ============================================================ items
+//
+// One workgroup; each of its 16 waves takes a run of tokens, 64 at a time.  The lanes of one id find each other by a
+// ballot for each bit of it; their first one counts them in the wave's own counters, so no atomic is needed and a token's
+// place among its wave's is known at once; it is kept in registers for the first 16 chunks (16384 tokens of the call) and
+// found again for the others.  8192 tokens of 8 adapters: LORA_ITEMS_US.
+constexpr int LORA_CHUNKS = 16;
+static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__restrict__ ids, int S, int n, LoraItems o) {
+  __shared__ int cnt[16][LORA_MOST_N], first[LORA_MOST_N], total[LORA_MOST_N], sums[16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int seg = (S + 1023) / 1024 * 64, p0 = w * seg, p1 = min(p0 + seg, S);
+  const int bits = n > 1 ? 32 - __builtin_clz((unsigned)(n - 1)) : 0;
+  auto load = [&](int p) {
+    const int e = p < p1 ? ids[p] : -1;
+    return (unsigned)e < (unsigned)n ? e : -1;
+  };
+  int e[LORA_CHUNKS], at[LORA_CHUNKS];
+#pragma unroll
+  for (int c = 0; c < LORA_CHUNKS; ++c) e[c] = 64 * c < seg ? load(p0 + 64 * c + lane) : -1;
+  for (int k = lane; k < n; k += 64) cnt[w][k] = 0;
+  stage_sync();
+  // the place of a token among those of its adapter in its wave
+  auto place = [&](int e) {
+    uint64_t same = __ballot(e >= 0);
+    for (int j = 0; j < bits; ++j) {
+      const uint64_t b = __ballot(e >= 0 && ((e >> j) & 1));
+      same &= ((e >> j) & 1) ? b : ~b;
+    }
+    const int rank = __builtin_popcountll(same & ((1ull << lane) - 1));
+    int at = 0;
+    if (e >= 0) at = cnt[w][e];
+    stage_sync();
+    if (e >= 0 && !rank) cnt[w][e] = at + __builtin_popcountll(same);
+    stage_sync();
+    return at + rank;
+  };
+#pragma unroll
+  for (int c = 0; c < LORA_CHUNKS; ++c)
+    if (64 * c < seg) at[c] = place(e[c]);
+  for (int p = p0 + 64 * LORA_CHUNKS; p < p1; p += 64) place(load(p + lane));
+  __syncthreads();
+  // by adapter: tokens of the waves before, all of them, and their items
+  int mine = 0;
+  if (tid < n) {
+    int run = 0;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int k = cnt[v][tid];
+      cnt[v][tid] = run;
+      run += k;
+    }
+    total[tid] = run;
+    mine = (run + LORA_TOKENS - 1) / LORA_TOKENS;
+  }
+  int incl = mine;  // (adapters are below 512: waves 0 to 7 hold them)
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int up = __shfl_up(incl, m, 64);
+    if (lane >= m) incl += up;
+  }
+  if (lane == 63) sums[w] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int v = 0; v < 8; ++v) {
+    if (v < w) before += sums[v];
+    all += sums[v];
+  }
+  if (tid < n) {
+    first[tid] = before + incl - mine;
+    o.first[tid] = first[tid];
+    o.counts[tid] = total[tid];
+  }
+  if (!tid) *o.n_items = all;
+  __syncthreads();
+  auto put = [&](int p, int e, int at) {
+    if (e < 0) return;
+    at += cnt[w][e];
+    o.tokens[(size_t)first[e] * LORA_TOKENS + at] = p;
+    if (!(at & (LORA_TOKENS - 1))) o.item_e[first[e] + at / LORA_TOKENS] = e;
+  };
+#pragma unroll
+  for (int c = 0; c < LORA_CHUNKS; ++c)
+    if (64 * c < seg) put(p0 + 64 * c + lane, e[c], at[c]);
+  for (int q = w; q < n; q += 16) {  // behind an adapter's last token
+    const int used = total[q] & (LORA_TOKENS - 1);
+    if (used && lane >= used && lane < LORA_TOKENS) o.tokens[((size_t)first[q] + total[q] / LORA_TOKENS) * LORA_TOKENS + lane] = -1;
+  }
+  if (seg <= 64 * LORA_CHUNKS) return;
+  // the chunks past the registers: their places again, on from those of the chunks before
+  stage_sync();
+  for (int c = 0; c < LORA_CHUNKS; ++c) {
+    const int k = load(p0 + 64 * c + lane);
+    if (k >= 0) atomicAdd(&cnt[w][k], 1);
+  }
+  stage_sync();
+  for (int p = p0 + 64 * LORA_CHUNKS; p < p1; p += 64) {
+    const int k = load(p + lane);
+    const int a = place(k);
+    if (k < 0) continue;
+    o.tokens[(size_t)first[k] * LORA_TOKENS + a] = p + lane;
+    if (!(a & (LORA_TOKENS - 1))) o.item_e[first[k] + a / LORA_TOKENS] = k;
+  }
+}
+
+// This thread's view of item i: its adapter, its tokens and how many there are (read side by side)
 struct LoraItem {
   int e, count;
   const int32_t *tokens;
+  // token t of the item; those past the last are its first
+  __device__ __forceinline__ int64_t token(int t) const {
+    const int s = tokens[t];
+    return s < 0 ? tokens[0] : s;
+  }
 };
 __device__ __forceinline__ bool lora_item(const LoraArgs &g, int i, LoraItem &it) {
-  if (i >= *g.n_items) return false;
-  const int32_t w = g.items[i];
-  it.e = mmq_item_expert(w);
-  const int first = mmq_item_first(w);
-  it.count = min(LORA_TOKENS, g.counts[it.e] - first);
-  it.tokens = g.pairs + g.offs[it.e] + first;
+  it.tokens = g.it.tokens + (size_t)i * LORA_TOKENS;
+  it.e = g.it.item_e[i];
+  const int t = it.tokens[threadIdx.x & (LORA_TOKENS - 1)];
+  if (i >= *g.it.n_items) return false;  // (before it.e is used)
+  it.e = uniform(it.e);
+  it.count = __builtin_popcount((uint32_t)__ballot(t >= 0));
   return true;
 }
 
 // ============================================================ fragments
 
 template <class T>
-struct Pack8 {
-  T v[8];
-};
-// 8 consecutive values, of which the first `left` exist (zeros past them); any alignment
+__device__ __forceinline__ uint32_t bits_of(T v) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(uint32_t, v);
+  else return __builtin_bit_cast(uint16_t, v);
+}
 template <class T>
-__device__ __forceinline__ void load_k(Pack8<T> &p, const T *at, int left) {
-  if (left >= 8) {
-    __builtin_memcpy(&p, at, sizeof(p));
+__device__ __forceinline__ float f32_of_bits(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+  else return to_f32(__builtin_bit_cast(T, (uint16_t)w));
+}
+// N neighbouring values as words (two of 16 bits a word, a single one by itself)
+template <class T, int N>
+struct Words {
+  static constexpr int W = (N * (int)sizeof(T) + 3) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    else return f32_of_bits<T>(j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu);
+  }
+};
+// N values at `at` of which the first `left` exist (zeros past them), at any alignment; `safe`: a value that exists
+template <class T, int N>
+__device__ __forceinline__ void load_words(Words<T, N> &p, const T *at, int left, const T *safe) {
+  if (left >= N) {
+    if constexpr (N * sizeof(T) < 4) p.w[0] = bits_of(*at);
+    else __builtin_memcpy(p.w, at, N * sizeof(T));
   } else {
+    uint32_t e[N];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) p.v[j] = j < left ? at[j] : from_f32<T>(0.f);
+    for (int j = 0; j < N; ++j) e[j] = bits_of(*(j < left ? at + j : safe));
+#pragma unroll
+    for (int j = 0; j < N; ++j) e[j] = j < left ? e[j] : 0u;
+#pragma unroll
+    for (int k = 0; k < Words<T, N>::W; ++k) {
+      if constexpr (sizeof(T) == 4) p.w[k] = e[k];
+      else p.w[k] = 2 * k + 1 < N ? e[2 * k] | e[2 * k + 1] << 16 : e[2 * k];
+    }
   }
 }
+// 8 values of the summed index as terms
 template <class T, int NT>
-__device__ __forceinline__ void frag_of(const Pack8<T> &p, v8bf (&t)[NT]) {
+__device__ __forceinline__ void frag_of(const Words<T, 8> &p, v8bf (&t)[NT]) {
   if constexpr (sizeof(T) == 2 && NT == 1) {
-    t[0] = __builtin_bit_cast(v8bf, p);
+    t[0] = __builtin_bit_cast(v8bf, v4u{p.w[0], p.w[1], p.w[2], p.w[3]});
   } else {
     float f[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = to_f32(p.v[j]);
+    for (int j = 0; j < 8; ++j) f[j] = p.get(j);
     split_terms<T, NT>(f, t);
   }
 }
-// NF neighbouring values at `at`, of which `left` exist
-template <class T, int NF>
-__device__ __forceinline__ void load_rows(T (&p)[NF], const T *at, int left) {
-  if (left >= NF) {
-    __builtin_memcpy(p, at, sizeof(p));
+// the same from 8 groups of NF neighbouring rows: row h of each
+template <class T, int NT, int NF>
+__device__ __forceinline__ void frag_of_rows(const Words<T, NF> (&p)[8], int h, v8bf (&t)[NT]) {
+  if constexpr (sizeof(T) == 2 && NT == 1) {
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] = __builtin_amdgcn_perm(p[2 * j + 1].w[h / 2], p[2 * j].w[h / 2], h & 1 ? 0x07060302u : 0x05040100u);
+    t[0] = __builtin_bit_cast(v8bf, v4u{o[0], o[1], o[2], o[3]});
   } else {
+    float f[8];
 #pragma unroll
-    for (int h = 0; h < NF; ++h) p[h] = h < left ? at[h] : from_f32<T>(0.f);
+    for (int j = 0; j < 8; ++j) f[j] = p[j].get(h);
+    split_terms<T, NT>(f, t);
   }
-}
-template <class T, int NF>
-__device__ __forceinline__ Pack8<T> column_of(const T (&p)[8][NF], int h) {
-  Pack8<T> r;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) r.v[j] = p[j][h];
-  return r;
 }
 // acc += all wanted products of the terms of a (rows of the result's lanes) and b (its columns)
 template <bool F16, int NA, int NB>
@@ -122,264 +263,346 @@ constexpr int terms_beside() {
   return std::is_same<T, float>::value ? 3 : std::is_same<T, O>::value ? 1 : std::is_same<T, bf16>::value ? 1 : 2;
 }
 
-// ============================================================ shrink
+// ============================================================ both products
 //
-// A workgroup takes an item, 16 NF of r and a slice of k; its four waves take 64 k of it in turn (whole lines of x) for
-// all 64 tokens, so each value of M is read once a workgroup, and their sums meet in LDS.
-template <class TX, class TW, bool KC, int NF>
-struct LoraShrink {
-  static constexpr int NX = terms_beside<TX, TW>(), NW = terms_beside<TW, TX>();
+// A workgroup takes an item.  Over the long axis its eight waves take a line of x (64 k of 16 bits, 32 of f32) in turn for
+// all of its tokens and 16 NF of r, so each value of M is read once a workgroup, from L2 as a rule; x's next line is asked
+// for before the wave waits for M's.  The waves' sums meet in LDS as v and become terms there.  Over the short axis a wave
+// takes 64 columns at a time; columns are given to fragments so that a lane ends with 16 neighbouring ones of a row:
+// residual and result go in whole lines.
+//
+// RL: values of r whose terms LDS has room for.  Workgroups from g.rest on look through 64 tokens each for those without
+// an adapter: their rows are the residual (or zeros), and NaN where the id names none.
+constexpr int LORA_WAVES = 8;
+template <class TX, class TW, bool KC, int NF, int RL, class TY>
+struct Lora {
+  static constexpr int NX = terms_beside<TX, TW>(), NM = terms_beside<TW, TX>(), NL = terms_beside<TW, float>();
   static constexpr bool F16 = std::is_same<TX, _Float16>::value && std::is_same<TW, _Float16>::value;
-  // the sums of MT tiles of 16 tokens over this wave's part of [k0, k1)
+  static constexpr int H = 4 / (int)sizeof(TX), LINE = 32 * H;  // matrix instructions and k of a step
+  static constexpr int NR = 16 * NF, LD = RL + 8;               // (8 more: 16 rows cover all banks)
+  static constexpr int C = 4;                                   // fragments of 16 columns of a wave
+  struct Lds {
+    float sums[LORA_WAVES][16][NR + 4];
+    uint16_t terms[3][LORA_TOKENS][LD];
+  };
+
+  // the sums of MT tiles of 16 tokens over this wave's lines
   template <int MT>
-  __device__ __forceinline__ static void sums(const LoraArgs &g, const LoraItem &it, int r0, int64_t k0, int64_t k1,
-                                              v4f (&acc)[MT][NF]) {
+  __device__ __forceinline__ static void long_axis(const LoraArgs &g, const LoraItem &it, int r0, v4f (&acc)[MT][NF]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
-    const TW *m = (const TW *)g.m + it.e * g.adapter;
-    const TX *x[MT];  // (tokens past the item's last repeat it, rows past R others: what they give is not stored)
+    const TW *m = (const TW *)g.m + it.e * g.m_adapter;
+    const TX *x[MT];  // (tokens past the item's last, and rows past R, repeat others: what they give is not used)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) x[i] = (const TX *)g.x + (int64_t)it.tokens[min(16 * i + fr, it.count - 1)] * g.ldx;
+    for (int i = 0; i < MT; ++i) x[i] = (const TX *)g.x + it.token(16 * i + fr) * g.ldx + 8 * fc;
     const int rc = NF * fr + r0 < g.R ? NF * fr + r0 : 0, rl = min(g.R - rc, NF);
+    const TW *row[NF];
+#pragma unroll
+    for (int h = 0; h < NF; ++h) row[h] = m + (int64_t)min(r0 + 16 * h + fr, g.R - 1) * g.ldm + 8 * fc;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int h = 0; h < NF; ++h) acc[i][h] = v4f{0.f, 0.f, 0.f, 0.f};
-    auto step = [&](int64_t k, auto whole) {
-      Pack8<TX> px[2][MT];
-      Pack8<TW> pk[2][NF];
-      TW pr[2][8][NF];
+    struct X {
+      Words<TX, 8> p[H][MT];
+    };
+    struct M {
+      Words<TW, 8> p[H][KC ? NF : 1];
+      Words<TW, NF> r[H][KC ? 1 : 8];
+    };
+    auto load_x = [&](X &to, int64_t k, auto whole) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int64_t ks = k + 32 * s + 8 * fc;
-        const int left = decltype(whole)::value ? 8 : (int)min(k1 - ks, (int64_t)8);
+      for (int s = 0; s < H; ++s)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) load_k(px[s][i], x[i] + ks, left);
+        for (int i = 0; i < MT; ++i)
+          load_words(to.p[s][i], x[i] + k + 32 * s, decltype(whole)::value ? 8 : (int)min(g.K - (k + 32 * s + 8 * fc), (int64_t)8),
+                 (const TX *)g.x);
+    };
+    auto load_m = [&](M &to, int64_t k, auto whole) {
+#pragma unroll
+      for (int s = 0; s < H; ++s) {
+        const int64_t ks = k + 32 * s;
+        const int left = decltype(whole)::value ? 8 : (int)min(g.K - (ks + 8 * fc), (int64_t)8);
         if constexpr (KC) {
 #pragma unroll
-          for (int h = 0; h < NF; ++h) load_k(pk[s][h], m + (int64_t)min(r0 + 16 * h + fr, g.R - 1) * g.ldm + ks, left);
+          for (int h = 0; h < NF; ++h) load_words(to.p[s][h], row[h] + ks, left, m);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) load_rows<TW, NF>(pr[s][j], m + (ks + j) * g.ldm + rc, j < left ? rl : 0);
+          for (int j = 0; j < 8; ++j)
+            load_words(to.r[s][j], m + (ks + 8 * fc + j) * g.ldm + rc, decltype(whole)::value ? NF : j < left ? rl : 0, m);
         }
       }
+    };
+    auto multiply = [&](const X &px, const M &pm) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        v8bf fw[NF][NW];
+      for (int s = 0; s < H; ++s) {
+        v8bf fm[NF][NM];
 #pragma unroll
         for (int h = 0; h < NF; ++h) {
-          if constexpr (KC) frag_of<TW, NW>(pk[s][h], fw[h]);
-          else frag_of<TW, NW>(column_of<TW, NF>(pr[s], h), fw[h]);
+          if constexpr (KC) frag_of(pm.p[s][h], fm[h]);
+          else frag_of_rows(pm.r[s], h, fm[h]);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           v8bf fx[NX];
-          frag_of<TX, NX>(px[s][i], fx);
+          frag_of(px.p[s][i], fx);
 #pragma unroll
-          for (int h = 0; h < NF; ++h) mul_terms<F16, NW, NX>(acc[i][h], fw[h], fx);
+          for (int h = 0; h < NF; ++h) mul_terms<F16, NM, NX>(acc[i][h], fm[h], fx);
         }
       }
     };
-    int64_t k = k0 + 64 * wave;
-    for (; k + 64 <= k1; k += 256) step(k, std::true_type());
-    if (k < k1) step(k, std::false_type());
-  }
-  // and those of all waves, to the slice's part of v
-  template <int MT>
-  __device__ __forceinline__ static void run(const LoraArgs &g, const LoraItem &it, int z, int r0,
-                                             float (&red)[4][16][16 * NF + 4]) {
-    constexpr int NR = 16 * NF;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
-    v4f acc[MT][NF];
-    const int64_t k0 = z * g.kslice;
-    sums<MT>(g, it, r0, k0, min(g.K, k0 + g.kslice), acc);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      if (16 * i >= it.count) break;
-      if (i) __syncthreads();
-#pragma unroll
-      for (int h = 0; h < NF; ++h)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) red[wave][fr][KC ? 16 * h + 4 * fc + q : NF * (4 * fc + q) + h] = acc[i][h][q];
-      __syncthreads();
-      for (int t = threadIdx.x; t < 16 * NR; t += 256) {
-        const int s = t / NR, r = t % NR;
-        if (16 * i + s >= it.count || r0 + r >= g.R) continue;
-        g.part[((size_t)z * g.S + it.tokens[16 * i + s]) * g.R + r0 + r] =
-            (red[0][s][r] + red[1][s][r]) + (red[2][s][r] + red[3][s][r]);
+    constexpr int STEP = LINE * LORA_WAVES;
+    int64_t k = LINE * wave;
+    if (k + LINE <= g.K && (KC || g.R % NF == 0)) {
+      X a, b;
+      M m0;
+      load_x(a, k, std::true_type());
+      // (the line after the last is asked for at the place of one that exists)
+      auto next = [&](int64_t k) { return k + STEP + LINE <= g.K ? k + STEP : k; };
+      for (;;) {
+        load_m(m0, k, std::true_type());
+        load_x(b, next(k), std::true_type());
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(a, m0);
+        __builtin_amdgcn_sched_barrier(0);
+        if ((k += STEP) + LINE > g.K) break;
+        load_m(m0, k, std::true_type());
+        load_x(a, next(k), std::true_type());
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(b, m0);
+        __builtin_amdgcn_sched_barrier(0);
+        if ((k += STEP) + LINE > g.K) break;
       }
     }
-  }
-};
-template <class TX, class TW, bool KC, int NF>
-__global__ __launch_bounds__(256) void k_lora_shrink(LoraArgs g) {
-  const int per = g.slices * g.chunks, b = blockIdx.x % per, z = b % g.slices, r0 = b / g.slices * 16 * NF;
-  __shared__ float red[4][16][16 * NF + 4];
-  LoraItem it;
-  if (!lora_item(g, blockIdx.x / per, it)) return;
-  if (it.count <= 16) LoraShrink<TX, TW, KC, NF>::template run<1>(g, it, z, r0, red);
-  else LoraShrink<TX, TW, KC, NF>::template run<LORA_TOKENS / 16>(g, it, z, r0, red);
-}
-
-// ============================================================ expand
-//
-// A workgroup takes an item and 256 columns, 64 a wave.  The slices of v are added, scaled and split into terms in LDS
-// once; matrices come straight from memory.  Columns are given to fragments so that a lane ends with 16 neighbouring
-// ones of a row: residual and result go in whole lines.  Workgroups from g.rest on look through 64 tokens each for those
-// without an adapter: their rows are the residual (or zeros), and NaN where the id names none.
-// r whose terms lie in LDS at a time: all up to 128 (52 KB)
-__host__ __device__ __forceinline__ int lora_r_step(int R) { return R < 128 ? (R + 31) & ~31 : 128; }
-__device__ __forceinline__ void load16(v4f (&v)[4], const void *p, int type, size_t i, int left) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (4 * q + 4 <= left) {
-      v[q] = lin_load4(p, type, i + 4 * q);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[q][j] = 4 * q + j < left ? lin_load(p, type, i + 4 * q + j) : 0.f;
+    for (; k < g.K; k += STEP) {
+      X a;
+      M m0;
+      load_x(a, k, std::false_type());
+      load_m(m0, k, std::false_type());
+      multiply(a, m0);
     }
   }
-}
-template <class TW, bool KC>
-__global__ __launch_bounds__(256) void k_lora_expand(LoraArgs g) {
-  constexpr int NW = terms_beside<TW, float>(), NF = 4, MT = LORA_TOKENS / 16;
-  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
-  const int chunk = blockIdx.x % g.chunks, item = blockIdx.x / g.chunks;
-  const int64_t o0 = (int64_t)chunk * 256 + 64 * wave;
-  if (item >= g.rest) {
-    const int s0 = (item - g.rest) * 64;
+
+  template <int MT>
+  __device__ __forceinline__ static void run(const LoraArgs &g, const LoraItem &it, Lds &lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
+    const float c = g.scale ? g.scale[it.e] : 1.f;
+    for (int r0 = 0; r0 < g.R; r0 += NR) {
+      v4f acc[MT][NF];
+      long_axis<MT>(g, it, r0, acc);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if (r0 || i) __syncthreads();
+#pragma unroll
+        for (int h = 0; h < NF; ++h) {
+          if constexpr (KC) {
+            *reinterpret_cast<v4f *>(&lds.sums[wave][fr][16 * h + 4 * fc]) = acc[i][h];
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) lds.sums[wave][fr][NF * (4 * fc + q) + h] = acc[i][h][q];
+          }
+        }
+        __syncthreads();
+        constexpr int WIDE = NR < 32 ? 32 : NR;  // (zeros up to the 32 of a matrix instruction)
+        for (int t = threadIdx.x; t < 16 * WIDE; t += 64 * LORA_WAVES) {
+          const int s = t / WIDE, r = t % WIDE;
+          float v = 0.f;
+          if (r < NR && r0 + r < g.R) {
+#pragma unroll
+            for (int u = 0; u < LORA_WAVES; ++u) v += lds.sums[u][s][r];
+            if (g.v && 16 * i + s < it.count) g.v[(size_t)it.tokens[16 * i + s] * g.R + r0 + r] = v;
+            v *= c;
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const bf16 e = from_f32<bf16>(k ? v : __builtin_amdgcn_fmed3f(v, -BF16_MOST, BF16_MOST));
+            lds.terms[k][16 * i + s][r0 + r] = e.u;
+            v -= to_f32(e);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    short_axis<MT>(g, it, lds);
+  }
+
+  template <int MT>
+  __device__ __forceinline__ static void short_axis(const LoraArgs &g, const LoraItem &it, const Lds &lds) {
+    constexpr int AHEAD = RL / 32 < 2 ? RL / 32 : 2;  // steps of r whose matrix is asked for ahead
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
+    const TW *l = (const TW *)g.l + it.e * g.l_adapter;
+    const TY *res[MT];
+    TY *y[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t s = it.token(16 * i + fr);
+      res[i] = (const TY *)g.res + s * g.ldr + 16 * fc;
+      y[i] = (TY *)g.y + s * g.ldy + 16 * fc;
+    }
+    struct Raw {
+      Words<TW, 8> p[KC ? C : 1];
+      Words<TW, C> r[KC ? 1 : 8];
+    };
+    // 32 of r from r on of 64 columns (zeros past R: v has zeros there, but what lies there may be no number); whole: all
+    // columns exist, and KC's packs of 8 end with R
+    auto load_l = [&](Raw &to, int64_t o0, int r, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      r += 8 * fc;
+      const int left = min(g.R - r, 8);
+      if constexpr (KC) {
+#pragma unroll
+        for (int h = 0; h < C; ++h) {
+          const TW *at = l + min(o0 + 16 * (fr >> 2) + 4 * h + (fr & 3), g.N - 1) * g.ldl;
+          if constexpr (WHOLE) {
+            load_words(to.p[h], at + (left > 0 ? r : 0), 8, at);
+#pragma unroll
+            for (int k = 0; k < Words<TW, 8>::W; ++k) to.p[h].w[k] = left > 0 ? to.p[h].w[k] : 0u;
+          } else {
+            load_words(to.p[h], at + r, left, at);
+          }
+        }
+      } else {
+        const int64_t o = WHOLE ? o0 + C * fr : min(o0 + C * fr, g.N - 1);
+        const int cols = (int)min(g.N - o, (int64_t)C);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          load_words(to.r[j], l + min(r + j, g.R - 1) * g.ldl + o, WHOLE ? C : cols, l);
+#pragma unroll
+          for (int k = 0; k < Words<TW, C>::W; ++k) to.r[j].w[k] = j < left ? to.r[j].w[k] : 0u;
+        }
+      }
+    };
+    auto columns = [&](int64_t o0, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      const int left = WHOLE ? 16 : (int)min(g.N - (o0 + 16 * fc), (int64_t)16);
+      Words<TY, 16> z[MT];
+      Raw raw[AHEAD];
+      if (g.res) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) load_words(z[i], res[i] + o0, left, (const TY *)g.res);
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (32 * k < g.R) load_l(raw[k], o0, 32 * k, whole);
+      __builtin_amdgcn_sched_barrier(0);
+      v4f acc[MT][C];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < C; ++h) acc[i][h] = v4f{0.f, 0.f, 0.f, 0.f};
+      auto step = [&](const Raw &raw, int r) {
+        v8bf fl[C][NL];
+#pragma unroll
+        for (int h = 0; h < C; ++h) {
+          if constexpr (KC) frag_of(raw.p[h], fl[h]);
+          else frag_of_rows(raw.r, h, fl[h]);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          v8bf fv[3];
+#pragma unroll
+          for (int k = 0; k < 3; ++k) fv[k] = *reinterpret_cast<const v8bf *>(&lds.terms[k][16 * i + fr][r + 8 * fc]);
+#pragma unroll
+          for (int h = 0; h < C; ++h) mul_terms<false, NL, 3>(acc[i][h], fl[h], fv);
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (32 * k < g.R) step(raw[k], 32 * k);
+      if constexpr (RL > 64) {
+        for (int r = 64; r < g.R; r += 32) {
+          load_l(raw[0], o0, r, whole);
+          step(raw[0], r);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if (16 * i + fr >= it.count) continue;
+        Words<TY, 16> out;
+        float f[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float a = KC ? acc[i][q][j] : acc[i][j][q];
+            f[4 * q + j] = g.res ? z[i].get(4 * q + j) + a : a;
+          }
+#pragma unroll
+        for (int k = 0; k < Words<TY, 16>::W; ++k) {
+          if constexpr (sizeof(TY) == 4) out.w[k] = bits_of(f[k]);
+          else out.w[k] = bits_of(from_f32<TY>(f[2 * k])) | bits_of(from_f32<TY>(f[2 * k + 1])) << 16;
+        }
+        if (left >= 16) {
+          __builtin_memcpy(y[i] + o0, out.w, sizeof(out.w));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (j < left) y[i][o0 + j] = from_f32<TY>(f[j]);
+        }
+      }
+    };
+    for (int64_t o0 = 64 * wave; o0 < g.N; o0 += 64 * LORA_WAVES) {
+      if (o0 + 64 <= g.N && (!KC || g.R % 8 == 0)) columns(o0, std::true_type());
+      else columns(o0, std::false_type());
+    }
+  }
+
+  // tokens without an adapter among 64
+  __device__ __forceinline__ static void rest(const LoraArgs &g, int s0) {
+    const int lane = threadIdx.x & 63;
     const int e = s0 + lane < g.S ? g.ids[s0 + lane] : 0;
     uint64_t todo = __ballot((unsigned)e >= (unsigned)g.n);
     while (todo) {
       const int k = __builtin_ctzll(todo);
       todo &= todo - 1;
-      const int s = s0 + k, ek = __builtin_amdgcn_readlane(e, k);
-      const float fill = ek < 0 ? 0.f : __builtin_nanf("");
-      const int64_t o = o0 + lane;
-      if (o < g.N) {
-        float y = fill;
-        if (ek < 0 && g.res) y = lin_load(g.res, g.type, (size_t)(s * g.ldr + o));
-        lin_store(g.y, g.type, (size_t)(s * g.ldy + o), y);
-      }
-      if (g.v && !chunk)
-        for (int r = threadIdx.x; r < g.R; r += 256) g.v[(size_t)s * g.R + r] = fill;
+      const int64_t s = s0 + k;
+      const bool none = __builtin_amdgcn_readlane(e, k) < 0;
+      const float fill = none ? 0.f : __builtin_nanf("");
+      for (int64_t o = threadIdx.x; o < g.N; o += 64 * LORA_WAVES)
+        ((TY *)g.y)[s * g.ldy + o] = none && g.res ? ((const TY *)g.res)[s * g.ldr + o] : from_f32<TY>(fill);
+      if (g.v)
+        for (int r = threadIdx.x; r < g.R; r += 64 * LORA_WAVES) g.v[(size_t)s * g.R + r] = fill;
     }
-    return;
   }
+};
+template <class TX, class TW, bool KC, int NF, int RL, class TY>
+__global__ __launch_bounds__(64 * LORA_WAVES) void k_lora(LoraArgs g) {
+  typedef Lora<TX, TW, KC, NF, RL, TY> L;
+  __shared__ __attribute__((aligned(16))) typename L::Lds lds;
+  if ((int)blockIdx.x >= g.rest) return L::rest(g, ((int)blockIdx.x - g.rest) * 64);
   LoraItem it;
-  if (!lora_item(g, item, it)) return;
-  const int mt = (it.count + 15) >> 4;
-  const int RP = lora_r_step(g.R), LD = RP + 8, PLANE = LORA_TOKENS * LD;  // (8 more: 16 rows cover all banks)
-  const float c = g.scale ? g.scale[it.e] : 1.f;
-  const TW *m = (const TW *)g.m + it.e * g.adapter;
-  v4f acc[MT][NF];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int h = 0; h < NF; ++h) acc[i][h] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int rb = 0; rb < g.R; rb += RP) {
-    if (rb) __syncthreads();
-    for (int t = threadIdx.x; t < 16 * mt * RP; t += 256) {  // v: added, scaled, split
-      const int s = t / RP, r = t - s * RP;
-      float f = 0.f;
-      if (s < it.count && rb + r < g.R) {
-        const size_t at = (size_t)it.tokens[s] * g.R + rb + r;
-        for (int z = 0; z < g.slices; ++z) f += g.part[(size_t)z * g.S * g.R + at];
-        if (g.v && !chunk) g.v[at] = f;
-        f *= c;
-      }
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        const bf16 e = from_f32<bf16>(k ? f : __builtin_amdgcn_fmed3f(f, -BF16_MOST, BF16_MOST));
-        lds[k * PLANE + s * LD + r] = e.u;
-        f -= to_f32(e);
-      }
-    }
-    __syncthreads();
-    if (o0 >= g.N) continue;
-    for (int rk = 0; rk < RP && rb + rk < g.R; rk += 32) {
-      const int r = rb + rk + 8 * fc, left = min(g.R - r, 8);
-      v8bf fw[NF][NW];
-      if constexpr (KC) {
-#pragma unroll
-        for (int h = 0; h < NF; ++h) {
-          Pack8<TW> p;
-          load_k(p, m + min(o0 + 16 * (fr >> 2) + 4 * h + (fr & 3), g.N - 1) * g.ldm + r, left);
-          frag_of<TW, NW>(p, fw[h]);
-        }
-      } else {
-        TW p[8][NF];
-        const int64_t o = min(o0 + NF * fr, g.N - 1);
-        const int cols = (int)min(g.N - o, (int64_t)NF);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) load_rows<TW, NF>(p[j], m + (r + j) * g.ldm + o, j < left ? cols : 0);
-#pragma unroll
-        for (int h = 0; h < NF; ++h) frag_of<TW, NW>(column_of<TW, NF>(p, h), fw[h]);
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        if (i >= mt) break;
-        v8bf fv[3];
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-          fv[k] = *reinterpret_cast<const v8bf *>(lds + k * PLANE + (16 * i + fr) * LD + rk + 8 * fc);
-#pragma unroll
-        for (int h = 0; h < NF; ++h) mul_terms<false, NW, 3>(acc[i][h], fw[h], fv);
-      }
-    }
-  }
-  if (o0 < g.N) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      if (16 * i + fr >= it.count) continue;
-      const int64_t s = it.tokens[16 * i + fr], o = o0 + 16 * fc;
-      const int left = (int)min(g.N - o, (int64_t)16);
-      v4f y[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[q][j] = KC ? acc[i][q][j] : acc[i][j][q];
-      if (g.res) {
-        v4f z[4];
-        load16(z, g.res, g.type, (size_t)(s * g.ldr + o), left);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) y[q] += z[q];
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (4 * q + 4 <= left) {
-          lin_store4(g.y, g.type, (size_t)(s * g.ldy + o + 4 * q), y[q]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (4 * q + j < left) lin_store(g.y, g.type, (size_t)(s * g.ldy + o + 4 * q + j), y[q][j]);
-        }
-      }
-    }
-  }
+  if (!lora_item(g, blockIdx.x, it)) return;
+  if (it.count <= 16) L::template run<1>(g, it, lds);
+  else L::template run<2>(g, it, lds);
 }
-inline size_t lora_expand_lds(int R) { return (size_t)3 * LORA_TOKENS * (lora_r_step(R) + 8) * 2; }
 
 // ============================================================ sums over an adapter's tokens
 //
 // result[e][r][j] = c[e] sum over its tokens of a[s][r] m[s][j], or with r and j changed (BY_R, dB's order).  A workgroup
 // takes an adapter, 64 columns j, 16 NR of r and a slice of its tokens; its waves take 32 tokens in turn, and their sums
 // meet in LDS.  Both operands are summed over their rows in memory.
+struct LoraSumArgs {
+  const float *a;        // [S][R]
+  const void *m;
+  int64_t ldm, N;
+  int R, n, slices, chunks;  // slices of tokens, chunks of r
+  const float *scale;
+  float *out;            // [slices][n][R][N], or [slices][n][N][R]
+};
 template <class TM, int NR, bool BY_R>
-__global__ __launch_bounds__(256) void k_lora_sums(LoraArgs g) {
-  constexpr int NM = terms_beside<TM, float>(), NF = 4;
-  __shared__ float red[4][NF][256];
+__device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraItems &items, unsigned b,
+                                             float (&red)[LORA_WAVES][4][256]) {
+  constexpr int NM = terms_beside<TM, float>(), NF = 4, STEP = 32 * LORA_WAVES;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
-  const int64_t cols = (g.N + 63) / 64;
-  int64_t b = blockIdx.x;
-  const int64_t j0 = b % cols * 64;
+  const unsigned cols = (unsigned)((g.N + 63) / 64);
+  const int64_t j0 = (int64_t)(b % cols) * 64;
   b /= cols;
   const int r0 = (int)(b % g.chunks) * 16 * NR;
   b /= g.chunks;
   const int z = (int)(b % g.slices), e = (int)(b / g.slices);
-  const int count = g.counts[e], per = ((count + g.slices - 1) / g.slices + 31) & ~31;
+  const int count = items.counts[e], per = ((count + g.slices - 1) / g.slices + 31) & ~31;
   const int t0 = min(z * per, count), t1 = min(t0 + per, count);
-  const int32_t *tokens = g.pairs + g.offs[e];
+  const int32_t *tokens = items.tokens + (size_t)items.first[e] * LORA_TOKENS;
+  const float c = g.scale ? g.scale[e] : 1.f;
   v4f acc[NR][NF];
 #pragma unroll
   for (int h = 0; h < NR; ++h)
@@ -388,33 +611,41 @@ __global__ __launch_bounds__(256) void k_lora_sums(LoraArgs g) {
   const int64_t j = min(j0 + NF * fr, g.N - 1);
   const int jl = (int)min(g.N - j, (int64_t)NF);
   const int r = min(r0 + NR * fr, g.R - 1), rl = min(g.R - r, NR);
-  for (int t = t0 + 32 * wave; t < t1; t += 128) {
-    float pa[8][NR];
-    TM pm[8][NF];
+  const float *a = g.a + r;
+  const TM *m = (const TM *)g.m + j;
+  auto step = [&](int t, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    int s[8];
+    Words<float, NR> pa[8];
+    Words<TM, NF> pm[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] = tokens[WHOLE ? t + 8 * fc + k : min(t + 8 * fc + k, t1 - 1)];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int at = t + 8 * fc + k;
-      const bool in = at < t1;
-      const int64_t s = tokens[in ? at : t0];
-      load_rows<float, NR>(pa[k], g.v + s * g.R + r, in ? rl : 0);
-      load_rows<TM, NF>(pm[k], (const TM *)g.x + s * g.ldx + j, in ? jl : 0);
+      const bool in = WHOLE || t + 8 * fc + k < t1;
+      load_words(pa[k], a + (int64_t)s[k] * g.R, WHOLE ? NR : in ? rl : 0, g.a);
+      load_words(pm[k], m + (int64_t)s[k] * g.ldm, WHOLE ? NF : in ? jl : 0, (const TM *)g.m);
     }
+    __builtin_amdgcn_sched_barrier(0);
     v8bf fm[NF][NM];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) frag_of<TM, NM>(column_of<TM, NF>(pm, f), fm[f]);
+    for (int f = 0; f < NF; ++f) frag_of_rows(pm, f, fm[f]);
 #pragma unroll
     for (int h = 0; h < NR; ++h) {
       v8bf fa[3];
-      frag_of<float, 3>(column_of<float, NR>(pa, h), fa);
+      frag_of_rows(pa, h, fa);
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
         if constexpr (BY_R) mul_terms<false, 3, NM>(acc[h][f], fa, fm[f]);
         else mul_terms<false, NM, 3>(acc[h][f], fm[f], fa);
       }
     }
-  }
-  const float c = g.scale ? g.scale[e] : 1.f;
-  float *out = (float *)g.y + ((size_t)z * g.n + e) * g.R * g.N;
+  };
+  int t = t0 + 32 * wave;
+  if (j0 + 64 <= g.N && r0 + 16 * NR <= g.R)
+    for (; t + 32 <= t1; t += STEP) step(t, std::true_type());
+  for (; t < t1; t += STEP) step(t, std::false_type());
+  float *out = g.out + ((size_t)z * g.n + e) * g.R * g.N;
 #pragma unroll
   for (int h = 0; h < NR; ++h) {
     if (h) __syncthreads();
@@ -425,17 +656,26 @@ __global__ __launch_bounds__(256) void k_lora_sums(LoraArgs g) {
     __syncthreads();
     // value (f, lane, q): index 4 fc + q of the operand that gives the rows, fr of the other; neighbours of the result
     // go to neighbouring threads
-    for (int t = threadIdx.x; t < NF * 256; t += 256) {
+    for (int t = threadIdx.x; t < NF * 256; t += 64 * LORA_WAVES) {
       const int jr = BY_R ? t >> 4 : t & 63, ri = BY_R ? t & 15 : t >> 6;  // j - j0, and r = r0 + NR ri + h
       const int f = jr & 3, row = BY_R ? ri : jr >> 2, col = BY_R ? jr >> 2 : ri;
       const int k = 64 * (row & 3) + 16 * (row >> 2) + col;
       const int64_t jj = j0 + jr;
       const int rr = r0 + NR * ri + h;
       if (jj >= g.N || rr >= g.R) continue;
-      const float v = c * ((red[0][f][k] + red[1][f][k]) + (red[2][f][k] + red[3][f][k]));
-      out[BY_R ? (size_t)jj * g.R + rr : (size_t)rr * g.N + jj] = v;
+      float v = 0.f;
+#pragma unroll
+      for (int u = 0; u < LORA_WAVES; ++u) v += red[u][f][k];
+      out[BY_R ? (size_t)jj * g.R + rr : (size_t)rr * g.N + jj] = c * v;
     }
   }
+}
+// dA by the first `na` workgroups, dB by the others: what they wait for is the same
+template <class TX, class TY, int NR>
+__global__ __launch_bounds__(64 * LORA_WAVES) void k_lora_sums(LoraItems items, LoraSumArgs a, LoraSumArgs b, unsigned na) {
+  __shared__ float red[LORA_WAVES][4][256];
+  if (blockIdx.x < na) lora_sums_wg<TX, NR, false>(a, items, blockIdx.x, red);
+  else lora_sums_wg<TY, NR, true>(b, items, blockIdx.x - na, red);
 }
 
 // ============================================================ few tokens
@@ -525,12 +765,21 @@ __global__ __launch_bounds__(512) void k_lora_few(LoraFewArgs g) {
   lin_store(g.y, g.type, (size_t)(s * g.ldy + o), y);
 }
 
-// the products by their operands' types; `kc`: the forward pass's order of the matrices
-void lora_shrink(int x_type, int w_type, bool kc, const LoraArgs &g, int grid, hipStream_t st);
-void lora_expand(int w_type, bool kc, const LoraArgs &g, int grid, hipStream_t st);
-void lora_sums(int m_type, bool by_r, const LoraArgs &g, int grid, hipStream_t st);
+// the kernels by their operands' types: of the rows, the adapters and the result
+void lora_forward(int x_type, int w_type, int y_type, const LoraArgs &g, int grid, hipStream_t st);
+void lora_backward(int x_type, int w_type, int y_type, const LoraArgs &g, int grid, hipStream_t st);
+void lora_sums(int x_type, int dy_type, const LoraItems &items, const LoraSumArgs &a, unsigned na, const LoraSumArgs &b,
+               unsigned nb, hipStream_t st);
 void lora_few(int x_type, int w_type, const LoraFewArgs &g, dim3 grid, hipStream_t st);
-// r of a workgroup: 16, 32 or 64
+template <class TX, class TW, bool KC, class TY>
+void lora_launch(const LoraArgs &g, int grid, hipStream_t st) {
+  const dim3 n(grid), wg(64 * LORA_WAVES);
+  if (g.R <= 16) hipLaunchKernelGGL((k_lora<TX, TW, KC, 1, 32, TY>), n, wg, 0, st, g);
+  else if (g.R <= 32) hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 32, TY>), n, wg, 0, st, g);
+  else if (g.R <= 64) hipLaunchKernelGGL((k_lora<TX, TW, KC, 4, 64, TY>), n, wg, 0, st, g);
+  else hipLaunchKernelGGL((k_lora<TX, TW, KC, 4, 256, TY>), n, wg, 0, st, g);
+}
+// r of a workgroup of sums: 16, 32 or 64
 inline int lora_r_of(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : 64; }
 
 }  // namespace zm

@@ -1,5 +1,4 @@
-// zm_lora_b.hip -- adapters: the product over the short axis, v by B and (backward) u by A; the sums over an adapter's
-// tokens; a few tokens at once
+// zm_lora_b.hip -- adapters: the sums over an adapter's tokens, and a few tokens at once
 #include <hip/hip_runtime.h>
 
 #include "zm_lora.hpp"
@@ -7,18 +6,13 @@
 namespace zm {
 namespace {
 
-template <class TW>
-void expand(bool kc, const LoraArgs &g, int grid, hipStream_t st) {
-  const size_t n = lora_expand_lds(g.R);
-  if (kc) hipLaunchKernelGGL((k_lora_expand<TW, true>), dim3(grid), dim3(256), n, st, g);
-  else hipLaunchKernelGGL((k_lora_expand<TW, false>), dim3(grid), dim3(256), n, st, g);
-}
-template <class TM, bool BY_R>
-void sums(const LoraArgs &g, int grid, hipStream_t st) {
-  switch (lora_r_of(g.R)) {
-  case 16: hipLaunchKernelGGL((k_lora_sums<TM, 1, BY_R>), dim3(grid), dim3(256), 0, st, g); break;
-  case 32: hipLaunchKernelGGL((k_lora_sums<TM, 2, BY_R>), dim3(grid), dim3(256), 0, st, g); break;
-  default: hipLaunchKernelGGL((k_lora_sums<TM, 4, BY_R>), dim3(grid), dim3(256), 0, st, g);
+template <class TX, class TY>
+void sums(const LoraItems &items, const LoraSumArgs &a, unsigned na, const LoraSumArgs &b, unsigned nb, hipStream_t st) {
+  const dim3 grid(na + nb), wg(64 * LORA_WAVES);
+  switch (lora_r_of(a.R)) {
+  case 16: hipLaunchKernelGGL((k_lora_sums<TX, TY, 1>), grid, wg, 0, st, items, a, b, na); break;
+  case 32: hipLaunchKernelGGL((k_lora_sums<TX, TY, 2>), grid, wg, 0, st, items, a, b, na); break;
+  default: hipLaunchKernelGGL((k_lora_sums<TX, TY, 4>), grid, wg, 0, st, items, a, b, na);
   }
 }
 template <class TX, class TW>
@@ -28,15 +22,17 @@ void few(const LoraFewArgs &g, dim3 grid, hipStream_t st) {
 
 }  // namespace
 
-void lora_expand(int w_type, bool kc, const LoraArgs &g, int grid, hipStream_t st) {
-  if (w_type == LIN_BF16) expand<bf16>(kc, g, grid, st);
-  else if (w_type == LIN_F16) expand<_Float16>(kc, g, grid, st);
-  else expand<float>(kc, g, grid, st);
-}
-void lora_sums(int m_type, bool by_r, const LoraArgs &g, int grid, hipStream_t st) {
-  if (m_type == LIN_BF16) by_r ? sums<bf16, true>(g, grid, st) : sums<bf16, false>(g, grid, st);
-  else if (m_type == LIN_F16) by_r ? sums<_Float16, true>(g, grid, st) : sums<_Float16, false>(g, grid, st);
-  else by_r ? sums<float, true>(g, grid, st) : sums<float, false>(g, grid, st);
+void lora_sums(int x_type, int dy_type, const LoraItems &items, const LoraSumArgs &a, unsigned na, const LoraSumArgs &b,
+               unsigned nb, hipStream_t st) {
+  if (x_type == LIN_BF16) {
+    if (dy_type == LIN_BF16) sums<bf16, bf16>(items, a, na, b, nb, st);
+    else sums<bf16, float>(items, a, na, b, nb, st);
+  } else if (x_type == LIN_F16) {
+    if (dy_type == LIN_F16) sums<_Float16, _Float16>(items, a, na, b, nb, st);
+    else sums<_Float16, float>(items, a, na, b, nb, st);
+  } else {
+    sums<float, float>(items, a, na, b, nb, st);
+  }
 }
 void lora_few(int x_type, int w_type, const LoraFewArgs &g, dim3 grid, hipStream_t st) {
   if (x_type == LIN_BF16) few<bf16, bf16>(g, grid, st);
