@@ -265,31 +265,32 @@ constexpr int terms_beside() {
 
 // ============================================================ both products
 //
-// A workgroup takes an item.  Over the long axis its eight waves take a line of x (64 k of 16 bits, 32 of f32) in turn for
-// all of its tokens and 16 NF of r, so each value of M is read once a workgroup, from L2 as a rule; x's next line is asked
-// for before the wave waits for M's.  The waves' sums meet in LDS as v and become terms there.  Over the short axis a wave
+// A workgroup takes an item.  Over the long axis its eight waves, in G groups of 16 NF of r each, take a line of x (64 k of
+// 16 bits, 32 of f32) in turn for all of its tokens, so each value of M is read once a workgroup, from L2 as a rule.  The
+// waves' sums meet in LDS as v and become terms there.  Over the short axis a wave
 // takes 64 columns at a time; columns are given to fragments so that a lane ends with 16 neighbouring ones of a row:
 // residual and result go in whole lines.
 //
 // RL: values of r whose terms LDS has room for.  Workgroups from g.rest on look through 64 tokens each for those without
 // an adapter: their rows are the residual (or zeros), and NaN where the id names none.
 constexpr int LORA_WAVES = 8;
-template <class TX, class TW, bool KC, int NF, int RL, class TY>
+template <class TX, class TW, bool KC, int NF, int G, int RL, class TY>
 struct Lora {
   static constexpr int NX = terms_beside<TX, TW>(), NM = terms_beside<TW, TX>(), NL = terms_beside<TW, float>();
   static constexpr bool F16 = std::is_same<TX, _Float16>::value && std::is_same<TW, _Float16>::value;
   static constexpr int H = 4 / (int)sizeof(TX), LINE = 32 * H;  // matrix instructions and k of a step
   static constexpr int NR = 16 * NF, LD = RL + 8;               // (8 more: 16 rows cover all banks)
+  static constexpr int SHARE = LORA_WAVES / G;                  // waves of a group
   static constexpr int C = 4;                                   // fragments of 16 columns of a wave
   struct Lds {
     float sums[LORA_WAVES][16][NR + 4];
     uint16_t terms[3][LORA_TOKENS][LD];
   };
 
-  // the sums of MT tiles of 16 tokens over this wave's lines
+  // the sums of MT tiles of 16 tokens over this wave's lines, r from r0 on
   template <int MT>
   __device__ __forceinline__ static void long_axis(const LoraArgs &g, const LoraItem &it, int r0, v4f (&acc)[MT][NF]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % SHARE, fr = lane & 15, fc = lane >> 4;
     const TW *m = (const TW *)g.m + it.e * g.m_adapter;
     const TX *x[MT];  // (tokens past the item's last, and rows past R, repeat others: what they give is not used)
 #pragma unroll
@@ -309,26 +310,21 @@ struct Lora {
       Words<TW, 8> p[H][KC ? NF : 1];
       Words<TW, NF> r[H][KC ? 1 : 8];
     };
-    auto load_x = [&](X &to, int64_t k, auto whole) {
+    auto load_x = [&](X &to, int64_t k) {
 #pragma unroll
       for (int s = 0; s < H; ++s)
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-          load_words(to.p[s][i], x[i] + k + 32 * s, decltype(whole)::value ? 8 : (int)min(g.K - (k + 32 * s + 8 * fc), (int64_t)8),
-                 (const TX *)g.x);
+        for (int i = 0; i < MT; ++i) load_words(to.p[s][i], x[i] + k + 32 * s, 8, x[i]);
     };
-    auto load_m = [&](M &to, int64_t k, auto whole) {
+    auto load_m = [&](M &to, int64_t k) {
 #pragma unroll
       for (int s = 0; s < H; ++s) {
-        const int64_t ks = k + 32 * s;
-        const int left = decltype(whole)::value ? 8 : (int)min(g.K - (ks + 8 * fc), (int64_t)8);
         if constexpr (KC) {
 #pragma unroll
-          for (int h = 0; h < NF; ++h) load_words(to.p[s][h], row[h] + ks, left, m);
+          for (int h = 0; h < NF; ++h) load_words(to.p[s][h], row[h] + k + 32 * s, 8, m);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            load_words(to.r[s][j], m + (ks + 8 * fc + j) * g.ldm + rc, decltype(whole)::value ? NF : j < left ? rl : 0, m);
+          for (int j = 0; j < 8; ++j) load_words(to.r[s][j], m + (k + 32 * s + 8 * fc + j) * g.ldm + rc, NF, m);
         }
       }
     };
@@ -350,45 +346,61 @@ struct Lora {
         }
       }
     };
-    constexpr int STEP = LINE * LORA_WAVES;
+    // a line of which only a part exists, or of M whose rows do not end with a pack: 32 k and a fragment at a time
+    auto part = [&](int64_t k) {
+#pragma unroll 1
+      for (int s = 0; s < H; ++s, k += 32) {
+        const int left = (int)min(g.K - (k + 8 * fc), (int64_t)8);
+        v8bf fx[MT][NX];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          Words<TX, 8> p;
+          load_words(p, x[i] + k, left, (const TX *)g.x);
+          frag_of(p, fx[i]);
+        }
+        Words<TW, NF> r[KC ? 1 : 8];
+        if constexpr (!KC) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) load_words(r[j], m + (k + 8 * fc + j) * g.ldm + rc, j < left ? rl : 0, m);
+        }
+#pragma unroll
+        for (int h = 0; h < NF; ++h) {
+          v8bf fm[NM];
+          if constexpr (KC) {
+            Words<TW, 8> p;
+            load_words(p, row[h] + k, left, m);
+            frag_of(p, fm);
+          } else {
+            frag_of_rows(r, h, fm);
+          }
+#pragma unroll
+          for (int i = 0; i < MT; ++i) mul_terms<F16, NM, NX>(acc[i][h], fm, fx[i]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+    constexpr int STEP = LINE * SHARE;
     int64_t k = LINE * wave;
-    if (k + LINE <= g.K && (KC || g.R % NF == 0)) {
-      X a, b;
-      M m0;
-      load_x(a, k, std::true_type());
-      // (the line after the last is asked for at the place of one that exists)
-      auto next = [&](int64_t k) { return k + STEP + LINE <= g.K ? k + STEP : k; };
-      for (;;) {
-        load_m(m0, k, std::true_type());
-        load_x(b, next(k), std::true_type());
+    if (KC || g.R % NF == 0) {
+      for (; k + LINE <= g.K; k += STEP) {
+        X px;
+        M pm;
+        load_x(px, k);
+        load_m(pm, k);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(a, m0);
-        __builtin_amdgcn_sched_barrier(0);
-        if ((k += STEP) + LINE > g.K) break;
-        load_m(m0, k, std::true_type());
-        load_x(a, next(k), std::true_type());
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(b, m0);
-        __builtin_amdgcn_sched_barrier(0);
-        if ((k += STEP) + LINE > g.K) break;
+        multiply(px, pm);
       }
     }
-    for (; k < g.K; k += STEP) {
-      X a;
-      M m0;
-      load_x(a, k, std::false_type());
-      load_m(m0, k, std::false_type());
-      multiply(a, m0);
-    }
+    for (; k < g.K; k += STEP) part(k);
   }
 
   template <int MT>
   __device__ __forceinline__ static void run(const LoraArgs &g, const LoraItem &it, Lds &lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
     const float c = g.scale ? g.scale[it.e] : 1.f;
-    for (int r0 = 0; r0 < g.R; r0 += NR) {
+    for (int r0 = 0; r0 < g.R; r0 += NR * G) {
       v4f acc[MT][NF];
-      long_axis<MT>(g, it, r0, acc);
+      long_axis<MT>(g, it, r0 + NR * (wave / SHARE), acc);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         if (r0 || i) __syncthreads();
@@ -402,13 +414,13 @@ struct Lora {
           }
         }
         __syncthreads();
-        constexpr int WIDE = NR < 32 ? 32 : NR;  // (zeros up to the 32 of a matrix instruction)
+        constexpr int WIDE = NR * G < 32 ? 32 : NR * G;  // (zeros up to the 32 of a matrix instruction)
         for (int t = threadIdx.x; t < 16 * WIDE; t += 64 * LORA_WAVES) {
           const int s = t / WIDE, r = t % WIDE;
           float v = 0.f;
-          if (r < NR && r0 + r < g.R) {
+          if (r < NR * G && r0 + r < g.R) {
 #pragma unroll
-            for (int u = 0; u < LORA_WAVES; ++u) v += lds.sums[u][s][r];
+            for (int u = 0; u < SHARE; ++u) v += lds.sums[r / NR * SHARE + u][s][r % NR];
             if (g.v && 16 * i + s < it.count) g.v[(size_t)it.tokens[16 * i + s] * g.R + r0 + r] = v;
             v *= c;
           }
@@ -427,7 +439,7 @@ struct Lora {
 
   template <int MT>
   __device__ __forceinline__ static void short_axis(const LoraArgs &g, const LoraItem &it, const Lds &lds) {
-    constexpr int AHEAD = RL / 32 < 2 ? RL / 32 : 2;  // steps of r whose matrix is asked for ahead
+    constexpr int AHEAD = KC && RL > 32 ? 2 : 1;  // steps of r whose matrix is asked for with the residual
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
     const TW *l = (const TW *)g.l + it.e * g.l_adapter;
     const TY *res[MT];
@@ -508,8 +520,9 @@ struct Lora {
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k)
         if (32 * k < g.R) step(raw[k], 32 * k);
-      if constexpr (RL > 64) {
-        for (int r = 64; r < g.R; r += 32) {
+      if constexpr (RL > 32 * AHEAD) {
+#pragma unroll 1
+        for (int r = 32 * AHEAD; r < g.R; r += 32) {
           load_l(raw[0], o0, r, whole);
           step(raw[0], r);
         }
@@ -564,9 +577,11 @@ struct Lora {
     }
   }
 };
-template <class TX, class TW, bool KC, int NF, int RL, class TY>
-__global__ __launch_bounds__(64 * LORA_WAVES) void k_lora(LoraArgs g) {
-  typedef Lora<TX, TW, KC, NF, RL, TY> L;
+// 16-bit rows leave room for two workgroups on a CU, 128 registers a lane: with one, a ninth more items than CUs took twice
+// the time
+template <class TX, class TW, bool KC, int NF, int G, int RL, class TY>
+__global__ __launch_bounds__(64 * LORA_WAVES, sizeof(TX) == 2 ? 4 : 2) void k_lora(LoraArgs g) {
+  typedef Lora<TX, TW, KC, NF, G, RL, TY> L;
   __shared__ __attribute__((aligned(16))) typename L::Lds lds;
   if ((int)blockIdx.x >= g.rest) return L::rest(g, ((int)blockIdx.x - g.rest) * 64);
   LoraItem it;
@@ -774,10 +789,10 @@ void lora_few(int x_type, int w_type, const LoraFewArgs &g, dim3 grid, hipStream
 template <class TX, class TW, bool KC, class TY>
 void lora_launch(const LoraArgs &g, int grid, hipStream_t st) {
   const dim3 n(grid), wg(64 * LORA_WAVES);
-  if (g.R <= 16) hipLaunchKernelGGL((k_lora<TX, TW, KC, 1, 32, TY>), n, wg, 0, st, g);
-  else if (g.R <= 32) hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 32, TY>), n, wg, 0, st, g);
-  else if (g.R <= 64) hipLaunchKernelGGL((k_lora<TX, TW, KC, 4, 64, TY>), n, wg, 0, st, g);
-  else hipLaunchKernelGGL((k_lora<TX, TW, KC, 4, 256, TY>), n, wg, 0, st, g);
+  if (g.R <= 16) hipLaunchKernelGGL((k_lora<TX, TW, KC, 1, 1, 32, TY>), n, wg, 0, st, g);
+  else if (g.R <= 32) hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 1, 32, TY>), n, wg, 0, st, g);
+  else if (g.R <= 64) hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 2, 64, TY>), n, wg, 0, st, g);
+  else hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 2, 256, TY>), n, wg, 0, st, g);
 }
 // r of a workgroup of sums: 16, 32 or 64
 inline int lora_r_of(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : 64; }
