@@ -24,21 +24,29 @@ int check_lora(const zm_lora_desc *d, const char *who) {
   if (d->x_stride < 0 || d->y_stride < 0 || d->res_stride < 0 || d->a_stride < 0 || d->b_stride < 0 || d->a_adapter < 0 ||
       d->b_adapter < 0)
     return fail("%s: negative stride", who);
+  const int64_t most = ((int64_t)1 << 31) / (int64_t)size_of(d->w_type);
+  if ((d->R - 1) * d->a_stride + d->I >= most || (d->O - 1) * d->b_stride + d->R >= most)
+    return fail("%s: an adapter's a and b are below 2^31 bytes", who);
   return 0;
 }
 
 // Work items are counted on the device; a launch has as many as there can be.
-int64_t most_items(const zm_lora_desc &d) { return d.S / LORA_TOKENS + std::min<int64_t>(d.S, d.n); }
+int64_t items_of(const zm_lora_desc &d, int T) { return d.S / T + std::min<int64_t>(d.S, d.n); }
+// Tokens of an item.  A CU runs one item at a time: 16 where the items then fit the 256 CUs (of the most there can be a
+// few are not there), else 32.
+int tokens_of(const zm_lora_desc &d) { return items_of(d, 16) <= 272 ? 16 : LORA_TOKENS; }
+int64_t most_items(const zm_lora_desc &d) { return items_of(d, tokens_of(d)); }
 
 // slices of an axis of K, `unit` at a time, for `want` workgroups where one slice has `n`
 int64_t slices_of(int64_t n, int64_t want, int64_t K, int64_t unit, int64_t most) {
   return std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want / std::max<int64_t>(n, 1), most), K / unit));
 }
 
-// slices of an adapter's tokens for its gradient of N columns; their sums take at most 64 MB
+// slices of an adapter's tokens for its gradient of N columns: both gradients are one launch, of a workgroup for each CU
+// where there are tokens for it; the slices' sums take at most 64 MB
 int sums_slices(const zm_lora_desc &d, int64_t N) {
-  const int64_t groups = (N + 63) / 64 * ((d.R + lora_r_of(d.R) - 1) / lora_r_of(d.R)) * d.n;
-  return (int)slices_of(groups, 512, d.S / d.n, 256, (64 << 20) / (4 * N * d.R * d.n));
+  const int64_t groups = ((d.I + 63) / 64 + (d.O + 63) / 64) * ((d.R + lora_r_of(d.R) - 1) / lora_r_of(d.R)) * d.n;
+  return (int)slices_of(groups, 256, d.S / d.n, 256, (64 << 20) / (4 * N * d.R * d.n));
 }
 size_t sums_space(const zm_lora_desc &d, int64_t N) {
   const int z = sums_slices(d, N);
@@ -49,7 +57,7 @@ size_t sums_space(const zm_lora_desc &d, int64_t N) {
 struct Space {
   size_t items, u, total;
 };
-size_t item_bytes(const zm_lora_desc &d) { return align256((2 * d.n + 1 + (LORA_TOKENS + 1) * most_items(d)) * 4); }
+size_t item_bytes(const zm_lora_desc &d) { return align256((2 * d.n + 1 + (tokens_of(d) + 1) * most_items(d)) * 4); }
 Space space_of(const zm_lora_desc &d, bool backward) {
   Space s{};
   s.items = item_bytes(d);
@@ -71,19 +79,19 @@ LoraArgs items(const zm_lora_desc &d, const int32_t *ids, const float *scale, ui
   g.n = d.n;
   g.ids = ids;
   g.scale = scale;
-  g.rest = (int)most_items(d);
   int32_t *p = (int32_t *)ws;
   const int64_t most = most_items(d);
+  g.rest = (int)((d.S + most - 1) / most);
+  g.it.T = tokens_of(d);
+  g.it.log_T = g.it.T == 16 ? 4 : 5;
   g.it.tokens = p;
-  g.it.item_e = p + LORA_TOKENS * most;
+  g.it.item_e = p + g.it.T * most;
   g.it.counts = g.it.item_e + most;
   g.it.first = g.it.counts + d.n;
   g.it.n_items = g.it.first + d.n;
   hipLaunchKernelGGL(k_lora_items, dim3(1), dim3(1024), 0, st, ids, (int)d.S, (int)d.n, g.it);
   return g;
 }
-// the workgroups of k_lora: one an item, and one for 64 tokens to look for those without an adapter
-int groups_of(const zm_lora_desc &d) { return (int)(most_items(d) + (d.S + 63) / 64); }
 LoraSumArgs sums_args(const zm_lora_desc &d, const float *a, const void *m, int64_t ldm, int64_t N, const float *scale,
                       float *dst, float *space) {
   LoraSumArgs g{};
@@ -151,7 +159,7 @@ int zm_lora(const zm_lora_desc *d, const void *x, const void *a, const void *b, 
   g.y = y;
   g.ldy = d->y_stride;
   g.v = v;
-  lora_forward(d->x_type, d->w_type, d->y_type, g, groups_of(*d), st);
+  lora_forward(d->x_type, d->w_type, d->y_type, g, (int)most_items(*d), st);
   return launched();
 }
 
@@ -191,7 +199,7 @@ int zm_lora_backward(const zm_lora_desc *d, const void *dy, const void *x, const
     g.y = dx;
     g.ldy = d->I;
     g.v = da ? u : nullptr;
-    lora_backward(d->y_type, d->w_type, d->x_type, g, groups_of(*d), st);
+    lora_backward(d->y_type, d->w_type, d->x_type, g, (int)most_items(*d), st);
   }
   if (da || db) {
     const LoraSumArgs ga = sums_args(*d, u, x, d->x_stride, d->I, scale, da, sa);

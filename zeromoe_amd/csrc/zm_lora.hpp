@@ -25,13 +25,14 @@
 
 namespace zm {
 
-constexpr int LORA_TOKENS = 32;  // of an item
+constexpr int LORA_TOKENS = 32;  // of an item, at most (16 or 32)
 constexpr int LORA_MOST_R = 256, LORA_MOST_N = 512;
 
-// The items: adapter e's tokens lie at tokens[32 first[e] ..], counts[e] of them, in ascending order, -1 behind them up to
-// the next item; item i is of adapter item_e[i].
+// The items, of up to T tokens: adapter e's tokens lie at tokens[T first[e] ..], counts[e] of them, in ascending order, -1
+// behind them up to the next item; item i is of adapter item_e[i].
 struct LoraItems {
-  int32_t *counts, *first, *item_e, *tokens, *n_items;  // [n], [n], [items], [items][32], one
+  int32_t *counts, *first, *item_e, *tokens, *n_items;  // [n], [n], [items], [items][T], one
+  int T, log_T;  // (a power of two)
 };
 struct LoraArgs {
   const void *x, *m, *l;  // rows, the matrices of the long axis and those of the short one
@@ -46,7 +47,7 @@ struct LoraArgs {
   const void *res;        // [S][ldr] or null
   void *y;
   int64_t ldr, ldy;
-  int rest;               // the first workgroup that looks for tokens without an adapter
+  int rest;               // tokens that a workgroup looks through for those without an adapter
 };
 
 // ============================================================ items
@@ -66,8 +67,14 @@ static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__res
     return (unsigned)e < (unsigned)n ? e : -1;
   };
   int e[LORA_CHUNKS], at[LORA_CHUNKS];
+  // all asked for before the first is waited for (a condition on the load would wait for each: 1 us a chunk)
 #pragma unroll
-  for (int c = 0; c < LORA_CHUNKS; ++c) e[c] = 64 * c < seg ? load(p0 + 64 * c + lane) : -1;
+  for (int c = 0; c < LORA_CHUNKS; ++c)
+    if (64 * c < seg) e[c] = ids[min(p0 + 64 * c + lane, S - 1)];
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int c = 0; c < LORA_CHUNKS; ++c)
+    e[c] = 64 * c < seg && p0 + 64 * c + lane < p1 && (unsigned)e[c] < (unsigned)n ? e[c] : -1;
   for (int k = lane; k < n; k += 64) cnt[w][k] = 0;
   stage_sync();
   // the place of a token among those of its adapter in its wave
@@ -101,7 +108,7 @@ static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__res
       run += k;
     }
     total[tid] = run;
-    mine = (run + LORA_TOKENS - 1) / LORA_TOKENS;
+    mine = (run + o.T - 1) >> o.log_T;
   }
   int incl = mine;  // (adapters are below 512: waves 0 to 7 hold them)
 #pragma unroll
@@ -127,15 +134,15 @@ static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__res
   auto put = [&](int p, int e, int at) {
     if (e < 0) return;
     at += cnt[w][e];
-    o.tokens[(size_t)first[e] * LORA_TOKENS + at] = p;
-    if (!(at & (LORA_TOKENS - 1))) o.item_e[first[e] + at / LORA_TOKENS] = e;
+    o.tokens[(size_t)first[e] * o.T + at] = p;
+    if (!(at & (o.T - 1))) o.item_e[first[e] + (at >> o.log_T)] = e;
   };
 #pragma unroll
   for (int c = 0; c < LORA_CHUNKS; ++c)
     if (64 * c < seg) put(p0 + 64 * c + lane, e[c], at[c]);
   for (int q = w; q < n; q += 16) {  // behind an adapter's last token
-    const int used = total[q] & (LORA_TOKENS - 1);
-    if (used && lane >= used && lane < LORA_TOKENS) o.tokens[((size_t)first[q] + total[q] / LORA_TOKENS) * LORA_TOKENS + lane] = -1;
+    const int used = total[q] & (o.T - 1);
+    if (used && lane >= used && lane < o.T) o.tokens[((size_t)first[q] + (total[q] >> o.log_T)) * o.T + lane] = -1;
   }
   if (seg <= 64 * LORA_CHUNKS) return;
   // the chunks past the registers: their places again, on from those of the chunks before
@@ -149,8 +156,8 @@ static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__res
     const int k = load(p + lane);
     const int a = place(k);
     if (k < 0) continue;
-    o.tokens[(size_t)first[k] * LORA_TOKENS + a] = p + lane;
-    if (!(a & (LORA_TOKENS - 1))) o.item_e[first[k] + a / LORA_TOKENS] = k;
+    o.tokens[(size_t)first[k] * o.T + a] = p + lane;
+    if (!(a & (o.T - 1))) o.item_e[first[k] + (a >> o.log_T)] = k;
   }
 }
 
@@ -165,12 +172,12 @@ struct LoraItem {
   }
 };
 __device__ __forceinline__ bool lora_item(const LoraArgs &g, int i, LoraItem &it) {
-  it.tokens = g.it.tokens + (size_t)i * LORA_TOKENS;
+  it.tokens = g.it.tokens + (size_t)i * g.it.T;
   it.e = g.it.item_e[i];
-  const int t = it.tokens[threadIdx.x & (LORA_TOKENS - 1)];
+  const int lane = threadIdx.x & 63, t = it.tokens[min(lane, g.it.T - 1)];
   if (i >= *g.it.n_items) return false;  // (before it.e is used)
   it.e = uniform(it.e);
-  it.count = __builtin_popcount((uint32_t)__ballot(t >= 0));
+  it.count = __builtin_popcountll(__ballot(t >= 0 && lane < g.it.T));
   return true;
 }
 
@@ -265,145 +272,181 @@ constexpr int terms_beside() {
 
 // ============================================================ both products
 //
-// A workgroup takes an item.  Over the long axis its eight waves, in G groups of 16 NF of r each, take a line of x (64 k of
-// 16 bits, 32 of f32) in turn for all of its tokens, so each value of M is read once a workgroup, from L2 as a rule.  The
-// waves' sums meet in LDS as v and become terms there.  Over the short axis a wave
-// takes 64 columns at a time; columns are given to fragments so that a lane ends with 16 neighbouring ones of a row:
-// residual and result go in whole lines.
+// A workgroup takes an item.  Over the long axis its eight waves take a line of x (64 k of 16 bits, 32 of f32) in turn for
+// all of its tokens and 16 NF of r, so each value of M is read once a workgroup, from L2 as a rule; the next line or two
+// are on their way while one is multiplied.  The waves' sums meet in LDS as v and become terms there.  Over the short axis a
+// wave takes 64 columns at a time, the next ones on their way.
 //
-// RL: values of r whose terms LDS has room for.  Workgroups from g.rest on look through 64 tokens each for those without
-// an adapter: their rows are the residual (or zeros), and NaN where the id names none.
+// A fragment's 16 neighbouring lanes hold 16 rows, and a load that follows that asks for 16 lines for each 16 lanes: the
+// address units take one a cycle, 16 bytes (such a kernel read 35 GB/s a CU, whatever was on its way).  So rows come in
+// whole lines, 8 neighbouring lanes each, and go to fragments through LDS of the wave's own (no barrier), and results go
+// back the same way.  RL: values of r whose terms LDS has room for.
+//
+// Every workgroup also looks through g.rest tokens for those without an adapter: their rows are the residual (or zeros),
+// and NaN where the id names none.  (Workgroups of their own waited for a CU behind the items: 68 us for LORA_US.)
 constexpr int LORA_WAVES = 8;
-template <class TX, class TW, bool KC, int NF, int G, int RL, class TY>
+
+// ROWS rows of PIECES x 16 bytes by way of registers into LDS, rows 128 bytes apart, their pieces permuted so that 16 rows
+// of a fragment cover all banks
+template <class T, int ROWS, int PIECES>
+struct Stage {
+  static constexpr int V = 16 / (int)sizeof(T), PER = ROWS * PIECES / 64;
+  Words<T, V> reg[PER];
+  __device__ __forceinline__ static int row(int i) { return (i * 64 + ((int)threadIdx.x & 63)) / PIECES; }
+  __device__ __forceinline__ static int piece() { return (int)threadIdx.x % PIECES; }
+  __device__ __forceinline__ static uint32_t at(int row, int piece) { return row * 128 + ((piece ^ (row >> 1)) & 7) * 16; }
+  // `left`: values that exist of the row's part, for this lane's piece at(i) = its row's first value
+  template <class At>
+  __device__ __forceinline__ void load(const At &at, int left, const T *safe) {
+    if (left >= PIECES * V) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) load_words(reg[i], at(i) + V * piece(), V, safe);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) load_words(reg[i], at(i) + V * piece(), left - V * piece(), safe);
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t *lds) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      *reinterpret_cast<v4u *>(lds + at(row(i), piece())) = v4u{reg[i].w[0], reg[i].w[1], reg[i].w[2], reg[i].w[3]};
+  }
+  // values 32 s + 8 fc .. of row `row`
+  __device__ __forceinline__ static Words<T, 8> frag(const uint8_t *lds, int row, int s) {
+    const int fc = ((int)threadIdx.x & 63) >> 4;
+    Words<T, 8> p;
+#pragma unroll
+    for (int q = 0; q < (int)sizeof(T) / 2; ++q) {
+      const v4u v = *reinterpret_cast<const v4u *>(lds + at(row, (4 * s + fc) * ((int)sizeof(T) / 2) + q));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p.w[4 * q + j] = v[j];
+    }
+    return p;
+  }
+};
+
+template <class TX, class TW, bool KC, int NF, int RL, class TY>
 struct Lora {
   static constexpr int NX = terms_beside<TX, TW>(), NM = terms_beside<TW, TX>(), NL = terms_beside<TW, float>();
   static constexpr bool F16 = std::is_same<TX, _Float16>::value && std::is_same<TW, _Float16>::value;
   static constexpr int H = 4 / (int)sizeof(TX), LINE = 32 * H;  // matrix instructions and k of a step
   static constexpr int NR = 16 * NF, LD = RL + 8;               // (8 more: 16 rows cover all banks)
-  static constexpr int SHARE = LORA_WAVES / G;                  // waves of a group
   static constexpr int C = 4;                                   // fragments of 16 columns of a wave
+  static constexpr int DEPTH = (KC ? sizeof(TW) == 2 : NF <= 2) ? 2 : 1;  // lines on their way (as registers allow)
+  static constexpr int BUF = 128 * (LORA_TOKENS + (NR < 32 ? 32 : NR));  // bytes of a wave: a line; 64 rows of L
   struct Lds {
-    float sums[LORA_WAVES][16][NR + 4];
+    union {
+      uint8_t wave[LORA_WAVES][BUF];
+      float sums[LORA_WAVES][16][NR + 4];
+    };
     uint16_t terms[3][LORA_TOKENS][LD];
   };
 
   // the sums of MT tiles of 16 tokens over this wave's lines, r from r0 on
   template <int MT>
-  __device__ __forceinline__ static void long_axis(const LoraArgs &g, const LoraItem &it, int r0, v4f (&acc)[MT][NF]) {
-    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % SHARE, fr = lane & 15, fc = lane >> 4;
+  __device__ __forceinline__ static void long_axis(const LoraArgs &g, const LoraItem &it, int r0, uint8_t *buf,
+                                                   v4f (&acc)[MT][NF]) {
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), fr = lane & 15, fc = lane >> 4;
+    constexpr int STEP = LINE * LORA_WAVES;
+    typedef Stage<TX, 16 * MT, 8> SX;
+    typedef Stage<TW, NR, LINE * (int)sizeof(TW) / 16> SM;  // KC
     const TW *m = (const TW *)g.m + it.e * g.m_adapter;
-    const TX *x[MT];  // (tokens past the item's last, and rows past R, repeat others: what they give is not used)
+    const TX *x[SX::PER];  // (tokens past the item's last, and rows past R, repeat others: what they give is not used)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) x[i] = (const TX *)g.x + it.token(16 * i + fr) * g.ldx + 8 * fc;
+    for (int i = 0; i < SX::PER; ++i) x[i] = (const TX *)g.x + it.token(SX::row(i)) * g.ldx;
+    uint32_t row[SM::PER];  // bytes (zm_lora admits adapters of less than 2^31)
+#pragma unroll
+    for (int i = 0; i < SM::PER; ++i) row[i] = (uint32_t)min(r0 + SM::row(i), g.R - 1) * (uint32_t)(g.ldm * sizeof(TW));
     const int rc = NF * fr + r0 < g.R ? NF * fr + r0 : 0, rl = min(g.R - rc, NF);
-    const TW *row[NF];
-#pragma unroll
-    for (int h = 0; h < NF; ++h) row[h] = m + (int64_t)min(r0 + 16 * h + fr, g.R - 1) * g.ldm + 8 * fc;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int h = 0; h < NF; ++h) acc[i][h] = v4f{0.f, 0.f, 0.f, 0.f};
-    struct X {
-      Words<TX, 8> p[H][MT];
+    struct Line {
+      SX x;
+      SM m;                        // KC
+      Words<TW, NF> r[KC ? 1 : H][8];  // else
     };
-    struct M {
-      Words<TW, 8> p[H][KC ? NF : 1];
-      Words<TW, NF> r[H][KC ? 1 : 8];
-    };
-    auto load_x = [&](X &to, int64_t k) {
+    if (LINE * wave >= g.K) return;
+    const int64_t last = LINE * wave + (g.K - 1 - LINE * wave) / STEP * STEP;
+    auto load = [&](Line &to, int64_t k) {
+      // (past the end the last line again: a load under a condition would be waited for where its paths meet)
+      k = min(k, last);
+      const int left = (int)min(g.K - k, (int64_t)LINE);
+      to.x.load([&](int i) { return x[i] + k; }, left, (const TX *)g.x);
+      if constexpr (KC) {
+        to.m.load([&](int i) { return (const TW *)((const uint8_t *)(m + k) + row[i]); }, left, m);
+      } else if (left == LINE && g.R % NF == 0) {
 #pragma unroll
-      for (int s = 0; s < H; ++s)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) load_words(to.p[s][i], x[i] + k + 32 * s, 8, x[i]);
-    };
-    auto load_m = [&](M &to, int64_t k) {
-#pragma unroll
-      for (int s = 0; s < H; ++s) {
-        if constexpr (KC) {
-#pragma unroll
-          for (int h = 0; h < NF; ++h) load_words(to.p[s][h], row[h] + k + 32 * s, 8, m);
-        } else {
+        for (int s = 0; s < H; ++s)
 #pragma unroll
           for (int j = 0; j < 8; ++j) load_words(to.r[s][j], m + (k + 32 * s + 8 * fc + j) * g.ldm + rc, NF, m);
-        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < H; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            load_words(to.r[s][j], m + (k + 32 * s + 8 * fc + j) * g.ldm + rc, 32 * s + 8 * fc + j < left ? rl : 0, m);
       }
     };
-    auto multiply = [&](const X &px, const M &pm) {
+    uint8_t *bx = buf, *bm = buf + 128 * 16 * MT;
+    auto step = [&](Line &line, int64_t k) {
+      line.x.store(bx);
+      v8bf fr_m[KC ? 1 : H][NF][NM];
+      if constexpr (KC) {
+        line.m.store(bm);
+      } else {
+#pragma unroll
+        for (int s = 0; s < H; ++s)
+#pragma unroll
+          for (int h = 0; h < NF; ++h) frag_of_rows(line.r[s], h, fr_m[s][h]);
+      }
+      load(line, k + DEPTH * STEP);
+      stage_sync();
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < H; ++s) {
         v8bf fm[NF][NM];
+        if constexpr (KC) {
 #pragma unroll
-        for (int h = 0; h < NF; ++h) {
-          if constexpr (KC) frag_of(pm.p[s][h], fm[h]);
-          else frag_of_rows(pm.r[s], h, fm[h]);
+          for (int h = 0; h < NF; ++h) frag_of(SM::frag(bm, 16 * h + fr, s), fm[h]);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           v8bf fx[NX];
-          frag_of(px.p[s][i], fx);
+          frag_of(SX::frag(bx, 16 * i + fr, s), fx);
 #pragma unroll
-          for (int h = 0; h < NF; ++h) mul_terms<F16, NM, NX>(acc[i][h], fm[h], fx);
-        }
-      }
-    };
-    // a line of which only a part exists, or of M whose rows do not end with a pack: 32 k and a fragment at a time
-    auto part = [&](int64_t k) {
-#pragma unroll 1
-      for (int s = 0; s < H; ++s, k += 32) {
-        const int left = (int)min(g.K - (k + 8 * fc), (int64_t)8);
-        v8bf fx[MT][NX];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          Words<TX, 8> p;
-          load_words(p, x[i] + k, left, (const TX *)g.x);
-          frag_of(p, fx[i]);
-        }
-        Words<TW, NF> r[KC ? 1 : 8];
-        if constexpr (!KC) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) load_words(r[j], m + (k + 8 * fc + j) * g.ldm + rc, j < left ? rl : 0, m);
-        }
-#pragma unroll
-        for (int h = 0; h < NF; ++h) {
-          v8bf fm[NM];
-          if constexpr (KC) {
-            Words<TW, 8> p;
-            load_words(p, row[h] + k, left, m);
-            frag_of(p, fm);
-          } else {
-            frag_of_rows(r, h, fm);
+          for (int h = 0; h < NF; ++h) {
+            if constexpr (KC) mul_terms<F16, NM, NX>(acc[i][h], fm[h], fx);
+            else mul_terms<F16, NM, NX>(acc[i][h], fr_m[s][h], fx);
           }
-#pragma unroll
-          for (int i = 0; i < MT; ++i) mul_terms<F16, NM, NX>(acc[i][h], fm, fx[i]);
-          __builtin_amdgcn_sched_barrier(0);
         }
       }
+      stage_sync();
     };
-    constexpr int STEP = LINE * SHARE;
+    Line a, b;
     int64_t k = LINE * wave;
-    if (KC || g.R % NF == 0) {
-      for (; k + LINE <= g.K; k += STEP) {
-        X px;
-        M pm;
-        load_x(px, k);
-        load_m(pm, k);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(px, pm);
+    load(a, k);
+    if constexpr (DEPTH == 2) load(b, k + STEP);
+    for (; k < g.K; k += DEPTH * STEP) {
+      step(a, k);
+      if constexpr (DEPTH == 2) {
+        if (k + STEP >= g.K) break;
+        step(b, k + STEP);
       }
     }
-    for (; k < g.K; k += STEP) part(k);
   }
 
   template <int MT>
   __device__ __forceinline__ static void run(const LoraArgs &g, const LoraItem &it, Lds &lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), fr = lane & 15, fc = lane >> 4;
     const float c = g.scale ? g.scale[it.e] : 1.f;
-    for (int r0 = 0; r0 < g.R; r0 += NR * G) {
+    for (int r0 = 0; r0 < g.R; r0 += NR) {
       v4f acc[MT][NF];
-      long_axis<MT>(g, it, r0 + NR * (wave / SHARE), acc);
+      long_axis<MT>(g, it, r0, lds.wave[wave], acc);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        if (r0 || i) __syncthreads();
+        __syncthreads();
 #pragma unroll
         for (int h = 0; h < NF; ++h) {
           if constexpr (KC) {
@@ -414,13 +457,13 @@ struct Lora {
           }
         }
         __syncthreads();
-        constexpr int WIDE = NR * G < 32 ? 32 : NR * G;  // (zeros up to the 32 of a matrix instruction)
+        constexpr int WIDE = NR < 32 ? 32 : NR;  // (zeros up to the 32 of a matrix instruction)
         for (int t = threadIdx.x; t < 16 * WIDE; t += 64 * LORA_WAVES) {
           const int s = t / WIDE, r = t % WIDE;
           float v = 0.f;
-          if (r < NR * G && r0 + r < g.R) {
+          if (r < NR && r0 + r < g.R) {
 #pragma unroll
-            for (int u = 0; u < SHARE; ++u) v += lds.sums[r / NR * SHARE + u][s][r % NR];
+            for (int u = 0; u < LORA_WAVES; ++u) v += lds.sums[u][s][r];
             if (g.v && 16 * i + s < it.count) g.v[(size_t)it.tokens[16 * i + s] * g.R + r0 + r] = v;
             v *= c;
           }
@@ -432,82 +475,95 @@ struct Lora {
           }
         }
       }
+      __syncthreads();
     }
-    __syncthreads();
     short_axis<MT>(g, it, lds);
   }
 
   template <int MT>
-  __device__ __forceinline__ static void short_axis(const LoraArgs &g, const LoraItem &it, const Lds &lds) {
-    constexpr int AHEAD = KC && RL > 32 ? 2 : 1;  // steps of r whose matrix is asked for with the residual
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
+  __device__ __forceinline__ static void short_axis(const LoraArgs &g, const LoraItem &it, Lds &lds) {
+    constexpr int STEP = 64 * LORA_WAVES;
+    constexpr bool STAGED = KC && RL > 32;                   // (shorter rows of L are several to a line)
+    constexpr int RS = STAGED ? 128 / (int)sizeof(TW) : 32;  // r of a step
+    typedef Stage<TW, 64, 8> SL;
+    // the result: a row of 64 columns in VY-value pieces, PY of them
+    constexpr int VY = 16 / (int)sizeof(TY), PY = 64 / VY, OUT = 16 * PY / 64;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), fr = lane & 15, fc = lane >> 4;
+    uint8_t *buf = lds.wave[wave];
     const TW *l = (const TW *)g.l + it.e * g.l_adapter;
-    const TY *res[MT];
-    TY *y[MT];
+    const int yr = lane / PY, yc = lane % PY * VY;  // the lane's row (of 64 / PY at once) and its first column
+    auto out_row = [&](int i, int q) { return 16 * i + yr + 64 / PY * q; };
+    int token[MT][OUT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int64_t s = it.token(16 * i + fr);
-      res[i] = (const TY *)g.res + s * g.ldr + 16 * fc;
-      y[i] = (TY *)g.y + s * g.ldy + 16 * fc;
-    }
-    struct Raw {
-      Words<TW, 8> p[KC ? C : 1];
-      Words<TW, C> r[KC ? 1 : 8];
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int q = 0; q < OUT; ++q) token[i][q] = (int)it.token(out_row(i, q));
+    struct Part {  // of the matrix: 64 columns, RS of r
+      SL s;                     // STAGED
+      Words<TW, 8> k[C];        // KC
+      Words<TW, C> r[8];        // else
     };
-    // 32 of r from r on of 64 columns (zeros past R: v has zeros there, but what lies there may be no number); whole: all
-    // columns exist, and KC's packs of 8 end with R
-    auto load_l = [&](Raw &to, int64_t o0, int r, auto whole) {
-      constexpr bool WHOLE = decltype(whole)::value;
-      r += 8 * fc;
-      const int left = min(g.R - r, 8);
-      if constexpr (KC) {
+    struct Columns {
+      Words<TY, VY> z[MT][OUT];
+      Part l;
+    };
+    auto load_part = [&](Part &to, int64_t o0, int r) {
+      const bool whole = o0 + 64 <= g.N;
+      if constexpr (STAGED) {
+        to.s.load([&](int i) {
+          const uint32_t o = (uint32_t)(whole ? o0 + SL::row(i) : min(o0 + SL::row(i), g.N - 1));
+          return (const TW *)((const uint8_t *)(l + r) + o * (uint32_t)(g.ldl * sizeof(TW)));
+        }, min(g.R - r, RS), l);
+      } else if constexpr (KC) {
+        const int left = min(g.R - (r + 8 * fc), 8);
 #pragma unroll
         for (int h = 0; h < C; ++h) {
-          const TW *at = l + min(o0 + 16 * (fr >> 2) + 4 * h + (fr & 3), g.N - 1) * g.ldl;
-          if constexpr (WHOLE) {
-            load_words(to.p[h], at + (left > 0 ? r : 0), 8, at);
+          const TW *at = l + min(o0 + 16 * h + fr, g.N - 1) * g.ldl;
+          if (g.R % 8 == 0) {  // a pack is whole or none: no condition on the load
+            load_words(to.k[h], at + (left > 0 ? r + 8 * fc : 0), 8, at);
 #pragma unroll
-            for (int k = 0; k < Words<TW, 8>::W; ++k) to.p[h].w[k] = left > 0 ? to.p[h].w[k] : 0u;
+            for (int k = 0; k < Words<TW, 8>::W; ++k) to.k[h].w[k] = left > 0 ? to.k[h].w[k] : 0u;
           } else {
-            load_words(to.p[h], at + r, left, at);
+            load_words(to.k[h], at + r + 8 * fc, left, at);
           }
         }
       } else {
-        const int64_t o = WHOLE ? o0 + C * fr : min(o0 + C * fr, g.N - 1);
-        const int cols = (int)min(g.N - o, (int64_t)C);
+        const int64_t o = min(o0 + C * fr, g.N - 1);
+        const int n = (int)min(g.N - o, (int64_t)C);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          load_words(to.r[j], l + min(r + j, g.R - 1) * g.ldl + o, WHOLE ? C : cols, l);
+          const int rj = r + 8 * fc + j;  // (past R v has zeros, but what lies there may be no number)
+          load_words(to.r[j], l + min(rj, g.R - 1) * g.ldl + o, whole ? C : n, l);
 #pragma unroll
-          for (int k = 0; k < Words<TW, C>::W; ++k) to.r[j].w[k] = j < left ? to.r[j].w[k] : 0u;
+          for (int k = 0; k < Words<TW, C>::W; ++k) to.r[j].w[k] = rj < g.R ? to.r[j].w[k] : 0u;
         }
       }
     };
-    auto columns = [&](int64_t o0, auto whole) {
-      constexpr bool WHOLE = decltype(whole)::value;
-      const int left = WHOLE ? 16 : (int)min(g.N - (o0 + 16 * fc), (int64_t)16);
-      Words<TY, 16> z[MT];
-      Raw raw[AHEAD];
+    int64_t o0 = 64 * wave;
+    if (o0 >= g.N) return;
+    const int64_t last = o0 + (g.N - 1 - o0) / STEP * STEP;
+    auto load = [&](Columns &to, int64_t o0) {
+      o0 = min(o0, last);
+      const int cols = (int)min(g.N - (o0 + yc), (int64_t)VY);
       if (g.res) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) load_words(z[i], res[i] + o0, left, (const TY *)g.res);
-      }
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        if (32 * k < g.R) load_l(raw[k], o0, 32 * k, whole);
-      __builtin_amdgcn_sched_barrier(0);
+          for (int q = 0; q < OUT; ++q) {
+            const TY *at = (const TY *)g.res + token[i][q] * g.ldr + o0 + yc;
+            load_words(to.z[i][q], at, o0 + 64 <= g.N ? VY : cols, (const TY *)g.res);
+          }
+      }
+      load_part(to.l, o0, 0);
+    };
+    auto columns = [&](Columns &now, Columns &next, int64_t o0) {
+      const int cols = (int)min(g.N - (o0 + yc), (int64_t)VY);
       v4f acc[MT][C];
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int h = 0; h < C; ++h) acc[i][h] = v4f{0.f, 0.f, 0.f, 0.f};
-      auto step = [&](const Raw &raw, int r) {
-        v8bf fl[C][NL];
-#pragma unroll
-        for (int h = 0; h < C; ++h) {
-          if constexpr (KC) frag_of(raw.p[h], fl[h]);
-          else frag_of_rows(raw.r, h, fl[h]);
-        }
+      auto multiply = [&](const v8bf (&fl)[C][NL], int r) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           v8bf fv[3];
@@ -517,52 +573,96 @@ struct Lora {
           for (int h = 0; h < C; ++h) mul_terms<false, NL, 3>(acc[i][h], fl[h], fv);
         }
       };
+      auto part = [&](const Part &p, int r) {
+        v8bf fl[C][NL];
+        if constexpr (STAGED) {
+          p.s.store(buf);
+          stage_sync();
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        if (32 * k < g.R) step(raw[k], 32 * k);
-      if constexpr (RL > 32 * AHEAD) {
-#pragma unroll 1
-        for (int r = 32 * AHEAD; r < g.R; r += 32) {
-          load_l(raw[0], o0, r, whole);
-          step(raw[0], r);
-        }
-      }
+          for (int s = 0; s < RS / 32; ++s) {
+            if (r + 32 * s >= g.R) break;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        if (16 * i + fr >= it.count) continue;
-        Words<TY, 16> out;
-        float f[16];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float a = KC ? acc[i][q][j] : acc[i][j][q];
-            f[4 * q + j] = g.res ? z[i].get(4 * q + j) + a : a;
+            for (int h = 0; h < C; ++h) frag_of(SL::frag(buf, 16 * h + fr, s), fl[h]);
+            multiply(fl, r + 32 * s);
           }
-#pragma unroll
-        for (int k = 0; k < Words<TY, 16>::W; ++k) {
-          if constexpr (sizeof(TY) == 4) out.w[k] = bits_of(f[k]);
-          else out.w[k] = bits_of(from_f32<TY>(f[2 * k])) | bits_of(from_f32<TY>(f[2 * k + 1])) << 16;
-        }
-        if (left >= 16) {
-          __builtin_memcpy(y[i] + o0, out.w, sizeof(out.w));
+          stage_sync();
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (j < left) y[i][o0 + j] = from_f32<TY>(f[j]);
+          for (int h = 0; h < C; ++h) {
+            if constexpr (KC) frag_of(p.k[h], fl[h]);
+            else frag_of_rows(p.r, h, fl[h]);
+          }
+          multiply(fl, r);
+        }
+      };
+      load(next, o0 + STEP);
+      __builtin_amdgcn_sched_barrier(0);
+      part(now.l, 0);
+      if constexpr (RL > RS) {
+#pragma unroll 1
+        for (int r = RS; r < g.R; r += RS) {
+          load_part(now.l, o0, r);
+          part(now.l, r);
         }
       }
+      // a tile of 16 tokens at a time, rows of 64 columns and 4 more
+      float *rows = (float *)buf;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if (16 * i >= it.count) break;
+#pragma unroll
+        for (int h = 0; h < C; ++h) {
+          if constexpr (KC) {
+            *reinterpret_cast<v4f *>(rows + fr * 68 + 16 * h + 4 * fc) = acc[i][h];
+          } else {
+            // columns 4 (4 fc + q) + h
+            *reinterpret_cast<v4f *>(rows + fr * 68 + 16 * fc + 4 * h) = v4f{acc[i][0][h], acc[i][1][h], acc[i][2][h], acc[i][3][h]};
+          }
+        }
+        stage_sync();
+#pragma unroll
+        for (int q = 0; q < OUT; ++q) {
+          const int s = out_row(i, q);
+          float f[VY];
+#pragma unroll
+          for (int j = 0; j < VY; j += 4) {
+            const v4f v = *reinterpret_cast<const v4f *>(rows + (s - 16 * i) * 68 + yc + j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[j + k] = g.res ? now.z[i][q].get(j + k) + v[k] : v[k];
+          }
+          if (s >= it.count) continue;
+          TY *at = (TY *)g.y + token[i][q] * g.ldy + o0 + yc;
+          if (cols >= VY) {
+            Words<TY, VY> out;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (sizeof(TY) == 4) out.w[k] = bits_of(f[k]);
+              else out.w[k] = bits_of(from_f32<TY>(f[2 * k])) | bits_of(from_f32<TY>(f[2 * k + 1])) << 16;
+            }
+            __builtin_memcpy(at, out.w, 16);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VY; ++j)
+              if (j < cols) at[j] = from_f32<TY>(f[j]);
+          }
+        }
+        stage_sync();
+      }
     };
-    for (int64_t o0 = 64 * wave; o0 < g.N; o0 += 64 * LORA_WAVES) {
-      if (o0 + 64 <= g.N && (!KC || g.R % 8 == 0)) columns(o0, std::true_type());
-      else columns(o0, std::false_type());
+    Columns a, b;
+    load(a, o0);
+    for (;;) {
+      columns(a, b, o0);
+      if ((o0 += STEP) >= g.N) break;
+      columns(b, a, o0);
+      if ((o0 += STEP) >= g.N) break;
     }
   }
 
-  // tokens without an adapter among 64
-  __device__ __forceinline__ static void rest(const LoraArgs &g, int s0) {
+  // tokens without an adapter among s0 .. s1 - 1, at most 64
+  __device__ __forceinline__ static void rest(const LoraArgs &g, int s0, int s1) {
     const int lane = threadIdx.x & 63;
-    const int e = s0 + lane < g.S ? g.ids[s0 + lane] : 0;
+    const int e = s0 + lane < s1 ? g.ids[s0 + lane] : 0;
     uint64_t todo = __ballot((unsigned)e >= (unsigned)g.n);
     while (todo) {
       const int k = __builtin_ctzll(todo);
@@ -577,24 +677,25 @@ struct Lora {
     }
   }
 };
-// 16-bit rows leave room for two workgroups on a CU, 128 registers a lane: with one, a ninth more items than CUs took twice
-// the time
-template <class TX, class TW, bool KC, int NF, int G, int RL, class TY>
-__global__ __launch_bounds__(64 * LORA_WAVES, sizeof(TX) == 2 ? 4 : 2) void k_lora(LoraArgs g) {
-  typedef Lora<TX, TW, KC, NF, G, RL, TY> L;
+template <class TX, class TW, bool KC, int NF, int RL, class TY>
+__global__ __launch_bounds__(64 * LORA_WAVES) void k_lora(LoraArgs g) {
+  typedef Lora<TX, TW, KC, NF, RL, TY> L;
   __shared__ __attribute__((aligned(16))) typename L::Lds lds;
-  if ((int)blockIdx.x >= g.rest) return L::rest(g, ((int)blockIdx.x - g.rest) * 64);
   LoraItem it;
-  if (!lora_item(g, blockIdx.x, it)) return;
-  if (it.count <= 16) L::template run<1>(g, it, lds);
-  else L::template run<2>(g, it, lds);
+  if (lora_item(g, blockIdx.x, it)) {
+    if (it.count <= 16) L::template run<1>(g, it, lds);
+    else L::template run<2>(g, it, lds);
+  }
+  const int64_t s0 = (int64_t)blockIdx.x * g.rest, s1 = min(s0 + g.rest, (int64_t)g.S);
+  for (int64_t s = s0; s < s1; s += 64) L::rest(g, (int)s, (int)s1);
 }
 
 // ============================================================ sums over an adapter's tokens
 //
 // result[e][r][j] = c[e] sum over its tokens of a[s][r] m[s][j], or with r and j changed (BY_R, dB's order).  A workgroup
 // takes an adapter, 64 columns j, 16 NR of r and a slice of its tokens; its waves take 32 tokens in turn, and their sums
-// meet in LDS.  Both operands are summed over their rows in memory.
+// meet in LDS.  Both operands are summed over their rows in memory; a step's rows are on their way while the one before it
+// is multiplied.
 struct LoraSumArgs {
   const float *a;        // [S][R]
   const void *m;
@@ -607,7 +708,7 @@ template <class TM, int NR, bool BY_R>
 __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraItems &items, unsigned b,
                                              float (&red)[LORA_WAVES][4][256]) {
   constexpr int NM = terms_beside<TM, float>(), NF = 4, STEP = 32 * LORA_WAVES;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), fr = lane & 15, fc = lane >> 4;
   const unsigned cols = (unsigned)((g.N + 63) / 64);
   const int64_t j0 = (int64_t)(b % cols) * 64;
   b /= cols;
@@ -616,7 +717,7 @@ __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraIte
   const int z = (int)(b % g.slices), e = (int)(b / g.slices);
   const int count = items.counts[e], per = ((count + g.slices - 1) / g.slices + 31) & ~31;
   const int t0 = min(z * per, count), t1 = min(t0 + per, count);
-  const int32_t *tokens = items.tokens + (size_t)items.first[e] * LORA_TOKENS;
+  const int32_t *tokens = items.tokens + (size_t)items.first[e] * items.T;
   const float c = g.scale ? g.scale[e] : 1.f;
   v4f acc[NR][NF];
 #pragma unroll
@@ -628,27 +729,31 @@ __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraIte
   const int r = min(r0 + NR * fr, g.R - 1), rl = min(g.R - r, NR);
   const float *a = g.a + r;
   const TM *m = (const TM *)g.m + j;
-  auto step = [&](int t, auto whole) {
+  struct Step {
+    Words<float, NR> a[8];
+    Words<TM, NF> m[8];
+  };
+  // the 32 tokens at t (of those past t1 the last one's, which take no part)
+  auto load = [&](Step &p, int t, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
     int s[8];
-    Words<float, NR> pa[8];
-    Words<TM, NF> pm[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s[k] = tokens[WHOLE ? t + 8 * fc + k : min(t + 8 * fc + k, t1 - 1)];
+    for (int k = 0; k < 8; ++k) s[k] = tokens[min(t + 8 * fc + k, t1 - 1)];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const bool in = WHOLE || t + 8 * fc + k < t1;
-      load_words(pa[k], a + (int64_t)s[k] * g.R, WHOLE ? NR : in ? rl : 0, g.a);
-      load_words(pm[k], m + (int64_t)s[k] * g.ldm, WHOLE ? NF : in ? jl : 0, (const TM *)g.m);
+      load_words(p.a[k], a + (int64_t)s[k] * g.R, WHOLE ? NR : in ? rl : 0, g.a);
+      load_words(p.m[k], m + (int64_t)s[k] * g.ldm, WHOLE ? NF : in ? jl : 0, (const TM *)g.m);
     }
-    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](const Step &p) {
     v8bf fm[NF][NM];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) frag_of_rows(pm, f, fm[f]);
+    for (int f = 0; f < NF; ++f) frag_of_rows(p.m, f, fm[f]);
 #pragma unroll
     for (int h = 0; h < NR; ++h) {
       v8bf fa[3];
-      frag_of_rows(pa, h, fa);
+      frag_of_rows(p.a, h, fa);
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
         if constexpr (BY_R) mul_terms<false, 3, NM>(acc[h][f], fa, fm[f]);
@@ -657,9 +762,24 @@ __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraIte
     }
   };
   int t = t0 + 32 * wave;
-  if (j0 + 64 <= g.N && r0 + 16 * NR <= g.R)
-    for (; t + 32 <= t1; t += STEP) step(t, std::true_type());
-  for (; t < t1; t += STEP) step(t, std::false_type());
+  Step p, q;
+  if (j0 + 64 <= g.N && r0 + 16 * NR <= g.R && t + 32 <= t1) {  // whole steps, the next one on its way
+    load(p, t, std::true_type());
+    for (;;) {
+      load(q, t + STEP, std::true_type());
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(p);
+      if ((t += STEP) + 32 > t1) break;
+      load(p, t + STEP, std::true_type());
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(q);
+      if ((t += STEP) + 32 > t1) break;
+    }
+  }
+  for (; t < t1; t += STEP) {
+    load(p, t, std::false_type());
+    multiply(p);
+  }
   float *out = g.out + ((size_t)z * g.n + e) * g.R * g.N;
 #pragma unroll
   for (int h = 0; h < NR; ++h) {
@@ -789,10 +909,10 @@ void lora_few(int x_type, int w_type, const LoraFewArgs &g, dim3 grid, hipStream
 template <class TX, class TW, bool KC, class TY>
 void lora_launch(const LoraArgs &g, int grid, hipStream_t st) {
   const dim3 n(grid), wg(64 * LORA_WAVES);
-  if (g.R <= 16) hipLaunchKernelGGL((k_lora<TX, TW, KC, 1, 1, 32, TY>), n, wg, 0, st, g);
-  else if (g.R <= 32) hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 1, 32, TY>), n, wg, 0, st, g);
-  else if (g.R <= 64) hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 2, 64, TY>), n, wg, 0, st, g);
-  else hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 2, 256, TY>), n, wg, 0, st, g);
+  if (g.R <= 16) hipLaunchKernelGGL((k_lora<TX, TW, KC, 1, 32, TY>), n, wg, 0, st, g);
+  else if (g.R <= 32) hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 32, TY>), n, wg, 0, st, g);
+  else if (g.R <= 64) hipLaunchKernelGGL((k_lora<TX, TW, KC, 4, 64, TY>), n, wg, 0, st, g);
+  else hipLaunchKernelGGL((k_lora<TX, TW, KC, 4, 256, TY>), n, wg, 0, st, g);
 }
 // r of a workgroup of sums: 16, 32 or 64
 inline int lora_r_of(int R) { return R <= 16 ? 16 : R <= 32 ? 32 : 64; }
