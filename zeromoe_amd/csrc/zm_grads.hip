@@ -54,19 +54,57 @@ __device__ __forceinline__ int entry_of(const Table &t, uint32_t u) {
   return lo;
 }
 
-// 16 values of a thread: four packs of four, 1024 apart, so that a wave reads whole lines
-__device__ __forceinline__ void load_unit(const void *p, int type, int64_t i, int64_t n, v4f (&v)[4]) {
+// 16 values of a thread: four packs of four, 1024 apart, so that a wave reads whole lines.  As they lie in memory, so that
+// nothing waits for a load before all are asked for.
+template <class T>
+struct Unit {
+  typedef uint32_t Pack __attribute__((ext_vector_type(sizeof(T))));  // (four values: sizeof(T) words)
+  typedef Pack PackU __attribute__((aligned(2)));
+  Pack p[4];
+  __device__ __forceinline__ void load(const T *at) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int64_t k = i + 1024 * q;
-    v[q] = v4f{0.f, 0.f, 0.f, 0.f};
-    if (k + 4 <= n) {
-      v[q] = lin_load4(p, type, (size_t)k);
-    } else {
+    for (int q = 0; q < 4; ++q) p[q] = *reinterpret_cast<const PackU *>(at + 1024 * q);
+  }
+  __device__ __forceinline__ void load_part(const T *at, int64_t left) {  // left: values from `at` on
+    T e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (k + j < n) v[q][j] = lin_load(p, type, (size_t)(k + j));
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = 1024 * q + j < left ? at[1024 * q + j] : from_f32<T>(0.f);
+      __builtin_memcpy(&p[q], e, sizeof(e));
     }
+  }
+  __device__ __forceinline__ float get(int q, int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(p[q][j]);
+    else return to_f32(__builtin_bit_cast(T, (uint16_t)(p[q][j / 2] >> 16 * (j & 1))));
+  }
+};
+
+// Units u0 .. u1 - 1 of a tensor, this thread's values
+template <class T>
+__device__ __forceinline__ void add_squares(const Entry &e, uint32_t u0, uint32_t u1, double (&s)[4]) {
+  const T *at = (const T *)e.g + (int64_t)u0 * UNIT + 4 * threadIdx.x;
+  int64_t left = e.n - (int64_t)u0 * UNIT;
+  auto add = [&](const Unit<T> &v) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = __builtin_fma((double)v.get(q, j), (double)v.get(q, j), s[j]);
+  };
+  constexpr int N = 8 / (int)sizeof(T);  // units on their way: 128 bytes a thread
+  for (; u0 + N <= u1 && left >= N * UNIT; u0 += N, left -= N * UNIT, at += N * UNIT) {
+    Unit<T> v[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k].load(at + k * UNIT);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < N; ++k) add(v[k]);
+  }
+  for (; u0 < u1; ++u0, left -= UNIT, at += UNIT) {
+    Unit<T> v;
+    if (left >= UNIT) v.load(at);
+    else v.load_part(at, left - 4 * (int)threadIdx.x);
+    add(v);
   }
 }
 
@@ -76,15 +114,13 @@ __global__ __launch_bounds__(256) void k_grad_squares(Table t, double *__restric
   double s[4] = {0.0, 0.0, 0.0, 0.0};
   if (u0 < u1) {
     int at = entry_of(t, u0);
-    for (uint32_t u = u0; u < u1; ++u) {
-      while (at + 1 < t.count && t.e[at + 1].first <= u) ++at;
+    for (uint32_t u = u0; u < u1; ++at) {
       const Entry &e = t.e[at];
-      v4f v[4];
-      load_unit(e.g, e.type, (int64_t)(u - e.first) * UNIT + 4 * threadIdx.x, e.n, v);
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = __builtin_fma((double)v[q][j], (double)v[q][j], s[j]);
+      const uint32_t end = min(u1, at + 1 < t.count ? t.e[at + 1].first : t.units);
+      if (e.type == LIN_F32) add_squares<float>(e, u - e.first, end - e.first, s);
+      else if (e.type == LIN_F16) add_squares<_Float16>(e, u - e.first, end - e.first, s);
+      else add_squares<bf16>(e, u - e.first, end - e.first, s);
+      u = end;
     }
   }
   const double w = wave_sum_f64((s[0] + s[1]) + (s[2] + s[3]));
@@ -117,6 +153,38 @@ __global__ __launch_bounds__(256) void k_grad_norm(const double *__restrict__ pa
 
 // out = c g, rounded to f32 and from there to its type (c in f64: it may lie below f32's range where the gradients are
 // huge).  A c of 1 leaves gradients that are scaled in place as they are, unread.
+template <class T, class O>
+__device__ __forceinline__ void scale_units(const Entry &e, uint32_t u0, uint32_t u1, double c) {  // from the last one down
+  for (uint32_t u = u1; u-- > u0;) {
+    const int64_t i = (int64_t)u * UNIT + 4 * threadIdx.x, left = e.n - i;
+    const T *at = (const T *)e.g + i;
+    O *to = (O *)e.out + i;
+    Unit<T> v;
+    const bool whole = e.n - (int64_t)u * UNIT >= UNIT;
+    if (whole) v.load(at);
+    else v.load_part(at, left);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v4f f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = (float)((double)v.get(q, j) * c);
+      constexpr int type = std::is_same<O, float>::value ? LIN_F32 : std::is_same<O, bf16>::value ? LIN_BF16 : LIN_F16;
+      if (whole) {
+        lin_store4(to, type, 1024 * q, f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (1024 * q + j < left) lin_store(to, type, 1024 * q + j, f[j]);
+      }
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ void scale_to(const Entry &e, uint32_t u0, uint32_t u1, double c) {
+  if (e.out_type == LIN_F32) scale_units<T, float>(e, u0, u1, c);
+  else if (e.out_type == LIN_F16) scale_units<T, _Float16>(e, u0, u1, c);
+  else scale_units<T, bf16>(e, u0, u1, c);
+}
 __global__ __launch_bounds__(256) void k_grad_scale(Table t, const double *__restrict__ part, int parts, double max_norm,
                                                     double eps, float *norm) {
   const double n = grad_norm(part, parts);
@@ -125,27 +193,16 @@ __global__ __launch_bounds__(256) void k_grad_scale(Table t, const double *__res
   if (norm && !blockIdx.x && !threadIdx.x) *norm = (float)n;
   const uint32_t u0 = run_start(t.units, blockIdx.x, gridDim.x), u1 = run_start(t.units, blockIdx.x + 1, gridDim.x);
   if (u0 >= u1) return;
-  int at = entry_of(t, u1 - 1);
-  for (uint32_t u = u1; u-- > u0;) {
-    while (t.e[at].first > u) --at;
+  uint32_t end = u1;
+  for (int at = entry_of(t, u1 - 1); end > u0; --at) {
     const Entry &e = t.e[at];
-    if (c == 1.0 && e.out == e.g) continue;
-    const int64_t i = (int64_t)(u - e.first) * UNIT + 4 * threadIdx.x;
-    v4f v[4];
-    load_unit(e.g, e.type, i, e.n, v);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[q][j] = (float)((double)v[q][j] * c);
-      const int64_t k = i + 1024 * q;
-      if (k + 4 <= e.n) {
-        lin_store4(e.out, e.out_type, (size_t)k, v[q]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (k + j < e.n) lin_store(e.out, e.out_type, (size_t)(k + j), v[q][j]);
-      }
+    const uint32_t from = max(u0, e.first);
+    if (!(c == 1.0 && e.out == e.g)) {
+      if (e.type == LIN_F32) scale_to<float>(e, from - e.first, end - e.first, c);
+      else if (e.type == LIN_F16) scale_to<_Float16>(e, from - e.first, end - e.first, c);
+      else scale_to<bf16>(e, from - e.first, end - e.first, c);
     }
+    end = from;
   }
 }
 

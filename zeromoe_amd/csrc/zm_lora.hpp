@@ -815,8 +815,8 @@ __global__ __launch_bounds__(64 * LORA_WAVES) void k_lora_sums(LoraItems items, 
 
 // ============================================================ few tokens
 //
-// A workgroup takes a token and 512 columns: it computes all of the token's v (a wave a row of A at a time, two in flight),
-// which costs reading A once for each 512 columns but no second launch, then a column a thread.
+// A workgroup takes a token and 512 columns: it computes all of the token's v (a wave NR rows of A at a time, 16 loads of
+// them in flight), which costs reading A once for each 512 columns but no second launch, then a column a thread.
 struct LoraFewArgs {
   const void *x, *a, *b;
   int64_t ldx, lda, ldb, a_adapter, b_adapter, I, O;
@@ -829,9 +829,9 @@ struct LoraFewArgs {
   int64_t ldr, ldy;
   int type;
 };
-template <class TX, class TW>
+template <class TX, class TW, int NR>
 __global__ __launch_bounds__(512) void k_lora_few(LoraFewArgs g) {
-  constexpr int V = 16 / (int)sizeof(TW), U = 4;
+  constexpr int V = 16 / (int)sizeof(TW), U = 16 / NR;
   __shared__ float vs[LORA_MOST_R];
   typedef v4u v4uu __attribute__((aligned(2)));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -848,17 +848,19 @@ __global__ __launch_bounds__(512) void k_lora_few(LoraFewArgs g) {
   const TX *x = (const TX *)g.x + s * g.ldx;
   const TW *a = (const TW *)g.a + e * g.a_adapter, *b = (const TW *)g.b + e * g.b_adapter;
   const int K = (int)g.I;
-  for (int r = 2 * wave; r < g.R; r += 16) {
-    const TW *w[2] = {a + r * g.lda, a + min(r + 1, g.R - 1) * g.lda};
-    float acc[2] = {0.f, 0.f};
+  for (int r = NR * wave; r < g.R; r += 8 * NR) {
+    const TW *w[NR];
+#pragma unroll
+    for (int h = 0; h < NR; ++h) w[h] = a + min(r + h, g.R - 1) * g.lda;
+    float acc[NR] = {};
     for (int k0 = lane * V; k0 + V <= K; k0 += U * 64 * V) {
-      v4u rw[2][U];
+      v4u rw[U][NR];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int k = k0 + u * 64 * V;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          rw[h][u] = k + V <= K ? *reinterpret_cast<const v4uu *>(w[h] + k) : v4u{0, 0, 0, 0};
+        for (int h = 0; h < NR; ++h)
+          rw[u][h] = k + V <= K ? *reinterpret_cast<const v4uu *>(w[h] + k) : v4u{0, 0, 0, 0};
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -867,9 +869,9 @@ __global__ __launch_bounds__(512) void k_lora_few(LoraFewArgs g) {
         TX f[V];
         __builtin_memcpy(f, x + k, sizeof(f));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < NR; ++h) {
           TW t[V];
-          __builtin_memcpy(t, &rw[h][u], 16);
+          __builtin_memcpy(t, &rw[u][h], 16);
 #pragma unroll
           for (int j = 0; j < V; ++j) acc[h] = __builtin_fmaf(to_f32(t[j]), to_f32(f[j]), acc[h]);
         }
@@ -878,10 +880,14 @@ __global__ __launch_bounds__(512) void k_lora_few(LoraFewArgs g) {
     const int last = K / V * V + lane;
     if (last < K)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) acc[h] = __builtin_fmaf(to_f32(w[h][last]), to_f32(x[last]), acc[h]);
+      for (int h = 0; h < NR; ++h) acc[h] = __builtin_fmaf(to_f32(w[h][last]), to_f32(x[last]), acc[h]);
+    float v = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) acc[h] = group_sum<64>(acc[h]);
-    if (lane < 2 && r + lane < g.R) vs[r + lane] = lane ? acc[1] : acc[0];
+    for (int h = 0; h < NR; ++h) {
+      const float s = group_sum<64>(acc[h]);
+      v = lane == h ? s : v;
+    }
+    if (lane < NR && r + lane < g.R) vs[r + lane] = v;
   }
   __syncthreads();
   if (g.v && !blockIdx.x && threadIdx.x < g.R) g.v[(size_t)s * g.R + threadIdx.x] = vs[threadIdx.x];

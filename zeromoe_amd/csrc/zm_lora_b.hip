@@ -17,7 +17,8 @@ void sums(const LoraItems &items, const LoraSumArgs &a, unsigned na, const LoraS
 }
 template <class TX, class TW>
 void few(const LoraFewArgs &g, dim3 grid, hipStream_t st) {
-  hipLaunchKernelGGL((k_lora_few<TX, TW>), grid, dim3(512), 0, st, g);
+  if (g.R <= 16) hipLaunchKernelGGL((k_lora_few<TX, TW, 2>), grid, dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((k_lora_few<TX, TW, 4>), grid, dim3(512), 0, st, g);
 }
 
 }  // namespace
