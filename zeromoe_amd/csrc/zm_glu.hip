@@ -147,6 +147,10 @@ Product by_w(const zm_glu_desc &d) {
           vec_shape(dz_ld(d), 2 * d.F, t, false) && vec_shape(d.x_stride, d.I, d.x_type, false), false, false, false, -1};
 }
 
+// chunks of rows of the factors' gradients: 8 rows each, at most 512, so that a thread has its few rows on their way at
+// once (2048 x 1536 in bf16, chunks of 32: 34 us)
+int64_t factor_chunks(int64_t S) { return std::min<int64_t>((S + 7) / 8, 512); }
+
 // Workspace of the backward pass: both factors' gradients | bias partials | the larger product's partials.
 struct BackwardSpace {
   size_t dz, bias, part, total;
@@ -154,7 +158,7 @@ struct BackwardSpace {
 BackwardSpace backward_space(const zm_glu_desc &d) {
   BackwardSpace w{};
   w.dz = align256((size_t)d.S * dz_ld(d) * (dz_type(d) == LIN_BF16 ? 6 : 4));
-  w.bias = align256((size_t)dz_chunks(d.S) * 2 * d.F * 4);
+  w.bias = align256((size_t)factor_chunks(d.S) * 2 * d.F * 4);
   w.part = align256(std::max(by_x(d).space(), by_w(d).space()));
   w.total = w.dz + w.bias + w.part;
   return w;
@@ -246,7 +250,7 @@ int zm_glu_backward(const zm_glu_desc *d, const void *dy, const void *x, const v
   }
   a.ldz = ldz;
   a.part = db ? bias_part : nullptr;
-  const int64_t n = dz_chunks(d->S);
+  const int64_t n = factor_chunks(d->S);
   a.chunk = (d->S + n - 1) / n;
   const bool v = !(d->F & 3);
   const int64_t packs = v ? d->F / 4 : d->F;

@@ -32,12 +32,13 @@ def _list(grads, who: str):
 
 
 def _check(grads, d: int, what: str):
+    mode, types = _grad_mode(), _TYPES
     for i, g in enumerate(grads):
         if not isinstance(g, torch.Tensor) or g.get_device() != d:
             raise ValueError(f"{what} {i} is not a tensor of the first one's device")
-        if g.dtype not in _TYPES:
+        if g.dtype not in types:
             raise ValueError(f"{what} {i} is {g.dtype}: float32, float16 or bfloat16 needed")
-        if g.requires_grad and _grad_mode():
+        if mode and g.requires_grad:
             _not_recorded(what)
 
 
@@ -70,23 +71,26 @@ def clip_grad_norm(grads, max_norm: float, eps: float = 1e-6, out=None, stream=N
     if stream is not None or d != _device():
         return _there(clip_grad_norm, d, stream, grads, max_norm, eps, out)
     _check(grads, d, "gradient")
+    flat, types = [], _TYPES
     if out is None:
-        out = grads
+        for i, g in enumerate(grads):
+            if not g.is_contiguous() and not _dense(g):
+                raise ValueError(f"gradient {i} does not fill one piece of memory: strides {g.stride()} of {tuple(g.shape)}")
+            p, k = g.data_ptr(), types[g.dtype]
+            flat += (p, p, g.numel(), k, k)
     else:
         _check(out, d, "result")
         if len(out) != len(grads):
             raise ValueError(f"{len(grads)} gradients and {len(out)} results")
         for i, (g, o) in enumerate(zip(grads, out)):
-            if g.shape != o.shape or (g.stride() != o.stride() and not (g.is_contiguous() and o.is_contiguous())):
+            if g.shape != o.shape or not (g.is_contiguous() and o.is_contiguous()) and g.stride() != o.stride():
                 raise ValueError(f"result {i} needs its gradient's shape and strides: {tuple(g.shape)}, {g.stride()}")
+            if not g.is_contiguous() and not _dense(g):
+                raise ValueError(f"gradient {i} does not fill one piece of memory: strides {g.stride()} of {tuple(g.shape)}")
             if o.dtype != g.dtype and o.dtype != _F32:
                 raise ValueError(f"result {i} is {o.dtype}: {g.dtype} or float32 needed")
-    for i, g in enumerate(grads):
-        if not _dense(g):
-            raise ValueError(f"gradient {i} does not fill one piece of memory: strides {g.stride()} of {tuple(g.shape)}")
+            flat += (g.data_ptr(), o.data_ptr(), g.numel(), types[g.dtype], types[o.dtype])
     n = len(grads)
-    flat = [v for g, o in zip(grads, out)
-            for v in (g.data_ptr(), o.data_ptr(), g.numel(), _TYPES[g.dtype], _TYPES[o.dtype])]
     norm = grads[0].new_empty((), dtype=_F32)
     L = lib()
     ws = _space(L.zm_grad_norm_workspace_size(n), norm)
