@@ -63,8 +63,12 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, 
         int kind, bm, bn;
         double one, two, start;
       };
-      static const Tile dma_tiles[] = {
-          {2, 256, 256, 1.9, 0, 0}, {3, 256, 128, 1.04, 0, 0}, {0, 128, 128, 0.75, 1.09, 0}};
+      // 16-bit operands: a tile alone on its CU starts and ends with nothing beside it, two of 128 x 128 hide each other's
+      // (8192 x 1024 by w of 8192 rows, 16 steps a tile: 256 x 256 250 us, 256 x 128 185, 128 x 128 159; gradient by x of
+      // 8192 x 7168 with k = 2048: 349, 337, 261; 8192^3: 256 x 256 997).  Two weights end a tile with twice the sums and
+      // the activation.
+      const double more = pair ? 8.0 : 0.0;
+      const Tile dma_tiles[] = {{2, 256, 256, 1.72, 0, 27 + more}, {3, 256, 128, 1.0, 0, 12}, {0, 128, 128, 0.76, 1.0, 3.3}};
       static const Tile term_tiles[] = {
           {0, 128, 128, 1.0, 1.5, 0}, {0, 128, 128, 1.2, 2.1, 0}, {0, 128, 128, 1.3, 0, 0}};
       // w's side of a product may be narrow, as a router's is: 160 rows fill one tile of 160, and 62% of two of 128
