@@ -27,6 +27,7 @@ int check_lora(const zm_lora_desc *d, const char *who) {
   const int64_t most = ((int64_t)1 << 31) / (int64_t)size_of(d->w_type);
   if ((d->R - 1) * d->a_stride + d->I >= most || (d->O - 1) * d->b_stride + d->R >= most)
     return fail("%s: an adapter's a and b are below 2^31 bytes", who);
+  if ((std::max(d->I, d->O) / 64 + 1) * ((d->R + 15) / 16) * d->n >= 1 << 26) return fail("%s: n x R x I or n x R x O too large", who);
   return 0;
 }
 
@@ -134,6 +135,7 @@ int zm_lora(const zm_lora_desc *d, const void *x, const void *a, const void *b, 
   if (check_rows(d->S, d->y_stride, d->O, "zm_lora", "y")) return -1;
   if (!d->S) return 0;
   if (!x || !a || !b || !ids || !y) return fail("zm_lora: null pointer");
+  if (residual == y && d->S > 1 && d->res_stride != d->y_stride) return fail("zm_lora: a residual in the place of y has y's stride");
   const hipStream_t st = (hipStream_t)stream;
   if (few_tokens(*d)) {
     LoraFewArgs g{x, a, b, d->x_stride, d->a_stride, d->b_stride, d->a_adapter, d->b_adapter, d->I, d->O, d->R, d->n, ids,

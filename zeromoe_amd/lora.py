@@ -12,26 +12,22 @@ from .dense import (_F32, _F32S, _I32S, _TYPES, _device, _flat, _grad_mode, _ind
 
 
 def _operands(d, x, a, b, ids, scale):
-    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3 or a.shape[2] != x.shape[1] or b.shape[2] != a.shape[1] \
-            or b.shape[0] != a.shape[0]:
-        raise ValueError(f"x (S, I), a (n, R, I) and b (n, O, R) are needed, not {tuple(x.shape)}, {tuple(a.shape)} and "
-                         f"{tuple(b.shape)}")
+    """ids, scale, the sizes (S, I, O, R, n) and the strides of both adapters; each tensor's are asked for once (0.2 us)."""
+    xs, sa, sb = x.shape, a.shape, b.shape
+    if len(xs) != 2 or len(sa) != 3 or len(sb) != 3 or sa[2] != xs[1] or sb[2] != sa[1] or sb[0] != sa[0]:
+        raise ValueError(f"x (S, I), a (n, R, I) and b (n, O, R) are needed, not {tuple(xs)}, {tuple(sa)} and {tuple(sb)}")
     if x.get_device() != d or a.get_device() != d or b.get_device() != d:
         raise ValueError("x, a or b is on another device")
-    if x.dtype not in _TYPES or a.dtype not in _TYPES or a.dtype != b.dtype or (x.dtype != _F32 and a.dtype != x.dtype):
-        raise ValueError(f"x {x.dtype} with a {a.dtype} and b {b.dtype}: float32 activations with float32, float16 or "
-                         "bfloat16 adapters, or all of one 16-bit type")
-    n, R, I = a.shape
-    if (a.stride(2) != 1 and I != 1) or (b.stride(2) != 1 and R != 1):
+    tx, ta = x.dtype, a.dtype
+    if tx not in _TYPES or ta not in _TYPES or ta != b.dtype or (tx != _F32 and ta != tx):
+        raise ValueError(f"x {tx} with a {ta} and b {b.dtype}: float32 activations with float32, float16 or bfloat16 "
+                         "adapters, or all of one 16-bit type")
+    n, R, I = sa
+    la, lb = a.stride(), b.stride()
+    if (la[2] != 1 and I != 1) or (lb[2] != 1 and R != 1):
         raise ValueError("a and b need contiguous columns")
-    ids = _flat(_need(ids, "ids", d, _I32S, (x.shape[0],)))
-    return ids, _vector(scale, "scale", d, n)
-
-
-def _desc(x, a, b, y, res_stride):
-    n, R, I = a.shape
-    return ZmLoraDesc(_TYPES[x.dtype], _TYPES[a.dtype], _TYPES[y.dtype], n, R, x.shape[0], I, b.shape[1], x.stride(0),
-                      y.stride(0), res_stride, a.stride(1), a.stride(0), b.stride(1), b.stride(0))
+    ids = _flat(_need(ids, "ids", d, _I32S, (xs[0],)))
+    return ids, _vector(scale, "scale", d, n), (xs[0], I, sb[1], R, n), la, lb
 
 
 def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, scale=None, residual=None, out=None,
@@ -50,8 +46,7 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, s
                          or residual is not None and residual.requires_grad or out is not None and out.requires_grad):
         _not_recorded("lora")
     st = _raw_stream(d)
-    ids, scale = _operands(d, x, a, b, ids, scale)
-    S, O, R = x.shape[0], b.shape[1], a.shape[1]
+    ids, scale, (S, I, O, R, n), la, lb = _operands(d, x, a, b, ids, scale)
     x = _rows(x)
     dtype = out_dtype or (out.dtype if out is not None else x.dtype)
     if dtype != _F32 and dtype != x.dtype:
@@ -60,7 +55,8 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, s
     if residual is not None:
         residual = _rows(_need(residual, "residual", d, (dtype,), (S, O)))
     v = x.new_empty((S, R), dtype=_F32) if save else None
-    desc = _desc(x, a, b, y, residual.stride(0) if residual is not None else 0)
+    desc = ZmLoraDesc(_TYPES[x.dtype], _TYPES[a.dtype], _TYPES[dtype], n, R, S, I, O, x.stride(0), y.stride(0),
+                      residual.stride(0) if residual is not None else 0, la[1], la[0], lb[1], lb[0])
     L = lib()
     ws = _space(L.zm_lora_workspace_size(desc), x)
     check(L.zm_lora(desc, x.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(), _ptr(scale), _ptr(residual), y.data_ptr(),
@@ -80,8 +76,7 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.T
                          or v is not None and v.requires_grad or scale is not None and scale.requires_grad):
         _not_recorded("lora_backward")
     st = _raw_stream(d)
-    ids, scale = _operands(d, x, a, b, ids, scale)
-    (n, R, I), (S, O) = a.shape, (x.shape[0], b.shape[1])
+    ids, scale, (S, I, O, R, n), la, lb = _operands(d, x, a, b, ids, scale)
     x = _rows(x)
     dy = _rows(_need(dy, "dy", d, (_F32, x.dtype), (S, O)))
     if v is not None:
@@ -91,7 +86,8 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.T
     dx = x.new_empty((S, I)) if need_dx else None
     da = x.new_empty((n, R, I), dtype=_F32) if need_da else None
     db = x.new_empty((n, O, R), dtype=_F32) if need_db else None
-    desc = _desc(x, a, b, dy, 0)
+    desc = ZmLoraDesc(_TYPES[x.dtype], _TYPES[a.dtype], _TYPES[dy.dtype], n, R, S, I, O, x.stride(0), dy.stride(0), 0, la[1],
+                      la[0], lb[1], lb[0])
     L = lib()
     ws = _space(L.zm_lora_backward_workspace_size(desc), x)
     check(L.zm_lora_backward(desc, dy.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(), _ptr(scale),
