@@ -12,8 +12,8 @@
 //
 // and the adapters' gradients are sums over an adapter's tokens of c a[s][r] m[s][j] (a = u, m = x for dA, a = v, m = dy
 // for dB).  Tokens are sorted by adapter first (a stable order, so sums have a fixed order) into items of up to 32 tokens
-// of one adapter.  (Two kernels with v in memory, the long axis in slices, took 50 + 58 us where the one takes LORA_US:
-// 8192 x 7168 x 2048, R 64, bf16.)
+// of one adapter.  (Two kernels with v in memory, the long axis in slices, took 50 + 58 us where the one takes 65:
+// 8192 x 7168 x 2048, R 64, bf16.  Where items are few and have much to read, each axis is a launch of its own after all.)
 //
 // The matrix instructions (16 x 16, 32 of the summed index) take 8 consecutive values of that index a lane: lane (fr, fc)
 // row fr, values 8 fc ..  Where memory has the rows contiguous instead (B in the backward pass, and all operands of a sum
@@ -48,6 +48,11 @@ struct LoraArgs {
   void *y;
   int64_t ldr, ldy;
   int rest;               // tokens that a workgroup looks through for those without an adapter
+  // both axes in one launch, or (few items) each in its own, the long one in slices of k, the short one in groups of columns
+  enum { BOTH, LONG, SHORT };
+  int phase, slices;
+  int64_t kslice;
+  float *part;            // [slices][S][R]
 };
 
 // ============================================================ items
@@ -55,7 +60,7 @@ struct LoraArgs {
 // One workgroup; each of its 16 waves takes a run of tokens, 64 at a time.  The lanes of one id find each other by a
 // ballot for each bit of it; their first one counts them in the wave's own counters, so no atomic is needed and a token's
 // place among its wave's is known at once; it is kept in registers for the first 16 chunks (16384 tokens of the call) and
-// found again for the others.  8192 tokens of 8 adapters: LORA_ITEMS_US.
+// found again for the others.  8192 tokens of 8 adapters: 7.6 us.
 constexpr int LORA_CHUNKS = 16;
 static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__restrict__ ids, int S, int n, LoraItems o) {
   __shared__ int cnt[16][LORA_MOST_N], first[LORA_MOST_N], total[LORA_MOST_N], sums[16];
@@ -283,7 +288,7 @@ constexpr int terms_beside() {
 // back the same way.  RL: values of r whose terms LDS has room for.
 //
 // Every workgroup also looks through g.rest tokens for those without an adapter: their rows are the residual (or zeros),
-// and NaN where the id names none.  (Workgroups of their own waited for a CU behind the items: 68 us for LORA_US.)
+// and NaN where the id names none.  (Workgroups of their own waited for a CU behind the items: 68.6 us for 65.)
 constexpr int LORA_WAVES = 8;
 
 // ROWS rows of PIECES x 16 bytes by way of registers into LDS, rows 128 bytes apart, their pieces permuted so that 16 rows
@@ -344,8 +349,8 @@ struct Lora {
 
   // the sums of MT tiles of 16 tokens over this wave's lines, r from r0 on
   template <int MT>
-  __device__ __forceinline__ static void long_axis(const LoraArgs &g, const LoraItem &it, int r0, uint8_t *buf,
-                                                   v4f (&acc)[MT][NF]) {
+  __device__ __forceinline__ static void long_axis(const LoraArgs &g, const LoraItem &it, int r0, int64_t k0, int64_t k1,
+                                                   uint8_t *buf, v4f (&acc)[MT][NF]) {
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), fr = lane & 15, fc = lane >> 4;
     constexpr int STEP = LINE * LORA_WAVES;
     typedef Stage<TX, 16 * MT, 8> SX;
@@ -367,12 +372,13 @@ struct Lora {
       SM m;                        // KC
       Words<TW, NF> r[KC ? 1 : H][8];  // else
     };
-    if (LINE * wave >= g.K) return;
-    const int64_t last = LINE * wave + (g.K - 1 - LINE * wave) / STEP * STEP;
+    int64_t k = k0 + LINE * wave;
+    if (k >= k1) return;
+    const int64_t last = k + (k1 - 1 - k) / STEP * STEP;
     auto load = [&](Line &to, int64_t k) {
       // (past the end the last line again: a load under a condition would be waited for where its paths meet)
       k = min(k, last);
-      const int left = (int)min(g.K - k, (int64_t)LINE);
+      const int left = (int)min(k1 - k, (int64_t)LINE);
       to.x.load([&](int i) { return x[i] + k; }, left, (const TX *)g.x);
       if constexpr (KC) {
         to.m.load([&](int i) { return (const TW *)((const uint8_t *)(m + k) + row[i]); }, left, m);
@@ -425,13 +431,12 @@ struct Lora {
       stage_sync();
     };
     Line a, b;
-    int64_t k = LINE * wave;
     load(a, k);
     if constexpr (DEPTH == 2) load(b, k + STEP);
-    for (; k < g.K; k += DEPTH * STEP) {
+    for (; k < k1; k += DEPTH * STEP) {
       step(a, k);
       if constexpr (DEPTH == 2) {
-        if (k + STEP >= g.K) break;
+        if (k + STEP >= k1) break;
         step(b, k + STEP);
       }
     }
@@ -441,9 +446,35 @@ struct Lora {
   __device__ __forceinline__ static void run(const LoraArgs &g, const LoraItem &it, Lds &lds) {
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), fr = lane & 15, fc = lane >> 4;
     const float c = g.scale ? g.scale[it.e] : 1.f;
+    auto put_terms = [&](int s, int r, float v) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const bf16 e = from_f32<bf16>(k ? v : __builtin_amdgcn_fmed3f(v, -BF16_MOST, BF16_MOST));
+        lds.terms[k][s][r] = e.u;
+        v -= to_f32(e);
+      }
+    };
+    if (g.phase == LoraArgs::SHORT) {
+      const int RP = (g.R + 31) & ~31;
+      for (int t = threadIdx.x; t < 16 * MT * RP; t += 64 * LORA_WAVES) {
+        const int s = t / RP, r = t - s * RP;
+        float v = 0.f;
+        if (s < it.count && r < g.R) {
+          const size_t at = (size_t)it.tokens[s] * g.R + r;
+          for (int z = 0; z < g.slices; ++z) v += g.part[(size_t)z * g.S * g.R + at];
+          if (g.v && !blockIdx.y) g.v[at] = v;
+        }
+        put_terms(s, r, v * c);
+      }
+      __syncthreads();
+      return short_axis<MT>(g, it, lds);
+    }
+    const int64_t k0 = g.phase == LoraArgs::LONG ? blockIdx.y * g.kslice : 0;
+    const int64_t k1 = g.phase == LoraArgs::LONG ? min(g.K, k0 + g.kslice) : g.K;
+    float *part = g.phase == LoraArgs::LONG ? g.part + (size_t)blockIdx.y * g.S * g.R : g.v;
     for (int r0 = 0; r0 < g.R; r0 += NR) {
       v4f acc[MT][NF];
-      long_axis<MT>(g, it, r0, lds.wave[wave], acc);
+      long_axis<MT>(g, it, r0, k0, k1, lds.wave[wave], acc);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         __syncthreads();
@@ -464,25 +495,19 @@ struct Lora {
           if (r < NR && r0 + r < g.R) {
 #pragma unroll
             for (int u = 0; u < LORA_WAVES; ++u) v += lds.sums[u][s][r];
-            if (g.v && 16 * i + s < it.count) g.v[(size_t)it.tokens[16 * i + s] * g.R + r0 + r] = v;
-            v *= c;
+            if (part && 16 * i + s < it.count) part[(size_t)it.tokens[16 * i + s] * g.R + r0 + r] = v;
           }
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const bf16 e = from_f32<bf16>(k ? v : __builtin_amdgcn_fmed3f(v, -BF16_MOST, BF16_MOST));
-            lds.terms[k][16 * i + s][r0 + r] = e.u;
-            v -= to_f32(e);
-          }
+          put_terms(16 * i + s, r0 + r, v * c);
         }
       }
       __syncthreads();
     }
-    short_axis<MT>(g, it, lds);
+    if (g.phase == LoraArgs::BOTH) short_axis<MT>(g, it, lds);
   }
 
   template <int MT>
   __device__ __forceinline__ static void short_axis(const LoraArgs &g, const LoraItem &it, Lds &lds) {
-    constexpr int STEP = 64 * LORA_WAVES;
+    const int STEP = 64 * LORA_WAVES * gridDim.y;  // (groups of columns)
     constexpr bool STAGED = KC && RL > 32;                   // (shorter rows of L are several to a line)
     constexpr int RS = STAGED ? 128 / (int)sizeof(TW) : 32;  // r of a step
     typedef Stage<TW, 64, 8> SL;
@@ -539,7 +564,7 @@ struct Lora {
         }
       }
     };
-    int64_t o0 = 64 * wave;
+    int64_t o0 = 64 * (LORA_WAVES * blockIdx.y + wave);
     if (o0 >= g.N) return;
     const int64_t last = o0 + (g.N - 1 - o0) / STEP * STEP;
     auto load = [&](Columns &to, int64_t o0) {
@@ -686,6 +711,7 @@ __global__ __launch_bounds__(64 * LORA_WAVES) void k_lora(LoraArgs g) {
     if (it.count <= 16) L::template run<1>(g, it, lds);
     else L::template run<2>(g, it, lds);
   }
+  if (g.phase == LoraArgs::LONG || blockIdx.y) return;
   const int64_t s0 = (int64_t)blockIdx.x * g.rest, s1 = min(s0 + g.rest, (int64_t)g.S);
   for (int64_t s = s0; s < s1; s += 64) L::rest(g, (int)s, (int)s1);
 }
@@ -907,14 +933,14 @@ __global__ __launch_bounds__(512) void k_lora_few(LoraFewArgs g) {
 }
 
 // the kernels by their operands' types: of the rows, the adapters and the result
-void lora_forward(int x_type, int w_type, int y_type, const LoraArgs &g, int grid, hipStream_t st);
-void lora_backward(int x_type, int w_type, int y_type, const LoraArgs &g, int grid, hipStream_t st);
+void lora_forward(int x_type, int w_type, int y_type, const LoraArgs &g, dim3 grid, hipStream_t st);
+void lora_backward(int x_type, int w_type, int y_type, const LoraArgs &g, dim3 grid, hipStream_t st);
 void lora_sums(int x_type, int dy_type, const LoraItems &items, const LoraSumArgs &a, unsigned na, const LoraSumArgs &b,
                unsigned nb, hipStream_t st);
 void lora_few(int x_type, int w_type, const LoraFewArgs &g, dim3 grid, hipStream_t st);
 template <class TX, class TW, bool KC, class TY>
-void lora_launch(const LoraArgs &g, int grid, hipStream_t st) {
-  const dim3 n(grid), wg(64 * LORA_WAVES);
+void lora_launch(const LoraArgs &g, dim3 n, hipStream_t st) {
+  const dim3 wg(64 * LORA_WAVES);
   if (g.R <= 16) hipLaunchKernelGGL((k_lora<TX, TW, KC, 1, 32, TY>), n, wg, 0, st, g);
   else if (g.R <= 32) hipLaunchKernelGGL((k_lora<TX, TW, KC, 2, 32, TY>), n, wg, 0, st, g);
   else if (g.R <= 64) hipLaunchKernelGGL((k_lora<TX, TW, KC, 4, 64, TY>), n, wg, 0, st, g);

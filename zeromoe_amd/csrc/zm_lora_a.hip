@@ -5,7 +5,7 @@
 
 namespace zm {
 
-void lora_forward(int x_type, int w_type, int y_type, const LoraArgs &g, int grid, hipStream_t st) {
+void lora_forward(int x_type, int w_type, int y_type, const LoraArgs &g, dim3 grid, hipStream_t st) {
   if (x_type == LIN_BF16) {
     if (y_type == LIN_BF16) lora_launch<bf16, bf16, true, bf16>(g, grid, st);
     else lora_launch<bf16, bf16, true, float>(g, grid, st);

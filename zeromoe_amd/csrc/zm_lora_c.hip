@@ -5,7 +5,7 @@
 
 namespace zm {
 
-void lora_backward(int dy_type, int w_type, int dx_type, const LoraArgs &g, int grid, hipStream_t st) {
+void lora_backward(int dy_type, int w_type, int dx_type, const LoraArgs &g, dim3 grid, hipStream_t st) {
   if (dx_type == LIN_BF16) {
     if (dy_type == LIN_BF16) lora_launch<bf16, bf16, false, bf16>(g, grid, st);
     else lora_launch<float, bf16, false, bf16>(g, grid, st);
