@@ -136,14 +136,14 @@ def test_lora_strides_and_alignment(xt, wt, S, I, R):
 
 
 def check_backward(S, I, O, R, n, xt, wt, kind="mixed", scaled=True, ydt=None, seed=1, need=(True, True, True), x=None, a=None,
-                   b=None, dy=None, v=None):
+                   b=None, dy=None, v=None, ids=None):
     import zeromoe_amd as Z
 
     dtype, yt = TYPES[xt], TYPES[ydt or xt]
     x = rand(S, I, seed=seed, dtype=dtype) if x is None else x
     if a is None:
         a, b = adapters(n, R, I, O, wt, seed + 1)
-    ids = some_ids(S, n, kind)
+    ids = some_ids(S, n, kind) if ids is None else ids
     scale = rand(n, seed=seed + 3) if scaled else None
     dy = rand(S, O, seed=seed + 4, scale=0.1, dtype=yt) if dy is None else dy
     v = rand(S, R, seed=seed + 5) if v is None else v
@@ -229,6 +229,17 @@ def test_lora_rows_without_a_valid_adapter(S, I, R):
     _, _, y64, ty = lora64(x[keep], a, b, ids[keep], None)
     y64 = y64 + res[keep].double()
     close(z[keep], y64, ty + 2 * U * res[keep].double().abs() + 2 * U * y64.abs() + 1e-37)
+
+
+@pytest.mark.parametrize("counts", [(4096,), (4097,), (4095, 0, 1), (2049, 2032), (2050, 2033, 0, 0, 7), (16 * 250 + 1, 1, 1, 1, 1),
+                                    (16 * 250 + 1, 1, 1, 1, 1, 1), tuple([17] * 128), tuple([17] * 129), (4096, 1500), (5500, 0)])
+def test_lora_tokens_of_an_item(counts):
+    """Up to 256 groups of 16 tokens of an adapter, and more (which are taken 32 at a time), with tokens of none between."""
+    n, I, O, R = len(counts), 1032, 264, 16
+    ids = torch.cat([torch.full((c,), e) for e, c in enumerate(counts)] + [torch.full((300,), -1)])
+    ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(1))].to(torch.int32).cuda()
+    check_lora(len(ids), I, O, R, n, "bf16", "bf16", ids=ids)
+    check_backward(len(ids), I, O, R, n, "bf16", "bf16", ids=ids)
 
 
 def test_lora_no_tokens():

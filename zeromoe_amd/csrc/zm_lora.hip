@@ -31,12 +31,11 @@ int check_lora(const zm_lora_desc *d, const char *who) {
   return 0;
 }
 
-// Work items are counted on the device; a launch has as many as there can be.
+// Work items are counted on the device; a launch has as many as there can be.  Items of 16 tokens are worth it where no CU
+// gets two of them: that may be so up to 384, with a third of the tokens without an adapter.
 int64_t items_of(const zm_lora_desc &d, int T) { return d.S / T + std::min<int64_t>(d.S, d.n); }
-// Tokens of an item.  A CU runs one item at a time: 16 where the items then fit the 256 CUs (of the most there can be a
-// few are not there), else 32.
-int tokens_of(const zm_lora_desc &d) { return items_of(d, 16) <= 272 ? 16 : LORA_TOKENS; }
-int64_t most_items(const zm_lora_desc &d) { return items_of(d, tokens_of(d)); }
+bool small_items(const zm_lora_desc &d) { return items_of(d, 16) <= LORA_CUS * 3 / 2; }
+int64_t most_items(const zm_lora_desc &d) { return items_of(d, small_items(d) ? 16 : LORA_TOKENS); }
 
 // slices of an axis of K, `unit` at a time, for `want` workgroups where one slice has `n`
 int64_t slices_of(int64_t n, int64_t want, int64_t K, int64_t unit, int64_t most) {
@@ -64,7 +63,7 @@ struct Split {
 };
 Split split_of(const zm_lora_desc &d, int64_t K, int64_t N) {
   Split s{1, 1, K, 0};
-  const int64_t n = most_items(d), cus = 256 / n;
+  const int64_t n = most_items(d), cus = LORA_CUS / n;
   if (cus < 2 || d.R * (K + N) * (int64_t)size_of(d.w_type) < 256 << 10) return s;
   const int64_t z = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(cus, 16), K / 512));
   s.kslice = ((K + z - 1) / z + 511) / 512 * 512;
@@ -78,7 +77,7 @@ Split split_of(const zm_lora_desc &d, int64_t K, int64_t N) {
 struct Space {
   size_t items, part, u, total;
 };
-size_t item_bytes(const zm_lora_desc &d) { return align256((2 * d.n + 1 + (tokens_of(d) + 1) * most_items(d)) * 4); }
+size_t item_bytes(const zm_lora_desc &d) { return align256((2 * d.n + 2 + (LORA_TOKENS + 1) * most_items(d)) * 4); }
 Space space_of(const zm_lora_desc &d, bool backward) {
   Space s{};
   s.items = item_bytes(d);
@@ -104,11 +103,10 @@ LoraArgs items(const zm_lora_desc &d, const int32_t *ids, const float *scale, ui
   int32_t *p = (int32_t *)ws;
   const int64_t most = most_items(d);
   g.rest = (int)((d.S + most - 1) / most);
-  g.it.T = tokens_of(d);
-  g.it.log_T = g.it.T == 16 ? 4 : 5;
+  g.it.small = small_items(d);
   g.it.tokens = p;
-  g.it.item_e = p + g.it.T * most;
-  g.it.counts = g.it.item_e + most;
+  g.it.item = p + LORA_TOKENS * most;
+  g.it.counts = g.it.item + most;
   g.it.first = g.it.counts + d.n;
   g.it.n_items = g.it.first + d.n;
   hipLaunchKernelGGL(k_lora_items, dim3(1), dim3(1024), 0, st, ids, (int)d.S, (int)d.n, g.it);

@@ -12,7 +12,7 @@
 //
 // and the adapters' gradients are sums over an adapter's tokens of c a[s][r] m[s][j] (a = u, m = x for dA, a = v, m = dy
 // for dB).  Tokens are sorted by adapter first (a stable order, so sums have a fixed order) into items of up to 32 tokens
-// of one adapter.  (Two kernels with v in memory, the long axis in slices, took 50 + 58 us where the one takes 65:
+// of one adapter.  (Two kernels with v in memory, the long axis in slices, took 50 + 58 us where the one takes 60:
 // 8192 x 7168 x 2048, R 64, bf16.  Where items are few and have much to read, each axis is a launch of its own after all.)
 //
 // The matrix instructions (16 x 16, 32 of the summed index) take 8 consecutive values of that index a lane: lane (fr, fc)
@@ -26,13 +26,18 @@
 namespace zm {
 
 constexpr int LORA_TOKENS = 32;  // of an item, at most (16 or 32)
+constexpr int LORA_CUS = 256;
 constexpr int LORA_MOST_R = 256, LORA_MOST_N = 512;
 
-// The items, of up to T tokens: adapter e's tokens lie at tokens[T first[e] ..], counts[e] of them, in ascending order, -1
-// behind them up to the next item; item i is of adapter item_e[i].
+// The items, of up to T tokens: item i's tokens lie at tokens[T i ..], in ascending order, and item[i] is its
+// adapter and (from bit 16 on) how many there are.  Adapter e has counts[e] tokens, in the items from first[e] on.
+//
+// A CU runs one item at a time, so T is 16 where no CU gets a second one then, else 32: dx alone of 4095 tokens of four
+// adapters, 4096 x 1536, R 16: 51 us a call in 258 items of 16, 39 in 130 of 32; 4060 tokens in 256 of 16: 34.  How
+// many there are depends on the ids, so that is decided on the device.
 struct LoraItems {
-  int32_t *counts, *first, *item_e, *tokens, *n_items;  // [n], [n], [items], [items][T], one
-  int T, log_T;  // (a power of two)
+  int32_t *counts, *first, *item, *tokens, *n_items;  // [n], [n], [items], [items][T], items and log2 T
+  int small;  // whether T may be 16
 };
 struct LoraArgs {
   const void *x, *m, *l;  // rows, the matrices of the long axis and those of the short one
@@ -102,7 +107,8 @@ static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__res
     if (64 * c < seg) at[c] = place(e[c]);
   for (int p = p0 + 64 * LORA_CHUNKS; p < p1; p += 64) place(load(p + lane));
   __syncthreads();
-  // by adapter: tokens of the waves before, all of them, and their items
+  // by adapter: tokens of the waves before, all of them, and their items (small: of 16 tokens in the low half, of 32 in the
+  // other; there are 384 at most)
   int mine = 0;
   if (tid < n) {
     int run = 0;
@@ -113,7 +119,8 @@ static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__res
       run += k;
     }
     total[tid] = run;
-    mine = (run + o.T - 1) >> o.log_T;
+    mine = (run + 31) >> 5;
+    if (o.small) mine = mine << 16 | (run + 15) >> 4;
   }
   int incl = mine;  // (adapters are below 512: waves 0 to 7 hold them)
 #pragma unroll
@@ -129,26 +136,25 @@ static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__res
     if (v < w) before += sums[v];
     all += sums[v];
   }
+  const int lg = o.small && (all & 0xffff) <= LORA_CUS ? 4 : 5, T = 1 << lg;
+  auto items = [&](int k) { return !o.small ? k : lg == 4 ? k & 0xffff : k >> 16; };
   if (tid < n) {
-    first[tid] = before + incl - mine;
+    first[tid] = items(before + incl - mine);
     o.first[tid] = first[tid];
     o.counts[tid] = total[tid];
   }
-  if (!tid) *o.n_items = all;
+  if (!tid) {
+    o.n_items[0] = items(all);
+    o.n_items[1] = lg;
+  }
   __syncthreads();
-  auto put = [&](int p, int e, int at) {
-    if (e < 0) return;
-    at += cnt[w][e];
-    o.tokens[(size_t)first[e] * o.T + at] = p;
-    if (!(at & (o.T - 1))) o.item_e[first[e] + (at >> o.log_T)] = e;
+  auto put = [&](int p, int e, int at) {  // token p, `at` among e's
+    o.tokens[((size_t)first[e] << lg) + at] = p;
+    if (!(at & (T - 1))) o.item[first[e] + (at >> lg)] = e | min(T, total[e] - at) << 16;
   };
 #pragma unroll
   for (int c = 0; c < LORA_CHUNKS; ++c)
-    if (64 * c < seg) put(p0 + 64 * c + lane, e[c], at[c]);
-  for (int q = w; q < n; q += 16) {  // behind an adapter's last token
-    const int used = total[q] & (o.T - 1);
-    if (used && lane >= used && lane < o.T) o.tokens[((size_t)first[q] + (total[q] >> o.log_T)) * o.T + lane] = -1;
-  }
+    if (64 * c < seg && e[c] >= 0) put(p0 + 64 * c + lane, e[c], at[c] + cnt[w][e[c]]);
   if (seg <= 64 * LORA_CHUNKS) return;
   // the chunks past the registers: their places again, on from those of the chunks before
   stage_sync();
@@ -160,29 +166,25 @@ static __global__ __launch_bounds__(1024) void k_lora_items(const int32_t *__res
   for (int p = p0 + 64 * LORA_CHUNKS; p < p1; p += 64) {
     const int k = load(p + lane);
     const int a = place(k);
-    if (k < 0) continue;
-    o.tokens[(size_t)first[k] * o.T + a] = p + lane;
-    if (!(a & (o.T - 1))) o.item_e[first[k] + (a >> o.log_T)] = k;
+    if (k >= 0) put(p + lane, k, a);
   }
 }
 
-// This thread's view of item i: its adapter, its tokens and how many there are (read side by side)
+// This wave's view of item i: its adapter, its tokens and how many there are.  All are asked for before any is waited for.
 struct LoraItem {
-  int e, count;
-  const int32_t *tokens;
-  // token t of the item; those past the last are its first
-  __device__ __forceinline__ int64_t token(int t) const {
-    const int s = tokens[t];
-    return s < 0 ? tokens[0] : s;
-  }
+  int e, count, lanes;  // lanes: token lane % 32 of the item
+  // token t of the item; those past the last are its first (all lanes of the wave take part)
+  __device__ __forceinline__ int64_t token(int t) const { return __shfl(lanes, t < count ? t : 0, 64); }
 };
 __device__ __forceinline__ bool lora_item(const LoraArgs &g, int i, LoraItem &it) {
-  it.tokens = g.it.tokens + (size_t)i * g.it.T;
-  it.e = g.it.item_e[i];
-  const int lane = threadIdx.x & 63, t = it.tokens[min(lane, g.it.T - 1)];
-  if (i >= *g.it.n_items) return false;  // (before it.e is used)
-  it.e = uniform(it.e);
-  it.count = __builtin_popcountll(__ballot(t >= 0 && lane < g.it.T));
+  // (its place follows from T: both are read)
+  const int32_t *at = g.it.tokens + threadIdx.x % LORA_TOKENS;
+  int item = g.it.item[i], n = g.it.n_items[0], lg = g.it.n_items[1], t16 = at[16 * (size_t)i], t32 = at[32 * (size_t)i];
+  asm volatile("" : "+v"(item), "+v"(n), "+v"(lg), "+v"(t16), "+v"(t32));  // (else some are asked for past the branch)
+  if (i >= uniform(n)) return false;  // (before item is used)
+  it.e = uniform(item & 0xffff);
+  it.count = uniform(item >> 16);
+  it.lanes = uniform(lg) == 4 ? t16 : t32;
   return true;
 }
 
@@ -460,7 +462,7 @@ struct Lora {
         const int s = t / RP, r = t - s * RP;
         float v = 0.f;
         if (s < it.count && r < g.R) {
-          const size_t at = (size_t)it.tokens[s] * g.R + r;
+          const size_t at = (size_t)g.it.tokens[((size_t)blockIdx.x << g.it.n_items[1]) + s] * g.R + r;
           for (int z = 0; z < g.slices; ++z) v += g.part[(size_t)z * g.S * g.R + at];
           if (g.v && !blockIdx.y) g.v[at] = v;
         }
@@ -491,11 +493,12 @@ struct Lora {
         constexpr int WIDE = NR < 32 ? 32 : NR;  // (zeros up to the 32 of a matrix instruction)
         for (int t = threadIdx.x; t < 16 * WIDE; t += 64 * LORA_WAVES) {
           const int s = t / WIDE, r = t % WIDE;
+          const int64_t to = part ? it.token(16 * i + s) : 0;  // (by all lanes of the wave)
           float v = 0.f;
           if (r < NR && r0 + r < g.R) {
 #pragma unroll
             for (int u = 0; u < LORA_WAVES; ++u) v += lds.sums[u][s][r];
-            if (part && 16 * i + s < it.count) part[(size_t)it.tokens[16 * i + s] * g.R + r0 + r] = v;
+            if (part && 16 * i + s < it.count) part[(size_t)to * g.R + r0 + r] = v;
           }
           put_terms(16 * i + s, r0 + r, v * c);
         }
@@ -684,10 +687,9 @@ struct Lora {
     }
   }
 
-  // tokens without an adapter among s0 .. s1 - 1, at most 64
-  __device__ __forceinline__ static void rest(const LoraArgs &g, int s0, int s1) {
-    const int lane = threadIdx.x & 63;
-    const int e = s0 + lane < s1 ? g.ids[s0 + lane] : 0;
+  // tokens without an adapter among the 64 from s0 on, e: this lane's id (any id behind the last token)
+  __device__ __forceinline__ static void rest(const LoraArgs &g, int s0, int e) {
+    constexpr int U = 8, STEP = 64 * LORA_WAVES;
     uint64_t todo = __ballot((unsigned)e >= (unsigned)g.n);
     while (todo) {
       const int k = __builtin_ctzll(todo);
@@ -695,10 +697,20 @@ struct Lora {
       const int64_t s = s0 + k;
       const bool none = __builtin_amdgcn_readlane(e, k) < 0;
       const float fill = none ? 0.f : __builtin_nanf("");
-      for (int64_t o = threadIdx.x; o < g.N; o += 64 * LORA_WAVES)
-        ((TY *)g.y)[s * g.ldy + o] = none && g.res ? ((const TY *)g.res)[s * g.ldr + o] : from_f32<TY>(fill);
+      for (int64_t o0 = threadIdx.x; o0 < g.N; o0 += U * STEP) {
+        TY v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = from_f32<TY>(fill);
+        if (none && g.res) {  // (all asked for before the first is waited for)
+#pragma unroll
+          for (int u = 0; u < U; ++u) v[u] = ((const TY *)g.res)[s * g.ldr + min(o0 + u * STEP, g.N - 1)];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (o0 + u * STEP < g.N) ((TY *)g.y)[s * g.ldy + o0 + u * STEP] = v[u];
+      }
       if (g.v)
-        for (int r = threadIdx.x; r < g.R; r += 64 * LORA_WAVES) g.v[(size_t)s * g.R + r] = fill;
+        for (int r = threadIdx.x; r < g.R; r += STEP) g.v[(size_t)s * g.R + r] = fill;
     }
   }
 };
@@ -706,14 +718,17 @@ template <class TX, class TW, bool KC, int NF, int RL, class TY>
 __global__ __launch_bounds__(64 * LORA_WAVES) void k_lora(LoraArgs g) {
   typedef Lora<TX, TW, KC, NF, RL, TY> L;
   __shared__ __attribute__((aligned(16))) typename L::Lds lds;
+  const int lane = threadIdx.x & 63;
+  const int64_t s0 = (int64_t)blockIdx.x * g.rest, s1 = min(s0 + g.rest, (int64_t)g.S);
+  auto id = [&](int64_t s) { return s + lane < s1 ? g.ids[s + lane] : 0; };
+  const int e = id(s0);  // (here already)
   LoraItem it;
   if (lora_item(g, blockIdx.x, it)) {
     if (it.count <= 16) L::template run<1>(g, it, lds);
     else L::template run<2>(g, it, lds);
   }
   if (g.phase == LoraArgs::LONG || blockIdx.y) return;
-  const int64_t s0 = (int64_t)blockIdx.x * g.rest, s1 = min(s0 + g.rest, (int64_t)g.S);
-  for (int64_t s = s0; s < s1; s += 64) L::rest(g, (int)s, (int)s1);
+  for (int64_t s = s0; s < s1; s += 64) L::rest(g, (int)s, s == s0 ? e : id(s));
 }
 
 // ============================================================ sums over an adapter's tokens
@@ -743,7 +758,7 @@ __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraIte
   const int z = (int)(b % g.slices), e = (int)(b / g.slices);
   const int count = items.counts[e], per = ((count + g.slices - 1) / g.slices + 31) & ~31;
   const int t0 = min(z * per, count), t1 = min(t0 + per, count);
-  const int32_t *tokens = items.tokens + (size_t)items.first[e] * items.T;
+  const int32_t *tokens = items.tokens + ((size_t)items.first[e] << items.n_items[1]);
   const float c = g.scale ? g.scale[e] : 1.f;
   v4f acc[NR][NF];
 #pragma unroll
@@ -759,7 +774,7 @@ __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraIte
     Words<float, NR> a[8];
     Words<TM, NF> m[8];
   };
-  // the 32 tokens at t (of those past t1 the last one's, which take no part)
+  // the 32 tokens at t (of those past t1, which take no part, the last one's)
   auto load = [&](Step &p, int t, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
     int s[8];
