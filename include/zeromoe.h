@@ -444,7 +444,8 @@ int zm_router_backward(const zm_router_spec *spec, const float *logits, const fl
  * token's request names its adapter; adapters of a smaller rank are filled up with zeros).  Types as
  * zm_linear's, the adapters in the place of w; y and residual F32 or of x's type; scale F32 [n] (NULL: 1).
  * e < 0: no adapter, y is the residual (zeros without one); e >= n: a NaN row.  v (optional, F32 [S][R])
- * receives x[s] . a[e]^T for the backward pass, 0 or NaN for those.  n <= 512, R <= 256, S < 2^24.  residual
+ * receives x[s] . a[e]^T for the backward pass, 0 or NaN for those.  n <= 512, R <= 256, S < 2^24, and an
+ * adapter's a and b lie within 2^31 bytes each.  residual
  * (optional) may be y itself, of y's stride.  Columns are contiguous, the other strides are in elements.
  * Among f32 operands an infinity may come out as a NaN of its row.  S may be 0. */
 typedef struct zm_lora_desc {

@@ -25,6 +25,10 @@ libzeromoe_hip.so (include/zeromoe.h):
   (unquantized matrix product with bias, activation and residual),
   :func:`layer_norm`, :func:`combine` (weighted sum of the experts' rows) and
   :func:`router_backward` (gradient of :func:`router`'s weights).
+* Fine-tuning over frozen experts and serving its result, with gradients:
+  :func:`glu` (both halves of a gated feed-forward block as one product),
+  :func:`lora` (a low-rank adapter named by each token) and
+  :func:`clip_grad_norm` / :func:`grad_norm` (the gradients of a whole step).
 
 Torch is used only for device memory and the current stream.
 """
