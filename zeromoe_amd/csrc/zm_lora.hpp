@@ -52,7 +52,7 @@ struct LoraArgs {
   const void *res;        // [S][ldr] or null
   void *y;
   int64_t ldr, ldy;
-  int rest;               // tokens that a workgroup looks through for those without an adapter
+  int rest;               // tokens that a workgroup looks through for those without an adapter, at most 32
   // both axes in one launch, or (few items) each in its own, the long one in slices of k, the short one in groups of columns
   enum { BOTH, LONG, SHORT };
   int phase, slices;
@@ -719,16 +719,15 @@ __global__ __launch_bounds__(64 * LORA_WAVES) void k_lora(LoraArgs g) {
   typedef Lora<TX, TW, KC, NF, RL, TY> L;
   __shared__ __attribute__((aligned(16))) typename L::Lds lds;
   const int lane = threadIdx.x & 63;
-  const int64_t s0 = (int64_t)blockIdx.x * g.rest, s1 = min(s0 + g.rest, (int64_t)g.S);
-  auto id = [&](int64_t s) { return s + lane < s1 ? g.ids[s + lane] : 0; };
-  const int e = id(s0);  // (here already)
+  const int s0 = min((int)blockIdx.x * g.rest, g.S), s = s0 + lane;
+  const int e = lane < g.rest && s < g.S ? g.ids[s] : 0;  // (asked for here already)
   LoraItem it;
   if (lora_item(g, blockIdx.x, it)) {
     if (it.count <= 16) L::template run<1>(g, it, lds);
     else L::template run<2>(g, it, lds);
   }
   if (g.phase == LoraArgs::LONG || blockIdx.y) return;
-  for (int64_t s = s0; s < s1; s += 64) L::rest(g, (int)s, s == s0 ? e : id(s));
+  L::rest(g, s0, e);
 }
 
 // ============================================================ sums over an adapter's tokens
