@@ -758,7 +758,8 @@ __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraIte
   const int count = items.counts[e], per = ((count + g.slices - 1) / g.slices + 31) & ~31;
   const int t0 = min(z * per, count), t1 = min(t0 + per, count);
   const int32_t *tokens = items.tokens + ((size_t)items.first[e] << items.n_items[1]);
-  const float c = g.scale ? g.scale[e] : 1.f;
+  // (the scale of an adapter without tokens may be no number: its sums are zero all the same)
+  const float c = g.scale && count ? g.scale[e] : 1.f;
   v4f acc[NR][NF];
 #pragma unroll
   for (int h = 0; h < NR; ++h)
