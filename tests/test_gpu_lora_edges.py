@@ -1,11 +1,12 @@
-"""Adapters at the edges of their formula: scales of adapters that no token names."""
+"""Adapters at the edges of their formula: scales of adapters that no token names, and the backward pass of few tokens whose
+long axis is shared by several workgroups.  Tolerances as in test_gpu_lora."""
 import math
 
 import pytest
 import torch
 
-from test_gpu_dense import TYPES, rand
-from test_gpu_lora import adapters, some_ids
+from test_gpu_dense import PAIRS, TYPES, rand
+from test_gpu_lora import adapters, check_backward, some_ids
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +31,16 @@ def test_scale_of_an_adapter_without_tokens(S, I, O, R, xt, wt):
         assert torch.equal(g, w)
     for g in got[2:]:
         assert (g[[0, 2, 4]] == 0).all()
+
+
+# O of several slices in the backward pass, ranks of each kind of kernel, odd sizes
+SPLIT = [(1, 520, 8200, 128, 3), (63, 300, 8192, 65, 1), (40, 260, 4099, 200, 3), (5, 1030, 4608, 30, 2), (2, 2100, 8191, 16, 1),
+         (100, 131, 5121, 100, 4)]
+
+
+@pytest.mark.parametrize("xt,wt", PAIRS)
+@pytest.mark.parametrize("S,I,O,R,n", SPLIT)
+def test_backward_of_few_tokens_and_a_long_axis(S, I, O, R, n, xt, wt):
+    for need in ((True, True, True), (True, False, False), (False, True, False)):
+        check_backward(S, I, O, R, n, xt, wt, need=need)
+    check_backward(S, I, O, R, n, xt, wt, "one", ydt="f32", seed=21)
