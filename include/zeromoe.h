@@ -447,7 +447,7 @@ int zm_router_backward(const zm_router_spec *spec, const float *logits, const fl
  * receives x[s] . a[e]^T for the backward pass, 0 or NaN for those.  n <= 512, R <= 256, S < 2^24, and an
  * adapter's a and b lie within 2^31 bytes each.  residual
  * (optional) may be y itself, of y's stride.  Columns are contiguous, the other strides are in elements.
- * Among f32 operands an infinity may come out as a NaN of its row.  S may be 0. */
+ * Sums and infinities as zm_linear's: by the formula, whatever the number of tokens.  S may be 0. */
 typedef struct zm_lora_desc {
   int32_t x_type, w_type, y_type; /* y_type: of y, residual and dy */
   int32_t n, R;

@@ -1,5 +1,5 @@
-"""Adapters at the edges of their formula: scales of adapters that no token names, and the backward pass of few tokens whose
-long axis is shared by several workgroups.  Tolerances as in test_gpu_lora."""
+"""Adapters where the formula leaves the ordinary: infinities, scales of adapters that no token names, and the backward pass
+of few tokens whose long axis is shared by several workgroups.  Tolerances as in test_gpu_lora."""
 import math
 
 import pytest
@@ -44,3 +44,100 @@ def test_backward_of_few_tokens_and_a_long_axis(S, I, O, R, n, xt, wt):
     for need in ((True, True, True), (True, False, False), (False, True, False)):
         check_backward(S, I, O, R, n, xt, wt, need=need)
     check_backward(S, I, O, R, n, xt, wt, "one", ydt="f32", seed=21)
+
+
+def same_as(got, want, ok, what):
+    """An infinity for an infinity, a NaN for a NaN, a finite value for a finite one, wherever the signs are sure."""
+    inf = want.isinf() & ok
+    assert torch.equal(got.isnan() & ok, want.isnan() & ok) and torch.equal(got.isinf() & ok, inf), what
+    assert torch.equal(got.double()[inf], want[inf]), what
+
+
+def by_definition(p, p_ok, q):
+    """p (S, K) times q (J, K)^T in 64 bits, each product formed (an infinity times zero is a NaN), and where its sign is
+    sure: not where the sum is within 1e-4 of its terms from zero (f32 sums are off by far less), nor where such a p meets
+    an infinity of q.  Signs matter only where an infinity follows."""
+    few = max(1, (1 << 26) // p.numel())
+    y, size = (torch.cat([f(p[:, None] * c[None]).sum(-1) for c in q.split(few)], 1) for f in (lambda t: t, torch.abs))
+    unsure = ((~p_ok).double() @ q.isinf().double().t().contiguous()) > 0
+    return y, ~unsure & (~y.isfinite() | (y.abs() > 1e-4 * size)), ~unsure
+
+
+# tokens, widths and ranks of the kernel of few tokens, of the items, and of items whose axes are launches of their own
+KINDS = [(12, 264, 72, 1), (12, 264, 300, 9), (12, 8200, 72, 72), (12, 8193, 40, 130), (5000, 260, 72, 1), (5000, 136, 100, 24),
+         (4500, 96, 130, 50), (4300, 72, 65, 100), (40, 9000, 260, 128), (300, 4100, 257, 33)]
+
+
+def unusual(S, I, O, R, xt, wt):
+    """Four adapters; infinities in x, a, b and the scale, each reaching tokens of its own among the first twelve."""
+    a, b = adapters(4, R, I, O, wt)
+    x = rand(S, I, seed=3, dtype=TYPES[xt])
+    ids = torch.arange(S, device="cuda").remainder(4).to(torch.int32)
+    scale = torch.tensor([1.5, -0.5, 2.0, 1.0], device="cuda")
+    b[:] = b.abs() + 0.01
+    a[0, :, 5] = a[0, :, 5].abs() + 0.01  # x: infinities of one sign in v
+    x[0, 5], x[4, 5] = math.inf, -math.inf
+    x[8, 7] = math.inf                    # of both
+    a[1, R // 2, 9] = math.inf            # one adapter's v by the sign of x
+    x[5, 9] = 0.0                         # (and zero times it)
+    b[2, 3, R - 1] = -math.inf            # one adapter's column
+    scale[3] = math.inf                   # one adapter's rows
+    return x, a, b, ids, scale
+
+
+@pytest.mark.parametrize("xt,wt", PAIRS)
+@pytest.mark.parametrize("S,I,O,R", KINDS)
+def test_infinities_go_by_the_formula(S, I, O, R, xt, wt):
+    import zeromoe_amd as Z
+
+    x, a, b, ids, scale = unusual(S, I, O, R, xt, wt)
+    res = rand(S, O, seed=8, dtype=TYPES[xt])
+    res[7, 1] = -math.inf
+    y, v = Z.lora(x, a, b, ids, scale=scale, residual=res, save=True)
+    for e in range(4):
+        at = (ids == e).nonzero()[:, 0]
+        v64, v_ok, ok = by_definition(x[at].double(), torch.ones(len(at), I, device="cuda", dtype=torch.bool), a[e].double())
+        same_as(v[at], v64, ok, ("v", e))
+        y64, y_ok, ok = by_definition(v64, v_ok, b[e].double())
+        same_as(y[at], y64 * scale[e].double() + res[at].double(), ok if scale[e].isfinite() else y_ok, ("y", e))
+
+
+@pytest.mark.parametrize("S,I,O,R", KINDS)
+def test_one_token_and_many_agree_on_infinities(S, I, O, R):
+    """The same rows alone: infinities and NaN in the same places."""
+    import zeromoe_amd as Z
+
+    x, a, b, ids, scale = unusual(S, I, O, R, "bf16", "bf16")
+    y = Z.lora(x, a, b, ids, scale=scale)
+    for s in range(12):
+        one = Z.lora(x[s:s + 1], a, b, ids[s:s + 1], scale=scale)[0]
+        same_as(one, y[s].double(), torch.ones_like(one, dtype=torch.bool), s)
+
+
+@pytest.mark.parametrize("xt,wt", PAIRS)
+@pytest.mark.parametrize("S,I,O,R", [(12, 264, 72, 1), (12, 264, 300, 9), (12, 72, 8200, 72), (5000, 130, 96, 1),
+                                     (5000, 100, 136, 24), (4500, 130, 72, 50), (40, 260, 4100, 128), (1030, 64, 33, 100)])
+def test_gradients_of_infinities_go_by_the_formula(S, I, O, R, xt, wt):
+    import zeromoe_amd as Z
+
+    a, b = adapters(4, R, I, O, wt)
+    x, dy, v = rand(S, I, seed=3, dtype=TYPES[xt]), rand(S, O, seed=4, dtype=TYPES[xt]), rand(S, R, seed=5)
+    ids = torch.arange(S, device="cuda").remainder(4).to(torch.int32)
+    scale = torch.tensor([1.5, -0.5, 2.0, math.inf], device="cuda")
+    a[0] = a[0].abs() + 0.01
+    b[0, 5] = b[0, 5].abs() + 0.01
+    dy[4, 5] = math.inf            # u of one token, all of its dx, da of the adapter
+    x[1, 3] = -math.inf            # one column of da
+    v[5, R // 2] = math.inf        # one column of db
+    b[2, 7, R - 1] = math.inf      # one r of u
+    dx, da, db = Z.lora_backward(dy, x, a, b, ids, v, scale=scale)
+    for e in range(4):
+        at, c = (ids == e).nonzero()[:, 0], scale[e].double()
+        d, xe, ve = dy[at].double(), x[at].double(), v[at].double()
+        sure = torch.ones(len(at), O, device="cuda", dtype=torch.bool)
+        u, u_ok, _ = by_definition(d, sure, b[e].double().t().contiguous())
+        t = lambda m: m.t().contiguous()  # noqa: E731
+        for name, got, (want, last, ok) in (("dx", dx[at], by_definition(u, u_ok, t(a[e].double()))),
+                                            ("da", da[e], by_definition(t(u), t(u_ok), t(xe))),
+                                            ("db", db[e], by_definition(t(d), t(sure), t(ve)))):
+            same_as(got, want * c, ok if c.isfinite() else last, (name, e))

@@ -172,9 +172,15 @@ constexpr int64_t BUF_ROW = 1 << 23;  // bytes of a row, less than: 256 rows of 
 // workgroup takes 16 packs of V columns; its 16 groups of 16 threads take every 16th part, eight loads in flight, and
 // their sums meet in LDS, all in a fixed order.  512 parts of 14336 columns (29 MB): 9 us, against 123 us with a
 // thread per column going through all parts.
+struct PartsScale {  // group k of `each` columns times scale[k] where counts[k] is not 0; null: none
+  const float *scale = nullptr;
+  const int32_t *counts = nullptr;
+  int64_t each = 1;
+};
 template <int V>
 static __global__ __launch_bounds__(256) void k_parts_sum(const float *__restrict__ part, int parts, int64_t n, int64_t n0,
-                                                          float *__restrict__ dst0, float *__restrict__ dst1) {
+                                                          float *__restrict__ dst0, float *__restrict__ dst1,
+                                                          PartsScale by) {
   __shared__ float red[16][16 * V];
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
   const int64_t i = ((int64_t)blockIdx.x * 16 + c) * V;
@@ -207,16 +213,19 @@ static __global__ __launch_bounds__(256) void k_parts_sum(const float *__restric
     float a = 0.f;
 #pragma unroll
     for (int q = 0; q < 16; ++q) a += red[q][j];
+    if (by.scale && by.counts[k / by.each]) a *= by.scale[k / by.each];
     float *dst = k < n0 ? dst0 : dst1;
     if (dst) dst[k < n0 ? k : k - n0] = a;
   }
 }
 static inline void parts_sum(const float *part, int parts, int64_t n, int64_t n0, float *dst0, float *dst1,
-                             hipStream_t st) {
+                             hipStream_t st, const PartsScale &by = {}) {
   if (!(n & 3) && !((uintptr_t)part & 15))
-    hipLaunchKernelGGL((k_parts_sum<4>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, part, parts, n, n0, dst0, dst1);
+    hipLaunchKernelGGL((k_parts_sum<4>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, part, parts, n, n0, dst0, dst1,
+                       by);
   else
-    hipLaunchKernelGGL((k_parts_sum<1>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, part, parts, n, n0, dst0, dst1);
+    hipLaunchKernelGGL((k_parts_sum<1>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, part, parts, n, n0, dst0, dst1,
+                       by);
 }
 
 // ============================================================ two weights

@@ -144,9 +144,9 @@ LoraSumArgs sums_args(const zm_lora_desc &d, const float *a, const void *m, int6
   return g;
 }
 unsigned sums_groups(const LoraSumArgs &g) { return (unsigned)((g.N + 63) / 64 * g.chunks * g.slices * g.n); }
-void join_sums(const LoraSumArgs &g, float *dst, hipStream_t st) {
+void join_sums(const LoraSumArgs &g, const LoraItems &it, float *dst, hipStream_t st) {
   const int64_t all = (int64_t)g.n * g.R * g.N;
-  if (g.slices > 1) parts_sum(g.out, g.slices, all, all, dst, nullptr, st);
+  if (g.slices > 1) parts_sum(g.out, g.slices, all, all, dst, nullptr, st, {g.scale, it.counts, g.R * g.N});
 }
 
 int check_space(void *ws, size_t size, size_t need, const char *who) {
@@ -242,8 +242,8 @@ int zm_lora_backward(const zm_lora_desc *d, const void *dy, const void *x, const
     const LoraSumArgs ga = sums_args(*d, u, x, d->x_stride, d->I, scale, da, sa);
     const LoraSumArgs gb = sums_args(*d, v, dy, d->y_stride, d->O, scale, db, sb);
     lora_sums(d->x_type, d->y_type, g.it, ga, da ? sums_groups(ga) : 0, gb, db ? sums_groups(gb) : 0, st);
-    if (da) join_sums(ga, da, st);
-    if (db) join_sums(gb, db, st);
+    if (da) join_sums(ga, g.it, da, st);
+    if (db) join_sums(gb, g.it, db, st);
   }
   return launched();
 }

@@ -291,6 +291,10 @@ constexpr int terms_beside() {
 //
 // Every workgroup also looks through g.rest tokens for those without an adapter: their rows are the residual (or zeros),
 // and NaN where the id names none.  (Workgroups of their own waited for a CU behind the items: 68.6 us for 65.)
+//
+// Sums of terms have NaN where the formula may have an infinity (zm_linear.hpp, lin_again).  A value of v or of the result
+// that is not finite is taken again value by value in f32, so that what an infinity gives does not go by the number of
+// tokens; v stays without the scale, which multiplies the sums, as k_lora_few has it.
 constexpr int LORA_WAVES = 8;
 
 // ROWS rows of PIECES x 16 bytes by way of registers into LDS, rows 128 bytes apart, their pieces permuted so that 16 rows
@@ -444,16 +448,49 @@ struct Lora {
     }
   }
 
+  // v of a token again
+  __device__ __forceinline__ static float long_again(const LoraArgs &g, const LoraItem &it, int64_t token, int r) {
+    const TX *x = (const TX *)g.x + token * g.ldx;
+    const int64_t step = KC ? 1 : g.ldm;
+    const TW *m = (const TW *)g.m + it.e * g.m_adapter + (KC ? r * g.ldm : r);
+    float v = 0.f;
+    for (int64_t k = 0; k < g.K && v == v; k += 4) {
+      float a[4], b[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        a[u] = k + u < g.K ? to_f32(x[k + u]) : 0.f;
+        b[u] = k + u < g.K ? to_f32(m[(k + u) * step]) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v = __builtin_fmaf(a[u], b[u], v);
+    }
+    return v;
+  }
+  // the sum of the item's token s in column o again, without the scale
+  __device__ __forceinline__ static float short_again(const LoraArgs &g, const LoraItem &it, const Lds &lds, int s, int64_t o) {
+    const int64_t step = KC ? 1 : g.ldl;
+    const TW *l = (const TW *)g.l + it.e * g.l_adapter + (KC ? o * g.ldl : o);
+    float sum = 0.f;
+    for (int r = 0; r < g.R && sum == sum; ++r) {
+      float t[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) t[k] = to_f32(bf16{lds.terms[k][s][r]});
+      sum = __builtin_fmaf(t[0] + (t[1] + t[2]), to_f32(l[r * step]), sum);  // (the terms' sum is v, in every bit)
+    }
+    return sum;
+  }
+
   template <int MT>
   __device__ __forceinline__ static void run(const LoraArgs &g, const LoraItem &it, Lds &lds) {
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), fr = lane & 15, fc = lane >> 4;
     const float c = g.scale ? g.scale[it.e] : 1.f;
-    auto put_terms = [&](int s, int r, float v) {
+    auto put_terms = [&](int s, int r, float v) {  // (an infinity or a NaN is the first one, zeros follow)
+      const bool number = lin_finite(v);
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
-        const bf16 e = from_f32<bf16>(k ? v : __builtin_amdgcn_fmed3f(v, -BF16_MOST, BF16_MOST));
+        const bf16 e = from_f32<bf16>(k || !number ? v : __builtin_amdgcn_fmed3f(v, -BF16_MOST, BF16_MOST));
         lds.terms[k][s][r] = e.u;
-        v -= to_f32(e);
+        v = number ? v - to_f32(e) : 0.f;
       }
     };
     if (g.phase == LoraArgs::SHORT) {
@@ -462,14 +499,16 @@ struct Lora {
         const int s = t / RP, r = t - s * RP;
         float v = 0.f;
         if (s < it.count && r < g.R) {
-          const size_t at = (size_t)g.it.tokens[((size_t)blockIdx.x << g.it.n_items[1]) + s] * g.R + r;
+          const int token = g.it.tokens[((size_t)blockIdx.x << g.it.n_items[1]) + s];
+          const size_t at = (size_t)token * g.R + r;
           for (int z = 0; z < g.slices; ++z) v += g.part[(size_t)z * g.S * g.R + at];
+          if (NX * NM > 1 && !lin_finite(v)) v = long_again(g, it, token, r);
           if (g.v && !blockIdx.y) g.v[at] = v;
         }
-        put_terms(s, r, v * c);
+        put_terms(s, r, v);
       }
       __syncthreads();
-      return short_axis<MT>(g, it, lds);
+      return short_axis<MT>(g, it, c, lds);
     }
     const int64_t k0 = g.phase == LoraArgs::LONG ? blockIdx.y * g.kslice : 0;
     const int64_t k1 = g.phase == LoraArgs::LONG ? min(g.K, k0 + g.kslice) : g.K;
@@ -493,23 +532,24 @@ struct Lora {
         constexpr int WIDE = NR < 32 ? 32 : NR;  // (zeros up to the 32 of a matrix instruction)
         for (int t = threadIdx.x; t < 16 * WIDE; t += 64 * LORA_WAVES) {
           const int s = t / WIDE, r = t % WIDE;
-          const int64_t to = part ? it.token(16 * i + s) : 0;  // (by all lanes of the wave)
+          const int64_t to = part || NX * NM > 1 ? it.token(16 * i + s) : 0;  // (by all lanes of the wave)
           float v = 0.f;
           if (r < NR && r0 + r < g.R) {
 #pragma unroll
             for (int u = 0; u < LORA_WAVES; ++u) v += lds.sums[u][s][r];
+            if (NX * NM > 1 && g.phase == LoraArgs::BOTH && !lin_finite(v)) v = long_again(g, it, to, r0 + r);
             if (part && 16 * i + s < it.count) part[(size_t)to * g.R + r0 + r] = v;
           }
-          put_terms(16 * i + s, r0 + r, v * c);
+          put_terms(16 * i + s, r0 + r, v);
         }
       }
       __syncthreads();
     }
-    if (g.phase == LoraArgs::BOTH) short_axis<MT>(g, it, lds);
+    if (g.phase == LoraArgs::BOTH) short_axis<MT>(g, it, c, lds);
   }
 
   template <int MT>
-  __device__ __forceinline__ static void short_axis(const LoraArgs &g, const LoraItem &it, Lds &lds) {
+  __device__ __forceinline__ static void short_axis(const LoraArgs &g, const LoraItem &it, float c, Lds &lds) {
     const int STEP = 64 * LORA_WAVES * gridDim.y;  // (groups of columns)
     constexpr bool STAGED = KC && RL > 32;                   // (shorter rows of L are several to a line)
     constexpr int RS = STAGED ? 128 / (int)sizeof(TW) : 32;  // r of a step
@@ -638,8 +678,11 @@ struct Lora {
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         if (16 * i >= it.count) break;
+        float most = 0.f;
 #pragma unroll
         for (int h = 0; h < C; ++h) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) most += fabsf(acc[i][h][q]);
           if constexpr (KC) {
             *reinterpret_cast<v4f *>(rows + fr * 68 + 16 * h + 4 * fc) = acc[i][h];
           } else {
@@ -648,6 +691,14 @@ struct Lora {
           }
         }
         stage_sync();
+        if (__ballot(!lin_finite(most))) {
+#pragma unroll 1
+          for (int s = 0; s < 16 && 16 * i + s < it.count; ++s) {
+            float &at = rows[s * 68 + lane];
+            if (o0 + lane < g.N && !lin_finite(at)) at = short_again(g, it, lds, 16 * i + s, o0 + lane);
+          }
+          stage_sync();
+        }
 #pragma unroll
         for (int q = 0; q < OUT; ++q) {
           const int s = out_row(i, q);
@@ -656,7 +707,7 @@ struct Lora {
           for (int j = 0; j < VY; j += 4) {
             const v4f v = *reinterpret_cast<const v4f *>(rows + (s - 16 * i) * 68 + yc + j);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) f[j + k] = g.res ? now.z[i][q].get(j + k) + v[k] : v[k];
+            for (int k = 0; k < 4; ++k) f[j + k] = g.res ? __builtin_fmaf(c, v[k], now.z[i][q].get(j + k)) : c * v[k];
           }
           if (s >= it.count) continue;
           TY *at = (TY *)g.y + token[i][q] * g.ldy + o0 + yc;
@@ -758,8 +809,9 @@ __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraIte
   const int count = items.counts[e], per = ((count + g.slices - 1) / g.slices + 31) & ~31;
   const int t0 = min(z * per, count), t1 = min(t0 + per, count);
   const int32_t *tokens = items.tokens + ((size_t)items.first[e] << items.n_items[1]);
-  // (the scale of an adapter without tokens may be no number: its sums are zero all the same)
-  const float c = g.scale && count ? g.scale[e] : 1.f;
+  // (the scale of an adapter without tokens may be no number: its sums are zero all the same; slices are joined before it;
+  // asked for beside the count)
+  const float by = g.scale && g.slices == 1 ? g.scale[e] : 1.f, c = count ? by : 1.f;
   v4f acc[NR][NF];
 #pragma unroll
   for (int h = 0; h < NR; ++h)
@@ -832,17 +884,33 @@ __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraIte
     __syncthreads();
     // value (f, lane, q): index 4 fc + q of the operand that gives the rows, fr of the other; neighbours of the result
     // go to neighbouring threads
-    for (int t = threadIdx.x; t < NF * 256; t += 64 * LORA_WAVES) {
+    auto result = [&](int t, auto again) {  // whether it is finite
       const int jr = BY_R ? t >> 4 : t & 63, ri = BY_R ? t & 15 : t >> 6;  // j - j0, and r = r0 + NR ri + h
       const int f = jr & 3, row = BY_R ? ri : jr >> 2, col = BY_R ? jr >> 2 : ri;
       const int k = 64 * (row & 3) + 16 * (row >> 2) + col;
       const int64_t jj = j0 + jr;
       const int rr = r0 + NR * ri + h;
-      if (jj >= g.N || rr >= g.R) continue;
+      if (jj >= g.N || rr >= g.R) return true;
       float v = 0.f;
 #pragma unroll
       for (int u = 0; u < LORA_WAVES; ++u) v += red[u][f][k];
+      const bool finite = lin_finite(v);
+      if (decltype(again)::value) {
+        if (finite) return true;
+        v = 0.f;
+        for (int t = t0; t < t1 && v == v; ++t) {
+          const int64_t s = tokens[t];
+          v = __builtin_fmaf(g.a[s * g.R + rr], to_f32(((const TM *)g.m)[s * g.ldm + jj]), v);
+        }
+      }
       out[BY_R ? (size_t)jj * g.R + rr : (size_t)rr * g.N + jj] = c * v;
+      return finite;
+    };
+    bool finite = true;
+    for (int t = threadIdx.x; t < NF * 256; t += 64 * LORA_WAVES) finite &= result(t, std::false_type());
+    if (__ballot(!finite)) {  // those that are not, value by value, as in the products
+#pragma unroll 1
+      for (int t = threadIdx.x; t < NF * 256; t += 64 * LORA_WAVES) result(t, std::true_type());
     }
   }
 }
