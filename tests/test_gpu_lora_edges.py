@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_dense import PAIRS, TYPES, rand
+from test_gpu_dense import PAIRS, TYPES, U, rand
 from test_gpu_lora import adapters, check_backward, some_ids
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +141,29 @@ def test_gradients_of_infinities_go_by_the_formula(S, I, O, R, xt, wt):
                                             ("da", da[e], by_definition(t(u), t(u_ok), t(xe))),
                                             ("db", db[e], by_definition(t(d), t(sure), t(ve)))):
             same_as(got, want * c, ok if c.isfinite() else last, (name, e))
+
+
+def test_gradients_of_the_widest_rows():
+    """An adapter of 2^29 columns: its gradient takes more workgroups than one launch has."""
+    import zeromoe_amd as Z
+
+    I, O = (1 << 29) + 70, 40
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    a = torch.randn((1, 1, I), device="cuda", generator=g, dtype=torch.bfloat16)
+    x = torch.randn((2, I), device="cuda", generator=g, dtype=torch.bfloat16)
+    b, dy, v = rand(1, O, 1, seed=2, dtype=torch.bfloat16), rand(2, O, seed=3, dtype=torch.bfloat16), rand(2, 1, seed=4)
+    ids, scale = torch.tensor([-1, 0], device="cuda", dtype=torch.int32), torch.tensor([0.5], device="cuda")
+    dx, da, db = Z.lora_backward(dy, x, a, b, ids, v, scale=scale)
+    u = (dy[1].double() @ b[0, :, 0].double()).item()
+    # u in f32: O products, as in test_gpu_lora; one product with it, the scale, and the rounding of the result
+    tu = U * (4 + 2 * math.sqrt(O)) * (dy[1].double().abs() @ b[0, :, 0].double().abs()).item()
+    assert not dx[0].any()
+    for at in range(0, I, 1 << 26):
+        k = slice(at, min(at + (1 << 26), I))
+        for got, m, step in ((da[0, 0, k], x[1, k], U), (dx[1, k], a[0, 0, k], 2.0 ** -8)):
+            want = 0.5 * u * m.double()
+            tol = 0.5 * tu * m.double().abs() + (step + 4 * U) * want.abs() + 1e-37
+            assert ((got.double() - want).abs() <= tol).all()
+    want = 0.5 * dy[1].double() * v[1].double()
+    assert ((db[0, :, 0].double() - want).abs() <= 4 * U * want.abs() + 1e-37).all()

@@ -914,12 +914,14 @@ __device__ __forceinline__ void lora_sums_wg(const LoraSumArgs &g, const LoraIte
     }
   }
 }
-// dA by the first `na` workgroups, dB by the others: what they wait for is the same
+// dA by the first `na` workgroups, dB by the others: what they wait for is the same.  `first`: of this launch
 template <class TX, class TY, int NR>
-__global__ __launch_bounds__(64 * LORA_WAVES) void k_lora_sums(LoraItems items, LoraSumArgs a, LoraSumArgs b, unsigned na) {
+__global__ __launch_bounds__(64 * LORA_WAVES) void k_lora_sums(LoraItems items, LoraSumArgs a, LoraSumArgs b, unsigned na,
+                                                               unsigned first) {
   __shared__ float red[LORA_WAVES][4][256];
-  if (blockIdx.x < na) lora_sums_wg<TX, NR, false>(a, items, blockIdx.x, red);
-  else lora_sums_wg<TY, NR, true>(b, items, blockIdx.x - na, red);
+  const unsigned wg = first + blockIdx.x;
+  if (wg < na) lora_sums_wg<TX, NR, false>(a, items, wg, red);
+  else lora_sums_wg<TY, NR, true>(b, items, wg - na, red);
 }
 
 // ============================================================ few tokens

@@ -1,6 +1,8 @@
 // zm_lora_b.hip -- adapters: the sums over an adapter's tokens, and a few tokens at once
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "zm_lora.hpp"
 
 namespace zm {
@@ -8,11 +10,15 @@ namespace {
 
 template <class TX, class TY>
 void sums(const LoraItems &items, const LoraSumArgs &a, unsigned na, const LoraSumArgs &b, unsigned nb, hipStream_t st) {
-  const dim3 grid(na + nb), wg(64 * LORA_WAVES);
-  switch (lora_r_of(a.R)) {
-  case 16: hipLaunchKernelGGL((k_lora_sums<TX, TY, 1>), grid, wg, 0, st, items, a, b, na); break;
-  case 32: hipLaunchKernelGGL((k_lora_sums<TX, TY, 2>), grid, wg, 0, st, items, a, b, na); break;
-  default: hipLaunchKernelGGL((k_lora_sums<TX, TY, 4>), grid, wg, 0, st, items, a, b, na);
+  // (2^22 workgroups at a time: a launch has less than 2^32 threads)
+  constexpr unsigned MOST = 1u << 22;
+  for (unsigned first = 0; first < na + nb; first += MOST) {
+    const dim3 grid(std::min(MOST, na + nb - first)), wg(64 * LORA_WAVES);
+    switch (lora_r_of(a.R)) {
+    case 16: hipLaunchKernelGGL((k_lora_sums<TX, TY, 1>), grid, wg, 0, st, items, a, b, na, first); break;
+    case 32: hipLaunchKernelGGL((k_lora_sums<TX, TY, 2>), grid, wg, 0, st, items, a, b, na, first); break;
+    default: hipLaunchKernelGGL((k_lora_sums<TX, TY, 4>), grid, wg, 0, st, items, a, b, na, first);
+    }
   }
 }
 template <class TX, class TW>
