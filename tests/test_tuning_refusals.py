@@ -102,6 +102,17 @@ def test_lora_descriptions(change, why):
     assert L.zm_lora_workspace_size(d) == 0 and L.zm_lora_backward_workspace_size(d) == 0
 
 
+@pytest.mark.parametrize("change", [dict(R=5, a_stride=1 << 62), dict(O=33, b_stride=1 << 59), dict(R=3, a_stride=(1 << 63) - 1)])
+def test_lora_strides_whose_extent_passes_64_bits(change):
+    d, L = lora_desc(**change), lib()
+    assert L.zm_lora_workspace_size(d) == 0 and "below 2^31 bytes" in error()
+    assert L.zm_lora_backward_workspace_size(d) == 0 and "below 2^31 bytes" in error()
+    assert L.zm_lora(d, P, P, P, P, None, None, P, None, P, 1 << 40, None) == -1 and "below 2^31 bytes" in error()
+    assert L.zm_lora_backward(d, P, P, P, P, P, None, P, P, P, P, P, 1 << 40, None) == -1 and "below 2^31 bytes" in error()
+    one = lora_desc(R=1, a_stride=1 << 62, a_adapter=64, S=20000)  # (a single row has no stride)
+    assert L.zm_lora_workspace_size(one) > 0
+
+
 def test_lora_pointers_strides_and_workspace():
     L = lib()
     assert L.zm_lora(None, P, P, P, P, None, None, P, None, P, 0, None) == -1 and "null" in error()

@@ -25,7 +25,10 @@ int check_lora(const zm_lora_desc *d, const char *who) {
       d->b_adapter < 0)
     return fail("%s: negative stride", who);
   const int64_t most = ((int64_t)1 << 31) / (int64_t)size_of(d->w_type);
-  if ((d->R - 1) * d->a_stride + d->I >= most || (d->O - 1) * d->b_stride + d->R >= most)
+  auto large = [&](int64_t rows, int64_t stride, int64_t width) {  // (a stride that large first: the product may pass 64 bits)
+    return rows > 1 && (stride >= most || (rows - 1) * stride + width >= most);
+  };
+  if (d->I >= most || large(d->R, d->a_stride, d->I) || large(d->O, d->b_stride, d->R))
     return fail("%s: an adapter's a and b are below 2^31 bytes", who);
   if ((std::max(d->I, d->O) / 64 + 1) * ((d->R + 15) / 16) * d->n >= 1 << 26) return fail("%s: n x R x I or n x R x O too large", who);
   return 0;
