@@ -81,8 +81,10 @@ __global__ __launch_bounds__(256) void k_glu_factors(FactorArgs g) {
         v4f dg = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          dg[j] = d[k][j] * u[k][j] * lin_act_slope(z[k][j], g.act);
-          du[j] = d[k][j] * factor_act(z[k][j], g.act);
+          float a, slope;
+          factor_and_slope(z[k][j], g.act, a, slope);
+          dg[j] = d[k][j] * u[k][j] * slope;
+          du[j] = d[k][j] * a;
           sg[j] += dg[j];
           su[j] += du[j];
         }
