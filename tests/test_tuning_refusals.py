@@ -183,6 +183,15 @@ def test_clip_refusals():
         assert clip(ok, 2, ws=ws, size=size) == -1 and "workspace" in error()
 
 
+def test_norm_in_the_place_of_a_gradient():
+    L = lib()
+    size = L.zm_grad_norm_workspace_size(2)
+    for g in ((P, P, 10, F32, F32), (P, 65536, 10, F32, F32), (65536, P, 10, F32, F32), (P, 65536, 20, BF16, BF16)):
+        for norm in (P - 3, P, P + 36, P + 39):
+            assert L.zm_grad_clip(grads((8192, 8192, 5, F32, F32), g), 2, 1.0, 1e-6, norm, 1 << 20, size, None) == -1
+            assert "norm overlaps" in error()
+
+
 def test_wrappers_refuse_host_tensors():
     x, a = torch.zeros(2, 4), torch.zeros(1, 2, 4)
     ids = torch.zeros(2, dtype=torch.int32)

@@ -256,6 +256,16 @@ int check_overlap(const zm_grad *g, int64_t count, const char *who) {
   return 0;
 }
 
+// the norm is written while gradients are still read
+int check_norm(const zm_grad *g, int64_t count, const float *norm, const char *who) {
+  const uintptr_t at = (uintptr_t)norm;
+  auto overlaps = [&](const void *p, size_t bytes) { return at < (uintptr_t)p + bytes && (uintptr_t)p < at + sizeof(float); };
+  for (int64_t i = 0; norm && i < count; ++i)
+    if (g[i].n && (overlaps(g[i].data, g[i].n * size_of(g[i].type)) || overlaps(g[i].out, g[i].n * size_of(g[i].out_type))))
+      return fail("%s: norm overlaps gradient %lld or its result", who, (long long)i);
+  return 0;
+}
+
 // the workgroups of each launch, by its share of all units
 int groups_of(int64_t units, int64_t all) {
   return (int)std::min<int64_t>(units, units * MOST_GROUPS / std::max<int64_t>(all, 1) + 1);
@@ -321,6 +331,7 @@ int zm_grad_clip(const zm_grad *g, int64_t count, double max_norm, double eps, f
     return fail("zm_grad_clip: max_norm >= 0 and a finite eps >= 0 are needed");
   if (check_overlap(g, count, "zm_grad_clip")) return -1;
   if (check_space(workspace, workspace_size, count, "zm_grad_clip")) return -1;
+  if (check_norm(g, count, norm, "zm_grad_clip")) return -1;
   const hipStream_t st = (hipStream_t)stream;
   double *part = (double *)workspace;
   const int64_t all = all_units(g, count);
