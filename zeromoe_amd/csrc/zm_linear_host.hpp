@@ -65,8 +65,10 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, 
       };
       // 16-bit operands: a tile alone on its CU starts and ends with nothing beside it, two of 128 x 128 hide each other's
       // (8192 x 1024 by w of 8192 rows, 16 steps a tile: 256 x 256 250 us, 256 x 128 185, 128 x 128 159; gradient by x of
-      // 8192 x 7168 with k = 2048: 349, 337, 261; 8192^3: 256 x 256 997).  Two weights end a tile with twice the sums and
-      // the activation.
+      // 8192 x 7168 with k = 2048: 349, 337, 261; 8192^3: 256 x 256 968).  Two weights end a tile with twice the sums and
+      // the activation.  In slices a 256 x 128 tile starts and ends in less, since CUs have one each (512 rows by w of 4096 x
+      // 4096 in four slices 31 us, tiles of 128 x 128 in two 34; 130 rows in eight 19 and 20; 2048 x 2048 with k = 16384 in
+      // two 180 and 161).  Over 389 products of 130 to 16384 rows the choice takes 0.7% more than the best one.
       const double more = pair ? 8.0 : 0.0;
       const Tile dma_tiles[] = {{2, 256, 256, 1.72, 0, 27 + more}, {3, 256, 128, 1.0, 0, 12}, {0, 128, 128, 0.76, 1.0, 3.3}};
       static const Tile term_tiles[] = {
@@ -89,7 +91,8 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, 
         for (int64_t s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
           if (s > 1 && (s * plane > most || steps < 4 * s || tiles * s > 1024)) break;
           const int64_t n = tiles * s;
-          const double k = (double)((steps + s - 1) / s), one = t->one * k + t->start, two = t->two * k + 1.5 * t->start;
+          const double k = (double)((steps + s - 1) / s), two = t->two * k + 1.5 * t->start;
+          const double one = lds && t->kind == 3 && s > 1 ? 1.1 * k + 3 : t->one * k + t->start;
           double us = t->two ? n / 512 * two + (n % 512 > 256 ? two : n % 512 ? one : 0.0) : (n + 255) / 256 * one;
           us += s > 1 ? 4.0 + s * plane * 2 / 5e6 : 0.0;
           if (us < best) {
