@@ -519,13 +519,14 @@ __device__ __forceinline__ bool lin_finite(float v) { return fabsf(v) <= F32_MOS
 // by the number of rows or by the kernel.  Finite sums cost a check (2048^3 in f32: 108 us with and without it); with an
 // infinity in every row all of them are taken again, 16 ms (512 x 4096 x 4096, f32 by bf16: 32); behind a NaN, where the
 // sum stays one, 0.14 ms.
+template <int FORM>  // (as a value of g it took the kernels of one weight 2 to 5% more: 32 scalar registers spilled)
 __device__ __forceinline__ float lin_again(const LinArgs &g, int64_t m, int64_t n) {
   const int64_t ak = g.a_kc ? 1 : g.lda, bk = g.b_kc ? 1 : g.ldb;
-  const int planes = g.form == LIN_SUM ? g.half : g.planes;
-  const void *from = g.form == LIN_PAIR && (n & 16) ? g.b2 : g.b;
-  if (g.form == LIN_PAIR) n = pair_row(n);
+  const int planes = FORM == LIN_SUM ? g.half : g.planes;
+  const void *from = FORM == LIN_PAIR && (n & 16) ? g.b2 : g.b;
+  if (FORM == LIN_PAIR) n = pair_row(n);
   float s = 0.f;
-  for (int h = 0; h < (g.form == LIN_SUM ? 2 : 1); ++h) {
+  for (int h = 0; h < (FORM == LIN_SUM ? 2 : 1); ++h) {
     size_t ia = (size_t)(g.a_kc ? m * g.lda : m) + (h ? g.K : 0), ib = (size_t)(g.b_kc ? n * g.ldb : n);
     if (h) from = g.b2;
     for (int64_t k = 0; k < g.K && s == s; k += 4, ia += 4 * ak, ib += 4 * bk) {
@@ -545,17 +546,19 @@ __device__ __forceinline__ float lin_again(const LinArgs &g, int64_t m, int64_t 
   return s;
 }
 // whether column n of the product is one of the result
+template <int FORM>
 __device__ __forceinline__ bool lin_column(const LinArgs &g, int64_t n) {
-  return g.form == LIN_PAIR ? pair_row(n) < g.F : n < g.N;
+  return FORM == LIN_PAIR ? pair_row(n) < g.F : n < g.N;
 }
 // sums of row m, columns n .. n + 3: those that are not finite again
+template <int FORM>
 __device__ __forceinline__ void lin_repair(const LinArgs &g, int64_t m, int64_t n, v4f &v) {
   if (m >= g.M || lin_finite((fabsf(v.x) + fabsf(v.y)) + (fabsf(v.z) + fabsf(v.w)))) return;
 #pragma unroll 1
   for (int q = 0; q < 4; ++q) {
     const float x = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
-    if (lin_finite(x) || !lin_column(g, n + q)) continue;
-    const float y = lin_again(g, m, n + q);
+    if (lin_finite(x) || !lin_column<FORM>(g, n + q)) continue;
+    const float y = lin_again<FORM>(g, m, n + q);
     v.x = q == 0 ? y : v.x;
     v.y = q == 1 ? y : v.y;
     v.z = q == 2 ? y : v.z;
@@ -564,7 +567,7 @@ __device__ __forceinline__ void lin_repair(const LinArgs &g, int64_t m, int64_t 
 }
 // the same for a wave's fragments, where there is one slice (else the slices' join does it); at(i, 0), at(j, 1): their m
 // and n; TERMS: whether the kernel's operands may come as terms
-template <bool TERMS, int FM, int FN, class At>
+template <int FORM, bool TERMS, int FM, int FN, class At>
 __device__ __forceinline__ void lin_repair_all(const LinArgs &g, v4f (&acc)[FM][FN], const At &at) {
   if (!TERMS || !g.terms || g.slices > 1) return;
   float most = 0.f;  // (a sum past f32's largest is looked at again value by value)
@@ -578,7 +581,7 @@ __device__ __forceinline__ void lin_repair_all(const LinArgs &g, v4f (&acc)[FM][
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) lin_repair(g, at(i, 0), at(j, 1), acc[i][j]);
+    for (int j = 0; j < FN; ++j) lin_repair<FORM>(g, at(i, 0), at(j, 1), acc[i][j]);
 }
 
 // four sums of slice z: into its plane, or finished where there is one slice
@@ -756,7 +759,7 @@ __global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinA
     if (t + 1 >= steps) break;
     step(lds[BUFS - 1], lds[0], p, BUFS == 2 ? q : p);
   }
-  lin_repair_all<(NA * NB > 1 || !KCB), FM, FN>(
+  lin_repair_all<FORM, (NA * NB > 1 || !KCB), FM, FN>(
       g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
   lin_results<FORM>(g, z, m0 + wm, n0 + wn, fr, fc, acc);
 }
@@ -951,14 +954,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear_dma(LinArgs g) {
   }
   wait_vm<0>();  // (what was asked for past the end writes zeros: not into another workgroup's LDS)
   const int fr = lane & 15, fc = lane >> 4;
-  lin_repair_all<!KCB, FM, FN>(
+  lin_repair_all<FORM, !KCB, FM, FN>(
       g, acc, [&](int i, int n) { return n ? n0 + wn + 16 * i + 4 * fc : m0 + wm + 16 * i + fr; });
   lin_results<FORM>(g, z, m0 + wm, n0 + wn, fr, fc, acc);
 }
 
 // Results of the k slices added in order (the same bits on every call), then the epilogue.  G threads share four
 // results where there are many slices: each adds every G-th, four loads in flight, and their sums meet in LDS.
-template <int G>
+template <int G, int FORM>
 static __global__ __launch_bounds__(256) void k_linear_join(LinArgs g) {
   constexpr int Q = 256 / G;  // quads of results of a workgroup
   __shared__ v4f red[G][Q];
@@ -998,14 +1001,19 @@ static __global__ __launch_bounds__(256) void k_linear_join(LinArgs g) {
     for (int k = 1; k < G; ++k) v += red[k][threadIdx.x];
   }
   if (!in) return;
-  if (g.terms) lin_repair(g, m, n, v);
+  if (g.terms) lin_repair<FORM>(g, m, n, v);
   lin_finish4(g.e, m, n, g.N, v);
 }
-static inline void lin_join(const LinArgs &g, hipStream_t st) {
+template <int FORM>
+void lin_join_of(const LinArgs &g, hipStream_t st) {
   const int64_t quads = g.M * ((g.N + 3) / 4);
   if (g.slices > 8 && quads < (1 << 26))
-    hipLaunchKernelGGL((k_linear_join<16>), dim3((unsigned)((quads + 15) / 16)), dim3(256), 0, st, g);
-  else hipLaunchKernelGGL((k_linear_join<1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((k_linear_join<16, FORM>), dim3((unsigned)((quads + 15) / 16)), dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((k_linear_join<1, FORM>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, g);
+}
+static inline void lin_join(const LinArgs &g, hipStream_t st) {
+  if (g.form == LIN_SUM) lin_join_of<LIN_SUM>(g, st);
+  else lin_join_of<LIN_ONE>(g, st);
 }
 
 // ============================================================ few rows
@@ -1220,7 +1228,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinArgs g) {
     if (k + 2 * KS < ke) load(p, k + 2 * KS);
     step(q, lds[1]);
   }
-  lin_repair_all<(NX * NW > 1), MT, NF>(g, acc, [&](int i, int n) { return n ? n1 + 16 * i + 4 * fc : m0 + 16 * i + fr; });
+  lin_repair_all<FORM, (NX * NW > 1), MT, NF>(
+      g, acc, [&](int i, int n) { return n ? n1 + 16 * i + 4 * fc : m0 + 16 * i + fr; });
   lin_results<FORM>(g, z, m0, n1, fr, fc, acc);
 }
 
@@ -1354,8 +1363,8 @@ static __global__ __launch_bounds__(256) void k_pair_join(LinArgs g) {
   }
   if (!in) return;
   if (g.terms) {
-    lin_repair(g, m, n, v[0]);
-    lin_repair(g, m, n + 16, v[1]);
+    lin_repair<LIN_PAIR>(g, m, n, v[0]);
+    lin_repair<LIN_PAIR>(g, m, n + 16, v[1]);
   }
   lin_finish_pair(g.e, m, f, g.F, v[0], v[1]);
 }
