@@ -673,16 +673,22 @@ struct Lora {
           part(now.l, r);
         }
       }
+      // (a product that is infinite or no number has a factor that is)
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < C; ++h)
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) most = __builtin_fmaf(acc[i][h][q], acc[i][h][q + 1], most);
+      const bool again = __ballot(!lin_finite(most));
       // a tile of 16 tokens at a time, rows of 64 columns and 4 more
       float *rows = (float *)buf;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         if (16 * i >= it.count) break;
-        float most = 0.f;
 #pragma unroll
         for (int h = 0; h < C; ++h) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) most += fabsf(acc[i][h][q]);
           if constexpr (KC) {
             *reinterpret_cast<v4f *>(rows + fr * 68 + 16 * h + 4 * fc) = acc[i][h];
           } else {
@@ -691,7 +697,7 @@ struct Lora {
           }
         }
         stage_sync();
-        if (__ballot(!lin_finite(most))) {
+        if (again) {
 #pragma unroll 1
           for (int s = 0; s < 16 && 16 * i + s < it.count; ++s) {
             float &at = rows[s * 68 + lane];
