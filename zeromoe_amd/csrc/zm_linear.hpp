@@ -526,7 +526,8 @@ __device__ __forceinline__ float lin_again(const LinArgs &g, int64_t m, int64_t 
   const void *from = FORM == LIN_PAIR && (n & 16) ? g.b2 : g.b;
   if (FORM == LIN_PAIR) n = pair_row(n);
   float s = 0.f;
-  for (int h = 0; h < (FORM == LIN_SUM ? 2 : 1); ++h) {
+  // (both weights; as a constant of 2 the compiler orders the kernel otherwise: 6333 x 334 by x, 59 us for 54)
+  for (int h = 0; h < (FORM == LIN_SUM ? g.planes / planes : 1); ++h) {
     size_t ia = (size_t)(g.a_kc ? m * g.lda : m) + (h ? g.K : 0), ib = (size_t)(g.b_kc ? n * g.ldb : n);
     if (h) from = g.b2;
     for (int64_t k = 0; k < g.K && s == s; k += 4, ia += 4 * ak, ib += 4 * bk) {
