@@ -29,6 +29,7 @@ libzeromoe_hip.so (include/zeromoe.h):
   :func:`glu` (both halves of a gated feed-forward block as one product),
   :func:`lora` (a low-rank adapter named by each token) and
   :func:`clip_grad_norm` / :func:`grad_norm` (the gradients of a whole step).
+  No gradient goes through the quantized experts: what lies beside them is trained.
 
 Torch is used only for device memory and the current stream.
 """

@@ -769,7 +769,7 @@ __global__ __launch_bounds__(64 * WM * WN, BUFS == 1 ? 4 : 1) void k_linear(LinA
 //
 // The same product for 16-bit operands of one type, bound by the matrix cores.  Tiles go from global memory straight
 // into LDS (16 bytes a lane, whole cache lines of 64 k), two steps deep; fragments are read into registers half a step
-// ahead; one barrier a step.  8192^3 in bf16: 945 us, 1160 TFLOP/s (without its loads the loop does 1460; with them
+// ahead; one barrier a step.  8192^3 in bf16: 968 us, 1136 TFLOP/s (without its loads the loop does 1460; with them
 // answered by L2 alone 1290; reading them where a step of 32 k is four deep, in half lines, 780).
 //
 // An operand whose k is contiguous lies in LDS in rows of 64 k, its 16-byte chunks permuted by the row so that 16 rows

@@ -64,9 +64,9 @@ Plan plan(Kind kind, int64_t M, int64_t N, int64_t K, int planes, int products, 
         double one, two, start;
       };
       // 16-bit operands: a tile alone on its CU starts and ends with nothing beside it, two of 128 x 128 hide each other's
-      // (8192 x 1024 by w of 8192 rows, 16 steps a tile: 256 x 256 250 us, 256 x 128 185, 128 x 128 159; gradient by x of
-      // 8192 x 7168 with k = 2048: 349, 337, 261; 8192^3: 256 x 256 968).  Two weights end a tile with twice the sums and
-      // the activation.  In slices a 256 x 128 tile starts and ends in less, since CUs have one each (512 rows by w of 4096 x
+      // (gradients by x of 8192 x 8192 with k = 1024: 256 x 256 304 us, 256 x 128 297, 128 x 128 181; of 8192 x 7168 with
+      // k = 2048: 387, 398, 277; 8192^3: 971, 1115, 1051).  Two weights end a tile with twice the sums and the activation
+      // (8192 x 7168 by two of 2048: 437, 450, 428 on one set of operands, 448, 558, 476 on three in turn).  In slices a 256 x 128 tile starts and ends in less, since CUs have one each (512 rows by w of 4096 x
       // 4096 in four slices 31 us, tiles of 128 x 128 in two 34; 130 rows in eight 19 and 20; 2048 x 2048 with k = 16384 in
       // two 180 and 161).  Over 389 products of 130 to 16384 rows the choice takes 0.7% more than the best one.
       const double more = pair ? 8.0 : 0.0;
