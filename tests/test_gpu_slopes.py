@@ -60,3 +60,18 @@ def test_slopes_far_out(act, low):
     gate = Z.glu_backward(d, x, w, w, z, d, act=act, need_dx=False, need_dw=False)[3]
     for g in (gate,) if act == "none" else (got, gate):
         assert torch.equal(g[:8], want) and (act == "none" or g[8].isnan())
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_no_activation_has_a_slope_of_one(t):
+    """A NaN of the gate reaches up's gradient, which it multiplies, and not its own."""
+    import zeromoe_amd as Z
+
+    S, I, F = 20, 264, 100
+    x, w, dy, gate, up = (rand(*s, seed=i, dtype=t) for i, s in enumerate(((S, I), (F, I), (S, F), (S, F), (S, F))))
+    gate[3, 7] = math.nan
+    dx, dwg, dwu, dbg, dbu = Z.glu_backward(dy, x, w, w, gate, up, act="none")
+    assert dwg.isfinite().all() and dbg.isfinite().all()
+    for m in (dwu, dbu):
+        assert m[7].isnan().all() and m[:7].isfinite().all() and m[8:].isfinite().all()
+    assert dx[3].isnan().all() and dx[:3].isfinite().all() and dx[4:].isfinite().all()

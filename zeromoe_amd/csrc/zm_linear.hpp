@@ -136,7 +136,7 @@ __device__ __forceinline__ float lin_slope_of_number(float z, int act) {
 // (the clamps and comparisons above would make a number of a NaN)
 __device__ __forceinline__ float lin_act_slope(float z, int act) {
   const float s = lin_slope_of_number(z, act);
-  return z == z ? s : z;
+  return z == z || act == ACT_NONE ? s : z;  // (without an activation 1, whatever z is)
 }
 
 // both of a factor; gelu's share their erfc (8192 x 4096 in bf16 with the bias sums: 101 -> 76 us)
