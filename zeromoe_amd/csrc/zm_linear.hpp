@@ -106,14 +106,29 @@ __device__ __forceinline__ float factor_act(float z, int act) {
   if (act == ACT_GELU_TANH) return z / (1.0f + expf(-1.5957691216057307f * (z + 0.044715f * z * z * z)));
   return lin_act(z, act);
 }
-// slopes keep their digits where they are small too: Phi(z) = erfc(-z / sqrt 2) / 2 for 1 + erf, and for 1 + tanh and 1 - tanh^2
-// the logistic function s of twice their argument, s and s (1 - s)
+// The normal distribution and its density.  The tail is exp(-x^2 / 2) t P(t), x = |z|, t = 1 / (1 + 0.32 x), so that one exp
+// gives both; P is fitted to erfcx(x / sqrt 2) / (2 t) for the least largest relative error, 3.2e-8, and 3.2e-7 in f32
+// (bias gradient of 8192 x 4096 in bf16: erff and expf 105 us, erfcf and expf 110, this 103).
+__device__ __forceinline__ void normal(float z, float &cdf, float &pdf) {
+  const float t = 1.0f / (1.0f + 0.32f * fabsf(z)), e = expf(-0.5f * (z * z));
+  constexpr float P[10] = {0.127661526f, 0.127660945f, 0.114622362f, 0.0878290758f, 0.0586541221f,
+                           -0.00937805325f, 0.0653288662f, -0.14670831f, 0.0954077169f, -0.0210782699f};
+  float p = P[9];
+#pragma unroll
+  for (int k = 8; k >= 0; --k) p = __builtin_fmaf(p, t, P[k]);
+  const float tail = e * (t * p);
+  cdf = z < 0.f ? tail : 1.0f - tail;
+  pdf = e * 0.39894228040143268f;
+}
+// slopes keep their digits where they are small too: no 1 + erf, and for 1 + tanh and 1 - tanh^2 the logistic function s of
+// twice their argument, s and s (1 - s)
 __device__ __forceinline__ float lin_slope_of_number(float z, int act) {
   switch (act) {
   case ACT_RELU: return z > 0.f ? 1.0f : 0.0f;
   case ACT_GELU: {
-    const float zc = fminf(fmaxf(z, -20.f), 20.f);  // exp(-z^2/2) is 0 there; z * exp() has no inf * 0
-    return 0.5f * erfcf(z * -0.70710678118654752f) + zc * expf(-0.5f * zc * zc) * 0.39894228040143268f;
+    float cdf, pdf;
+    normal(z, cdf, pdf);
+    return cdf + fminf(fmaxf(z, -20.f), 20.f) * pdf;  // (pdf is 0 there: no inf * 0)
   }
   case ACT_GELU_TANH: {
     const float zc = fminf(fmaxf(z, -20.f), 20.f);  // s is 0 or 1 there
@@ -139,12 +154,13 @@ __device__ __forceinline__ float lin_act_slope(float z, int act) {
   return z == z || act == ACT_NONE ? s : z;  // (without an activation 1, whatever z is)
 }
 
-// both of a factor; gelu's share their erfc (8192 x 4096 in bf16 with the bias sums: 101 -> 76 us)
+// both of a factor, gelu's from one distribution
 __device__ __forceinline__ void factor_and_slope(float z, int act, float &a, float &s) {
   if (act == ACT_GELU) {
-    const float zc = fminf(fmaxf(z, -20.f), 20.f), c = erfcf(z * -0.70710678118654752f);
-    a = 0.5f * z * c;
-    s = z == z ? 0.5f * c + zc * expf(-0.5f * zc * zc) * 0.39894228040143268f : z;
+    float cdf, pdf;
+    normal(z, cdf, pdf);
+    a = z * cdf;
+    s = z == z ? cdf + fminf(fmaxf(z, -20.f), 20.f) * pdf : z;
   } else {
     a = factor_act(z, act);
     s = lin_act_slope(z, act);
