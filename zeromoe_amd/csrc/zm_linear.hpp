@@ -535,15 +535,18 @@ __device__ __forceinline__ bool lin_finite(float v) { return fabsf(v) <= F32_MOS
 // by the number of rows or by the kernel.  Finite sums cost a check (2048^3 in f32: 108 us with and without it); with an
 // infinity in every row all of them are taken again, 16 ms (512 x 4096 x 4096, f32 by bf16: 32); behind a NaN, where the
 // sum stays one, 0.14 ms.
-template <int FORM>  // (as a value of g it took the kernels of one weight 2 to 5% more: 32 scalar registers spilled)
+// (One weight knows its form here: with the branches of two, 32 more scalar registers spill, 2 to 5% on products of 10 to 40
+// us.  With two weights a form or a count of loops that the compiler knows took dx of 6333 x 334 x 416 from 54 us to 59, or
+// dx of 7232 x 288 x 96 from 16 to 19.)
+template <int FORM>
 __device__ __forceinline__ float lin_again(const LinArgs &g, int64_t m, int64_t n) {
+  const int form = FORM == LIN_ONE ? LIN_ONE : g.form;
   const int64_t ak = g.a_kc ? 1 : g.lda, bk = g.b_kc ? 1 : g.ldb;
-  const int planes = FORM == LIN_SUM ? g.half : g.planes;
-  const void *from = FORM == LIN_PAIR && (n & 16) ? g.b2 : g.b;
-  if (FORM == LIN_PAIR) n = pair_row(n);
+  const int planes = form == LIN_SUM ? g.half : g.planes;
+  const void *from = form == LIN_PAIR && (n & 16) ? g.b2 : g.b;
+  if (form == LIN_PAIR) n = pair_row(n);
   float s = 0.f;
-  // (both weights; as a constant of 2 the compiler orders the kernel otherwise: 6333 x 334 by x, 59 us for 54)
-  for (int h = 0; h < (FORM == LIN_SUM ? g.planes / planes : 1); ++h) {
+  for (int h = 0; h < (form == LIN_SUM ? 2 : 1); ++h) {
     size_t ia = (size_t)(g.a_kc ? m * g.lda : m) + (h ? g.K : 0), ib = (size_t)(g.b_kc ? n * g.ldb : n);
     if (h) from = g.b2;
     for (int64_t k = 0; k < g.K && s == s; k += 4, ia += 4 * ak, ib += 4 * bk) {
@@ -565,7 +568,7 @@ __device__ __forceinline__ float lin_again(const LinArgs &g, int64_t m, int64_t 
 // whether column n of the product is one of the result
 template <int FORM>
 __device__ __forceinline__ bool lin_column(const LinArgs &g, int64_t n) {
-  return FORM == LIN_PAIR ? pair_row(n) < g.F : n < g.N;
+  return (FORM == LIN_ONE ? LIN_ONE : g.form) == LIN_PAIR ? pair_row(n) < g.F : n < g.N;
 }
 // sums of row m, columns n .. n + 3: those that are not finite again
 template <int FORM>
