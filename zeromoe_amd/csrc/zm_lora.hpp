@@ -713,7 +713,7 @@ struct Lora {
           for (int j = 0; j < VY; j += 4) {
             const v4f v = *reinterpret_cast<const v4f *>(rows + (s - 16 * i) * 68 + yc + j);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) f[j + k] = g.res ? __builtin_fmaf(c, v[k], now.z[i][q].get(j + k)) : c * v[k];
+            for (int k = 0; k < 4; ++k) f[j + k] = __builtin_fmaf(c, v[k], g.res ? now.z[i][q].get(j + k) : 0.f);
           }
           if (s >= it.count) continue;
           TY *at = (TY *)g.y + token[i][q] * g.ldy + o0 + yc;
